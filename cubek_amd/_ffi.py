@@ -14,6 +14,7 @@ from typing import Sequence
 from .scheme import _CScheme
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libcubek_quant_hip.so")
+MATMUL_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libcubek_matmul_hip.so")
 
 #: every symbol include/cubek_quant.h declares
 EXPORTED_SYMBOLS = (
@@ -23,6 +24,10 @@ EXPORTED_SYMBOLS = (
     "cq_into_contiguous_packed", "cq_quantize_dynamic_static",
     "cq_gemv_quantized", "cq_plan_kind",
 )
+
+#: every symbol include/cubek_matmul.h declares
+MATMUL_SYMBOLS = ("cq_matmul_quantized", "cq_matmul_workspace_bytes", "cq_experts_quantized", "cq_experts_workspace_bytes", "cq_route",
+                  "cq_route_workspace_bytes", "cq_combine", "cq_matmul_last_hip_error")
 
 
 class CTensor(ctypes.Structure):
@@ -34,6 +39,17 @@ class CTensor(ctypes.Structure):
         ("strides", ctypes.POINTER(ctypes.c_uint64)),
         ("rank", ctypes.c_uint32),
         ("elem_size", ctypes.c_uint32),
+    ]
+
+
+class CEpilogue(ctypes.Structure):
+    """Binary layout of ``cq_epilogue`` (include/cubek_matmul.h)."""
+
+    _fields_ = [
+        ("activation", ctypes.c_uint32),
+        ("gated", ctypes.c_uint32),
+        ("bias", ctypes.POINTER(CTensor)),
+        ("residual", ctypes.POINTER(CTensor)),
     ]
 
 
@@ -51,6 +67,7 @@ OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED_SCHEME, ERR_BLOCK_NOT_DIVISIBLE, ERR_S
     ERR_SCRATCH_TOO_SMALL = range(11)
 
 _lib = None
+_matmul_lib = None
 _calls = None
 
 
@@ -105,6 +122,48 @@ def lib() -> ctypes.CDLL:
     return L
 
 
+def matmul_lib() -> ctypes.CDLL:
+    """The library of include/cubek_matmul.h: products of many tokens, grouped products, routing."""
+    global _matmul_lib
+    if _matmul_lib is not None:
+        return _matmul_lib
+    if not os.path.exists(MATMUL_LIB_PATH):
+        raise RuntimeError(f"native library not built: {MATMUL_LIB_PATH} is missing; there is no fallback path. "
+                           "Build it with `make -C cubek_amd/csrc` (needs hipcc).")
+    lib()
+    L = ctypes.CDLL(MATMUL_LIB_PATH)
+    tp, sp, ep = ctypes.POINTER(CTensor), ctypes.POINTER(_CScheme), ctypes.POINTER(CEpilogue)
+    space = [ctypes.c_void_p, ctypes.c_size_t]
+    L.cq_matmul_quantized.restype = ctypes.c_int
+    L.cq_matmul_quantized.argtypes = [ctypes.c_void_p, tp, tp, sp, tp, tp, ctypes.c_int, ctypes.c_int, ep] + space
+    L.cq_matmul_workspace_bytes.restype = ctypes.c_size_t
+    L.cq_matmul_workspace_bytes.argtypes = [tp, sp, tp, ctypes.c_int, ep]
+    L.cq_experts_quantized.restype = ctypes.c_int
+    L.cq_experts_quantized.argtypes = [ctypes.c_void_p, tp, tp, sp, tp, tp, tp, tp, ctypes.c_int, ctypes.c_int, ep] + space
+    L.cq_experts_workspace_bytes.restype = ctypes.c_size_t
+    L.cq_experts_workspace_bytes.argtypes = [tp, sp, tp, ctypes.c_int, ep]
+    L.cq_route.restype = ctypes.c_int
+    L.cq_route.argtypes = [ctypes.c_void_p] + [tp] * 6 + [ctypes.c_int, ctypes.c_int, ctypes.c_uint32] + space
+    L.cq_route_workspace_bytes.restype = ctypes.c_size_t
+    L.cq_route_workspace_bytes.argtypes = [ctypes.c_uint64] * 3
+    L.cq_combine.restype = ctypes.c_int
+    L.cq_combine.argtypes = [ctypes.c_void_p] + [tp] * 5 + [ctypes.c_int, ctypes.c_int]
+    L.cq_matmul_last_hip_error.restype = ctypes.c_int
+    L.cq_matmul_last_hip_error.argtypes = []
+    _matmul_lib = L
+    return L
+
+
+def epilogue_to_c(epilogue) -> CEpilogue:
+    """The ``cq_epilogue`` of an ``Epilogue``; its tensors live as long as their handles."""
+    c = CEpilogue(int(epilogue.activation), int(epilogue.gated))
+    for name in ("bias", "residual"):
+        t = getattr(epilogue, name)
+        if t is not None:
+            setattr(c, name, ctypes.pointer(t.as_c()))
+    return c
+
+
 def calls():
     """The module of the package's calls (csrc/py_call.cpp): each takes the Python objects of a call and returns its status."""
     global _calls
@@ -129,6 +188,13 @@ def check(status: int) -> None:
         if status == ERR_HIP:
             msg += f" (hipError_t {lib().cq_last_hip_error()})"
         raise QuantError(status, msg)
+
+
+def check_matmul(status: int) -> None:
+    """check() for the calls of include/cubek_matmul.h, whose library keeps its own last HIP error."""
+    if status == ERR_HIP:
+        raise QuantError(status, f"{lib().cq_strerror(status).decode()} (hipError_t {matmul_lib().cq_matmul_last_hip_error()})")
+    check(status)
 
 
 def make_tensor(ptr: int, shape: Sequence[int], strides: Sequence[int], elem_size: int):

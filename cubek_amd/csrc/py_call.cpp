@@ -1,5 +1,5 @@
 // The package's calls without ctypes: a CPython module that reads the handles, the scheme and the numbers of a call from the
-// Python objects and calls the C ABI (include/cubek_quant.h).
+// Python objects and calls the C ABI (include/cubek_quant.h, include/cubek_matmul.h).
 //
 // A call that launches one kernel takes the HIP runtime 3.2 us of the host.  Through ctypes (a lookup of the scheme's
 // struct by its hash, a cached struct per handle, a conversion per argument) the package added 1.2 us to that: quantize
@@ -12,6 +12,7 @@
 #include <initializer_list>
 #include <utility>
 
+#include "../../include/cubek_matmul.h"
 #include "../../include/cubek_quant.h"
 
 namespace {
@@ -275,6 +276,101 @@ PyObject* repack(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// A tensor argument that may be None.
+struct OptionalTensor {
+    Tensor tensor;
+    const cq_tensor* t = nullptr;
+    bool read(PyObject* o) {
+        if (o == Py_None) return true;
+        t = &tensor.t;
+        return tensor.read(o);
+    }
+};
+
+// activation, gated, bias, residual, workspace, bytes: what the products with an epilogue end in
+struct EpilogueArgs {
+    cq_epilogue e{};
+    OptionalTensor bias, residual;
+    void* workspace;
+    uint64_t bytes;
+    static constexpr Py_ssize_t kArgs = 6;
+
+    bool read(PyObject* const* a) {
+        uint64_t activation, gated;
+        if (!number(a[0], &activation) || !number(a[1], &gated) || !bias.read(a[2]) || !residual.read(a[3]) || !pointer(a[4], &workspace) ||
+            !integer(a[5], &bytes))
+            return false;
+        e.activation = static_cast<uint32_t>(activation);
+        e.gated = static_cast<uint32_t>(gated);
+        e.bias = bias.t;
+        e.residual = residual.t;
+        return true;
+    }
+};
+
+// stream, values, params, scheme, x, y, elem, y_elem, epilogue
+PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* stream;
+    Tensor values, params, x, y;
+    cq_scheme scheme;
+    cq_dtype elem, y_elem;
+    EpilogueArgs epi;
+    if (!count(n, 8 + epi.kArgs) || !pointer(a[0], &stream) || !values.read(a[1]) || !params.read(a[2]) || !read_scheme(a[3], &scheme) || !x.read(a[4]) ||
+        !y.read(a[5]) || !Common<1>::read_elem(a[6], &elem) || !Common<1>::read_elem(a[7], &y_elem) || !epi.read(a + 8))
+        return nullptr;
+    return status_of([&] {
+        return cq_matmul_quantized(static_cast<cq_stream_t>(stream), &values.t, &params.t, &scheme, &x.t, &y.t, elem, y_elem, &epi.e, epi.workspace,
+                                   epi.bytes);
+    });
+}
+
+// stream, values, params, scheme, x, offsets, rows, y, elem, y_elem, epilogue
+PyObject* experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* stream;
+    Tensor values, params, x, offsets, y;
+    OptionalTensor rows;
+    cq_scheme scheme;
+    cq_dtype elem, y_elem;
+    EpilogueArgs epi;
+    if (!count(n, 10 + epi.kArgs) || !pointer(a[0], &stream) || !values.read(a[1]) || !params.read(a[2]) || !read_scheme(a[3], &scheme) || !x.read(a[4]) ||
+        !offsets.read(a[5]) || !rows.read(a[6]) || !y.read(a[7]) || !Common<1>::read_elem(a[8], &elem) || !Common<1>::read_elem(a[9], &y_elem) ||
+        !epi.read(a + 10))
+        return nullptr;
+    return status_of([&] {
+        return cq_experts_quantized(static_cast<cq_stream_t>(stream), &values.t, &params.t, &scheme, &x.t, &offsets.t, rows.t, &y.t, elem, y_elem, &epi.e,
+                                    epi.workspace, epi.bytes);
+    });
+}
+
+// stream, logits, weights, experts, offsets, rows, slots, elem, score, normalize, workspace, bytes
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void *stream, *workspace;
+    Tensor t[6];
+    cq_dtype elem;
+    uint64_t score, normalize, bytes;
+    if (!count(n, 12) || !pointer(a[0], &stream)) return nullptr;
+    for (int i = 0; i < 6; i++)
+        if (!t[i].read(a[1 + i])) return nullptr;
+    if (!Common<1>::read_elem(a[7], &elem) || !number(a[8], &score) || !number(a[9], &normalize) || !pointer(a[10], &workspace) || !integer(a[11], &bytes))
+        return nullptr;
+    return status_of([&] {
+        return cq_route(static_cast<cq_stream_t>(stream), &t[0].t, &t[1].t, &t[2].t, &t[3].t, &t[4].t, &t[5].t, elem,
+                        static_cast<cq_score>(static_cast<int>(score)), static_cast<uint32_t>(normalize), workspace, bytes);
+    });
+}
+
+// stream, h, slots, weights, residual, y, h_elem, y_elem
+PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* stream;
+    Tensor h, slots, weights, y;
+    OptionalTensor residual;
+    cq_dtype h_elem, y_elem;
+    if (!count(n, 8) || !pointer(a[0], &stream) || !h.read(a[1]) || !slots.read(a[2]) || !weights.read(a[3]) || !residual.read(a[4]) || !y.read(a[5]) ||
+        !Common<1>::read_elem(a[6], &h_elem) || !Common<1>::read_elem(a[7], &y_elem))
+        return nullptr;
+    return status_of([&] { return cq_combine(static_cast<cq_stream_t>(stream), &h.t, &slots.t, &weights.t, residual.t, &y.t, h_elem, y_elem); });
+}
+
 template <class F>
 constexpr PyMethodDef method(const char* name, F f) {
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr};
@@ -294,6 +390,7 @@ PyMethodDef methods[] = {
     method("quantize", quantize), method("dequantize", dequantize), method("compute_scales", compute_scales),
     method("quantize_dynamic", quantize_dynamic), method("quantize_dynamic_static", quantize_dynamic_static),
     method("gemv", gemv), method("max_abs", max_abs), method("repack", repack),
+    method("matmul", matmul), method("experts", experts), method("route", route), method("combine", combine),
     {"bind", bind, METH_VARARGS, "bind(TensorHandleRef, QuantScheme)"}, {nullptr, nullptr, 0, nullptr},
 };
 
