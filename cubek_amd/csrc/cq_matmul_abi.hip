@@ -1,5 +1,5 @@
 // C ABI of libcubek_matmul_hip.so (include/cubek_matmul.h): argument checks, the choice of a kernel, launches.
-#include "cq_matmul_internal.hpp"
+#include "cq_matmul_tiles.hpp"
 
 namespace {
 
@@ -166,7 +166,11 @@ cq_status read_indexes(const cq_tensor* t, uint64_t n, const int32_t** out) {
     return CQ_OK;
 }
 
-cq_status launch(cq_stream_t stream, const cq::MatmulArgs& a) { return hip_status(cq::launch_matmul_general(stream, a)); }
+cq_status launch(cq_stream_t stream, cq::MatmulArgs& a) {
+    const uint64_t size = dtype_size(a.y_dtype);
+    a.vector_stores = aligned(a.y, 16) && a.y_stride * size % 16 == 0 && (!a.residual || (aligned(a.residual, 16) && a.residual_stride * size % 16 == 0));
+    return hip_status(cq::tiles_take(a) ? cq::launch_matmul_tiles(stream, a) : cq::launch_matmul_general(stream, a));
+}
 
 }  // namespace
 

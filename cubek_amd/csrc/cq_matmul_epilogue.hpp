@@ -21,13 +21,32 @@ __device__ __forceinline__ void store_float(int dtype, char* p, uint64_t i, floa
         reinterpret_cast<__bf16*>(p)[i] = static_cast<__bf16>(v);
 }
 
+// 1 / (1 + exp(-v)), by the hardware's exp2 and reciprocal (one unit in the last place each).
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f)); }
+
+// erfc(x) for x >= 0 by Abramowitz and Stegun 7.1.26 (Hastings), a fifth-order polynomial in 1 / (1 + p x) times exp(-x^2): within 1.5e-7, and in
+// the tail as small as erfc itself, so that a product with it loses nothing to cancellation.  The library's erff takes three times the
+// instructions (gelu of 4096 x 28672 values).
+__device__ __forceinline__ float erfc_positive(float x) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    return p * t * __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
+}
+
 // `activation` is uniform over the launch.
 __device__ __forceinline__ float activated(uint32_t activation, float v) {
     switch (activation) {
         case CQ_ACT_RELU: return v < 0.0f ? 0.0f : v;
-        case CQ_ACT_SILU: return v / (1.0f + expf(-v));
-        case CQ_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-        case CQ_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+        case CQ_ACT_SILU: return v * sigmoid(v);
+        case CQ_ACT_GELU: {
+            const float half = 0.5f * v * erfc_positive(__builtin_fabsf(v) * 0.70710678118654752f);
+            return v < 0.0f ? half : v - half;
+        }
+        // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
+        case CQ_ACT_GELU_TANH: return v * sigmoid(1.5957691216057308f * __builtin_fmaf(0.044715f * v * v, v, v));
         default: return v;
     }
 }
@@ -74,15 +93,61 @@ __device__ __forceinline__ bool find_tile(const MatmulArgs& a, uint32_t tile, ui
     return false;
 }
 
-// Tiles that a launch has to hold for any offsets: every expert may end in a tile that is not full.
-inline uint64_t most_tiles(const MatmulArgs& a, uint32_t size_log2) {
-    const uint64_t full = (static_cast<uint64_t>(a.positions) + (1u << size_log2) - 1u) >> size_log2;
-    return a.offsets ? full + (a.experts < a.positions ? a.experts : a.positions) : full;
-}
-
 __device__ __forceinline__ uint32_t row_of_position(const MatmulArgs& a, uint32_t p) {
     if (a.row_of == nullptr) return p;
     return static_cast<uint32_t>(min(max(a.row_of[p], 0), static_cast<int32_t>(a.tokens) - 1));
+}
+
+// Columns col .. col + 7 of position p, as far as y has them, from their sums (and those of the gated ones) in LDS.
+__device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, const float* sums, const float* gated) {
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const bool whole = col + 8 <= a.out_cols;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    const auto with_bias = [&](const float* from, uint32_t row) {
+        const f32x4 low = *reinterpret_cast<const f32x4*>(from), high = *reinterpret_cast<const f32x4*>(from + 4);
+        f32x8 v = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+        if (a.bias) {
+            const uint64_t at = expert * a.bias_expert;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) v[k] += load_float(a.bias_dtype, a.bias, at + (whole ? row + k : min(row + k, a.wide - 1u)) * a.bias_stride);
+        }
+        return v;
+    };
+    f32x8 v = with_bias(sums, col);
+    if (a.activation != CQ_ACT_IDENTITY) {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) v[k] = activated(a.activation, v[k]);
+    }
+    if (a.gated) {
+        const f32x8 up = with_bias(gated, a.out_cols + col);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) v[k] *= up[k];
+    }
+    const uint64_t y_at = p * a.y_stride + col, r_at = p * a.residual_stride + col;
+    if (whole && a.vector_stores) {  // eight columns lie on a boundary of 16 bytes
+        if (a.y_dtype == CQ_F32) {
+            if (a.residual) v += *reinterpret_cast<const f32x8*>(a.residual + r_at * 4);
+            *reinterpret_cast<f32x8*>(a.y + y_at * 4) = v;
+            return;
+        }
+        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+        typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+        if (a.residual) {
+            const u32x4 r = *reinterpret_cast<const u32x4*>(a.residual + r_at * 2);
+            v += a.y_dtype == CQ_F16 ? __builtin_convertvector(__builtin_bit_cast(f16x8, r), f32x8) : __builtin_convertvector(__builtin_bit_cast(bf16x8, r), f32x8);
+        }
+        *reinterpret_cast<u32x4*>(a.y + y_at * 2) = a.y_dtype == CQ_F16 ? __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8))
+                                                                        : __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
+        return;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++)
+        if (whole || col + k < a.out_cols) {
+            float out = v[k];
+            if (a.residual) out += load_float(a.y_dtype, a.residual, r_at + k);
+            store_float(a.y_dtype, a.y, y_at + k, out);
+        }
 }
 
 }  // namespace

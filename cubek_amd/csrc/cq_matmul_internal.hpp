@@ -30,9 +30,16 @@ struct MatmulArgs {
     uint64_t scale_row, scale_col, scale_expert;  // strides of the scales, in elements
     uint64_t x_stride, y_stride, residual_stride, bias_stride, bias_expert;  // in elements
     uint32_t activation, gated;
+    uint32_t vector_stores;  // eight columns of y and of the residual, from any multiple of eight on, lie on a boundary of 16 bytes
     void* workspace;
     uint64_t workspace_bytes;
 };
+// Tiles that a launch has to hold for any offsets: every expert may end in a tile that is not full.
+inline uint64_t most_tiles(const MatmulArgs& a, uint32_t size_log2) {
+    const uint64_t full = (static_cast<uint64_t>(a.positions) + (1u << size_log2) - 1u) >> size_log2;
+    return a.offsets ? full + (a.experts < a.positions ? a.experts : a.positions) : full;
+}
+
 hipError_t launch_matmul_general(hipStream_t s, const MatmulArgs& a);
 
 struct RouteArgs {
