@@ -81,11 +81,7 @@ __global__ __launch_bounds__(256) void matmul_general_kernel(MatmulArgs a) {
             for (uint32_t j = 0; j < 4; j++) {
                 const uint32_t p = at.first + ty + 16 * i, n = n0 + tx + 16 * j;
                 if (p >= at.last || n >= a.out_cols) continue;
-                const auto bias = [&](uint32_t row) { return a.bias ? load_float(a.bias_dtype, a.bias, e * a.bias_expert + row * a.bias_stride) : 0.0f; };
-                float out = activated(a.activation, v[i][j] + bias(n));
-                if (a.gated) out *= w[i][j] + bias(a.out_cols + n);
-                if (a.residual) out += load_float(a.y_dtype, a.residual, p * a.residual_stride + n);
-                store_float(a.y_dtype, a.y, p * a.y_stride + n, out);
+                finish1(a, e, p, n, v[i][j], w[i][j]);
             }
     }
 }

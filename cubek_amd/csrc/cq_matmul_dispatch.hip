@@ -1,21 +1,27 @@
-// Which object holds the kernels for a product on the matrix cores.
+// Which kernel on the matrix cores a product takes, and which object holds it.
 #include "cq_matmul_tiles.hpp"
 
 namespace cq {
 
+#define CQ_BY_CODE(kernel, f, ...)                                                             \
+    switch (a.native == 1 ? 100u : a.native == 2 ? 101u : a.native == 3 ? 102u : a.bits) {     \
+        case 2: return kernel##_##f##_2(__VA_ARGS__);                                          \
+        case 4: return kernel##_##f##_4(__VA_ARGS__);                                          \
+        case 100: return kernel##_##f##_100(__VA_ARGS__);                                      \
+        case 101: return kernel##_##f##_101(__VA_ARGS__);                                      \
+        case 102: return kernel##_##f##_102(__VA_ARGS__);                                      \
+        default: return kernel##_##f##_8(__VA_ARGS__);                                         \
+    }
+
 hipError_t launch_matmul_tiles(hipStream_t s, const MatmulArgs& a) {
+    FewShape few;
+    if (few_takes(a, &few)) {
+        if (a.dtype == CQ_BF16) CQ_BY_CODE(matmul_few, BF16, s, a, few)
+        CQ_BY_CODE(matmul_few, F16, s, a, few)
+    }
     const TilesShape shape = tiles_shape(a);
-    const bool bf16 = a.dtype == CQ_BF16;
-    switch (a.native) {
-        case 1: return bf16 ? matmul_tiles_BF16_100(s, a, shape) : matmul_tiles_F16_100(s, a, shape);
-        case 2: return bf16 ? matmul_tiles_BF16_101(s, a, shape) : matmul_tiles_F16_101(s, a, shape);
-        case 3: return bf16 ? matmul_tiles_BF16_102(s, a, shape) : matmul_tiles_F16_102(s, a, shape);
-    }
-    switch (a.bits) {
-        case 2: return bf16 ? matmul_tiles_BF16_2(s, a, shape) : matmul_tiles_F16_2(s, a, shape);
-        case 4: return bf16 ? matmul_tiles_BF16_4(s, a, shape) : matmul_tiles_F16_4(s, a, shape);
-        default: return bf16 ? matmul_tiles_BF16_8(s, a, shape) : matmul_tiles_F16_8(s, a, shape);
-    }
+    if (a.dtype == CQ_BF16) CQ_BY_CODE(matmul_tiles, BF16, s, a, shape)
+    CQ_BY_CODE(matmul_tiles, F16, s, a, shape)
 }
 
 }  // namespace cq

@@ -98,6 +98,18 @@ __device__ __forceinline__ uint32_t row_of_position(const MatmulArgs& a, uint32_
     return static_cast<uint32_t>(min(max(a.row_of[p], 0), static_cast<int32_t>(a.tokens) - 1));
 }
 
+// Column col of position p from its sum, and the gated one's.
+__device__ __forceinline__ void finish1(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, float v, float up) {
+    if (a.bias) {
+        v += load_float(a.bias_dtype, a.bias, expert * a.bias_expert + col * a.bias_stride);
+        if (a.gated) up += load_float(a.bias_dtype, a.bias, expert * a.bias_expert + (a.out_cols + col) * a.bias_stride);
+    }
+    v = activated(a.activation, v);
+    if (a.gated) v *= up;
+    if (a.residual) v += load_float(a.y_dtype, a.residual, p * a.residual_stride + col);
+    store_float(a.y_dtype, a.y, p * a.y_stride + col, v);
+}
+
 // Columns col .. col + 7 of position p, as far as y has them, from their sums (and those of the gated ones) in LDS.
 __device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, const float* sums, const float* gated) {
     typedef float f32x8 __attribute__((ext_vector_type(8)));

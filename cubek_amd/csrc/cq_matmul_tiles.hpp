@@ -36,6 +36,34 @@ struct TilesGrid {
     }
 };
 
+// The kernel of a decode step (cq_kernels_matmul_few.hip): positions of a tile, stages that a wave's loads are ahead.
+constexpr uint32_t kFewLog2 = 3, kFewDepth = 2;
+
+struct FewGrid {
+    uint32_t shares_log2, scale_size, scale_col_bytes;
+    cubek_quant::device::FastDivmod units_per_block;
+
+    FewGrid(const MatmulArgs& a, uint32_t unit, uint32_t shares_log2)
+        : shares_log2(shares_log2), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u), scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)),
+          units_per_block(a.block_cols ? a.block_cols / unit : 0x7fffffffu) {}
+};
+
+struct FewShape {
+    uint32_t groups, tokens, shares_log2;  // groups of 16 rows of a wave; most tokens of a tile; shares of a row's columns
+};
+
+// Whether it takes a product that tiles_take() lets through: a unit of 16 bytes of codes has one scale.
+inline bool few_takes(const MatmulArgs& a, FewShape* shape) {
+    const uint32_t unit = 128 / a.bits, stages = (a.cols / unit + 7) / 8;
+    const uint64_t each = a.offsets ? (a.positions + a.experts - 1ull) / a.experts : a.positions;
+    if (each > (a.offsets ? 4u : 8u) || a.block_cols % unit || most_tiles(a, kFewLog2) > 65535) return false;
+    shape->tokens = a.positions < 8 ? a.positions : 8;
+    shape->groups = a.gated ? 2 : 1;
+    if (a.bits == 2 && shape->tokens > 4) return false;  // a stage of x, 512 columns of each token, is more than a wave's part of LDS
+    shape->shares_log2 = stages >= 8 ? 3 : stages >= 4 ? 2 : stages >= 2 ? 1 : 0;
+    return true;
+}
+
 // Whether the kernels on the matrix cores take a product: 16-bit x, rows of whole 16-byte pieces on boundaries of 16 bytes, scales that serve
 // 32 columns at least, and distances within a tile that fit 32 bits.
 inline bool tiles_take(const MatmulArgs& a) {
@@ -60,7 +88,9 @@ inline TilesShape tiles_shape(const MatmulArgs& a) {
 hipError_t launch_matmul_tiles(hipStream_t s, const MatmulArgs& a);
 
 #define CQ_TILES_CODES(X, f) X(f, 2) X(f, 4) X(f, 8) X(f, 100) X(f, 101) X(f, 102)
-#define CQ_TILES_DECLARE(f, c) hipError_t matmul_tiles_##f##_##c(hipStream_t s, const MatmulArgs& a, TilesShape shape);
+#define CQ_TILES_DECLARE(f, c)                                                              \
+    hipError_t matmul_tiles_##f##_##c(hipStream_t s, const MatmulArgs& a, TilesShape shape); \
+    hipError_t matmul_few_##f##_##c(hipStream_t s, const MatmulArgs& a, const FewShape& shape);
 CQ_TILES_CODES(CQ_TILES_DECLARE, BF16)
 CQ_TILES_CODES(CQ_TILES_DECLARE, F16)
 
