@@ -172,6 +172,17 @@ cq_status launch(cq_stream_t stream, cq::MatmulArgs& a) {
     return hip_status(cq::tiles_take(a) ? cq::launch_matmul_tiles(stream, a) : cq::launch_matmul_general(stream, a));
 }
 
+// What the product with these sizes would share its columns by, if it had the room; 0 where it does not share them.
+size_t workspace_for(cq::MatmulArgs& a, cq_dtype dtype, const cq_scheme* scheme, uint64_t cols) {
+    if (a.positions == 0 || a.out_cols == 0 || a.experts == 0 || cols != a.cols || a.positions > kMostExtent) return 0;
+    a.dtype = dtype;
+    if (scheme->level == CQ_LEVEL_BLOCK) a.block_cols = scheme->block[scheme->block_rank - 1], a.block_rows = 1;
+    a.workspace_bytes = ~0ull;
+    if (!cq::tiles_take(a)) return 0;
+    const cq::MatmulChoice c = cq::matmul_choice(a);
+    return c.few ? 0 : cq::sums_bytes(a, c.tiles.splits);
+}
+
 }  // namespace
 
 extern "C" {
@@ -181,7 +192,8 @@ size_t cq_matmul_workspace_bytes(const cq_tensor* values, const cq_scheme* schem
     if (check_scheme(scheme) != CQ_OK || read_weights(values, nullptr, scheme, false, &a) != CQ_OK || !tensor_ok(x) || !valid_dtype(dtype) ||
         read_epilogue(epilogue, nullptr, false, &a) != CQ_OK)
         return 0;
-    return 0;
+    a.positions = a.tokens = static_cast<uint32_t>(x->rank == 1 ? 1 : x->shape[0]);
+    return workspace_for(a, dtype, scheme, x->shape[x->rank - 1]);
 }
 
 cq_status cq_matmul_quantized(cq_stream_t stream, const cq_tensor* values, const cq_tensor* params, const cq_scheme* scheme, const cq_tensor* x,
@@ -205,9 +217,12 @@ cq_status cq_matmul_quantized(cq_stream_t stream, const cq_tensor* values, const
 size_t cq_experts_workspace_bytes(const cq_tensor* values, const cq_scheme* scheme, const cq_tensor* y, cq_dtype dtype, const cq_epilogue* epilogue) {
     cq::MatmulArgs a{};
     if (check_scheme(scheme) != CQ_OK || read_weights(values, nullptr, scheme, true, &a) != CQ_OK || !tensor_ok(y) || !valid_dtype(dtype) ||
-        read_epilogue(epilogue, nullptr, true, &a) != CQ_OK)
+        read_epilogue(epilogue, nullptr, true, &a) != CQ_OK || y->rank != 2)
         return 0;
-    return 0;
+    const int32_t offsets = 0;
+    a.positions = a.tokens = static_cast<uint32_t>(y->shape[0]);
+    a.offsets = &offsets;  // not read: only that there are some
+    return workspace_for(a, dtype, scheme, a.cols);
 }
 
 cq_status cq_experts_quantized(cq_stream_t stream, const cq_tensor* values, const cq_tensor* params, const cq_scheme* scheme, const cq_tensor* x,

@@ -14,14 +14,17 @@ namespace cq {
     }
 
 hipError_t launch_matmul_tiles(hipStream_t s, const MatmulArgs& a) {
-    FewShape few;
-    if (few_takes(a, &few)) {
-        if (a.dtype == CQ_BF16) CQ_BY_CODE(matmul_few, BF16, s, a, few)
-        CQ_BY_CODE(matmul_few, F16, s, a, few)
+    const MatmulChoice choice = matmul_choice(a);
+    if (choice.few) {
+        if (a.dtype == CQ_BF16) CQ_BY_CODE(matmul_few, BF16, s, a, choice.few_shape)
+        CQ_BY_CODE(matmul_few, F16, s, a, choice.few_shape)
     }
-    const TilesShape shape = tiles_shape(a);
-    if (a.dtype == CQ_BF16) CQ_BY_CODE(matmul_tiles, BF16, s, a, shape)
-    CQ_BY_CODE(matmul_tiles, F16, s, a, shape)
+    const auto product = [&]() -> hipError_t {
+        if (a.dtype == CQ_BF16) CQ_BY_CODE(matmul_tiles, BF16, s, a, choice.tiles)
+        CQ_BY_CODE(matmul_tiles, F16, s, a, choice.tiles)
+    };
+    const hipError_t err = product();
+    return err != hipSuccess || choice.tiles.splits == 1 ? err : launch_matmul_finish(s, a, choice.tiles.splits);
 }
 
 }  // namespace cq

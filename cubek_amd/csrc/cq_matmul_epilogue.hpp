@@ -110,29 +110,33 @@ __device__ __forceinline__ void finish1(const MatmulArgs& a, uint32_t expert, ui
     store_float(a.y_dtype, a.y, p * a.y_stride + col, v);
 }
 
-// Columns col .. col + 7 of position p, as far as y has them, from their sums (and those of the gated ones) in LDS.
-__device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, const float* sums, const float* gated) {
-    typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// Eight floats from a boundary of 16 bytes.
+__device__ __forceinline__ f32x8 load8(const float* p) {
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    const f32x4 low = *reinterpret_cast<const f32x4*>(p), high = *reinterpret_cast<const f32x4*>(p + 4);
+    return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Columns col .. col + 7 of position p, as far as y has them, from their sums and those of the gated ones.
+__device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, f32x8 v, f32x8 up) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const bool whole = col + 8 <= a.out_cols;
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-    const auto with_bias = [&](const float* from, uint32_t row) {
-        const f32x4 low = *reinterpret_cast<const f32x4*>(from), high = *reinterpret_cast<const f32x4*>(from + 4);
-        f32x8 v = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
-        if (a.bias) {
+    if (a.bias) {
+        const auto add_bias = [&](f32x8& to, uint32_t row) {
             const uint64_t at = expert * a.bias_expert;
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) v[k] += load_float(a.bias_dtype, a.bias, at + (whole ? row + k : min(row + k, a.wide - 1u)) * a.bias_stride);
-        }
-        return v;
-    };
-    f32x8 v = with_bias(sums, col);
+            for (uint32_t k = 0; k < 8; k++) to[k] += load_float(a.bias_dtype, a.bias, at + (whole ? row + k : min(row + k, a.wide - 1u)) * a.bias_stride);
+        };
+        add_bias(v, col);
+        if (a.gated) add_bias(up, a.out_cols + col);
+    }
     if (a.activation != CQ_ACT_IDENTITY) {
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) v[k] = activated(a.activation, v[k]);
     }
     if (a.gated) {
-        const f32x8 up = with_bias(gated, a.out_cols + col);
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) v[k] *= up[k];
     }

@@ -6,21 +6,43 @@
 
 namespace cq {
 
-enum class TilesShape { k256x256, k256x128, k256x64, k256x32 };  // rows of W x positions
+enum class TilesShape { k256x128, k128x64, k128x32, k32x32 };  // rows of W x positions
+struct TilesChoice {
+    TilesShape shape;
+    uint32_t splits;  // workgroups that share the columns of a tile
+};
+
+// kNT, kTT: tiles of 32 rows and of 32 positions of a wave; kWN, kWT, kWK: waves along rows, positions and columns; kLine: bytes of a row in a
+// chunk of codes.
+template <int kNT, int kTT, int kWN, int kWT, int kWK, int kLine>
+struct TilesTraits {
+    static constexpr uint32_t kRows = 32 * kNT * kWN, kTokens = 32 * kTT * kWT;
+    static constexpr uint32_t kXBytes = kTokens * 128, kCodeBytes = kRows * kLine;  // a step of x; a chunk of codes
+    static constexpr uint32_t kPitch = 32 * kNT + 4;                              // of the sums on their way to y
+    static constexpr uint32_t kImages = kWK * 2 * (kXBytes + kCodeBytes), kParts = kWN * kWT * kWK * 32 * kPitch * 4;
+    static constexpr uint32_t kLds = kImages > kParts ? kImages : kParts;
+    static_assert(kLds <= 160 * 1024, "a compute unit's LDS");
+    static constexpr uint32_t kWaves = kWN * kWT * kWK, kFit = 160 * 1024 / kLds;
+    static constexpr uint32_t kMost = kNT * kTT >= 8 ? 2 : 4;  // waves of a SIMD that the registers of the sums leave room for
+    static constexpr uint32_t kWavesPerSimd = kWaves / 4 * kFit < kMost ? kWaves / 4 * kFit : kMost;
+};
 
 struct TilesGrid {
-    uint32_t n_tiles, p_tiles;
+    uint32_t n_tiles, p_tiles, splits, pitch;  // pitch: floats of a position's sums in the workspace
     uint32_t scale_size, scale_col_bytes;
     cubek_quant::device::FastDivmod halves_per_block, by_group;  // by 32 columns; by kGroup * n_tiles
 
     static constexpr uint32_t kUnits = 8, kGroup = 4;  // dies with an L2 each; tiles of positions that share one die's weights
 
-    TilesGrid(const MatmulArgs& a, uint32_t n_tiles, uint64_t p_tiles)
-        : n_tiles(n_tiles), p_tiles(static_cast<uint32_t>(p_tiles)), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u),
-          scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)), halves_per_block(a.block_cols ? a.block_cols / 32u : 0x7fffffffu),
-          by_group(kGroup * n_tiles) {}
+    TilesGrid(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t splits)
+        : n_tiles((a.out_cols + (a.gated ? rows / 2 : rows) - 1) / (a.gated ? rows / 2 : rows)), p_tiles(static_cast<uint32_t>(most_tiles(a, __builtin_ctz(tokens)))),
+          splits(splits), pitch(sums_pitch(a)), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u), scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)),
+          halves_per_block(a.block_cols ? a.block_cols / 32u : 0x7fffffffu), by_group(kGroup * n_tiles) {}
 
     uint32_t workgroups() const { return n_tiles * p_tiles; }
+
+    // Floats of a position's sums: whole eights of columns, gated two of them.
+    static uint32_t sums_pitch(const MatmulArgs& a) { return (a.out_cols + 7u) / 8u * 8u * (a.gated ? 2u : 1u); }
 
     // Workgroups go round the dies one by one.  Each die gets a run of tiles of its own, in groups of kGroup tiles of positions by all tiles of
     // rows, positions first: what its workgroups read at a time are few rows of x and few of W.
@@ -36,33 +58,32 @@ struct TilesGrid {
     }
 };
 
-// The kernel of a decode step (cq_kernels_matmul_few.hip): positions of a tile, stages that a wave's loads are ahead.
-constexpr uint32_t kFewLog2 = 3, kFewDepth = 2;
-
-struct FewGrid {
-    uint32_t shares_log2, scale_size, scale_col_bytes;
-    cubek_quant::device::FastDivmod units_per_block;
-
-    FewGrid(const MatmulArgs& a, uint32_t unit, uint32_t shares_log2)
-        : shares_log2(shares_log2), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u), scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)),
-          units_per_block(a.block_cols ? a.block_cols / unit : 0x7fffffffu) {}
-};
+// The kernel of a decode step (cq_kernels_matmul_few.hip): stages that a wave's loads are ahead.
+constexpr uint32_t kFewAhead = 1;
 
 struct FewShape {
-    uint32_t groups, tokens, shares_log2;  // groups of 16 rows of a wave; most tokens of a tile; shares of a row's columns
+    uint32_t groups, tokens_log2, shares_log2;  // groups of 16 rows of a wave; positions of a tile; shares of a row's columns
+    uint32_t x_bytes;                           // of a stage: whole loads of 1 KiB
+
+    uint32_t x_loads() const { return (x_bytes / 1024 + (8 >> shares_log2) - 1) / (8 >> shares_log2); }  // of a wave
+    uint32_t lds() const {
+        const uint32_t images = (kFewAhead + 1) * ((x_bytes << shares_log2) + 8 * groups * 2560), sums = 8 * groups * (tokens_log2 == 5 ? 2048 : 1024);
+        return images > sums ? images : sums;
+    }
 };
 
-// Whether it takes a product that tiles_take() lets through: a unit of 16 bytes of codes has one scale.
-inline bool few_takes(const MatmulArgs& a, FewShape* shape) {
-    const uint32_t unit = 128 / a.bits, stages = (a.cols / unit + 7) / 8;
-    const uint64_t each = a.offsets ? (a.positions + a.experts - 1ull) / a.experts : a.positions;
-    if (each > (a.offsets ? 4u : 8u) || a.block_cols % unit || most_tiles(a, kFewLog2) > 65535) return false;
-    shape->tokens = a.positions < 8 ? a.positions : 8;
-    shape->groups = a.gated ? 2 : 1;
-    if (a.bits == 2 && shape->tokens > 4) return false;  // a stage of x, 512 columns of each token, is more than a wave's part of LDS
-    shape->shares_log2 = stages >= 8 ? 3 : stages >= 4 ? 2 : stages >= 2 ? 1 : 0;
-    return true;
-}
+struct FewGrid {
+    uint32_t shares_log2, tokens_log2, x_bytes, scale_size, scale_col_bytes, block_magic;
+
+    FewGrid(const MatmulArgs& a, const FewShape& c)
+        : shares_log2(c.shares_log2), tokens_log2(c.tokens_log2), x_bytes(c.x_bytes), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u),
+          scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)) {
+        const uint32_t each = a.block_cols * a.bits / 128;  // units of 16 bytes of codes under a scale
+        block_magic = each ? (0x80000000u + each - 1) / each : 0u;
+    }
+    // unit / each, for less than 2^27 units and each < 32: 2 unit ceil(2^31 / each) / 2^32
+    __device__ uint32_t block_of(uint32_t unit) const { return __umulhi(2u * unit, block_magic); }
+};
 
 // Whether the kernels on the matrix cores take a product: 16-bit x, rows of whole 16-byte pieces on boundaries of 16 bytes, scales that serve
 // 32 columns at least, and distances within a tile that fit 32 bits.
@@ -80,16 +101,96 @@ inline bool tiles_take(const MatmulArgs& a) {
     return (a.out_cols / 16ull + 1) * most_tiles(a, 5) < (1ull << 22);  // workgroups of a launch
 }
 
-inline TilesShape tiles_shape(const MatmulArgs& a) {
-    const uint64_t each = a.positions / (a.offsets ? a.experts : 1u);
-    return each >= 192 ? TilesShape::k256x256 : each >= 96 ? TilesShape::k256x128 : each >= 48 ? TilesShape::k256x64 : TilesShape::k256x32;
+inline uint64_t sums_bytes(const MatmulArgs& a, uint32_t splits) { return splits > 1 ? 4ull * splits * a.positions * TilesGrid::sums_pitch(a) : 0; }
+
+// Which kernel a product takes, by what it would take.  Times in microseconds, fitted to sweeps over shapes, splits and 1 to 2048 positions
+// (blocks of 32, bf16; f16 and the other codes of a width alike): a launch is its rounds of steps, and a round costs little less when half
+// of a compute unit's workgroups are there.  Measured against the model: [28672, 8192] 4 bits, tiles of 256 x 128, 2048 positions 833 us for 850,
+// 1024 450 for 468, 128 in four parts 91 for 88; [4096, 4096] 512 positions, 256 x 128 in four parts 39.3 for 38.8, 128 x 64 in two 37.6 for 40.2;
+// 128 positions, 128 x 64 in four parts 21.7 for 20.0, 32 x 32 23.7 for 22.4; a decode step of 16 on [28672, 8192] 36.3 for 36.
+struct MatmulChoice {
+    bool few = false;
+    FewShape few_shape{};
+    TilesChoice tiles{TilesShape::k256x128, 1};
+    double us = 1e30;
+};
+
+constexpr double kStartUs = 4.0;  // a launch without a step
+
+// Workgroups that a launch may be taken to have: the experts' sizes lie in device memory, and as many end in half a tile as in a whole one.
+inline double likely_tiles(const MatmulArgs& a, uint32_t size) {
+    if (!a.offsets) return static_cast<double>((a.positions + static_cast<uint64_t>(size) - 1) / size);
+    const double experts = a.experts < a.positions ? a.experts : a.positions, each = a.positions / experts;
+    return experts * (each > 0.5 * size ? each / size + 0.5 : 1.0);
 }
 
+// What `workgroups` take for a round of steps that takes `half` with one workgroup on a compute unit and `full` with two.
+inline double rounds_us(double workgroups, double half, double full) {
+    const double whole = static_cast<double>(static_cast<uint64_t>(workgroups / 512.0)), rest = workgroups - 512.0 * whole;
+    return whole * full + (rest <= 0.0 ? 0.0 : rest <= 256.0 ? half : full);
+}
+
+inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows, uint32_t tokens, uint32_t along, uint32_t line, double half, double full, MatmulChoice* best) {
+    const uint32_t columns = a.gated ? rows / 2 : rows, steps = line / 8 / a.bits, chunks = ((a.cols + 63) / 64 + steps - 1) / steps;
+    const double tiles = (a.out_cols + columns - 1) / columns * likely_tiles(a, tokens);
+    for (uint32_t splits = 1; splits <= 16; splits *= 2) {
+        if (splits > 1 && (splits * along > chunks || sums_bytes(a, splits) > a.workspace_bytes)) break;
+        const double rounds = static_cast<double>((chunks + splits * along - 1) / (splits * along) * steps);
+        const double sums = splits > 1 ? 3.0 + 2.0 * static_cast<double>(sums_bytes(a, splits)) / 5e6 : 0.0;  // written and read at 5 TB/s
+        const double us = kStartUs + rounds * rounds_us(tiles * splits, half, full) + sums;
+        if (us < best->us) {
+            best->few = false;
+            best->tiles = TilesChoice{shape, splits};
+            best->us = us;
+        }
+    }
+}
+
+// The kernel of a decode step, where a unit of 16 bytes of codes has one scale: as many shares of the columns as leave all workgroups
+// running at once.
+inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
+    const uint32_t unit = 128 / a.bits, stages = (a.cols / unit + 7) / 8;
+    if (a.block_cols % unit) return;
+    for (uint32_t tokens_log2 = 3; tokens_log2 <= 5; tokens_log2++) {
+        FewShape c{};
+        const uint32_t most = 1u << tokens_log2, tokens = a.positions < most ? a.positions : most;
+        if (a.offsets == nullptr && a.positions > most) continue;  // the weights would be read again for every tile
+        c.tokens_log2 = tokens_log2;
+        c.x_bytes = (tokens * (2048 / a.bits) + 1023) / 1024 * 1024;
+        c.groups = a.gated ? 2 : 1;
+        const double waves = (a.out_cols + 15) / 16 * likely_tiles(a, most);
+        for (c.shares_log2 = 3; c.shares_log2 > 0; c.shares_log2--) {
+            const uint32_t fit = c.lds() ? 160 * 1024 / c.lds() : 2;
+            if ((1u << c.shares_log2) <= stages && c.x_loads() <= 8 && waves * (1u << c.shares_log2) / 8 <= 256.0 * (fit < 2 ? fit : 2)) break;
+        }
+        if (c.lds() > 160 * 1024 || c.x_loads() > 8 || most_tiles(a, tokens_log2) > 65535) continue;
+        const double half = (0.45 + unit * 8 * (0.0025 + (tokens_log2 == 5 ? 0.0022 : 0.0)) + (tokens_log2 == 4 ? 0.15 : 0.0)) * (c.groups == 2 ? 1.7 : 1.0);
+        const double rounds = static_cast<double>((stages + (1u << c.shares_log2) - 1) >> c.shares_log2);
+        const double us = 3.0 + rounds * rounds_us(waves * (1u << c.shares_log2) / 8, half, 1.85 * half);
+        if (us < best->us) {
+            best->few = true;
+            best->few_shape = c;
+            best->us = us;
+        }
+    }
+}
+
+inline MatmulChoice matmul_choice(const MatmulArgs& a) {
+    MatmulChoice c;
+    consider_few(a, &c);
+    consider_tiles(a, TilesShape::k256x128, 256, 128, 1, 64, 1.15, 1.83, &c);
+    consider_tiles(a, TilesShape::k128x64, 128, 64, 2, 64, 1.2, 1.65, &c);
+    consider_tiles(a, TilesShape::k128x32, 128, 32, 2, 64, 1.13, 1.8, &c);
+    consider_tiles(a, TilesShape::k32x32, 32, 32, 8, 128, 1.15, 2.3, &c);
+    return c;
+}
+
+hipError_t launch_matmul_finish(hipStream_t s, const MatmulArgs& a, uint32_t splits);
 hipError_t launch_matmul_tiles(hipStream_t s, const MatmulArgs& a);
 
 #define CQ_TILES_CODES(X, f) X(f, 2) X(f, 4) X(f, 8) X(f, 100) X(f, 101) X(f, 102)
 #define CQ_TILES_DECLARE(f, c)                                                              \
-    hipError_t matmul_tiles_##f##_##c(hipStream_t s, const MatmulArgs& a, TilesShape shape); \
+    hipError_t matmul_tiles_##f##_##c(hipStream_t s, const MatmulArgs& a, const TilesChoice& choice); \
     hipError_t matmul_few_##f##_##c(hipStream_t s, const MatmulArgs& a, const FewShape& shape);
 CQ_TILES_CODES(CQ_TILES_DECLARE, BF16)
 CQ_TILES_CODES(CQ_TILES_DECLARE, F16)
