@@ -119,6 +119,21 @@ __device__ __forceinline__ f32x8 load8(const float* p) {
     return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Eight columns to a boundary of 16 bytes, rounded once.
+__device__ __forceinline__ void store8(int dtype, char* y, uint64_t at, f32x8 v) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    if (dtype == CQ_F32) {
+        *reinterpret_cast<f32x4*>(y + at * 4) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(y + at * 4 + 16) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+        *reinterpret_cast<u32x4*>(y + at * 2) = dtype == CQ_F16 ? __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8))
+                                                                : __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
+    }
+}
+
 // Columns col .. col + 7 of position p, as far as y has them, from their sums and those of the gated ones.
 __device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, f32x8 v, f32x8 up) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -142,19 +157,15 @@ __device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, ui
     }
     const uint64_t y_at = p * a.y_stride + col, r_at = p * a.residual_stride + col;
     if (whole && a.vector_stores) {  // eight columns lie on a boundary of 16 bytes
-        if (a.y_dtype == CQ_F32) {
-            if (a.residual) v += *reinterpret_cast<const f32x8*>(a.residual + r_at * 4);
-            *reinterpret_cast<f32x8*>(a.y + y_at * 4) = v;
-            return;
-        }
-        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-        typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-        if (a.residual) {
+        if (a.residual && a.y_dtype == CQ_F32) {
+            v += load8(reinterpret_cast<const float*>(a.residual) + r_at);
+        } else if (a.residual) {
+            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+            typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
             const u32x4 r = *reinterpret_cast<const u32x4*>(a.residual + r_at * 2);
             v += a.y_dtype == CQ_F16 ? __builtin_convertvector(__builtin_bit_cast(f16x8, r), f32x8) : __builtin_convertvector(__builtin_bit_cast(bf16x8, r), f32x8);
         }
-        *reinterpret_cast<u32x4*>(a.y + y_at * 2) = a.y_dtype == CQ_F16 ? __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8))
-                                                                        : __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
+        store8(a.y_dtype, a.y, y_at, v);
         return;
     }
 #pragma unroll

@@ -50,6 +50,7 @@ struct RouteArgs {
     int32_t *experts, *offsets, *rows, *slots;
     uint32_t tokens, num_experts, chosen;
     uint32_t sigmoid, normalize;
+    uint32_t vector_logits;  // a lane's logits are contiguous and on a boundary of their own size, up to 16 bytes
     void* workspace;
 };
 uint64_t route_workspace_bytes(uint64_t tokens, uint64_t experts, uint64_t chosen);

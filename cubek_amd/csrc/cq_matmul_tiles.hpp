@@ -138,7 +138,7 @@ inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows,
         const double rounds = static_cast<double>((chunks + splits * along - 1) / (splits * along) * steps);
         const double sums = splits > 1 ? 3.0 + 2.0 * static_cast<double>(sums_bytes(a, splits)) / 5e6 : 0.0;  // written and read at 5 TB/s
         const double us = kStartUs + rounds * rounds_us(tiles * splits, half, full) + sums;
-        if (us < best->us) {
+        if (us < best->us * (splits > 1 ? 0.92 : 1.0)) {  // (workgroups of many rounds do not wait for one another)
             best->few = false;
             best->tiles = TilesChoice{shape, splits};
             best->us = us;
