@@ -36,16 +36,16 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
 // kNT, kTT: tiles of 32 rows and 32 positions of a wave; kWN, kWT, kWK: waves along rows, positions and columns.  Waves along the columns
 // take a run of chunks each, with images of their own; their sums meet in LDS at the end.  Several workgroups may share the columns too: then they
 // leave their sums in the workspace, and matmul_finish_kernel adds them up.
-template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWT, int kWK, int kLine>
-__global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine>::kWavesPerSimd)) void matmul_tiles_kernel(MatmulArgs a, TilesGrid grid) {
-    using Traits = TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine>;
+template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWT, int kWK, int kLine, int kXRing, int kCodeRing>
+__global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>::kWavesPerSimd)) void matmul_tiles_kernel(MatmulArgs a, TilesGrid grid) {
+    using Traits = TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>;
     constexpr uint32_t kWaves = kWN * kWT, kRows = Traits::kRows, kTokens = Traits::kTokens, kTokensLog2 = __builtin_ctz(kTokens);
     constexpr uint32_t kBits = bits_of(kCode), kSteps = kLine / 8 / kBits;  // steps of a chunk: 128 bytes of codes are 1024 / kBits columns
     constexpr uint32_t kUnits = kLine / 16, kTurn = 256 / kLine;            // 16-byte pieces of a line; rows side by side in the 256 bytes of all banks
     static_assert(kSteps >= 1, "whole steps");
     constexpr uint32_t kXBytes = Traits::kXBytes, kCodeBytes = Traits::kCodeBytes;
-    constexpr uint32_t kXLoads = kTokens / 8 / kWaves, kCodeLoads = kCodeBytes / 1024 / kWaves;
-    static_assert(kXLoads * 8 * kWaves == kTokens && kCodeLoads * 1024 * kWaves == kCodeBytes, "whole loads of 1 KiB");
+    constexpr uint32_t kXLoads = kTokens / 8 / kWaves, kCodeLoads = kCodeBytes / 1024 / kWaves, kScaleLoads = kRows * 2 / 64 / kWaves;
+    static_assert(kXLoads * 8 * kWaves == kTokens && kCodeLoads * 1024 * kWaves == kCodeBytes && kScaleLoads * 32 * kWaves == kRows, "whole loads of 1 KiB");
     extern __shared__ char lds[];
 
     uint32_t n_tile, p_tile;
@@ -58,8 +58,9 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     const uint32_t positions = at.last - at.first;
     const uint32_t out0 = n_tile * (a.gated ? kRows / 2 : kRows);  // the workgroup's first column of y
     const uint32_t last_unit = a.cols / (128u / kBits) - 1u;
-    char* const x_img = lds + wave_k * (2 * kXBytes + 2 * kCodeBytes);
-    char* const code_img = x_img + 2 * kXBytes;
+    char* const x_img = lds + wave_k * Traits::kImage;
+    char* const code_img = x_img + kXRing * kXBytes;
+    char* const scale_img = code_img + kCodeRing * kCodeBytes;
 
     // this wave's run of chunks, and the steps that the workgroup's longest one has
     const uint32_t all_steps = (a.cols + 63u) / 64u, chunks = (all_steps + kSteps - 1u) / kSteps;
@@ -89,49 +90,60 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
 #pragma unroll
     for (uint32_t q = 0; q < kXLoads; q++) {
         const uint32_t t = (q * kWaves + wave) * 8u + lane / 8u;
-        x_from[q] = (row_of_position(a, min(at.first + t, at.last - 1u)) - x_row0) * static_cast<uint32_t>(a.x_stride * 2u);
         x_piece[q] = (lane & 7u) ^ ((t >> 1) & 7u);
+        x_from[q] = (row_of_position(a, min(at.first + t, at.last - 1u)) - x_row0) * static_cast<uint32_t>(a.x_stride * 2u) + x_piece[q] * 16u;
     }
     // (scales start on multiples of 4 bytes from an address that is one)
     const uint32_t scale_row0 = a.block_rows ? row0 / a.block_rows : 0u;
     const uint64_t scale_at = (at.expert * a.scale_expert + scale_row0 * a.scale_row) * grid.scale_size + (reinterpret_cast<uintptr_t>(a.scales) & 3u);
     const char* const scales = a.scales - (reinterpret_cast<uintptr_t>(a.scales) & 3u) + (scale_at & ~3ull);
-    uint32_t scale_from[kNT];
+    // a step's scales lie [row][half of its columns], a word around each
+    const auto scale_row = [&](uint32_t r) {
+        return static_cast<uint32_t>(scale_at & 3u) +
+               (a.block_rows ? (weight_row(r) / a.block_rows - scale_row0) * static_cast<uint32_t>(a.scale_row * grid.scale_size) : 0u);
+    };
+    uint32_t scale_from[kScaleLoads], scale_own[kNT];
 #pragma unroll
-    for (uint32_t n = 0; n < kNT; n++)
-        scale_from[n] = static_cast<uint32_t>(scale_at & 3u) +
-                        (a.block_rows ? (weight_row((wave_n * kNT + n) * 32u + i) / a.block_rows - scale_row0) * static_cast<uint32_t>(a.scale_row * grid.scale_size) : 0u);
+    for (uint32_t q = 0; q < kScaleLoads; q++) scale_from[q] = scale_row((q * kWaves + wave) * 32u + lane / 2u);
+#pragma unroll
+    for (uint32_t n = 0; n < kNT; n++) scale_own[n] = scale_row((wave_n * kNT + n) * 32u + i);
+    const auto scale_block = [&](uint32_t step, uint32_t half) { return grid.block_of(min(step * 2u + half, a.cols / 32u - 1u)) * grid.scale_col_bytes; };
 
     const auto load_x = [&](uint32_t step, uint32_t into) {
         const char* const from = x + step * 128ull;
         const uint32_t pieces = a.cols / 8u - step * 8u;
+        const auto load = [&](auto all) {
 #pragma unroll
-        for (uint32_t q = 0; q < kXLoads; q++) {
-            // positions that the tile does not have leave what was there: they have columns of their own in every product
-            if (kTokens <= 64 && (q * kWaves + wave) * 8u >= positions) continue;
-            const char* p = from + (x_from[q] + x_piece[q] * 16u);
-            if (pieces < 8u && x_piece[q] >= pieces) p = kZeros;  // columns past the row's end
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(p), CQ_LDS_PTR(x_img + into * kXBytes + (q * kWaves + wave) * 1024u), 16, 0, 0);
-        }
+            for (uint32_t q = 0; q < kXLoads; q++) {
+                // positions that the tile does not have leave what was there: they have columns of their own in every product
+                if (kTokens <= 64 && (q * kWaves + wave) * 8u >= positions) continue;
+                const char* p = from + x_from[q];
+                if (!decltype(all)::value && x_piece[q] >= pieces) p = kZeros;  // columns past the row's end
+                __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(p), CQ_LDS_PTR(x_img + into * kXBytes + (q * kWaves + wave) * 1024u), 16, 0, 0);
+            }
+        };
+        if (pieces >= 8u)
+            load(std::true_type{});
+        else
+            load(std::false_type{});
     };
-    const auto load_codes = [&](uint32_t chunk) {
+    const auto load_codes = [&](uint32_t chunk, uint32_t into) {
 #pragma unroll
         for (uint32_t q = 0; q < kCodeLoads; q++)
             __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(words + (code_from[q] + min(chunk * kUnits + code_unit[q], last_unit) * 16u)),
-                                             CQ_LDS_PTR(code_img + (chunk & 1u) * kCodeBytes + (q * kWaves + wave) * 1024u), 16, 0, 0);
+                                             CQ_LDS_PTR(code_img + into * kCodeBytes + (q * kWaves + wave) * 1024u), 16, 0, 0);
     };
-    uint32_t scale_words[kNT], scale_offsets[kNT];
-    const auto load_scales = [&](uint32_t step) {
-        const uint32_t block = grid.halves_per_block.div(min(step * 2u + h, a.cols / 32u - 1u));
+    const auto load_scales = [&](uint32_t step, uint32_t into) {
+        const uint32_t block = scale_block(step, lane & 1u);
 #pragma unroll
-        for (uint32_t n = 0; n < kNT; n++) {
-            scale_offsets[n] = scale_from[n] + block * grid.scale_col_bytes;
-            scale_words[n] = scale_word(scales, scale_offsets[n]);
-        }
+        for (uint32_t q = 0; q < kScaleLoads; q++)
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(scales + ((scale_from[q] + block) & ~3u)),
+                                             CQ_LDS_PTR(scale_img + into * Traits::kScaleBytes + (q * kWaves + wave) * 256u), 4, 0, 0);
     };
-    const auto read_codes = [&](uint32_t step, uint32_t n) {
-        const uint32_t r = (wave_n * kNT + n) * 32u + i, chunk = step / kSteps, s = step % kSteps;
-        const char* const line = code_img + (chunk & 1u) * kCodeBytes + r * kLine;
+    // `in`: a step of the wave's run, from 0 on
+    const auto read_codes = [&](uint32_t in, uint32_t n) {
+        const uint32_t r = (wave_n * kNT + n) * 32u + i, s = in % kSteps;
+        const char* const line = code_img + in / kSteps % kCodeRing * kCodeBytes + r * kLine;
         const uint32_t turn = r / kTurn % kUnits;
         Codes<kCode> c;
         if constexpr (kBits == 2) {
@@ -154,12 +166,14 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     Codes<kCode> codes[kNT];
     float rounded_scale[kNT];
     bool all_short = true;
-    const auto fetch = [&](uint32_t step) {  // codes and scales of a step, to be dequantized
+    const auto fetch = [&](uint32_t in) {  // codes and scales of a step, to be dequantized
         bool mine = true;
+        const uint32_t block = scale_block(first_step + in, h);
 #pragma unroll
         for (uint32_t n = 0; n < kNT; n++) {
-            codes[n] = read_codes(step, n);
-            rounded_scale[n] = dev::round_to<kF>(scale_of(a.param_dtype, scale_words[n], scale_offsets[n]));
+            codes[n] = read_codes(in, n);
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(scale_img + in % Traits::kScaleRing * Traits::kScaleBytes + ((wave_n * kNT + n) * 32u + i) * 8u + h * 4u);
+            rounded_scale[n] = dev::round_to<kF>(scale_of(a.param_dtype, word, scale_own[n] + block));
             mine = mine && takes_short<kF, kCode>(rounded_scale[n]);
         }
         all_short = kCode > 8 || __builtin_amdgcn_ballot_w64(!mine) == 0;
@@ -185,46 +199,72 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
             xv[t] = *reinterpret_cast<const u32x4*>(x_img + from * kXBytes + row * 128u + ((h * 4u + m) ^ ((row >> 1) & 7u)) * 16u);
         }
     };
-    // x of a step, codes and scales of the next one are there, and everybody has left the step before, whose places the next loads take
-    const auto arrive = [] {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // What is asked for in an iteration: scales three steps ahead, x kXAhead steps ahead, and in the last step of a chunk the chunk that comes
+    // kCodeRing - 1 behind the next one's; all into places whose last reader was done an iteration before.
+    constexpr uint32_t kXAhead = kXRing - 1, kCodeLead = (kCodeRing - 1) * kSteps;  // iterations until a chunk is read
+    const auto begin = [](auto outstanding) {
+        // everybody's loads up to those that may still be on their way are there, and everybody has left the iteration before
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(outstanding)::value) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    bool codes_after_x = false;  // a chunk's loads were issued behind the x that an iteration waits for, and are not wanted yet
+    const auto issue = [&](uint32_t in) {
+        if (in + 3 < steps) load_scales(first_step + in + 3, (in + 3) % Traits::kScaleRing);
+        if (in + kXAhead < steps) load_x(first_step + in + kXAhead, (in + kXAhead) % kXRing);
+        const uint32_t chunk = (in + 1) / kSteps - 1 + kCodeRing;
+        codes_after_x = (in + 1) % kSteps == 0 && chunk * kSteps < steps;
+        if (codes_after_x) load_codes(first_chunk + chunk, chunk % kCodeRing);
+    };
+    constexpr uint32_t kPerMfma = 5;
     u32x4 xv[2][kTT];
+#pragma unroll
+    for (uint32_t k = 0; k < kCodeRing; k++)
+        if (k * kSteps < steps) load_codes(first_chunk + k, k);
+#pragma unroll
+    for (uint32_t k = 0; k < 3; k++)
+        if (k < steps) load_scales(first_step + k, k);
+#pragma unroll
+    for (uint32_t k = 0; k < kXAhead; k++)
+        if (k < steps) load_x(first_step + k, k);
+    begin(std::integral_constant<int, 0>{});
     if (kWK == 1 || steps != 0) {
-        load_codes(first_chunk);
-        load_x(first_step, 0);
-        load_scales(first_step);
-        if (kSteps < steps) load_codes(first_chunk + 1u);
-    }
-    arrive();
-    if (kWK == 1 || steps != 0) {
-        fetch(first_step);
+        fetch(0);
         dequantize_any(first_step);
-        load_scales(first_step + min(1u, steps - 1u));
     }
 #pragma unroll 1
-    for (uint32_t n_step = 0; n_step < rounds; n_step++) {
-        arrive();
-        if (kWK > 1 && n_step >= steps) continue;  // waves along the columns may have a chunk less than others
-        const uint32_t from = n_step & 1u, next = first_step + min(n_step + 1u, steps - 1u);
-        read_x(from, 0, xv[0]);
+    for (uint32_t in = 0; in < rounds; in++) {
+        static_assert(kXAhead == 1, "the x of an iteration is what the one before asked for");
+        if (kCodeLead >= 2 && codes_after_x)
+            begin(std::integral_constant<int, kCodeLoads>{});
+        else
+            begin(std::integral_constant<int, 0>{});
+        codes_after_x = false;
+        if (kWK > 1 && in >= steps) continue;  // waves along the columns may have a chunk less than others
+        const uint32_t next = min(in + 1u, steps - 1u);
+        read_x(in % kXRing, 0, xv[0]);
         fetch(next);
-        if (n_step + 1 < steps) load_x(next, from ^ 1u);
-        if ((n_step + 1) % kSteps == 0 && n_step + 1 + kSteps < steps) load_codes(first_chunk + (n_step + 1) / kSteps + 1);
-        load_scales(first_step + min(n_step + 2u, steps - 1u));
+        issue(in);
         // the next step's weights take the places of this one's as they are used up
 #pragma unroll
         for (uint32_t m = 0; m < 4; m++) {
-            if (m < 3) read_x(from, m + 1, xv[(m + 1) & 1]);
+            if (m < 3) read_x(in % kXRing, m + 1, xv[(m + 1) & 1]);
 #pragma unroll
             for (uint32_t t = 0; t < kTT; t++)
 #pragma unroll
                 for (uint32_t n = 0; n < kNT; n++) acc[n][t] = mfma<kF>(w[n][m], xv[m & 1][t], acc[n][t]);
             dequantize(m);
         }
-        if (!all_short || (next + 1) * 64u > a.cols) dequantize_any(next);
+        if constexpr (kTT >= 4) {
+            // a matrix instruction keeps its unit busy for 32 cycles, in which the wave may issue seven others
+#pragma unroll
+            for (uint32_t k = 0; k < 4 * kNT * kTT; k++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, kPerMfma, 0);
+                if (k % (kNT * kTT) < kTT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
+        if (!all_short || (first_step + next + 1) * 64u > a.cols) dequantize_any(first_step + next);
     }
 
     // Lane (i, h) holds position i of each 32, rows 8 q + 4 h + 0 .. 3 of each 32.  They go through the wave's own part of LDS, 32 positions at a
@@ -279,21 +319,21 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     }
 }
 
-template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWT, int kWK, int kLine>
+template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWT, int kWK, int kLine, int kXRing, int kCodeRing>
 hipError_t launch_tile(hipStream_t s, const MatmulArgs& a, uint32_t splits) {
-    using Traits = TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine>;
+    using Traits = TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>;
     const TilesGrid grid(a, Traits::kRows, Traits::kTokens, splits);
-    hipLaunchKernelGGL((matmul_tiles_kernel<kF, kCode, kNT, kTT, kWN, kWT, kWK, kLine>), dim3(grid.workgroups(), splits), dim3(64 * kWN * kWT * kWK), Traits::kLds, s, a, grid);
+    hipLaunchKernelGGL((matmul_tiles_kernel<kF, kCode, kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>), dim3(grid.workgroups(), splits), dim3(64 * kWN * kWT * kWK), Traits::kLds, s, a, grid);
     return hipGetLastError();
 }
 
 template <dev::Float kF, int kCode>
 hipError_t launch_shape(hipStream_t s, const MatmulArgs& a, const TilesChoice& c) {
     switch (c.shape) {
-        case TilesShape::k256x128: return launch_tile<kF, kCode, 2, 4, 4, 1, 1, 64>(s, a, c.splits);
-        case TilesShape::k128x64: return launch_tile<kF, kCode, 1, 2, 4, 1, 2, 64>(s, a, c.splits);
-        case TilesShape::k128x32: return launch_tile<kF, kCode, 1, 1, 4, 1, 2, 64>(s, a, c.splits);
-        case TilesShape::k32x32: return launch_tile<kF, kCode, 1, 1, 1, 1, 8, 128>(s, a, c.splits);
+        case TilesShape::k256x128: return launch_tile<kF, kCode, 2, 4, 4, 1, 1, 64, 2, 2>(s, a, c.splits);
+        case TilesShape::k128x64: return launch_tile<kF, kCode, 1, 2, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
+        case TilesShape::k128x32: return launch_tile<kF, kCode, 1, 1, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
+        case TilesShape::k32x32: return launch_tile<kF, kCode, 1, 1, 1, 1, 8, 128, 2, 2>(s, a, c.splits);
     }
     return hipErrorInvalidValue;
 }

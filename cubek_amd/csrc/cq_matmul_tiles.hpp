@@ -14,12 +14,14 @@ struct TilesChoice {
 
 // kNT, kTT: tiles of 32 rows and of 32 positions of a wave; kWN, kWT, kWK: waves along rows, positions and columns; kLine: bytes of a row in a
 // chunk of codes.
-template <int kNT, int kTT, int kWN, int kWT, int kWK, int kLine>
+// kXRing, kCodeRing: images of x (a step) and of codes (a chunk).
+template <int kNT, int kTT, int kWN, int kWT, int kWK, int kLine, int kXRing, int kCodeRing>
 struct TilesTraits {
     static constexpr uint32_t kRows = 32 * kNT * kWN, kTokens = 32 * kTT * kWT;
-    static constexpr uint32_t kXBytes = kTokens * 128, kCodeBytes = kRows * kLine;  // a step of x; a chunk of codes
+    static constexpr uint32_t kXBytes = kTokens * 128, kCodeBytes = kRows * kLine, kScaleBytes = kRows * 8;  // a step of x; a chunk of codes; a step's scales
+    static constexpr uint32_t kScaleRing = 4;
     static constexpr uint32_t kPitch = 32 * kNT + 4;                              // of the sums on their way to y
-    static constexpr uint32_t kImages = kWK * 2 * (kXBytes + kCodeBytes), kParts = kWN * kWT * kWK * 32 * kPitch * 4;
+    static constexpr uint32_t kImage = kXRing * kXBytes + kCodeRing * kCodeBytes + kScaleRing * kScaleBytes, kImages = kWK * kImage, kParts = kWN * kWT * kWK * 32 * kPitch * 4;
     static constexpr uint32_t kLds = kImages > kParts ? kImages : kParts;
     static_assert(kLds <= 160 * 1024, "a compute unit's LDS");
     static constexpr uint32_t kWaves = kWN * kWT * kWK, kFit = 160 * 1024 / kLds;
@@ -27,18 +29,23 @@ struct TilesTraits {
     static constexpr uint32_t kWavesPerSimd = kWaves / 4 * kFit < kMost ? kWaves / 4 * kFit : kMost;
 };
 
+// n / each as 2 n ceil(2^31 / each) / 2^32, for n < 2^27 and each < 32; 0 for each = 0, one scale for everything
+inline uint32_t magic_of(uint32_t each) { return each ? (0x80000000u + each - 1u) / each : 0u; }
+
 struct TilesGrid {
     uint32_t n_tiles, p_tiles, splits, pitch;  // pitch: floats of a position's sums in the workspace
     uint32_t scale_size, scale_col_bytes;
-    cubek_quant::device::FastDivmod halves_per_block, by_group;  // by 32 columns; by kGroup * n_tiles
+    uint32_t block_magic;                          // of the division of 32 columns by those under a scale
+    cubek_quant::device::FastDivmod by_group;      // by kGroup * n_tiles
 
     static constexpr uint32_t kUnits = 8, kGroup = 4;  // dies with an L2 each; tiles of positions that share one die's weights
 
     TilesGrid(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t splits)
         : n_tiles((a.out_cols + (a.gated ? rows / 2 : rows) - 1) / (a.gated ? rows / 2 : rows)), p_tiles(static_cast<uint32_t>(most_tiles(a, __builtin_ctz(tokens)))),
           splits(splits), pitch(sums_pitch(a)), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u), scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)),
-          halves_per_block(a.block_cols ? a.block_cols / 32u : 0x7fffffffu), by_group(kGroup * n_tiles) {}
+          block_magic(magic_of(a.block_cols / 32u)), by_group(kGroup * n_tiles) {}
 
+    __device__ uint32_t block_of(uint32_t half) const { return __umulhi(2u * half, block_magic); }
     uint32_t workgroups() const { return n_tiles * p_tiles; }
 
     // Floats of a position's sums: whole eights of columns, gated two of them.
@@ -77,11 +84,7 @@ struct FewGrid {
 
     FewGrid(const MatmulArgs& a, const FewShape& c)
         : shares_log2(c.shares_log2), tokens_log2(c.tokens_log2), x_bytes(c.x_bytes), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u),
-          scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)) {
-        const uint32_t each = a.block_cols * a.bits / 128;  // units of 16 bytes of codes under a scale
-        block_magic = each ? (0x80000000u + each - 1) / each : 0u;
-    }
-    // unit / each, for less than 2^27 units and each < 32: 2 unit ceil(2^31 / each) / 2^32
+          scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)), block_magic(magic_of(a.block_cols * a.bits / 128)) {}
     __device__ uint32_t block_of(uint32_t unit) const { return __umulhi(2u * unit, block_magic); }
 };
 
