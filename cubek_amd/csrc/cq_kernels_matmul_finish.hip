@@ -19,7 +19,9 @@ __global__ __launch_bounds__(256) void matmul_finish_kernel(MatmulArgs a, uint32
                 v += load8(from);
                 if (a.gated) up += load8(from + pitch / 2);
             }
-            finish8(a, at.expert, p, col, v, up);
+            v += load_bias8(a, at.expert, col);
+            if (a.gated) up += load_bias8(a, at.expert, a.out_cols + col);
+            finish8(a, p, col, v, up);
         }
     }
 }

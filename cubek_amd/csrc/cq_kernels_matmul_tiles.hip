@@ -275,6 +275,12 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     float* const parts_of = reinterpret_cast<float*>(lds) + wave * kPart;  // those of the other waves along the columns behind it
     const bool pairs = a.gated && grid.splits == 1;                        // (with shared columns the rows are stored as they are)
     const uint32_t columns = pairs ? 16u * kNT : 32u * kNT, lanes = columns / 8u;
+    const uint32_t in = lane % lanes * 8u, own_col = out0 + wave_n * columns + in;
+    f32x8 bias = {}, bias_up = {};
+    if (grid.splits == 1 && own_col < a.out_cols) {
+        bias = load_bias8(a, at.expert, own_col);
+        if (a.gated) bias_up = load_bias8(a, at.expert, a.out_cols + own_col);
+    }
     __syncthreads();
 #pragma unroll
     for (uint32_t t = 0; t < kTT; t++) {
@@ -292,7 +298,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         const uint32_t p0 = at.first + (wave_t * kTT + t) * 32u;
 #pragma unroll 1
         for (uint32_t r = (wave_k * 64u + lane) / lanes; r < 32; r += 64u * kWK / lanes) {
-            const uint32_t in = lane % lanes * 8u, p = p0 + r;
+            const uint32_t p = p0 + r;
             if (p >= at.last) continue;
             const float* const from = parts_of + r * kPitch + (pairs ? in / 16u * 32u + in % 16u : in);
             const auto sum_at = [&](const float* at_part) {
@@ -311,8 +317,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
                 *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};  // (the pitch has room for whole eights)
                 *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
             } else {
-                const uint32_t col = out0 + wave_n * columns + in;
-                if (col < a.out_cols) finish8(a, at.expert, p, col, sum_at(from), a.gated ? sum_at(from + 16) : f32x8{});
+                if (own_col < a.out_cols) finish8(a, p, own_col, sum_at(from) + bias, a.gated ? sum_at(from + 16) + bias_up : f32x8{});
             }
         }
         if (kWK == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

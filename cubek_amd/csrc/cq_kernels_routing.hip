@@ -296,20 +296,7 @@ __device__ __forceinline__ void load_columns(int dtype, const char* p, uint64_t 
     if constexpr (kN == 1) {
         out[0] = load_float(dtype, p, i);
     } else {
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-        f32x8 v;
-        if (dtype == CQ_F32) {
-            v = load8(reinterpret_cast<const float*>(p) + i);
-        } else {
-            const u32x4 bits = *reinterpret_cast<const u32x4*>(p + i * 2);
-            if (dtype == CQ_F16) {
-                v = __builtin_convertvector(__builtin_bit_cast(f16x8, bits), f32x8);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[2 * k] = __builtin_bit_cast(float, bits[k] << 16), v[2 * k + 1] = __builtin_bit_cast(float, bits[k] & 0xffff0000u);
-            }
-        }
+        const f32x8 v = load_floats8(dtype, p, i);
 #pragma unroll
         for (int k = 0; k < 8; k++) out[k] = v[k];
     }

@@ -119,6 +119,19 @@ __device__ __forceinline__ f32x8 load8(const float* p) {
     return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Eight floats of any type from a boundary of 16 bytes.
+__device__ __forceinline__ f32x8 load_floats8(int dtype, const char* p, uint64_t i) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    if (dtype == CQ_F32) return load8(reinterpret_cast<const float*>(p) + i);
+    const u32x4 bits = *reinterpret_cast<const u32x4*>(p + i * 2);
+    if (dtype == CQ_F16) return __builtin_convertvector(__builtin_bit_cast(f16x8, bits), f32x8);
+    f32x8 v;
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[2 * k] = __builtin_bit_cast(float, bits[k] << 16), v[2 * k + 1] = __builtin_bit_cast(float, bits[k] & 0xffff0000u);
+    return v;
+}
+
 // Eight columns to a boundary of 16 bytes, rounded once.
 __device__ __forceinline__ void store8(int dtype, char* y, uint64_t at, f32x8 v) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -134,19 +147,20 @@ __device__ __forceinline__ void store8(int dtype, char* y, uint64_t at, f32x8 v)
     }
 }
 
-// Columns col .. col + 7 of position p, as far as y has them, from their sums and those of the gated ones.
-__device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, uint32_t p, uint32_t col, f32x8 v, f32x8 up) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const bool whole = col + 8 <= a.out_cols;
-    if (a.bias) {
-        const auto add_bias = [&](f32x8& to, uint32_t row) {
-            const uint64_t at = expert * a.bias_expert;
+// The bias of rows row .. row + 7 of W, as far as W has them; for all positions of a lane, which asks for it once.
+__device__ __forceinline__ f32x8 load_bias8(const MatmulArgs& a, uint32_t expert, uint32_t row) {
+    f32x8 v = {};
+    if (a.bias == nullptr) return v;
+    const uint64_t at = expert * a.bias_expert;
+    if (a.vector_bias && row % 8u == 0 && row + 8u <= a.wide) return load_floats8(a.bias_dtype, a.bias, at + row);
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) to[k] += load_float(a.bias_dtype, a.bias, at + (whole ? row + k : min(row + k, a.wide - 1u)) * a.bias_stride);
-        };
-        add_bias(v, col);
-        if (a.gated) add_bias(up, a.out_cols + col);
-    }
+    for (uint32_t k = 0; k < 8; k++) v[k] = load_float(a.bias_dtype, a.bias, at + min(row + k, a.wide - 1u) * a.bias_stride);
+    return v;
+}
+
+// Columns col .. col + 7 of position p, as far as y has them, from their sums and those of the gated ones, bias and all.
+__device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t p, uint32_t col, f32x8 v, f32x8 up) {
+    const bool whole = col + 8 <= a.out_cols;
     if (a.activation != CQ_ACT_IDENTITY) {
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) v[k] = activated(a.activation, v[k]);
@@ -157,14 +171,7 @@ __device__ __forceinline__ void finish8(const MatmulArgs& a, uint32_t expert, ui
     }
     const uint64_t y_at = p * a.y_stride + col, r_at = p * a.residual_stride + col;
     if (whole && a.vector_stores) {  // eight columns lie on a boundary of 16 bytes
-        if (a.residual && a.y_dtype == CQ_F32) {
-            v += load8(reinterpret_cast<const float*>(a.residual) + r_at);
-        } else if (a.residual) {
-            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-            typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-            const u32x4 r = *reinterpret_cast<const u32x4*>(a.residual + r_at * 2);
-            v += a.y_dtype == CQ_F16 ? __builtin_convertvector(__builtin_bit_cast(f16x8, r), f32x8) : __builtin_convertvector(__builtin_bit_cast(bf16x8, r), f32x8);
-        }
+        if (a.residual) v += load_floats8(a.y_dtype, a.residual, r_at);
         store8(a.y_dtype, a.y, y_at, v);
         return;
     }
