@@ -102,6 +102,7 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
         }
     };
 
+    const ScaleMasks masks(a.param_dtype);
     f32x4 acc[kNT][kTT][2] = {};
     uint32_t scale_of_row[kNT], column[kTT];
 #pragma unroll
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
             const uint32_t block = grid.block_of(min(stage * 8u + q * 4u + g, units - 1u)) * grid.scale_col_bytes;
 #pragma unroll
             for (uint32_t t = 0; t < kNT; t++) {
-                scale[t][q] = dev::round_to<kF>(scale_of(a.param_dtype, word[t][q], scale_of_row[t] + block));
+                scale[t][q] = dev::round_to<kF>(scale_of(masks, word[t][q], scale_of_row[t] + block));
                 mine_short = mine_short && takes_short<kF, kCode>(scale[t][q]);
             }
         }

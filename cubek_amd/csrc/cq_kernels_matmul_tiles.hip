@@ -49,9 +49,8 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     extern __shared__ char lds[];
 
     uint32_t n_tile, p_tile;
-    grid.tile(blockIdx.x, &n_tile, &p_tile);
     TileOfPositions at;
-    if (!find_tile(a, p_tile, kTokensLog2, &at)) return;
+    if (!grid.tile(blockIdx.x, &n_tile, &p_tile) || !find_tile(a, p_tile, kTokensLog2, &at)) return;
     const uint32_t lane = threadIdx.x & 63u, any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wave = any_wave % kWaves, wave_k = any_wave / kWaves;
     const uint32_t wave_n = wave % kWN, wave_t = wave / kWN, i = lane & 31u, h = lane >> 5;
@@ -161,6 +160,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         return c;
     };
 
+    const ScaleMasks masks(a.param_dtype);
     f32x16 acc[kNT][kTT] = {};
     u32x4 w[kNT][4];  // the step's weights, by instruction
     Codes<kCode> codes[kNT];
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         for (uint32_t n = 0; n < kNT; n++) {
             codes[n] = read_codes(in, n);
             const uint32_t word = *reinterpret_cast<const uint32_t*>(scale_img + in % Traits::kScaleRing * Traits::kScaleBytes + ((wave_n * kNT + n) * 32u + i) * 8u + h * 4u);
-            rounded_scale[n] = dev::round_to<kF>(scale_of(a.param_dtype, word, scale_own[n] + block));
+            rounded_scale[n] = dev::round_to<kF>(scale_of(masks, word, scale_own[n] + block));
             mine = mine && takes_short<kF, kCode>(rounded_scale[n]);
         }
         all_short = kCode > 8 || __builtin_amdgcn_ballot_w64(!mine) == 0;
@@ -182,15 +182,21 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
 #pragma unroll
         for (uint32_t n = 0; n < kNT; n++) w[n][m] = slice<kF, kCode, true>(codes[n], m, rounded_scale[n]);
     };
-    const auto dequantize_any = [&](uint32_t step) {  // scales that are not ordinary, and the last step where it is a half
-        const bool past = step * 2u + h >= a.cols / 32u;
+    // What the short way does not do: scales that are not ordinary; and where the row ends in the middle of a step, whose second half counts
+    // nothing.
+    const auto amend = [&](uint32_t step) {
+        if (kCode <= 8 && !all_short) {
 #pragma unroll
-        for (uint32_t n = 0; n < kNT; n++)
+            for (uint32_t n = 0; n < kNT; n++)
 #pragma unroll
-            for (uint32_t m = 0; m < 4; m++) {
-                w[n][m] = slice<kF, kCode, false>(codes[n], m, rounded_scale[n]);
-                if (past) w[n][m] = u32x4{0, 0, 0, 0};
-            }
+                for (uint32_t m = 0; m < 4; m++) w[n][m] = slice<kF, kCode, false>(codes[n], m, rounded_scale[n]);
+        }
+        if ((step + 1) * 64u > a.cols) {
+#pragma unroll
+            for (uint32_t n = 0; n < kNT; n++)
+#pragma unroll
+                for (uint32_t m = 0; m < 4; m++) w[n][m] = h == 1 ? u32x4{0, 0, 0, 0} : w[n][m];
+        }
     };
     const auto read_x = [&](uint32_t from, uint32_t m, u32x4* xv) {
 #pragma unroll
@@ -216,7 +222,6 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         codes_after_x = (in + 1) % kSteps == 0 && chunk * kSteps < steps;
         if (codes_after_x) load_codes(first_chunk + chunk, chunk % kCodeRing);
     };
-    constexpr uint32_t kPerMfma = 5;
     u32x4 xv[2][kTT];
 #pragma unroll
     for (uint32_t k = 0; k < kCodeRing; k++)
@@ -230,7 +235,9 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     begin(std::integral_constant<int, 0>{});
     if (kWK == 1 || steps != 0) {
         fetch(0);
-        dequantize_any(first_step);
+#pragma unroll
+        for (uint32_t m = 0; m < 4; m++) dequantize(m);
+        amend(first_step);
     }
 #pragma unroll 1
     for (uint32_t in = 0; in < rounds; in++) {
@@ -255,16 +262,17 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
                 for (uint32_t n = 0; n < kNT; n++) acc[n][t] = mfma<kF>(w[n][m], xv[m & 1][t], acc[n][t]);
             dequantize(m);
         }
-        if constexpr (kTT >= 4) {
-            // a matrix instruction keeps its unit busy for 32 cycles, in which the wave may issue seven others
+        if constexpr (kTT >= 4 && kCode != 8) {
+            // A matrix instruction keeps its unit busy for 32 cycles, in which the wave may issue seven others; x of the next products comes in front of the
+            // next weights ([28672, 8192] 4 bits, 4096 positions 1.96 -> 1.88 ms; the 8-bit fields have no registers left for it).
 #pragma unroll
             for (uint32_t k = 0; k < 4 * kNT * kTT; k++) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, kPerMfma, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
                 if (k % (kNT * kTT) < kTT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         }
-        if (!all_short || (first_step + next + 1) * 64u > a.cols) dequantize_any(first_step + next);
+        amend(first_step + next);
     }
 
     // Lane (i, h) holds position i of each 32, rows 8 q + 4 h + 0 .. 3 of each 32.  They go through the wave's own part of LDS, 32 positions at a
@@ -336,6 +344,7 @@ template <dev::Float kF, int kCode>
 hipError_t launch_shape(hipStream_t s, const MatmulArgs& a, const TilesChoice& c) {
     switch (c.shape) {
         case TilesShape::k256x128: return launch_tile<kF, kCode, 2, 4, 4, 1, 1, 64, 2, 2>(s, a, c.splits);
+        case TilesShape::k256x128x2: return launch_tile<kF, kCode, 2, 4, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
         case TilesShape::k128x64: return launch_tile<kF, kCode, 1, 2, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
         case TilesShape::k128x32: return launch_tile<kF, kCode, 1, 1, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
         case TilesShape::k32x32: return launch_tile<kF, kCode, 1, 1, 1, 1, 8, 128, 2, 2>(s, a, c.splits);

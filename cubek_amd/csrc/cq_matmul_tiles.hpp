@@ -6,7 +6,7 @@
 
 namespace cq {
 
-enum class TilesShape { k256x128, k128x64, k128x32, k32x32 };  // rows of W x positions
+enum class TilesShape { k256x128, k256x128x2, k128x64, k128x32, k32x32 };  // rows of W x positions; x2: by twice the waves, along the columns
 struct TilesChoice {
     TilesShape shape;
     uint32_t splits;  // workgroups that share the columns of a tile
@@ -34,34 +34,49 @@ inline uint32_t magic_of(uint32_t each) { return each ? (0x80000000u + each - 1u
 
 struct TilesGrid {
     uint32_t n_tiles, p_tiles, splits, pitch;  // pitch: floats of a position's sums in the workspace
-    uint32_t scale_size, scale_col_bytes;
-    uint32_t block_magic;                          // of the division of 32 columns by those under a scale
-    cubek_quant::device::FastDivmod by_group;      // by kGroup * n_tiles
+    uint32_t scale_size, scale_col_bytes, block_magic;
 
-    static constexpr uint32_t kUnits = 8, kGroup = 4;  // dies with an L2 each; tiles of positions that share one die's weights
+    // Workgroups go round the dies, which have an L2 each, one by one.  Tiles are dealt out in rectangles of up to kGroup tiles of positions by
+    // up to kChunk of rows, whose workgroups read few rows of x and few of W at a time: rectangle r to die r % kDies, as many to each die
+    // as to any other where that can be had, and the experts' sizes, which the host does not know, spread over all of them (in runs of
+    // tiles the last dies had those that do not exist: 64 experts, 6126 positions 209 -> 204 us).
+    static constexpr uint32_t kDies = 8, kGroup = 4, kChunk = 8;
+    uint32_t group, chunk, rectangles;
+    cubek_quant::device::FastDivmod by_rectangle, by_chunks, by_group;
 
     TilesGrid(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t splits)
         : n_tiles((a.out_cols + (a.gated ? rows / 2 : rows) - 1) / (a.gated ? rows / 2 : rows)), p_tiles(static_cast<uint32_t>(most_tiles(a, __builtin_ctz(tokens)))),
           splits(splits), pitch(sums_pitch(a)), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u), scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)),
-          block_magic(magic_of(a.block_cols / 32u)), by_group(kGroup * n_tiles) {}
+          block_magic(magic_of(a.block_cols / 32u)) {
+        group = p_tiles < kGroup ? p_tiles : kGroup;
+        const uint32_t groups = (p_tiles + group - 1) / group;
+        uint32_t even = kDies;  // chunks come in multiples of this many, so that all rectangles do in multiples of kDies
+        while (even > 1 && groups % (kDies / even * 2) == 0) even /= 2;
+        uint32_t chunks = ((n_tiles + kChunk - 1) / kChunk + even - 1) / even * even;
+        if (chunks > n_tiles) chunks = n_tiles;
+        chunk = (n_tiles + chunks - 1) / chunks;
+        chunks = (n_tiles + chunk - 1) / chunk;
+        rectangles = groups * chunks;
+        by_rectangle = cubek_quant::device::FastDivmod(group * chunk);
+        by_chunks = cubek_quant::device::FastDivmod(chunks);
+        by_group = cubek_quant::device::FastDivmod(group);
+    }
 
     __device__ uint32_t block_of(uint32_t half) const { return __umulhi(2u * half, block_magic); }
-    uint32_t workgroups() const { return n_tiles * p_tiles; }
+    uint32_t workgroups() const { return (rectangles + kDies - 1) / kDies * kDies * group * chunk; }
 
     // Floats of a position's sums: whole eights of columns, gated two of them.
     static uint32_t sums_pitch(const MatmulArgs& a) { return (a.out_cols + 7u) / 8u * 8u * (a.gated ? 2u : 1u); }
 
-    // Workgroups go round the dies one by one.  Each die gets a run of tiles of its own, in groups of kGroup tiles of positions by all tiles of
-    // rows, positions first: what its workgroups read at a time are few rows of x and few of W.
-    __device__ void tile(uint32_t block, uint32_t* n, uint32_t* p) const {
-        const uint32_t total = n_tiles * p_tiles, each = total / kUnits, rest = total % kUnits;
-        const uint32_t die = block % kUnits, in = block / kUnits;
-        const uint32_t id = die * each + min(die, rest) + in;
-        uint32_t group, within;
-        by_group.div_mod(id, &group, &within);
-        const uint32_t size = min(kGroup, p_tiles - group * kGroup);
-        *n = within / size;
-        *p = group * kGroup + within % size;
+    // false: a workgroup beyond the last tile
+    __device__ bool tile(uint32_t block, uint32_t* n, uint32_t* p) const {
+        uint32_t round, within, p_group, n_chunk, in_chunk, in_group;
+        by_rectangle.div_mod(block / kDies, &round, &within);
+        by_chunks.div_mod(round * kDies + block % kDies, &p_group, &n_chunk);
+        by_group.div_mod(within, &in_chunk, &in_group);
+        *n = n_chunk * chunk + in_chunk;
+        *p = p_group * group + in_group;
+        return *n < n_tiles && *p < p_tiles;
     }
 };
 
@@ -118,8 +133,6 @@ struct MatmulChoice {
     double us = 1e30;
 };
 
-constexpr double kStartUs = 4.0;  // a launch without a step
-
 // Workgroups that a launch may be taken to have: the experts' sizes lie in device memory, and as many end in half a tile as in a whole one.
 inline double likely_tiles(const MatmulArgs& a, uint32_t size) {
     if (!a.offsets) return static_cast<double>((a.positions + static_cast<uint64_t>(size) - 1) / size);
@@ -133,14 +146,15 @@ inline double rounds_us(double workgroups, double half, double full) {
     return whole * full + (rest <= 0.0 ? 0.0 : rest <= 256.0 ? half : full);
 }
 
-inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows, uint32_t tokens, uint32_t along, uint32_t line, double half, double full, MatmulChoice* best) {
+inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows, uint32_t tokens, uint32_t along, uint32_t line, double start, double half, double full,
+                           MatmulChoice* best) {
     const uint32_t columns = a.gated ? rows / 2 : rows, steps = line / 8 / a.bits, chunks = ((a.cols + 63) / 64 + steps - 1) / steps;
     const double tiles = (a.out_cols + columns - 1) / columns * likely_tiles(a, tokens);
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
         if (splits > 1 && (splits * along > chunks || sums_bytes(a, splits) > a.workspace_bytes)) break;
         const double rounds = static_cast<double>((chunks + splits * along - 1) / (splits * along) * steps);
         const double sums = splits > 1 ? 3.0 + 2.0 * static_cast<double>(sums_bytes(a, splits)) / 5e6 : 0.0;  // written and read at 5 TB/s
-        const double us = kStartUs + rounds * rounds_us(tiles * splits, half, full) + sums;
+        const double us = start + rounds * rounds_us(tiles * splits, half, full) + sums;
         if (us < best->us * (splits > 1 ? 0.92 : 1.0)) {  // (workgroups of many rounds do not wait for one another)
             best->few = false;
             best->tiles = TilesChoice{shape, splits};
@@ -181,10 +195,12 @@ inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
 inline MatmulChoice matmul_choice(const MatmulArgs& a) {
     MatmulChoice c;
     consider_few(a, &c);
-    consider_tiles(a, TilesShape::k256x128, 256, 128, 1, 64, 1.15, 1.83, &c);
-    consider_tiles(a, TilesShape::k128x64, 128, 64, 2, 64, 1.2, 1.65, &c);
-    consider_tiles(a, TilesShape::k128x32, 128, 32, 2, 64, 1.13, 1.8, &c);
-    consider_tiles(a, TilesShape::k32x32, 32, 32, 8, 128, 1.15, 2.3, &c);
+    // start: a launch without its rounds, from the first loads to the last sums
+    consider_tiles(a, TilesShape::k256x128, 256, 128, 1, 64, 6.0, 1.05, 1.75, &c);
+    consider_tiles(a, TilesShape::k256x128x2, 256, 128, 2, 64, 9.0, 1.85, 3.7, &c);
+    consider_tiles(a, TilesShape::k128x64, 128, 64, 2, 64, 5.0, 1.15, 1.65, &c);
+    consider_tiles(a, TilesShape::k128x32, 128, 32, 2, 64, 4.5, 1.1, 1.75, &c);
+    consider_tiles(a, TilesShape::k32x32, 32, 32, 8, 128, 4.0, 1.15, 2.3, &c);
     return c;
 }
 

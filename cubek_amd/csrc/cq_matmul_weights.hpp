@@ -13,10 +13,15 @@ constexpr int bits_of(int code) { return code <= 8 ? code : (code == kCodeE2M1x2
 // A stored scale of type `dtype` (uniform over the launch) at an address, as the word around it and as a number: apart, so that a load is
 // not waited for where it is issued, and without branches, which would cut a step's instructions into pieces.
 __device__ __forceinline__ uint32_t scale_word(const char* base, uint32_t offset) { return *reinterpret_cast<const uint32_t*>(base + (offset & ~3u)); }
-__device__ __forceinline__ float scale_of(int dtype, uint32_t word, uint32_t offset) {
-    const uint32_t half = offset & 2u ? word >> 16 : word & 0xffffu;
-    const float wide = __builtin_bit_cast(float, dtype == CQ_BF16 ? half << 16 : word);
-    return dtype == CQ_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(half))) : wide;
+// All bits or none of a word, by the type of the scales: uniform over the launch.
+struct ScaleMasks {
+    uint32_t f32, bf16, f16;
+    __device__ explicit ScaleMasks(int dtype) : f32(dtype == CQ_F32 ? ~0u : 0u), bf16(dtype == CQ_BF16 ? ~0u : 0u), f16(dtype == CQ_F16 ? ~0u : 0u) {}
+};
+__device__ __forceinline__ float scale_of(const ScaleMasks& m, uint32_t word, uint32_t offset) {
+    const uint32_t half = word >> ((offset & 2u) * 8u);
+    const uint32_t from_f16 = __builtin_bit_cast(uint32_t, static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(half))));
+    return __builtin_bit_cast(float, (word & m.f32) | (half << 16 & m.bf16) | (from_f16 & m.f16));
 }
 
 __device__ const char kZeros[16] __attribute__((aligned(16))) = {};
