@@ -290,64 +290,49 @@ __global__ __launch_bounds__(256) void route_nothing_kernel(RouteArgs a) {
     for (uint32_t e = threadIdx.x; e <= a.num_experts; e += 256) a.offsets[e] = 0;
 }
 
-// kN floats in a row: eight on a boundary of 16 bytes, or one.
-template <int kN>
-__device__ __forceinline__ void load_columns(int dtype, const char* p, uint64_t i, float* out) {
-    if constexpr (kN == 1) {
-        out[0] = load_float(dtype, p, i);
-    } else {
-        const f32x8 v = load_floats8(dtype, p, i);
-#pragma unroll
-        for (int k = 0; k < 8; k++) out[k] = v[k];
-    }
-}
-template <int kN>
-__device__ __forceinline__ void store_columns(int dtype, char* p, uint64_t i, const float* v) {
-    if constexpr (kN == 1) {
-        store_float(dtype, p, i, v[0]);
-    } else {
-        f32x8 all;
-#pragma unroll
-        for (int k = 0; k < 8; k++) all[k] = v[k];
-        store8(dtype, p, i, all);
-    }
-}
-
-// A thread makes kN columns of a token, kN = 8 where everything lies on boundaries of 16 bytes: bound by the read of h, eight rows of it
-// in flight.
-template <int kN>
+// A thread makes eight columns of a token, or the last ones: bound by the read of h, eight rows of it in flight.
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, uint32_t parts, uint32_t tokens_each) {
     // parts of a token, 256 of them or whole tokens to a workgroup
     const uint32_t in = parts < 256u ? threadIdx.x / parts : 0u, part = parts < 256u ? threadIdx.x % parts : blockIdx.x * 256u + threadIdx.x;
     if (part >= parts || in >= tokens_each) return;
-    const uint32_t n = part * kN;
+    const uint32_t n = part * 8u, rest = a.cols - n;
+    const auto load = [&](int dtype, const char* p, uint64_t at) {
+        if (rest >= 8u) return load_floats8(dtype, p, at);
+        f32x8 v;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) v[k] = load_float(dtype, p, at + min(k, rest - 1u));
+        return v;
+    };
     for (uint64_t t = static_cast<uint64_t>(blockIdx.y) * tokens_each + in; t < a.tokens; t += static_cast<uint64_t>(gridDim.y) * tokens_each) {
         const int32_t* const slots = a.slots + t * a.chosen;
         const float* const weights = a.weights + t * a.chosen;
-        float sum[kN] = {};
+        f32x8 sum = {};
 #pragma unroll 1
         for (uint32_t j0 = 0; j0 < a.chosen; j0 += 8) {
-            float v[8][kN], w[8];
+            f32x8 v[8];
+            float w[8];
             bool there[8];
 #pragma unroll
             for (uint32_t j = 0; j < 8; j++) {
                 const uint32_t slot = j0 + j < a.chosen ? static_cast<uint32_t>(slots[j0 + j]) : ~0u;
                 there[j] = slot < a.positions;
                 w[j] = there[j] ? weights[j0 + j] : 0.0f;
-                if (there[j]) load_columns<kN>(a.h_dtype, a.h, slot * a.h_stride + n, v[j]);
+                if (there[j]) v[j] = load(a.h_dtype, a.h, slot * a.h_stride + n);
             }
 #pragma unroll
             for (uint32_t j = 0; j < 8; j++)
 #pragma unroll
-                for (int k = 0; k < kN; k++) sum[k] = there[j] ? __builtin_fmaf(w[j], v[j][k], sum[k]) : sum[k];
+                for (int k = 0; k < 8; k++) sum[k] = there[j] ? __builtin_fmaf(w[j], v[j][k], sum[k]) : sum[k];
         }
-        if (a.residual) {
-            float r[kN];
-            load_columns<kN>(a.y_dtype, a.residual, t * a.residual_stride + n, r);
+        if (a.residual) sum += load(a.y_dtype, a.residual, t * a.residual_stride + n);
+        const uint64_t at = t * a.y_stride + n;
+        if (rest >= 8u) {
+            store8(a.y_dtype, a.y, at, sum);
+        } else {
 #pragma unroll
-            for (int k = 0; k < kN; k++) sum[k] += r[k];
+            for (uint32_t k = 0; k < 8; k++)
+                if (k < rest) store_float(a.y_dtype, a.y, at + k, sum[k]);
         }
-        store_columns<kN>(a.y_dtype, a.y, t * a.y_stride + n, sum);
     }
 }
 
@@ -375,15 +360,8 @@ hipError_t launch_route(hipStream_t s, const RouteArgs& a) {
 }
 
 hipError_t launch_combine(hipStream_t s, const CombineArgs& a) {
-    const auto on16 = [](const void* p, uint64_t stride, int dtype) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (dtype == CQ_F32 ? 4 : 2) % 16 == 0; };
-    const bool vectors = a.cols % 8 == 0 && on16(a.h, a.h_stride, a.h_dtype) && on16(a.y, a.y_stride, a.y_dtype) &&
-                         (!a.residual || on16(a.residual, a.residual_stride, a.y_dtype));
-    const uint32_t parts = vectors ? a.cols / 8 : a.cols, each = parts < 256 ? 256 / parts : 1, ys = (a.tokens + each - 1) / each;
-    const dim3 grid(parts < 256 ? 1 : (parts + 255) / 256, ys < 65535 ? ys : 65535);
-    if (vectors)
-        hipLaunchKernelGGL(combine_kernel<8>, grid, dim3(256), 0, s, a, parts, each);
-    else
-        hipLaunchKernelGGL(combine_kernel<1>, grid, dim3(256), 0, s, a, parts, each);
+    const uint32_t parts = (a.cols + 7) / 8, each = parts < 256 ? 256 / parts : 1, ys = (a.tokens + each - 1) / each;
+    hipLaunchKernelGGL(combine_kernel, dim3(parts < 256 ? 1 : (parts + 255) / 256, ys < 65535 ? ys : 65535), dim3(256), 0, s, a, parts, each);
     return hipGetLastError();
 }
 

@@ -167,10 +167,6 @@ cq_status read_indexes(const cq_tensor* t, uint64_t n, const int32_t** out) {
 }
 
 cq_status launch(cq_stream_t stream, cq::MatmulArgs& a) {
-    const uint64_t size = dtype_size(a.y_dtype);
-    a.vector_stores = aligned(a.y, 16) && a.y_stride * size % 16 == 0 && (!a.residual || (aligned(a.residual, 16) && a.residual_stride * size % 16 == 0));
-    const uint64_t bias_size = dtype_size(a.bias_dtype);
-    a.vector_bias = a.bias && a.bias_stride == 1 && aligned(a.bias, 16) && a.bias_expert * bias_size % 16 == 0;
     return hip_status(cq::tiles_take(a) ? cq::launch_matmul_tiles(stream, a) : cq::launch_matmul_general(stream, a));
 }
 

@@ -30,8 +30,6 @@ struct MatmulArgs {
     uint64_t scale_row, scale_col, scale_expert;  // strides of the scales, in elements
     uint64_t x_stride, y_stride, residual_stride, bias_stride, bias_expert;  // in elements
     uint32_t activation, gated;
-    uint32_t vector_stores;  // eight columns of y and of the residual, from any multiple of eight on, lie on a boundary of 16 bytes
-    uint32_t vector_bias;    // eight rows of the bias too
     void* workspace;
     uint64_t workspace_bytes;
 };
