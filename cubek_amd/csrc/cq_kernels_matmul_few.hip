@@ -1,9 +1,9 @@
 // Products with quantized weights for up to 32 positions of an expert (or of the whole product): a decode step.
 //
 // A wave takes 16 or 32 rows of W (gated: 16 and their gated ones) and a share of their columns, in stages of a line of 128 bytes of every
-// row.  Codes, scales and x of a stage come into LDS by direct loads, kAhead stages ahead: codes and scales into the wave's own part, x into one
-// that the waves of a share have together.  16 x 16 x 32 matrix instructions take lane (i, g)'s eight columns of row i, and the same of
-// token i.  The eight waves of a workgroup are one to eight groups of rows by eight to one shares of the columns; the shares' sums meet
+// row or of half a line (few_units).  Codes, scales and x of a stage come into LDS by direct loads, kAhead stages ahead: codes and scales into
+// the wave's own part, x into one that the waves of a share have together.  16 x 16 x 32 matrix instructions take lane (i, g)'s eight columns
+// of row i, and the same of token i.  The eight waves of a workgroup are one to eight groups of rows by eight to one shares of the columns; the shares' sums meet
 // in LDS at the end.  Bound by the read of W and the instructions of its dequantization side by side, and in launches of few stages by the
 // time from a workgroup's start to its first stage and from its last one to its sums.
 #include <hip/hip_runtime.h>
@@ -30,10 +30,10 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 // kNT: groups of 16 rows of a wave; kTT: groups of 16 positions; kX: loads of 1 KiB by which a wave takes part in a stage of its share's x.
 template <dev::Float kF, int kCode, int kNT, int kTT, int kX>
 __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid grid) {
-    constexpr uint32_t kBits = bits_of(kCode), kUnit = 128 / kBits;  // columns of 16 bytes of codes
-    constexpr uint32_t kM = kUnit / 8, kPieces = 8 * kM;             // matrix instructions of a unit; a stage's 16-byte pieces of x of a token
-    constexpr uint32_t kCodeBytes = kNT * 2048, kSlot = kCodeBytes + kNT * 512, kAhead = kFewAhead, kRing = kAhead + 1;
-    constexpr uint32_t kLoads = kNT * 4 + kX;
+    constexpr uint32_t kBits = bits_of(kCode), kUnit = 128 / kBits, kUnits = few_units(kTT == 1 ? 4 : 5, kBits);  // columns of 16 bytes of codes; of those, in a stage
+    constexpr uint32_t kQ = kUnits / 4, kM = kUnit / 8, kPieces = kUnits * kM;  // a lane's units; matrix instructions of one; 16-byte pieces of x of a token
+    constexpr uint32_t kCodeBytes = kNT * 16 * kUnits * 16, kSlot = kCodeBytes + kNT * 16 * kUnits * 4, kAhead = kFewAhead, kRing = kAhead + 1;
+    constexpr uint32_t kCodeLoads = kCodeBytes / 1024, kScaleLoads = kNT * kUnits / 4, kLoads = kCodeLoads + kScaleLoads + kX;
     extern __shared__ char lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t i = lane & 15u, g = lane >> 4;
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
     const auto weight_row = [&](uint32_t r) {
         return a.gated ? min(row0 + r % 16u, a.out_cols - 1u) + r / 16u * a.out_cols : min(row0 + r, a.out_cols - 1u);
     };
-    const uint32_t units = a.cols / kUnit, stages = (units + 7u) / 8u;
+    const uint32_t units = a.cols / kUnit, stages = (units + kUnits - 1u) / kUnits;
     const char* const words = a.words + at.expert * a.expert_bytes + row0 * a.row_bytes;
     const uint32_t scale_row0 = a.block_rows ? row0 / a.block_rows : 0u;
     const uint64_t scale_at = (at.expert * a.scale_expert + scale_row0 * a.scale_row) * grid.scale_size + (reinterpret_cast<uintptr_t>(a.scales) & 3u);
@@ -61,43 +61,50 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
         return scale_base + (a.block_rows ? (weight_row(r) / a.block_rows - scale_row0) * static_cast<uint32_t>(a.scale_row * grid.scale_size) : 0u);
     };
 
-    // Where a lane's pieces come from.  Codes: place p of row r holds unit p ^ (r / 2 % 8); scales: place u of row r that of unit u; x: place p of
-    // token v piece p ^ (v % 16).  Positions past the last are the last again.
-    uint32_t code_from[2 * kNT], code_unit[2 * kNT], scale_from[2 * kNT], x_piece[kX], x_to[kX], x_from[kX];
+    // Where a lane's pieces come from.  Codes: place p of row r holds unit p ^ (r / 2 % 8), of half lines p ^ (r / 4 % 4); scales: place u of row
+    // r that of unit u; x: place p of token v piece p ^ (v % 16), of fewer than 16 pieces p ^ (v / 2 % 8): sixteen lanes' reads fall on
+    // different banks.  Positions past the last are the last again.
+    const auto code_turn = [](uint32_t r) { return kUnits == 8 ? (r >> 1) & 7u : (r >> 2) & 3u; };
+    const auto x_turn = [](uint32_t v) { return kPieces >= 16 ? v & 15u : (v >> 1) & 7u; };
+    uint32_t code_from[kCodeLoads], code_unit[kCodeLoads], scale_from[kScaleLoads], x_to[kX], x_from[kX];
     const uint32_t x_row0 = a.row_of ? 0u : at.first;
     const char* const x = a.x + x_row0 * a.x_stride * 2u;
 #pragma unroll
-    for (uint32_t q = 0; q < 2 * kNT; q++) {
-        const uint32_t r = q * 8u + lane / 8u;
-        code_unit[q] = (lane & 7u) ^ ((r >> 1) & 7u);
+    for (uint32_t q = 0; q < kCodeLoads; q++) {
+        const uint32_t r = (q * 64u + lane) / kUnits;
+        code_unit[q] = (lane % kUnits) ^ code_turn(r);
         code_from[q] = (weight_row(r) - row0) * static_cast<uint32_t>(a.row_bytes);
-        scale_from[q] = scale_row_of(r);
     }
 #pragma unroll
+    for (uint32_t q = 0; q < kScaleLoads; q++) scale_from[q] = scale_row_of((q * 64u + lane) / kUnits);
+    const auto x_token = [&](uint32_t q, uint32_t lane) { return min((x_to[q] / 16u + lane) / kPieces, tokens - 1u); };
+    const auto x_piece = [&](uint32_t q, uint32_t lane) { return lane % kPieces ^ x_turn(x_token(q, lane)); };
+#pragma unroll
     for (uint32_t q = 0; q < kX; q++) {
-        const uint32_t l = min(q * groups + group, grid.x_bytes / 1024u - 1u);  // (some waves may bring the last one together)
-        const uint32_t pl = l * 64u + lane, v = min(pl / kPieces, tokens - 1u);
-        x_to[q] = l * 1024u;
-        x_piece[q] = (pl % kPieces) ^ (v & 15u);
-        x_from[q] = (row_of_position(a, at.first + v) - x_row0) * static_cast<uint32_t>(a.x_stride * 2u) + x_piece[q] * 16u;
+        x_to[q] = min(q * groups + group, grid.x_bytes / 1024u - 1u) * 1024u;  // (some waves may bring the last one together)
+        x_from[q] = (row_of_position(a, at.first + x_token(q, lane)) - x_row0) * static_cast<uint32_t>(a.x_stride * 2u) + x_piece(q, lane) * 16u;
     }
     const auto load = [&](uint32_t stage, uint32_t slot) {
         char* const to = mine + slot * kSlot;
-        const uint32_t unit0 = stage * 8u;
+        const uint32_t unit0 = stage * kUnits;
 #pragma unroll
-        for (uint32_t q = 0; q < 2 * kNT; q++)
+        for (uint32_t q = 0; q < kCodeLoads; q++)
             __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(words + (code_from[q] + min(unit0 + code_unit[q], units - 1u) * 16u)),
-                                             CQ_LDS_PTR(to + q * 1024u), 16, 0, 2 /* nt */);
-        const uint32_t block = grid.block_of(min(unit0 + (lane & 7u), units - 1u)) * grid.scale_col_bytes;
+                                             CQ_LDS_PTR(to + q * 1024u), 16, 0, kUnits == 8 ? 2 : 0 /* whole lines past the caches */);
+        const uint32_t block = grid.block_of(min(unit0 + lane % kUnits, units - 1u)) * grid.scale_col_bytes;
 #pragma unroll
-        for (uint32_t q = 0; q < 2 * kNT; q++)
+        for (uint32_t q = 0; q < kScaleLoads; q++)
             __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(scales + ((scale_from[q] + block) & ~3u)), CQ_LDS_PTR(to + kCodeBytes + q * 256u), 4, 0, 0);
         const char* const from = x + static_cast<uint64_t>(unit0) * (kM * 16u);
         const uint32_t pieces = (units - unit0) * kM;
 #pragma unroll
         for (uint32_t q = 0; q < kX; q++) {
             const char* p = from + x_from[q];
-            if (pieces < kPieces && x_piece[q] >= pieces) p = kZeros;  // columns past the row's end
+            if (pieces < kPieces) {  // columns past the row's end; the piece is worked out again here, so that no register holds it in the loop
+                uint32_t again = lane;
+                asm volatile("" : "+v"(again));
+                if (x_piece(q, again) >= pieces) p = kZeros;
+            }
             __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(p), CQ_LDS_PTR(x_img + slot * grid.x_bytes + x_to[q]), 16, 0, 0);
         }
     };
@@ -126,54 +133,52 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
         slot = slot == kAhead ? 0 : slot + 1;
         free_slot = free_slot == kAhead ? 0 : free_slot + 1;
         if (stage >= stages) continue;  // a share may have a stage less than others
-        u32x4 w[kNT][2];
-        uint32_t word[kNT][2];
+        u32x4 w[kNT][kQ];
+        uint32_t word[kNT][kQ];
 #pragma unroll
-        for (uint32_t q = 0; q < 2; q++)
+        for (uint32_t q = 0; q < kQ; q++)
 #pragma unroll
-            for (uint32_t t = 0; t < kNT; t++) {
+            for (uint32_t k = 0; k < kNT; k++) {
                 const uint32_t unit = q * 4u + g;
-                word[t][q] = *reinterpret_cast<const uint32_t*>(from + kCodeBytes + t * 512u + i * 32u + unit * 4u);
-                w[t][q] = *reinterpret_cast<const u32x4*>(from + t * 2048u + i * 128u + (unit ^ ((i >> 1) & 7u)) * 16u);
+                word[k][q] = *reinterpret_cast<const uint32_t*>(from + kCodeBytes + ((k * 16u + i) * kUnits + unit) * 4u);
+                w[k][q] = *reinterpret_cast<const u32x4*>(from + ((k * 16u + i) * kUnits + (unit ^ code_turn(i))) * 16u);
             }
-        // everything that a stage's first half needs is asked of LDS at once, the second half's x while the first is worked on
-        u32x4 xv[2][kM][kTT];
-        const auto read_x = [&](uint32_t q) {
+        // x of eight columns' products, asked of LDS kEarly products before they come: for few tokens everything at once
+        constexpr uint32_t kProducts = kQ * kM, kEarly = kTT == 1 ? kProducts : 2;
+        u32x4 xv[kProducts][kTT];
+        const auto read_x = [&](uint32_t k) {
 #pragma unroll
-            for (uint32_t m = 0; m < kM; m++)
-#pragma unroll
-                for (uint32_t t = 0; t < kTT; t++)
-                    xv[q][m][t] = *reinterpret_cast<const u32x4*>(x_now + (column[t] * kPieces + (((q * 4u + g) * kM + m) ^ (column[t] & 15u))) * 16u);
+            for (uint32_t t = 0; t < kTT; t++)
+                xv[k][t] = *reinterpret_cast<const u32x4*>(x_now + (column[t] * kPieces + ((((k / kM) * 4u + g) * kM + k % kM) ^ x_turn(column[t]))) * 16u);
         };
-        read_x(0);
-        if (kTT == 1) read_x(1);
+#pragma unroll
+        for (uint32_t k = 0; k < kEarly; k++) read_x(k);
         __builtin_amdgcn_sched_barrier(0);
-        float scale[kNT][2];
+        float scale[kNT][kQ];
         bool mine_short = true;
 #pragma unroll
-        for (uint32_t q = 0; q < 2; q++) {
-            const uint32_t block = grid.block_of(min(stage * 8u + q * 4u + g, units - 1u)) * grid.scale_col_bytes;
+        for (uint32_t q = 0; q < kQ; q++) {
+            const uint32_t block = grid.block_of(min(stage * kUnits + q * 4u + g, units - 1u)) * grid.scale_col_bytes;
 #pragma unroll
-            for (uint32_t t = 0; t < kNT; t++) {
-                scale[t][q] = dev::round_to<kF>(scale_of(masks, word[t][q], scale_of_row[t] + block));
-                mine_short = mine_short && takes_short<kF, kCode>(scale[t][q]);
+            for (uint32_t k = 0; k < kNT; k++) {
+                scale[k][q] = dev::round_to<kF>(scale_of(masks, word[k][q], scale_of_row[k] + block));
+                mine_short = mine_short && takes_short<kF, kCode>(scale[k][q]);
             }
         }
-        const bool whole = stage * 8u + 8u <= units;
-        const bool plain = whole && (kCode > 8 || __builtin_amdgcn_ballot_w64(!mine_short) == 0);
+        const bool plain = (stage + 1u) * kUnits <= units && (kCode > 8 || __builtin_amdgcn_ballot_w64(!mine_short) == 0);
         const auto multiply = [&](auto ordinary) {
-            if (kTT > 1) read_x(1);
 #pragma unroll
-            for (uint32_t q = 0; q < 2; q++)
+            for (uint32_t k = 0; k < kProducts; k++) {
+                if (k + kEarly < kProducts) read_x(k + kEarly);
+                const uint32_t q = k / kM, m = k % kM;
 #pragma unroll
-                for (uint32_t m = 0; m < kM; m++)
+                for (uint32_t n_ = 0; n_ < kNT; n_++) {
+                    u32x4 v = unit_slice<kF, kCode, decltype(ordinary)::value>(w[n_][q], m, scale[n_][q]);
+                    if (!decltype(ordinary)::value && stage * kUnits + q * 4u + g >= units) v = u32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (uint32_t k = 0; k < kNT; k++) {
-                        u32x4 v = unit_slice<kF, kCode, decltype(ordinary)::value>(w[k][q], m, scale[k][q]);
-                        if (!decltype(ordinary)::value && stage * 8u + q * 4u + g >= units) v = u32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (uint32_t t = 0; t < kTT; t++) acc[k][t][m & 1] = mfma<kF>(v, xv[q][m][t], acc[k][t][m & 1]);
-                    }
+                    for (uint32_t t = 0; t < kTT; t++) acc[n_][t][k & 1] = mfma<kF>(v, xv[k][t], acc[n_][t][k & 1]);
+                }
+            }
         };
         if (plain)
             multiply(std::true_type{});

@@ -82,14 +82,19 @@ struct TilesGrid {
 
 // The kernel of a decode step (cq_kernels_matmul_few.hip): stages that a wave's loads are ahead.
 constexpr uint32_t kFewAhead = 1;
+// 16-byte units of codes of a row in a stage: a line, or half of one where x of a whole one is so large that a compute unit holds one workgroup
+// (32 positions [4096, 14336] 4 bits 35.5 -> 22.0 us, one position [8192, 8192] 2 bits 12.4 -> 10.0; lines of 4 and 8 bits for up to 16
+// positions stay whole: [28672, 8192] 4 bits, one position, 36.6 us and 40.8 in halves).
+__host__ __device__ constexpr uint32_t few_units(uint32_t tokens_log2, uint32_t bits) { return tokens_log2 <= 4 && bits > 2 ? 8 : 4; }
 
 struct FewShape {
-    uint32_t groups, tokens_log2, shares_log2;  // groups of 16 rows of a wave; positions of a tile; shares of a row's columns
-    uint32_t x_bytes;                           // of a stage: whole loads of 1 KiB
+    uint32_t groups, tokens_log2, shares_log2, units;  // groups of 16 rows of a wave; positions of a tile; shares of a row's columns; units of a stage
+    uint32_t x_bytes;                                  // of a stage: whole loads of 1 KiB
 
     uint32_t x_loads() const { return (x_bytes / 1024 + (8 >> shares_log2) - 1) / (8 >> shares_log2); }  // of a wave
     uint32_t lds() const {
-        const uint32_t images = (kFewAhead + 1) * ((x_bytes << shares_log2) + 8 * groups * 2560), sums = 8 * groups * (tokens_log2 == 5 ? 2048 : 1024);
+        const uint32_t images = (kFewAhead + 1) * ((x_bytes << shares_log2) + 8 * groups * 16 * units * 20);
+        const uint32_t sums = 8 * groups * (tokens_log2 == 5 ? 2048u : 1024u);
         return images > sums ? images : sums;
     }
 };
@@ -166,24 +171,28 @@ inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows,
 // The kernel of a decode step, where a unit of 16 bytes of codes has one scale: as many shares of the columns as leave all workgroups
 // running at once.
 inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
-    const uint32_t unit = 128 / a.bits, stages = (a.cols / unit + 7) / 8;
+    const uint32_t unit = 128 / a.bits;
     if (a.block_cols % unit) return;
     for (uint32_t tokens_log2 = 3; tokens_log2 <= 5; tokens_log2++) {
         FewShape c{};
-        const uint32_t most = 1u << tokens_log2, tokens = a.positions < most ? a.positions : most;
-        if (a.offsets == nullptr && a.positions > most) continue;  // the weights would be read again for every tile
+        const uint32_t most = 1u << tokens_log2, tokens = a.positions < most ? a.positions : most, units = few_units(tokens_log2, a.bits);
+        const uint32_t stages = (a.cols / unit + units - 1) / units;
+        // every further tile of positions reads the weights again: of experts as many have one more as one less
+        if (a.positions > (a.offsets ? 1.5 * most * a.experts : most)) continue;
         c.tokens_log2 = tokens_log2;
-        c.x_bytes = (tokens * (2048 / a.bits) + 1023) / 1024 * 1024;
+        c.units = units;
+        c.x_bytes = (tokens * (units * unit * 2) + 1023) / 1024 * 1024;
         c.groups = a.gated ? 2 : 1;
         const double waves = (a.out_cols + 15) / 16 * likely_tiles(a, most);
         for (c.shares_log2 = 3; c.shares_log2 > 0; c.shares_log2--) {
-            const uint32_t fit = c.lds() ? 160 * 1024 / c.lds() : 2;
+            const uint32_t fit = 160 * 1024 / c.lds();
             if ((1u << c.shares_log2) <= stages && c.x_loads() <= 8 && waves * (1u << c.shares_log2) / 8 <= 256.0 * (fit < 2 ? fit : 2)) break;
         }
         if (c.lds() > 160 * 1024 || c.x_loads() > 8 || most_tiles(a, tokens_log2) > 65535) continue;
-        const double half = (0.45 + unit * 8 * (0.0025 + (tokens_log2 == 5 ? 0.0022 : 0.0)) + (tokens_log2 == 4 ? 0.15 : 0.0)) * (c.groups == 2 ? 1.7 : 1.0);
+        const double columns = units * unit, round = tokens_log2 == 3 ? 0.45 + 0.0025 * columns : tokens_log2 == 4 ? 0.6 + 0.0025 * columns : 0.35 + 0.0055 * columns;
+        const double half = round * (c.groups == 2 ? 1.7 : 1.0);
         const double rounds = static_cast<double>((stages + (1u << c.shares_log2) - 1) >> c.shares_log2);
-        const double us = 3.0 + rounds * rounds_us(waves * (1u << c.shares_log2) / 8, half, 1.85 * half);
+        const double us = 3.0 + rounds * rounds_us(waves * (1u << c.shares_log2) / 8, half, (tokens_log2 == 5 ? 1.5 : 1.85) * half);
         if (us < best->us) {
             best->few = true;
             best->few_shape = c;
