@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     constexpr uint32_t kWaves = kWN * kWT, kRows = Traits::kRows, kTokens = Traits::kTokens, kTokensLog2 = __builtin_ctz(kTokens);
     constexpr uint32_t kBits = bits_of(kCode), kSteps = kLine / 8 / kBits;  // steps of a chunk: 128 bytes of codes are 1024 / kBits columns
     constexpr uint32_t kUnits = kLine / 16, kTurn = 256 / kLine;            // 16-byte pieces of a line; rows side by side in the 256 bytes of all banks
-    static_assert(kSteps >= 1, "whole steps");
+    static_assert(kSteps >= 1 && kWT == 1, "whole steps; all waves have the same positions");
     constexpr uint32_t kXBytes = Traits::kXBytes, kCodeBytes = Traits::kCodeBytes;
     constexpr uint32_t kXLoads = kTokens / 8 / kWaves, kCodeLoads = kCodeBytes / 1024 / kWaves, kScaleLoads = kRows * 2 / 64 / kWaves;
     static_assert(kXLoads * 8 * kWaves == kTokens && kCodeLoads * 1024 * kWaves == kCodeBytes && kScaleLoads * 32 * kWaves == kRows, "whole loads of 1 KiB");
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     Codes<kCode> codes[kNT];
     float rounded_scale[kNT];
     bool all_short = true;
-    const auto fetch = [&](uint32_t in) {  // codes and scales of a step, to be dequantized
+    const auto fetch = [&](uint32_t in) __attribute__((always_inline)) {  // codes and scales of a step, to be dequantized
         bool mine = true;
         const uint32_t block = scale_block(first_step + in, h);
 #pragma unroll
@@ -178,13 +178,13 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         }
         all_short = kCode > 8 || __builtin_amdgcn_ballot_w64(!mine) == 0;
     };
-    const auto dequantize = [&](uint32_t m) {
+    const auto dequantize = [&](uint32_t m) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t n = 0; n < kNT; n++) w[n][m] = slice<kF, kCode, true>(codes[n], m, rounded_scale[n]);
     };
     // What the short way does not do: scales that are not ordinary; and where the row ends in the middle of a step, whose second half counts
     // nothing.
-    const auto amend = [&](uint32_t step) {
+    const auto amend = [&](uint32_t step) __attribute__((always_inline)) {
         if (kCode <= 8 && !all_short) {
 #pragma unroll
             for (uint32_t n = 0; n < kNT; n++)
@@ -198,9 +198,9 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
                 for (uint32_t m = 0; m < 4; m++) w[n][m] = h == 1 ? u32x4{0, 0, 0, 0} : w[n][m];
         }
     };
-    const auto read_x = [&](uint32_t from, uint32_t m, u32x4* xv) {
+    const auto read_x = [&](auto tiles, uint32_t from, uint32_t m, u32x4* xv) __attribute__((always_inline)) {
 #pragma unroll
-        for (uint32_t t = 0; t < kTT; t++) {
+        for (uint32_t t = 0; t < decltype(tiles)::value; t++) {
             const uint32_t row = (wave_t * kTT + t) * 32u + i;
             xv[t] = *reinterpret_cast<const u32x4*>(x_img + from * kXBytes + row * 128u + ((h * 4u + m) ^ ((row >> 1) & 7u)) * 16u);
         }
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         asm volatile("" ::: "memory");
     };
     bool codes_after_x = false;  // a chunk's loads were issued behind the x that an iteration waits for, and are not wanted yet
-    const auto issue = [&](uint32_t in) {
+    const auto issue = [&](uint32_t in) __attribute__((always_inline)) {
         if (in + 3 < steps) load_scales(first_step + in + 3, (in + 3) % Traits::kScaleRing);
         if (in + kXAhead < steps) load_x(first_step + in + kXAhead, (in + kXAhead) % kXRing);
         const uint32_t chunk = (in + 1) / kSteps - 1 + kCodeRing;
@@ -239,41 +239,51 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
         for (uint32_t m = 0; m < 4; m++) dequantize(m);
         amend(first_step);
     }
+    // The steps, for all tiles of 32 positions or for the first half of them, where an expert's last positions need no more (64 experts with 25
+    // positions each, [10707, 608] 4 bits, 149 -> 133 us; a version for three of four would leave the sums no registers).
+    const auto run = [&](auto tiles) __attribute__((always_inline)) {
+        constexpr uint32_t kHave = decltype(tiles)::value;
 #pragma unroll 1
-    for (uint32_t in = 0; in < rounds; in++) {
-        static_assert(kXAhead == 1, "the x of an iteration is what the one before asked for");
-        if (kCodeLead >= 2 && codes_after_x)
-            begin(std::integral_constant<int, kCodeLoads>{});
-        else
-            begin(std::integral_constant<int, 0>{});
-        codes_after_x = false;
-        if (kWK > 1 && in >= steps) continue;  // waves along the columns may have a chunk less than others
-        const uint32_t next = min(in + 1u, steps - 1u);
-        read_x(in % kXRing, 0, xv[0]);
-        fetch(next);
-        issue(in);
-        // the next step's weights take the places of this one's as they are used up
+        for (uint32_t in = 0; in < rounds; in++) {
+            static_assert(kXAhead == 1, "the x of an iteration is what the one before asked for");
+            if (kCodeLead >= 2 && codes_after_x)
+                begin(std::integral_constant<int, kCodeLoads>{});
+            else
+                begin(std::integral_constant<int, 0>{});
+            codes_after_x = false;
+            if (kWK > 1 && in >= steps) continue;  // waves along the columns may have a chunk less than others
+            const uint32_t next = min(in + 1u, steps - 1u);
+            read_x(tiles, in % kXRing, 0, xv[0]);
+            fetch(next);
+            issue(in);
+            // the next step's weights take the places of this one's as they are used up
 #pragma unroll
-        for (uint32_t m = 0; m < 4; m++) {
-            if (m < 3) read_x(in % kXRing, m + 1, xv[(m + 1) & 1]);
+            for (uint32_t m = 0; m < 4; m++) {
+                if (m < 3) read_x(tiles, in % kXRing, m + 1, xv[(m + 1) & 1]);
 #pragma unroll
-            for (uint32_t t = 0; t < kTT; t++)
+                for (uint32_t t = 0; t < kHave; t++)
 #pragma unroll
-                for (uint32_t n = 0; n < kNT; n++) acc[n][t] = mfma<kF>(w[n][m], xv[m & 1][t], acc[n][t]);
-            dequantize(m);
-        }
-        if constexpr (kTT >= 4 && kCode != 8) {
-            // A matrix instruction keeps its unit busy for 32 cycles, in which the wave may issue seven others; x of the next products comes in front of the
-            // next weights ([28672, 8192] 4 bits, 4096 positions 1.96 -> 1.88 ms; the 8-bit fields have no registers left for it).
-#pragma unroll
-            for (uint32_t k = 0; k < 4 * kNT * kTT; k++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-                if (k % (kNT * kTT) < kTT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    for (uint32_t n = 0; n < kNT; n++) acc[n][t] = mfma<kF>(w[n][m], xv[m & 1][t], acc[n][t]);
+                dequantize(m);
             }
+            if constexpr (kHave >= 4 && kCode != 8) {
+                // A matrix instruction keeps its unit busy for 32 cycles, in which the wave may issue seven others; x of the next products comes in front of
+                // the next weights ([28672, 8192] 4 bits, 4096 positions 1.96 -> 1.88 ms; the 8-bit fields have no registers left for it).
+#pragma unroll
+                for (uint32_t k = 0; k < 4 * kNT * kHave; k++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+                    if (k % (kNT * kHave) < kHave) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+            }
+            amend(first_step + next);
         }
-        amend(first_step + next);
-    }
+    };
+    const uint32_t have = min((positions + 31u) / 32u, static_cast<uint32_t>(kTT));
+    if (kTT == 1 || have > kTT / 2u)
+        run(std::integral_constant<int, kTT>{});
+    else if constexpr (kTT > 1)
+        run(std::integral_constant<int, kTT / 2>{});
 
     // Lane (i, h) holds position i of each 32, rows 8 q + 4 h + 0 .. 3 of each 32.  They go through the wave's own part of LDS, 32 positions at a
     // time, so that a lane ends up with eight columns side by side, the waves along the columns meet, and the activation stands in the
@@ -292,6 +302,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     __syncthreads();
 #pragma unroll
     for (uint32_t t = 0; t < kTT; t++) {
+        if (kTT > 1 && t >= have) break;
         if (t != 0 && kWK > 1) __syncthreads();
 #pragma unroll
         for (uint32_t n = 0; n < kNT; n++)
