@@ -32,27 +32,43 @@ struct TilesTraits {
 // n / each as 2 n ceil(2^31 / each) / 2^32, for n < 2^27 and each < 32; 0 for each = 0, one scale for everything
 inline uint32_t magic_of(uint32_t each) { return each ? (0x80000000u + each - 1u) / each : 0u; }
 
+// Tiles of `size` positions that a launch may be taken to have: the experts' sizes lie in device memory, and as many end in half a tile as in a whole one.
+inline double likely_tiles(const MatmulArgs& a, uint32_t size) {
+    if (!a.offsets) return static_cast<double>((a.positions + static_cast<uint64_t>(size) - 1) / size);
+    const double experts = a.experts < a.positions ? a.experts : a.positions, each = a.positions / experts;
+    return experts * (each > 0.5 * size ? each / size + 0.5 : 1.0);
+}
+
 struct TilesGrid {
     uint32_t n_tiles, p_tiles, splits, pitch;  // pitch: floats of a position's sums in the workspace
     uint32_t scale_size, scale_col_bytes, block_magic;
 
-    // Workgroups go round the dies, which have an L2 each, one by one.  Tiles are dealt out in rectangles of up to kGroup tiles of positions by
-    // up to kChunk of rows, whose workgroups read few rows of x and few of W at a time: rectangle r to die r % kDies, as many to each die
-    // as to any other where that can be had, and the experts' sizes, which the host does not know, spread over all of them (in runs of
-    // tiles the last dies had those that do not exist: 64 experts, 6126 positions 209 -> 204 us).
-    static constexpr uint32_t kDies = 8, kGroup = 4, kChunk = 8;
-    uint32_t group, chunk, rectangles;
+    // Workgroups go round the dies, which have an L2 each, one by one.  Tiles are dealt out in rectangles of `group` tiles of positions by
+    // `chunk` of rows, whose workgroups read few rows of x and few of W at a time: as many to each die as to any other, the same rows to the
+    // same die.  Of experts the host does not know how many tiles there are: a die may have a rectangle more than another.  Where its compute
+    // units do not hold all of its workgroups at once, that is kept to a sixteenth of them, and the next rectangles go one die further on, as the
+    // narrower ones at the rows' end would all come to the same dies (64 experts, 6126 positions, 11 tiles of rows: 204 -> 177 us; of fewer
+    // workgroups the larger rectangles' shared reads count for more: 4 experts of 324 positions, [1360, 11104] 8 bits, 152 us, and 230 in single tiles).
+    static constexpr uint32_t kDies = 8, kSlots = 64, kGroup = 4, kChunk = 8, kParts = 16;
+    uint32_t group, chunk, rectangles, turn = 0;
     cubek_quant::device::FastDivmod by_rectangle, by_chunks, by_group;
 
     TilesGrid(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t splits)
         : n_tiles((a.out_cols + (a.gated ? rows / 2 : rows) - 1) / (a.gated ? rows / 2 : rows)), p_tiles(static_cast<uint32_t>(most_tiles(a, __builtin_ctz(tokens)))),
           splits(splits), pitch(sums_pitch(a)), scale_size(a.param_dtype == CQ_F32 ? 4u : 2u), scale_col_bytes(static_cast<uint32_t>(a.scale_col * scale_size)),
           block_magic(magic_of(a.block_cols / 32u)) {
-        group = p_tiles < kGroup ? p_tiles : kGroup;
-        const uint32_t groups = (p_tiles + group - 1) / group;
-        uint32_t even = kDies;  // chunks come in multiples of this many, so that all rectangles do in multiples of kDies
+        uint32_t area = kGroup * kChunk, widest = kGroup, even = kDies;  // chunks come in multiples of `even`, so that all rectangles do in multiples of kDies
+        const double likely = likely_tiles(a, tokens) * n_tiles;
+        if (a.offsets && likely * splits > kDies * kSlots) {
+            const double fits = likely / (kDies * kParts);
+            if (fits < area) area = fits < 1.0 ? 1u : static_cast<uint32_t>(fits);
+            while (widest > area) widest /= 2;
+            even = 1, turn = 1;
+        }
+        group = p_tiles < widest ? p_tiles : widest;
+        const uint32_t groups = (p_tiles + group - 1) / group, most = area / group;
         while (even > 1 && groups % (kDies / even * 2) == 0) even /= 2;
-        uint32_t chunks = ((n_tiles + kChunk - 1) / kChunk + even - 1) / even * even;
+        uint32_t chunks = ((n_tiles + most - 1) / most + even - 1) / even * even;
         if (chunks > n_tiles) chunks = n_tiles;
         chunk = (n_tiles + chunks - 1) / chunks;
         chunks = (n_tiles + chunk - 1) / chunk;
@@ -72,7 +88,7 @@ struct TilesGrid {
     __device__ bool tile(uint32_t block, uint32_t* n, uint32_t* p) const {
         uint32_t round, within, p_group, n_chunk, in_chunk, in_group;
         by_rectangle.div_mod(block / kDies, &round, &within);
-        by_chunks.div_mod(round * kDies + block % kDies, &p_group, &n_chunk);
+        by_chunks.div_mod(round * kDies + (block + round * turn) % kDies, &p_group, &n_chunk);
         by_group.div_mod(within, &in_chunk, &in_group);
         *n = n_chunk * chunk + in_chunk;
         *p = p_group * group + in_group;
@@ -84,7 +100,8 @@ struct TilesGrid {
 constexpr uint32_t kFewAhead = 1;
 // 16-byte units of codes of a row in a stage: a line, or half of one where x of a whole one is so large that a compute unit holds one workgroup
 // (32 positions [4096, 14336] 4 bits 35.5 -> 22.0 us, one position [8192, 8192] 2 bits 12.4 -> 10.0; lines of 4 and 8 bits for up to 16
-// positions stay whole: [28672, 8192] 4 bits, one position, 36.6 us and 40.8 in halves).
+// positions stay whole: [28672, 8192] 4 bits, one position, 36.6 us and 40.8 in halves; rows of few stages take the halves of 32 positions:
+// 2 positions, [6376, 576] 4 bits gated, 8.7 us and 11.1 in whole lines).
 __host__ __device__ constexpr uint32_t few_units(uint32_t tokens_log2, uint32_t bits) { return tokens_log2 <= 4 && bits > 2 ? 8 : 4; }
 
 struct FewShape {
@@ -137,13 +154,6 @@ struct MatmulChoice {
     TilesChoice tiles{TilesShape::k256x128, 1};
     double us = 1e30;
 };
-
-// Workgroups that a launch may be taken to have: the experts' sizes lie in device memory, and as many end in half a tile as in a whole one.
-inline double likely_tiles(const MatmulArgs& a, uint32_t size) {
-    if (!a.offsets) return static_cast<double>((a.positions + static_cast<uint64_t>(size) - 1) / size);
-    const double experts = a.experts < a.positions ? a.experts : a.positions, each = a.positions / experts;
-    return experts * (each > 0.5 * size ? each / size + 0.5 : 1.0);
-}
 
 // What `workgroups` take for a round of steps that takes `half` with one workgroup on a compute unit and `full` with two.
 inline double rounds_us(double workgroups, double half, double full) {
