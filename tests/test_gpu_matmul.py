@@ -171,6 +171,48 @@ def test_infinities_and_nan_stay_in_their_token(oracle, tokens):
             Product(wide(x), w).check(wide(y.cpu()), cols)
 
 
+# tokens, rows of W, columns, with a workspace: few tokens by shares of a row; each shape of tile whole, and with its columns shared out
+LARGER = [(12, 260, 2112, True), (30, 400, 1056, True), (31, 972, 7008, True), (44, 70, 96, True), (88, 34, 3584, True), (61, 40, 4416, True),
+          (300, 700, 4128, True), (700, 1000, 2848, True), (668, 4564, 96, True), (1100, 1040, 1024, False), (4275, 928, 1984, False)]
+
+
+@pytest.mark.parametrize("elem", [BF16, F16], ids=lambda e: e.name)
+@pytest.mark.parametrize("which", range(len(LARGER)))
+def test_larger_products(oracle, which, elem):
+    tokens, rows, cols, with_workspace = LARGER[which]
+    value, store, block = [(V.Q4S, U32, [32]), (V.Q8S, U32, [32]), (V.E4M3, NATIVE, None), (V.Q2S, U32, [32])][(which + (elem == F16)) % 4]
+    rng, gated = np.random.default_rng(which), which % 3 == 1
+    scheme = scheme_of(value, block, 0, store)
+    codes, scales = random_weight(rng, scheme, (rows, cols))
+    x, bias = floats(rng, (tokens, cols), elem), floats(rng, (rows,), elem)
+    gb = bias.cuda()
+    y = run_matmul(on_gpu(codes), scales.cuda(), scheme, x.cuda(), elem, elem, Epilogue(Activation.Silu, gated, bias=h(gb)), with_workspace=with_workspace)
+    w = dequantized(oracle, codes, scales, (rows, cols), elem, scheme)
+    Product(wide(x), w, Activation.Silu, gated, wide(bias), y_elem=elem).check(wide(y.cpu()))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("sizes,rows", [([0, 1, 64, 65, 128, 129, 0, 300, 32, 33, 96, 500, 7, 200, 256, 189], 2050), ([100, 0, 40] * 13 + [400], 1300)])
+def test_groups_of_larger_tiles(oracle, sizes, rows, gated):
+    """Tiles that are full, at most half full and hardly begun, on grids of more workgroups than run at once."""
+    import torch
+
+    rng = np.random.default_rng(rows)
+    scheme = scheme_of(V.Q8S if gated else V.Q4S, [32])
+    e, cols, positions, elem = len(sizes), 96, sum(sizes), F16 if gated else BF16
+    n = rows // 2 if gated else rows
+    codes, scales = random_weight(rng, scheme, (e, rows, cols))
+    x = floats(rng, (positions, cols), elem)
+    at = offsets_of(sizes)
+    gc, gs, gx, go = on_gpu(codes), scales.cuda(), x.cuda(), torch.from_numpy(at).cuda()
+    y = torch.full((positions, n), 9.0, device="cuda")
+    experts.launch_ref(ComputeClient.current(), h(gc), h(gs), scheme, h(gx), h(go), h(y), elem, F32, epilogue=Epilogue(Activation.Relu, gated))
+    w, got = dequantized(oracle, codes, scales, (e, rows, cols), elem, scheme), wide(y.cpu())
+    for i in range(e):
+        if sizes[i]:
+            Product(wide(x)[at[i]:at[i + 1]], w[i], Activation.Relu, gated).check(got[at[i]:at[i + 1]], i)
+
+
 def test_no_tokens_and_no_columns(oracle):
     import torch
 
