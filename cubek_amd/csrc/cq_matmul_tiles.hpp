@@ -51,6 +51,7 @@ struct TilesGrid {
     // workgroups the larger rectangles' shared reads count for more: 4 experts of 324 positions, [1360, 11104] 8 bits, 152 us, and 230 in single tiles).
     static constexpr uint32_t kDies = 8, kSlots = 64, kGroup = 4, kChunk = 8, kParts = 16;
     uint32_t group, chunk, rectangles, turn = 0;
+    uint32_t group_width, wider_groups, chunk_width, wider_chunks;  // groups and chunks are as even as can be: the first ones a tile wider
     cubek_quant::device::FastDivmod by_rectangle, by_chunks, by_group;
 
     TilesGrid(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t splits)
@@ -65,13 +66,14 @@ struct TilesGrid {
             while (widest > area) widest /= 2;
             even = 1, turn = 1;
         }
-        group = p_tiles < widest ? p_tiles : widest;
-        const uint32_t groups = (p_tiles + group - 1) / group, most = area / group;
+        const uint32_t groups = (p_tiles + widest - 1) / widest;
+        group = a.offsets ? (p_tiles < widest ? p_tiles : widest) : (p_tiles + groups - 1) / groups;
+        group_width = a.offsets ? group : p_tiles / groups, wider_groups = a.offsets ? 0 : p_tiles % groups;
+        const uint32_t most = area / group;
         while (even > 1 && groups % (kDies / even * 2) == 0) even /= 2;
         uint32_t chunks = ((n_tiles + most - 1) / most + even - 1) / even * even;
         if (chunks > n_tiles) chunks = n_tiles;
-        chunk = (n_tiles + chunks - 1) / chunks;
-        chunks = (n_tiles + chunk - 1) / chunk;
+        chunk = (n_tiles + chunks - 1) / chunks, chunk_width = n_tiles / chunks, wider_chunks = n_tiles % chunks;
         rectangles = groups * chunks;
         by_rectangle = cubek_quant::device::FastDivmod(group * chunk);
         by_chunks = cubek_quant::device::FastDivmod(chunks);
@@ -90,9 +92,9 @@ struct TilesGrid {
         by_rectangle.div_mod(block / kDies, &round, &within);
         by_chunks.div_mod(round * kDies + (block + round * turn) % kDies, &p_group, &n_chunk);
         by_group.div_mod(within, &in_chunk, &in_group);
-        *n = n_chunk * chunk + in_chunk;
-        *p = p_group * group + in_group;
-        return *n < n_tiles && *p < p_tiles;
+        *n = n_chunk * chunk_width + min(n_chunk, wider_chunks) + in_chunk;
+        *p = p_group * group_width + min(p_group, wider_groups) + in_group;
+        return in_chunk < chunk_width + (n_chunk < wider_chunks) && in_group < group_width + (p_group < wider_groups) && *p < p_tiles;
     }
 };
 

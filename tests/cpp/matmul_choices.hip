@@ -1,5 +1,6 @@
 // The host's side of the products, walked over random shapes: every choice fits the compute unit's LDS, the loads that a wave may take
 // part in and the workspace it was given, and every tile of a grid is dealt out once, whatever the experts and the shares of the columns.
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <vector>
@@ -51,12 +52,16 @@ int main() {
         static const uint32_t rows[] = {256, 256, 128, 128, 32}, tokens[] = {128, 128, 64, 32, 32};
         const int shape = c.few ? rand() % 5 : static_cast<int>(c.tiles.shape);
         const TilesGrid g(a, rows[shape], tokens[shape], c.few ? 1u << rand() % 5 : c.tiles.splits);
-        const uint32_t each = g.group * g.chunk, chunks = (g.n_tiles + g.chunk - 1) / g.chunk;
+        const uint32_t each = g.group * g.chunk, chunks = (g.n_tiles - g.wider_chunks) / g.chunk_width;
         std::vector<uint8_t> dealt(static_cast<size_t>(g.n_tiles) * g.p_tiles);
         for (uint32_t block = 0; block < g.workgroups(); block++) {  // as TilesGrid::tile divides on the device
             const uint32_t round = block / 8 / each, within = block / 8 % each, r = round * 8 + (block + round * g.turn) % 8;
-            const uint32_t row_tile = r % chunks * g.chunk + within / g.group, tile = r / chunks * g.group + within % g.group;
-            if (row_tile < g.n_tiles && tile < g.p_tiles) dealt[static_cast<size_t>(tile) * g.n_tiles + row_tile]++;
+            const uint32_t n_chunk = r % chunks, p_group = r / chunks, in_chunk = within / g.group, in_group = within % g.group;
+            if (in_chunk >= g.chunk_width + (n_chunk < g.wider_chunks) || in_group >= g.group_width + (p_group < g.wider_groups)) continue;
+            const uint32_t row_tile = n_chunk * g.chunk_width + std::min(n_chunk, g.wider_chunks) + in_chunk;
+            const uint32_t tile = p_group * g.group_width + std::min(p_group, g.wider_groups) + in_group;
+            CHECK(row_tile < g.n_tiles);
+            if (tile < g.p_tiles) dealt[static_cast<size_t>(tile) * g.n_tiles + row_tile]++;
         }
         for (const uint8_t times : dealt) CHECK(times == 1);
     }
