@@ -1,7 +1,7 @@
 // Products with quantized weights for up to 32 positions of an expert (or of the whole product): a decode step.
 //
 // A wave takes 16 or 32 rows of W (gated: 16 and their gated ones) and a share of their columns, in stages of a line of 128 bytes of every
-// row or of half a line (few_units).  Codes, scales and x of a stage come into LDS by direct loads, kAhead stages ahead: codes and scales into
+// row or of half a line (FewShape).  Codes, scales and x of a stage come into LDS by direct loads, kAhead stages ahead: codes and scales into
 // the wave's own part, x into one that the waves of a share have together.  16 x 16 x 32 matrix instructions take lane (i, g)'s eight columns
 // of row i, and the same of token i.  The eight waves of a workgroup are one to eight groups of rows by eight to one shares of the columns; the shares' sums meet
 // in LDS at the end.  Bound by the read of W and the instructions of its dequantization side by side, and in launches of few stages by the
@@ -27,10 +27,10 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     }
 }
 
-// kNT: groups of 16 rows of a wave; kTT: groups of 16 positions; kX: loads of 1 KiB by which a wave takes part in a stage of its share's x.
-template <dev::Float kF, int kCode, int kNT, int kTT, int kX>
+// kNT: groups of 16 rows of a wave; kTT: groups of 16 positions; kUnits: units of a row in a stage; kX: loads of 1 KiB by which a wave takes part in a stage of its share's x.
+template <dev::Float kF, int kCode, int kNT, int kTT, int kUnits, int kX>
 __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid grid) {
-    constexpr uint32_t kBits = bits_of(kCode), kUnit = 128 / kBits, kUnits = few_units(kTT == 1 ? 4 : 5, kBits);  // columns of 16 bytes of codes; of those, in a stage
+    constexpr uint32_t kBits = bits_of(kCode), kUnit = 128 / kBits;  // columns of 16 bytes of codes
     constexpr uint32_t kQ = kUnits / 4, kM = kUnit / 8, kPieces = kUnits * kM;  // a lane's units; matrix instructions of one; 16-byte pieces of x of a token
     constexpr uint32_t kCodeBytes = kNT * 16 * kUnits * 16, kSlot = kCodeBytes + kNT * 16 * kUnits * 4, kAhead = kFewAhead, kRing = kAhead + 1;
     constexpr uint32_t kCodeLoads = kCodeBytes / 1024, kScaleLoads = kNT * kUnits / 4, kLoads = kCodeLoads + kScaleLoads + kX;
@@ -211,29 +211,37 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
     }
 }
 
-template <dev::Float kF, int kCode, int kNT, int kTT, int kX>
+template <dev::Float kF, int kCode, int kNT, int kTT, int kUnits, int kX>
 hipError_t launch_few(hipStream_t s, const MatmulArgs& a, const FewShape& c) {
     const uint32_t columns = (8u >> c.shares_log2) * (a.gated ? 8u : 16u) * kNT;
     const FewGrid grid(a, c);
-    hipLaunchKernelGGL((matmul_few_kernel<kF, kCode, kNT, kTT, kX>), dim3((a.out_cols + columns - 1) / columns, static_cast<uint32_t>(most_tiles(a, c.tokens_log2))),
+    hipLaunchKernelGGL((matmul_few_kernel<kF, kCode, kNT, kTT, kUnits, kX>), dim3((a.out_cols + columns - 1) / columns, static_cast<uint32_t>(most_tiles(a, c.tokens_log2))),
                        dim3(512), c.lds(), s, a, grid);
     return hipGetLastError();
 }
 
-template <dev::Float kF, int kCode, int kNT, int kTT>
+template <dev::Float kF, int kCode, int kNT, int kTT, int kUnits>
 hipError_t launch_loads(hipStream_t s, const MatmulArgs& a, const FewShape& c) {
     switch (c.x_loads()) {
-        case 1: return launch_few<kF, kCode, kNT, kTT, 1>(s, a, c);
-        case 2: return launch_few<kF, kCode, kNT, kTT, 2>(s, a, c);
-        case 3: case 4: return launch_few<kF, kCode, kNT, kTT, 4>(s, a, c);
-        default: return launch_few<kF, kCode, kNT, kTT, 8>(s, a, c);
+        case 1: return launch_few<kF, kCode, kNT, kTT, kUnits, 1>(s, a, c);
+        case 2: return launch_few<kF, kCode, kNT, kTT, kUnits, 2>(s, a, c);
+        case 3: case 4: return launch_few<kF, kCode, kNT, kTT, kUnits, 4>(s, a, c);
+        default: return launch_few<kF, kCode, kNT, kTT, kUnits, 8>(s, a, c);
     }
+}
+
+template <dev::Float kF, int kCode, int kNT>
+hipError_t launch_units(hipStream_t s, const MatmulArgs& a, const FewShape& c) {
+    if (c.tokens_log2 == 5) return launch_loads<kF, kCode, kNT, 2, 4>(s, a, c);
+    if constexpr (kCode != 2) {
+        if (c.units == 8) return launch_loads<kF, kCode, kNT, 1, 8>(s, a, c);
+    }
+    return launch_loads<kF, kCode, kNT, 1, 4>(s, a, c);
 }
 
 template <dev::Float kF, int kCode>
 hipError_t launch_shape(hipStream_t s, const MatmulArgs& a, const FewShape& c) {
-    if (c.tokens_log2 == 5) return c.groups == 1 ? launch_loads<kF, kCode, 1, 2>(s, a, c) : launch_loads<kF, kCode, 2, 2>(s, a, c);
-    return c.groups == 1 ? launch_loads<kF, kCode, 1, 1>(s, a, c) : launch_loads<kF, kCode, 2, 1>(s, a, c);
+    return c.groups == 1 ? launch_units<kF, kCode, 1>(s, a, c) : launch_units<kF, kCode, 2>(s, a, c);
 }
 
 }  // namespace

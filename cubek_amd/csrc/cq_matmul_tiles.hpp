@@ -100,12 +100,10 @@ struct TilesGrid {
 
 // The kernel of a decode step (cq_kernels_matmul_few.hip): stages that a wave's loads are ahead.
 constexpr uint32_t kFewAhead = 1;
-// 16-byte units of codes of a row in a stage: a line, or half of one where x of a whole one is so large that a compute unit holds one workgroup
-// (32 positions [4096, 14336] 4 bits 35.5 -> 22.0 us, one position [8192, 8192] 2 bits 12.4 -> 10.0; lines of 4 and 8 bits for up to 16
-// positions stay whole: [28672, 8192] 4 bits, one position, 36.6 us and 40.8 in halves; rows of few stages take the halves of 32 positions:
-// 2 positions, [6376, 576] 4 bits gated, 8.7 us and 11.1 in whole lines).
-__host__ __device__ constexpr uint32_t few_units(uint32_t tokens_log2, uint32_t bits) { return tokens_log2 <= 4 && bits > 2 ? 8 : 4; }
-
+// units: of 16 bytes of codes of a row in a stage, 8 for a line or 4 for half of one.  x of 32 positions or of 2-bit codes is so large that a compute
+// unit would hold one workgroup of whole lines (32 positions [4096, 14336] 4 bits 35.5 -> 22.0 us, one position [8192, 8192] 2 bits 12.4 -> 10.0);
+// otherwise halves are for what has few stages or many workgroups of gated rows, whole lines for the rest ([28672, 8192] 4 bits, one
+// position, 36.6 us and 40.8 in halves).
 struct FewShape {
     uint32_t groups, tokens_log2, shares_log2, units;  // groups of 16 rows of a wave; positions of a tile; shares of a row's columns; units of a stage
     uint32_t x_bytes;                                  // of a stage: whole loads of 1 KiB
@@ -163,15 +161,25 @@ inline double rounds_us(double workgroups, double half, double full) {
     return whole * full + (rest <= 0.0 ? 0.0 : rest <= 256.0 ? half : full);
 }
 
+// Experts of unlike sizes have more tiles than as many of the same size, though never more than one that is not full for each.
+inline double uneven_tiles(const MatmulArgs& a, uint32_t size, double more) {
+    const double likely = likely_tiles(a, size);
+    if (!a.offsets) return likely;
+    const double most = static_cast<double>(a.positions / size + (a.experts < a.positions ? a.experts : a.positions));
+    return likely * more < most ? likely * more : most;
+}
+
 inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows, uint32_t tokens, uint32_t along, uint32_t line, double start, double half, double full,
                            MatmulChoice* best) {
     const uint32_t columns = a.gated ? rows / 2 : rows, steps = line / 8 / a.bits, chunks = ((a.cols + 63) / 64 + steps - 1) / steps;
-    const double tiles = (a.out_cols + columns - 1) / columns * likely_tiles(a, tokens);
+    const double row_tiles = (a.out_cols + columns - 1) / columns, tiles = row_tiles * uneven_tiles(a, tokens, 1.0), more = row_tiles * uneven_tiles(a, tokens, 1.25);
+    // weights that only one or two tiles of positions share come from memory, later than out of the L2
+    const double wait = a.offsets ? (rows == 256 ? 1.15 : rows == 32 ? 1.1 : tokens == 32 ? 1.2 : 1.0) : a.positions <= 32 ? 1.3 : 1.0;
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
         if (splits > 1 && (splits * along > chunks || sums_bytes(a, splits) > a.workspace_bytes)) break;
         const double rounds = static_cast<double>((chunks + splits * along - 1) / (splits * along) * steps);
         const double sums = splits > 1 ? 3.0 + 2.0 * static_cast<double>(sums_bytes(a, splits)) / 5e6 : 0.0;  // written and read at 5 TB/s
-        const double us = start + rounds * rounds_us(tiles * splits, half, full) + sums;
+        const double us = (start + rounds * 0.5 * (rounds_us(tiles * splits, half, full) + rounds_us(more * splits, half, full))) * wait + sums;
         if (us < best->us * (splits > 1 ? 0.92 : 1.0)) {  // (workgroups of many rounds do not wait for one another)
             best->few = false;
             best->tiles = TilesChoice{shape, splits};
@@ -180,35 +188,46 @@ inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows,
     }
 }
 
-// The kernel of a decode step, where a unit of 16 bytes of codes has one scale: as many shares of the columns as leave all workgroups
-// running at once.
+// The kernel of a decode step, where a unit of 16 bytes of codes has one scale: `round` is what a stage takes with one workgroup on a compute unit,
+// every further one adds 0.45 of it, as many as LDS holds, up to four.  Fitted to 170 random products of up to 40 positions or experts of up to
+// 400 each, for which every kernel was timed: what the model takes is 1.03 times the fastest in the geometric mean.
 inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
     const uint32_t unit = 128 / a.bits;
     if (a.block_cols % unit) return;
-    for (uint32_t tokens_log2 = 3; tokens_log2 <= 5; tokens_log2++) {
+    const double experts = a.offsets ? (a.experts < a.positions ? a.experts : a.positions) : 1;
+    const double read = experts * a.wide * a.cols * a.bits / 8 / 4.5e6;  // halves of lines at 4.5 TB/s
+    for (uint32_t way = 0; way < 5; way++) {
         FewShape c{};
-        const uint32_t most = 1u << tokens_log2, tokens = a.positions < most ? a.positions : most, units = few_units(tokens_log2, a.bits);
-        const uint32_t stages = (a.cols / unit + units - 1) / units;
+        c.tokens_log2 = way < 3 ? 3 + way : way, c.units = way < 2 ? 8 : 4;  // 8 and 16 positions by whole lines, 32, 8 and 16 by halves
+        if (c.units == 8 && a.bits == 2) continue;
+        const uint32_t most = 1u << c.tokens_log2, tokens = a.positions < most ? a.positions : most, columns = c.units * unit;
+        const uint32_t stages = (a.cols / unit + c.units - 1) / c.units;
         // every further tile of positions reads the weights again: of experts as many have one more as one less
-        if (a.positions > (a.offsets ? 1.5 * most * a.experts : most)) continue;
-        c.tokens_log2 = tokens_log2;
-        c.units = units;
-        c.x_bytes = (tokens * (units * unit * 2) + 1023) / 1024 * 1024;
+        if (a.positions > (a.offsets ? 1.5 * most * a.experts : most) || most_tiles(a, c.tokens_log2) > 65535) continue;
+        c.x_bytes = (tokens * (columns * 2) + 1023) / 1024 * 1024;
         c.groups = a.gated ? 2 : 1;
-        const double waves = (a.out_cols + 15) / 16 * likely_tiles(a, most);
-        for (c.shares_log2 = 3; c.shares_log2 > 0; c.shares_log2--) {
-            const uint32_t fit = 160 * 1024 / c.lds();
-            if ((1u << c.shares_log2) <= stages && c.x_loads() <= 8 && waves * (1u << c.shares_log2) / 8 <= 256.0 * (fit < 2 ? fit : 2)) break;
-        }
-        if (c.lds() > 160 * 1024 || c.x_loads() > 8 || most_tiles(a, tokens_log2) > 65535) continue;
-        const double columns = units * unit, round = tokens_log2 == 3 ? 0.45 + 0.0025 * columns : tokens_log2 == 4 ? 0.6 + 0.0025 * columns : 0.35 + 0.0055 * columns;
-        const double half = round * (c.groups == 2 ? 1.7 : 1.0);
-        const double rounds = static_cast<double>((stages + (1u << c.shares_log2) - 1) >> c.shares_log2);
-        const double us = 3.0 + rounds * rounds_us(waves * (1u << c.shares_log2) / 8, half, (tokens_log2 == 5 ? 1.5 : 1.85) * half);
-        if (us < best->us) {
-            best->few = true;
-            best->few_shape = c;
-            best->us = us;
+        const double round = (c.tokens_log2 == 5 ? 0.35 + 0.0055 * columns : c.units == 8 ? 0.6 + 0.0031 * columns : c.tokens_log2 == 4 ? 0.4 + 0.0022 * columns : 0.45 + 0.0025 * columns) *
+                             (c.groups == 2 ? 1.7 : 1.0);
+        for (c.shares_log2 = 0; c.shares_log2 <= 3; c.shares_log2++) {
+            if (c.shares_log2 && (1u << c.shares_log2) > stages) break;
+            if (c.lds() > 160 * 1024 || c.x_loads() > 8) continue;
+            const uint32_t held = 160 * 1024 / c.lds(), fit = held < 4 ? held : 4;
+            const double stages_each = (stages + (1u << c.shares_log2) - 1) >> c.shares_log2;
+            double us = 0.0;
+            for (const double more : {1.0, 1.25}) {
+                const double workgroups = (a.out_cols + 15) / 16 * uneven_tiles(a, most, more) * (1u << c.shares_log2) / 8;
+                const double whole = static_cast<double>(static_cast<uint64_t>(workgroups / (256.0 * fit))), rest = (workgroups - whole * 256.0 * fit) / 256.0;
+                us += 0.5 * round * (whole * (1.0 + 0.45 * (fit - 1)) + (rest <= 0.0 ? 0.0 : rest <= 1.0 ? 1.0 : rest <= 2.0 ? 1.45 : rest <= 3.0 ? 1.9 : 2.35));
+            }
+            us *= stages_each;
+            if (c.units == 4 && us < read) us = read;
+            if (a.offsets && c.tokens_log2 == 5) us *= 1.1;
+            us += 2.5 + 0.5 * c.shares_log2;
+            if (us < best->us) {
+                best->few = true;
+                best->few_shape = c;
+                best->us = us;
+            }
         }
     }
 }

@@ -45,7 +45,7 @@ int main() {
             const FewShape& f = c.few_shape;
             CHECK(f.lds() <= 160 * 1024 && f.x_loads() <= 8 && f.shares_log2 <= 3 && a.block_cols % (128 / a.bits) == 0);
             CHECK(a.offsets || a.positions <= 1u << f.tokens_log2);
-            CHECK(f.units == few_units(f.tokens_log2, a.bits) && f.x_bytes >= (a.positions < 1u << f.tokens_log2 ? a.positions : 1u << f.tokens_log2) * f.units * (128 / a.bits) * 2);
+            CHECK((f.units == 4 || (f.units == 8 && a.bits > 2 && f.tokens_log2 < 5)) && f.x_bytes >= (a.positions < 1u << f.tokens_log2 ? a.positions : 1u << f.tokens_log2) * f.units * (128 / a.bits) * 2);
         } else {
             CHECK(c.tiles.splits >= 1 && sums_bytes(a, c.tiles.splits) <= a.workspace_bytes);
         }
