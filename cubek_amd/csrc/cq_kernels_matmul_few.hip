@@ -6,6 +6,9 @@
 // of row i, and the same of token i.  The eight waves of a workgroup are one to eight groups of rows by eight to one shares of the columns; the shares' sums meet
 // in LDS at the end.  Bound by the read of W and the instructions of its dequantization side by side, and in launches of few stages by the
 // time from a workgroup's start to its first stage and from its last one to its sums.
+//
+// bf16, 4 bits: one token on [4096, 4096] 5.6 us (a launch 3.5), on [28672, 8192] 35, 16 tokens 37; 32 positions of eight experts [28672, 4096]
+// gated 127 us, 4.6 TB/s, with 2.4 vector instructions per weight; 24 tokens on [28672, 4096] f16 gated 25 us.
 #include <hip/hip_runtime.h>
 
 #include "cq_gemv_operand.hpp"

@@ -102,8 +102,8 @@ struct TilesGrid {
 constexpr uint32_t kFewAhead = 1;
 // units: of 16 bytes of codes of a row in a stage, 8 for a line or 4 for half of one.  x of 32 positions or of 2-bit codes is so large that a compute
 // unit would hold one workgroup of whole lines (32 positions [4096, 14336] 4 bits 35.5 -> 22.0 us, one position [8192, 8192] 2 bits 12.4 -> 10.0);
-// otherwise halves are for what has few stages or many workgroups of gated rows, whole lines for the rest ([28672, 8192] 4 bits, one
-// position, 36.6 us and 40.8 in halves).
+// otherwise halves leave room for more workgroups on a compute unit, whole lines are read faster ([28672, 8192] 4 bits, one position,
+// 36.6 us and 40.8 in halves; eight experts [28672, 4096] gated, 32 positions, 153 us and 127 in halves).
 struct FewShape {
     uint32_t groups, tokens_log2, shares_log2, units;  // groups of 16 rows of a wave; positions of a tile; shares of a row's columns; units of a stage
     uint32_t x_bytes;                                  // of a stage: whole loads of 1 KiB
@@ -190,7 +190,8 @@ inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows,
 
 // The kernel of a decode step, where a unit of 16 bytes of codes has one scale: `round` is what a stage takes with one workgroup on a compute unit,
 // every further one adds 0.45 of it, as many as LDS holds, up to four.  Fitted to 170 random products of up to 40 positions or experts of up to
-// 400 each, for which every kernel was timed: what the model takes is 1.03 times the fastest in the geometric mean.
+// 400 each, for which every kernel was timed: what the model takes is 1.04 times the fastest in the geometric mean (70 positions of 16 experts,
+// [5468, 3936] e2m1 gated 57 us, and 91 by whole lines).
 inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
     const uint32_t unit = 128 / a.bits;
     if (a.block_cols % unit) return;
