@@ -42,8 +42,9 @@ __device__ __forceinline__ float activated(uint32_t activation, float v) {
         case CQ_ACT_RELU: return v < 0.0f ? 0.0f : v;
         case CQ_ACT_SILU: return v * sigmoid(v);
         case CQ_ACT_GELU: {
-            const float half = 0.5f * v * erfc_positive(__builtin_fabsf(v) * 0.70710678118654752f);
-            return v < 0.0f ? half : v - half;
+            // v times the share of it that counts: v less the share's complement would be inf - inf * 0 at infinity
+            const float tail = 0.5f * erfc_positive(__builtin_fabsf(v) * 0.70710678118654752f);
+            return v * (v < 0.0f ? tail : 1.0f - tail);
         }
         // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
         case CQ_ACT_GELU_TANH: return v * sigmoid(1.5957691216057308f * __builtin_fmaf(0.044715f * v * v, v, v));
