@@ -216,9 +216,8 @@ __global__ __launch_bounds__(512) void matmul_few_kernel(MatmulArgs a, FewGrid g
 
 template <dev::Float kF, int kCode, int kNT, int kTT, int kUnits, int kX>
 hipError_t launch_few(hipStream_t s, const MatmulArgs& a, const FewShape& c) {
-    const uint32_t columns = (8u >> c.shares_log2) * (a.gated ? 8u : 16u) * kNT;
     const FewGrid grid(a, c);
-    hipLaunchKernelGGL((matmul_few_kernel<kF, kCode, kNT, kTT, kUnits, kX>), dim3((a.out_cols + columns - 1) / columns, static_cast<uint32_t>(most_tiles(a, c.tokens_log2))),
+    hipLaunchKernelGGL((matmul_few_kernel<kF, kCode, kNT, kTT, kUnits, kX>), dim3(c.workgroups(a), static_cast<uint32_t>(most_tiles(a, c.tokens_log2))),
                        dim3(512), c.lds(), s, a, grid);
     return hipGetLastError();
 }

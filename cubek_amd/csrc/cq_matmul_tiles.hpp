@@ -98,6 +98,17 @@ struct TilesGrid {
     }
 };
 
+// Threads of a launch along one dimension.
+constexpr uint64_t kLaunchThreads = 1ull << 32;
+
+// Whether one launch holds the workgroups of a shape of tile.  Along each side less than half of a rectangle's places are empty, and seven rectangles may be.
+inline bool tiles_fit(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t threads, uint32_t splits) {
+    const uint32_t columns = a.gated ? rows / 2 : rows;
+    const uint64_t most = kLaunchThreads / threads, p_tiles = most_tiles(a, __builtin_ctz(tokens)), n_tiles = (a.out_cols + columns - 1) / columns;
+    if (p_tiles >= most || n_tiles * p_tiles >= most) return false;
+    return 4 * n_tiles * p_tiles + TilesGrid::kDies * TilesGrid::kGroup * TilesGrid::kChunk < most || TilesGrid(a, rows, tokens, splits).workgroups() < most;
+}
+
 // The kernel of a decode step (cq_kernels_matmul_few.hip): stages that a wave's loads are ahead.
 constexpr uint32_t kFewAhead = 1;
 // units: of 16 bytes of codes of a row in a stage, 8 for a line or 4 for half of one.  x of 32 positions or of 2-bit codes is so large that a compute
@@ -109,6 +120,10 @@ struct FewShape {
     uint32_t x_bytes;                                  // of a stage: whole loads of 1 KiB
 
     uint32_t x_loads() const { return (x_bytes / 1024 + (8 >> shares_log2) - 1) / (8 >> shares_log2); }  // of a wave
+    uint32_t workgroups(const MatmulArgs& a) const {  // of a tile of positions
+        const uint32_t columns = (8u >> shares_log2) * (a.gated ? 8u : 16u) * groups;
+        return (a.out_cols + columns - 1) / columns;
+    }
     uint32_t lds() const {
         const uint32_t images = (kFewAhead + 1) * ((x_bytes << shares_log2) + 8 * groups * 16 * units * 20);
         const uint32_t sums = 8 * groups * (tokens_log2 == 5 ? 2048u : 1024u);
@@ -138,7 +153,7 @@ inline bool tiles_take(const MatmulArgs& a) {
     if (a.block_rows && (a.scale_row >= kFits / scale_size / 4 / (rows / a.block_rows + 2) ||
                          a.scale_col >= kFits / scale_size / 4 / (a.cols / a.block_cols + 1)))
         return false;
-    return (a.out_cols / 16ull + 1) * most_tiles(a, 5) < (1ull << 22);  // workgroups of a launch
+    return tiles_fit(a, 256, 128, 256, 1);  // the largest tiles; smaller ones are left out where a launch does not hold theirs
 }
 
 inline uint64_t sums_bytes(const MatmulArgs& a, uint32_t splits) { return splits > 1 ? 4ull * splits * a.positions * TilesGrid::sums_pitch(a) : 0; }
@@ -171,12 +186,14 @@ inline double uneven_tiles(const MatmulArgs& a, uint32_t size, double more) {
 
 inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows, uint32_t tokens, uint32_t along, uint32_t line, double start, double half, double full,
                            MatmulChoice* best) {
+    const uint32_t threads = (rows >= 128 ? 256 : 64) * along;
     const uint32_t columns = a.gated ? rows / 2 : rows, steps = line / 8 / a.bits, chunks = ((a.cols + 63) / 64 + steps - 1) / steps;
     const double row_tiles = (a.out_cols + columns - 1) / columns, tiles = row_tiles * uneven_tiles(a, tokens, 1.0), more = row_tiles * uneven_tiles(a, tokens, 1.25);
     // weights that only one or two tiles of positions share come from memory, later than out of the L2
     const double wait = a.offsets ? (rows == 256 ? 1.15 : rows == 32 ? 1.1 : tokens == 32 ? 1.2 : 1.0) : a.positions <= 32 ? 1.3 : 1.0;
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
         if (splits > 1 && (splits * along > chunks || sums_bytes(a, splits) > a.workspace_bytes)) break;
+        if (!tiles_fit(a, rows, tokens, threads, splits)) break;
         const double rounds = static_cast<double>((chunks + splits * along - 1) / (splits * along) * steps);
         const double sums = splits > 1 ? 3.0 + 2.0 * static_cast<double>(sums_bytes(a, splits)) / 5e6 : 0.0;  // written and read at 5 TB/s
         const double us = (start + rounds * 0.5 * (rounds_us(tiles * splits, half, full) + rounds_us(more * splits, half, full))) * wait + sums;
@@ -212,6 +229,7 @@ inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
         for (c.shares_log2 = 0; c.shares_log2 <= 3; c.shares_log2++) {
             if (c.shares_log2 && (1u << c.shares_log2) > stages) break;
             if (c.lds() > 160 * 1024 || c.x_loads() > 8) continue;
+            if (c.workgroups(a) >= kLaunchThreads / 512) continue;
             const uint32_t held = 160 * 1024 / c.lds(), fit = held < 4 ? held : 4;
             const double stages_each = (stages + (1u << c.shares_log2) - 1) >> c.shares_log2;
             double us = 0.0;
