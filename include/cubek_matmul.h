@@ -76,7 +76,7 @@ size_t cq_experts_workspace_bytes(const cq_tensor* values, const cq_scheme* sche
 
 typedef enum cq_score {
     CQ_SCORE_SOFTMAX = 0, /* over all experts of the token */
-    CQ_SCORE_SIGMOID = 1
+    CQ_SCORE_SIGMOID = 1  /* 0 for logits of -709.7827 and below, such as masks of a type's lowest value: 1 / s passes the range of 64 bits */
 } cq_score;
 
 #define CQ_MAX_EXPERTS 1024
