@@ -175,10 +175,7 @@ size_t workspace_for(cq::MatmulArgs& a, cq_dtype dtype, const cq_scheme* scheme,
     if (a.positions == 0 || a.out_cols == 0 || a.experts == 0 || cols != a.cols || a.positions > kMostExtent) return 0;
     a.dtype = dtype;
     if (scheme->level == CQ_LEVEL_BLOCK) a.block_cols = scheme->block[scheme->block_rank - 1], a.block_rows = 1;
-    a.workspace_bytes = ~0ull;
-    if (!cq::tiles_take(a)) return 0;
-    const cq::MatmulChoice c = cq::matmul_choice(a);
-    return c.few ? 0 : cq::sums_bytes(a, c.tiles.splits);
+    return cq::tiles_take(a) ? cq::room_of(a, cq::choice_within(a, ~0ull)) : 0;
 }
 
 }  // namespace

@@ -185,14 +185,14 @@ inline double uneven_tiles(const MatmulArgs& a, uint32_t size, double more) {
 }
 
 inline void consider_tiles(const MatmulArgs& a, TilesShape shape, uint32_t rows, uint32_t tokens, uint32_t along, uint32_t line, double start, double half, double full,
-                           MatmulChoice* best) {
+                           uint64_t room, MatmulChoice* best) {
     const uint32_t threads = (rows >= 128 ? 256 : 64) * along;
     const uint32_t columns = a.gated ? rows / 2 : rows, steps = line / 8 / a.bits, chunks = ((a.cols + 63) / 64 + steps - 1) / steps;
     const double row_tiles = (a.out_cols + columns - 1) / columns, tiles = row_tiles * uneven_tiles(a, tokens, 1.0), more = row_tiles * uneven_tiles(a, tokens, 1.25);
     // weights that only one or two tiles of positions share come from memory, later than out of the L2
     const double wait = a.offsets ? (rows == 256 ? 1.15 : rows == 32 ? 1.1 : tokens == 32 ? 1.2 : 1.0) : a.positions <= 32 ? 1.3 : 1.0;
     for (uint32_t splits = 1; splits <= 16; splits *= 2) {
-        if (splits > 1 && (splits * along > chunks || sums_bytes(a, splits) > a.workspace_bytes)) break;
+        if (splits > 1 && (splits * along > chunks || sums_bytes(a, splits) > room)) break;
         if (!tiles_fit(a, rows, tokens, threads, splits)) break;
         const double rounds = static_cast<double>((chunks + splits * along - 1) / (splits * along) * steps);
         const double sums = splits > 1 ? 3.0 + 2.0 * static_cast<double>(sums_bytes(a, splits)) / 5e6 : 0.0;  // written and read at 5 TB/s
@@ -251,16 +251,26 @@ inline void consider_few(const MatmulArgs& a, MatmulChoice* best) {
     }
 }
 
-inline MatmulChoice matmul_choice(const MatmulArgs& a) {
+// The fastest within `room` bytes of workspace.
+inline MatmulChoice choice_within(const MatmulArgs& a, uint64_t room) {
     MatmulChoice c;
     consider_few(a, &c);
     // start: a launch without its rounds, from the first loads to the last sums
-    consider_tiles(a, TilesShape::k256x128, 256, 128, 1, 64, 6.0, 1.05, 1.75, &c);
-    consider_tiles(a, TilesShape::k256x128x2, 256, 128, 2, 64, 9.0, 1.85, 3.7, &c);
-    consider_tiles(a, TilesShape::k128x64, 128, 64, 2, 64, 5.0, 1.15, 1.65, &c);
-    consider_tiles(a, TilesShape::k128x32, 128, 32, 2, 64, 4.5, 1.1, 1.75, &c);
-    consider_tiles(a, TilesShape::k32x32, 32, 32, 8, 128, 4.0, 1.15, 2.3, &c);
+    consider_tiles(a, TilesShape::k256x128, 256, 128, 1, 64, 6.0, 1.05, 1.75, room, &c);
+    consider_tiles(a, TilesShape::k256x128x2, 256, 128, 2, 64, 9.0, 1.85, 3.7, room, &c);
+    consider_tiles(a, TilesShape::k128x64, 128, 64, 2, 64, 5.0, 1.15, 1.65, room, &c);
+    consider_tiles(a, TilesShape::k128x32, 128, 32, 2, 64, 4.5, 1.1, 1.75, room, &c);
+    consider_tiles(a, TilesShape::k32x32, 32, 32, 8, 128, 4.0, 1.15, 2.3, room, &c);
     return c;
+}
+
+inline uint64_t room_of(const MatmulArgs& a, const MatmulChoice& c) { return c.few ? 0 : sums_bytes(a, c.tiles.splits); }
+
+// The fastest of all where its sums find room, so that a workspace of the size that was asked for gives the kernel it was asked for: within that room alone
+// another one may come out, as a smaller one in front of it sets another mark.
+inline MatmulChoice matmul_choice(const MatmulArgs& a) {
+    const MatmulChoice c = choice_within(a, ~0ull);
+    return room_of(a, c) <= a.workspace_bytes ? c : choice_within(a, a.workspace_bytes);
 }
 
 hipError_t launch_matmul_finish(hipStream_t s, const MatmulArgs& a, uint32_t splits);

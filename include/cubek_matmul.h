@@ -50,7 +50,7 @@ typedef struct cq_epilogue {
  *   workspace : optional device scratch of cq_matmul_workspace_bytes() bytes, 16-byte aligned; lets products of few tokens and
  *            few rows spread their columns over the GPU.  Without it they are right, and slower.
  * Every weight enters as the value cq_dequantize would store for `dtype`, F(F(scale) * F(code)); sums are f32, their order
- * depends on the shapes alone.  No tokens: nothing is launched.  No columns: sums of nothing. */
+ * depends on the shapes, on strides and alignment, and on whether the workspace has the bytes that were asked for: not on the values.  No tokens: nothing is launched.  No columns: sums of nothing. */
 cq_status cq_matmul_quantized(cq_stream_t stream, const cq_tensor* values, const cq_tensor* params, const cq_scheme* scheme,
                               const cq_tensor* x, const cq_tensor* y, cq_dtype dtype, cq_dtype y_dtype,
                               const cq_epilogue* epilogue, void* workspace, size_t workspace_bytes);

@@ -1,11 +1,14 @@
-"""The limits of the products' kernels, walked over sizes up to a card's memory without a GPU."""
+"""The limits of the products' kernels and the room they ask for, walked over random sizes without a GPU."""
 import os
+
+import pytest
 
 from test_matmul_host import ROOT, run
 
 
-def test_no_size_leaves_the_matrix_cores(tmp_path):
-    program = str(tmp_path / "matmul_limits")
+@pytest.mark.parametrize("name", ["matmul_limits", "matmul_workspace"])
+def test_walk(tmp_path, name):
+    program = str(tmp_path / name)
     run("/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-        os.path.join(ROOT, "tests", "cpp", "matmul_limits.hip"), "-o", program)
+        os.path.join(ROOT, "tests", "cpp", name + ".hip"), "-o", program)
     assert run(program).endswith("ok\n")
