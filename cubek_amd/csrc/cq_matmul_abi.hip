@@ -80,7 +80,7 @@ cq_status read_weights(const cq_tensor* values, const cq_tensor* params, const c
         a->native = scheme->value == CQ_VALUE_E4M3 ? 1u : scheme->value == CQ_VALUE_E5M2 ? 2u : scheme->value == CQ_VALUE_E2M1 ? 3u : 0u;
     a->param_dtype = scheme->param == CQ_PARAM_F32 ? CQ_F32 : (scheme->param == CQ_PARAM_F16 ? CQ_F16 : CQ_BF16);
     if (!params) return CQ_OK;  // a question about sizes
-    if (!tensor_ok(params)) return CQ_ERR_INVALID_ARGUMENT;
+    if (!tensor_ok(params) || !aligned(params->ptr, dtype_size(a->param_dtype))) return CQ_ERR_INVALID_ARGUMENT;
     if (params->elem_size != dtype_size(a->param_dtype)) return CQ_ERR_SHAPE_MISMATCH;
     a->scales = static_cast<const char*>(params->ptr);
     if (scheme->level == CQ_LEVEL_TENSOR) {
@@ -138,7 +138,7 @@ cq_status read_epilogue(const cq_epilogue* epi, const cq_tensor* y, bool experts
 
 // x: [tokens, cols], y: [positions, out_cols]; or both without their first dimension
 cq_status read_activations(const cq_tensor* x, const cq_tensor* y, cq_dtype dtype, cq_dtype y_dtype, bool experts, cq::MatmulArgs* a) {
-    if (!tensor_ok(x) || !tensor_ok(y)) return CQ_ERR_INVALID_ARGUMENT;
+    if (!tensor_ok(x) || !tensor_ok(y) || !aligned(x->ptr, dtype_size(dtype))) return CQ_ERR_INVALID_ARGUMENT;
     if (x->rank > 2 || y->rank != x->rank || (experts && x->rank != 2) || x->elem_size != dtype_size(dtype) || y->elem_size != dtype_size(y_dtype))
         return CQ_ERR_SHAPE_MISMATCH;
     const uint32_t last = x->rank - 1;

@@ -44,7 +44,8 @@ typedef struct cq_epilogue {
  *   values : U32-store [rows, cols / num_quants] or native-store [rows, cols] ([rows, cols / 2] for e2m1), rows may be pitched
  *   params : scales typed scheme->param, [1] per tensor or [rows / block_rows, cols / block_cols] for blocks over the last one or
  *            two dimensions, any strides
- *   x      : [tokens, cols] typed `dtype` (or [cols]: one token), its last dimension contiguous
+ *   x      : [tokens, cols] typed `dtype` (or [cols]: one token), its last dimension contiguous; x and params start on a multiple of their
+ *            elements' size (CQ_ERR_INVALID_ARGUMENT)
  *   y      : [tokens, N] typed `y_dtype` (or [N]), its last dimension contiguous; N as in cq_epilogue
  *   epilogue : NULL for the bare product
  *   workspace : optional device scratch of cq_matmul_workspace_bytes() bytes, 16-byte aligned; lets products of few tokens and
