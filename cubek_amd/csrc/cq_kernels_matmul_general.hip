@@ -35,13 +35,13 @@ __device__ __forceinline__ float decoded(const MatmulArgs& a, uint32_t byte, uin
 // 4 x 4 results of a thread in tiles of 64 positions x 64 columns, steps of 32 columns of W; for up to 16 positions one result of a thread in
 // tiles of 16 x 16, steps of 128 columns: four times the workgroups, and a quarter of the products for nobody.
 template <dev::Float kF, int kEach, int kStep>
-__global__ __launch_bounds__(256) void matmul_general_kernel(MatmulArgs a) {
+__global__ __launch_bounds__(256) void matmul_general_kernel(MatmulArgs a, uint32_t first) {
     constexpr uint32_t kTile = 16 * kEach, kTileLog2 = kEach == 4 ? 6 : 4;
     typedef float vec __attribute__((ext_vector_type(kEach)));
     constexpr uint32_t kPitch = kTile + kEach;  // a thread's numbers are read at once
     __shared__ alignas(16) float xs[kStep][kPitch], gate[kStep][kPitch], up[kStep][kPitch];
     const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const uint32_t n0 = blockIdx.x * kTile;
+    const uint32_t n0 = (first + blockIdx.x) * kTile;
     constexpr uint32_t kLoads = kTile * kStep / 256, kRowsApart = 256 / kStep;
     const uint32_t own_k = threadIdx.x % kStep, own_row = threadIdx.x / kStep;  // a thread brings the same column of kLoads rows in every step
     const Around x(a.x), scales(a.scales);
@@ -139,9 +139,13 @@ template <dev::Float kF, int kEach, int kStep>
 hipError_t launch(hipStream_t s, const MatmulArgs& a) {
     constexpr uint32_t kTile = 16 * kEach;
     const uint64_t tiles = most_tiles(a, kEach == 4 ? 6 : 4);  // beyond what a launch's second dimension holds: some more each
-    hipLaunchKernelGGL((matmul_general_kernel<kF, kEach, kStep>), dim3((a.out_cols + kTile - 1) / kTile, static_cast<uint32_t>(tiles < 65535 ? tiles : 65535)),
-                       dim3(256), 0, s, a);
-    return hipGetLastError();
+    const uint32_t all = (a.out_cols + kTile - 1) / kTile, most = kLaunchThreads / 256 - 1;
+    for (uint32_t first = 0; first < all; first += most) {
+        hipLaunchKernelGGL((matmul_general_kernel<kF, kEach, kStep>), dim3(all - first < most ? all - first : most, static_cast<uint32_t>(tiles < 65535 ? tiles : 65535)),
+                           dim3(256), 0, s, a, first);
+        if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 template <dev::Float kF>

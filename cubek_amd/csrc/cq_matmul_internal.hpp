@@ -7,6 +7,9 @@
 
 namespace cq {
 
+// Threads of a launch along one dimension.
+constexpr uint64_t kLaunchThreads = 1ull << 32;
+
 // y[p] = epilogue(x[row(p)] * dequantize(W[e])^T) for the positions p of expert e; a product without experts is one expert that has all
 // positions.
 struct MatmulArgs {

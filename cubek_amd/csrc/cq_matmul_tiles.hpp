@@ -98,9 +98,6 @@ struct TilesGrid {
     }
 };
 
-// Threads of a launch along one dimension.
-constexpr uint64_t kLaunchThreads = 1ull << 32;
-
 // Whether one launch holds the workgroups of a shape of tile.  Along each side less than half of a rectangle's places are empty, and seven rectangles may be.
 inline bool tiles_fit(const MatmulArgs& a, uint32_t rows, uint32_t tokens, uint32_t threads, uint32_t splits) {
     const uint32_t columns = a.gated ? rows / 2 : rows;
