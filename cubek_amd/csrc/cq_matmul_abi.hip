@@ -15,6 +15,7 @@ cq_status hip_status(hipError_t e) {
 void drop_stale_hip_error() { (void)hipGetLastError(); }
 
 constexpr uint64_t kMostExtent = 0x7fffffffull;  // rows, columns, positions and tokens are 32-bit numbers in the kernels
+constexpr uint64_t kMostRouted = (cq::kLaunchThreads / 1024 - 1) * 64;  // tokens of a routing: 64 of them are a workgroup of 1024 threads
 
 uint32_t dtype_size(int dtype) { return dtype == CQ_F32 ? 4u : 2u; }
 bool valid_dtype(int dtype) { return dtype == CQ_F32 || dtype == CQ_F16 || dtype == CQ_BF16; }
@@ -242,7 +243,7 @@ cq_status cq_experts_quantized(cq_stream_t stream, const cq_tensor* values, cons
 }
 
 size_t cq_route_workspace_bytes(uint64_t tokens, uint64_t experts, uint64_t chosen) {
-    if (experts > CQ_MAX_EXPERTS || chosen > CQ_MAX_CHOSEN || chosen > experts || tokens > kMostExtent) return 0;
+    if (experts > CQ_MAX_EXPERTS || chosen > CQ_MAX_CHOSEN || chosen > experts || tokens > kMostRouted) return 0;
     return cq::route_workspace_bytes(tokens, experts, chosen);
 }
 
@@ -254,7 +255,7 @@ cq_status cq_route(cq_stream_t stream, const cq_tensor* logits, const cq_tensor*
         return CQ_ERR_INVALID_ARGUMENT;
     if (logits->rank != 2 || logits->elem_size != dtype_size(dtype) || weights->rank != 2) return CQ_ERR_SHAPE_MISMATCH;
     const uint64_t tokens = logits->shape[0], num = logits->shape[1], chosen = weights->shape[1];
-    if (num > CQ_MAX_EXPERTS || chosen > CQ_MAX_CHOSEN || tokens > kMostExtent || tokens * chosen > kMostExtent) return CQ_ERR_TOO_LARGE;
+    if (num > CQ_MAX_EXPERTS || chosen > CQ_MAX_CHOSEN || tokens > kMostRouted || tokens * chosen > kMostExtent) return CQ_ERR_TOO_LARGE;
     if (chosen < 1 || chosen > num) return CQ_ERR_INVALID_ARGUMENT;
     for (const cq_tensor* t : {weights, experts, slots}) {
         if (t->rank != 2 || t->elem_size != 4 || t->shape[0] != tokens || t->shape[1] != chosen) return CQ_ERR_SHAPE_MISMATCH;

@@ -92,7 +92,7 @@ typedef enum cq_score {
  *             each pair.  All outputs contiguous.
  *   normalize : a token's weights are divided by their sum (0 stays 0).  A token whose logits are all -infinity gets weights of 0.
  *   workspace : cq_route_workspace_bytes() bytes of device memory, 16-byte aligned (0 for few tokens)
- * tokens * chosen < 2^31.  No tokens: the offsets are set to 0. */
+ * tokens <= 2^28 - 64 and tokens * chosen < 2^31.  No tokens: the offsets are set to 0. */
 cq_status cq_route(cq_stream_t stream, const cq_tensor* logits, const cq_tensor* weights, const cq_tensor* experts,
                    const cq_tensor* offsets, const cq_tensor* rows, const cq_tensor* slots, cq_dtype dtype, cq_score score,
                    uint32_t normalize, void* workspace, size_t workspace_bytes);
