@@ -41,6 +41,9 @@ bool is_contiguous(const cq_tensor* t) {
     return true;
 }
 
+// The stride of dimension d; one entry counts as 0, whatever the tensor says, and keeps no product from a kernel by its alignment.
+uint64_t stride_of(const cq_tensor* t, uint32_t d) { return t->shape[d] > 1 ? t->strides[d] : 0; }
+
 cq_status check_scheme(const cq_scheme* s) {
     if (!s) return CQ_ERR_INVALID_ARGUMENT;
     if (cq_value_size_bits(s->value) == 0 || s->param > CQ_PARAM_BF16 || s->store > CQ_STORE_NATIVE || s->level > CQ_LEVEL_BLOCK || s->reserved != 0)
@@ -63,17 +66,17 @@ cq_status read_weights(const cq_tensor* values, const cq_tensor* params, const c
     const uint32_t lead = experts ? 1u : 0u;
     if (!tensor_ok(values)) return CQ_ERR_INVALID_ARGUMENT;
     if (values->rank != 2 + lead || values->elem_size != (native ? 1u : 4u)) return CQ_ERR_SHAPE_MISMATCH;
-    const uint64_t *const shape = values->shape + lead, *const strides = values->strides + lead;
+    const uint64_t* const shape = values->shape + lead;
     a->bits = cq_value_size_bits(scheme->value);
     const uint64_t nq = cq_scheme_num_quants(scheme);
     if (shape[0] > kMostExtent || shape[1] > kMostExtent / nq || (experts && values->shape[0] > kMostExtent)) return CQ_ERR_TOO_LARGE;
-    if (shape[1] > 1 && strides[1] != 1) return CQ_ERR_NON_CONTIGUOUS;
+    if (shape[1] > 1 && values->strides[lead + 1] != 1) return CQ_ERR_NON_CONTIGUOUS;
     a->words = static_cast<const char*>(values->ptr);
     a->wide = static_cast<uint32_t>(shape[0]);
     a->cols = static_cast<uint32_t>(shape[1] * nq);
     a->experts = experts ? static_cast<uint32_t>(values->shape[0]) : 1u;
-    a->row_bytes = strides[0] * values->elem_size;
-    a->expert_bytes = experts ? values->strides[0] * values->elem_size : 0;
+    a->row_bytes = stride_of(values, lead) * values->elem_size;
+    a->expert_bytes = experts ? stride_of(values, 0) * values->elem_size : 0;
     // i8 bytes are the 8-bit fields of the U32 store, and e2m1 nibbles lie alike in both stores
     if (scheme->value == CQ_VALUE_E2M1_OCP)
         a->native = 3;
@@ -97,9 +100,9 @@ cq_status read_weights(const cq_tensor* values, const cq_tensor* params, const c
     if (a->wide % a->block_rows || a->cols % a->block_cols || params->shape[lead] != a->wide / a->block_rows ||
         params->shape[lead + 1] != a->cols / a->block_cols || (experts && params->shape[0] != a->experts))
         return CQ_ERR_SHAPE_MISMATCH;
-    a->scale_row = params->strides[lead];
-    a->scale_col = params->strides[lead + 1];
-    a->scale_expert = experts ? params->strides[0] : 0;
+    a->scale_row = stride_of(params, lead);
+    a->scale_col = stride_of(params, lead + 1);
+    a->scale_expert = experts ? stride_of(params, 0) : 0;
     return CQ_OK;
 }
 
@@ -153,7 +156,7 @@ cq_status read_activations(const cq_tensor* x, const cq_tensor* y, cq_dtype dtyp
     a->y_dtype = y_dtype;
     a->tokens = static_cast<uint32_t>(tokens);
     a->positions = static_cast<uint32_t>(positions);
-    a->x_stride = last ? x->strides[0] : 0;
+    a->x_stride = last ? stride_of(x, 0) : 0;
     a->y_stride = last ? y->strides[0] : 0;
     return CQ_OK;
 }
