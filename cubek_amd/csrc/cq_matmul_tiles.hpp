@@ -142,11 +142,11 @@ struct FewGrid {
 inline bool tiles_take(const MatmulArgs& a) {
     const auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
     const uint64_t scale_size = a.param_dtype == CQ_F32 ? 4 : 2, rows = 256 + (a.gated ? a.out_cols : 0);
-    const uint64_t x_rows = a.row_of ? a.tokens : 256;
+    const uint64_t x_rows = a.row_of ? a.tokens : 256, row = static_cast<uint64_t>(a.cols) * a.bits / 8;  // (rows of codes may overlap)
     constexpr uint64_t kFits = 0xf0000000ull;
     if (a.dtype == CQ_F32 || a.cols == 0 || a.cols % 32 || static_cast<uint64_t>(a.cols) * a.bits % 128 || a.block_cols % 32) return false;
     if (!on16(a.words) || !on16(a.x) || a.row_bytes % 16 || a.expert_bytes % 16 || a.x_stride % 8) return false;
-    if (a.row_bytes >= kFits / rows || a.x_stride * 2 >= kFits / x_rows) return false;
+    if (a.row_bytes >= (kFits - row) / rows || a.x_stride * 2 >= kFits / x_rows) return false;
     if (a.block_rows && (a.scale_row >= kFits / scale_size / 4 / (rows / a.block_rows + 2) ||
                          a.scale_col >= kFits / scale_size / 4 / (a.cols / a.block_cols + 1)))
         return false;

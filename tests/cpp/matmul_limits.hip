@@ -56,7 +56,7 @@ int main() {
         } while (positions * out_cols > 1ull << 36);
         const MatmulArgs a = product(positions, out_cols, 512 + static_cast<uint32_t>(spread(14)), gated, rand() % 2 ? static_cast<uint32_t>(spread(11)) : 0);
         if (static_cast<uint64_t>(a.experts) * a.wide * a.row_bytes > 1ull << 38) continue;  // more than the card holds
-        if (a.row_bytes >= 0xf0000000ull / (256 + (gated ? a.out_cols : 0))) continue;  // distances within a tile: another limit
+        if (a.row_bytes >= (0xf0000000ull - a.row_bytes) / (256 + (gated ? a.out_cols : 0))) continue;  // distances within a tile: another limit
         CHECK(tiles_take(a));
         const MatmulChoice c = matmul_choice(a);
         CHECK(c.us < 1e30);
@@ -70,6 +70,13 @@ int main() {
             CHECK(rectangles * each * threads[shape] < 1ull << 32);
             CHECK(static_cast<uint64_t>(g.rectangles) * each >= static_cast<uint64_t>(g.n_tiles) * g.p_tiles);
         }
+    }
+    {   // rows that overlap: the last one of a tile ends past 32 bits though their distances are within
+        MatmulArgs a = product(4, 1000, 1u << 30, 0, 0);
+        a.bits = 8, a.block_rows = a.block_cols = 0, a.cols = 1u << 30, a.row_bytes = 14u << 20, a.x_stride = 8;
+        CHECK(!tiles_take(a));
+        a.row_bytes = 4u << 20;
+        CHECK(tiles_take(a));
     }
     // a block has at most 255 columns: up to 15 units of 16 bytes of codes, of which a row has fewer than 2^27
     const MatmulArgs a{};
