@@ -38,16 +38,17 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     }
 }
 
-// kNT, kTT: tiles of 32 rows and 32 positions of a wave; kWN, kWT, kWK: waves along rows, positions and columns.  Waves along the columns
-// take a run of chunks each, with images of their own; their sums meet in LDS at the end.  Several workgroups may share the columns too: then they
-// leave their sums in the workspace, and matmul_finish_kernel adds them up.
-template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWT, int kWK, int kLine, int kXRing, int kCodeRing>
-__global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>::kWavesPerSimd)) void matmul_tiles_kernel(MatmulArgs a, TilesGrid grid) {
-    using Traits = TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>;
-    constexpr uint32_t kWaves = kWN * kWT, kRows = Traits::kRows, kTokens = Traits::kTokens, kTokensLog2 = __builtin_ctz(kTokens);
+// kNT, kTT: tiles of 32 rows and 32 positions of a wave; kWN, kWK: waves along rows and columns.  Waves along the columns take a run of chunks
+// each, with images of their own; their sums meet in LDS at the end.  Several workgroups may share the columns too: then they leave their sums in the
+// workspace, and matmul_finish_kernel adds them up.
+template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWK, int kLine>
+__global__ __launch_bounds__(64 * kWN * kWK, (TilesTraits<kNT, kTT, kWN, kWK, kLine>::kWavesPerSimd)) void matmul_tiles_kernel(MatmulArgs a, TilesGrid grid) {
+    using Traits = TilesTraits<kNT, kTT, kWN, kWK, kLine>;
+    constexpr uint32_t kWaves = kWN, kRows = Traits::kRows, kTokens = Traits::kTokens, kTokensLog2 = __builtin_ctz(kTokens);
     constexpr uint32_t kBits = bits_of(kCode), kSteps = kLine / 8 / kBits;  // steps of a chunk: 128 bytes of codes are 1024 / kBits columns
     constexpr uint32_t kUnits = kLine / 16, kTurn = 256 / kLine;            // 16-byte pieces of a line; rows side by side in the 256 bytes of all banks
-    static_assert(kSteps >= 1 && kWT == 1, "whole steps; all waves have the same positions");
+    static_assert(kSteps >= 1, "whole steps");
+    constexpr uint32_t kXRing = Traits::kXRing, kCodeRing = Traits::kCodeRing;
     constexpr uint32_t kXBytes = Traits::kXBytes, kCodeBytes = Traits::kCodeBytes;
     constexpr uint32_t kXLoads = kTokens / 8 / kWaves, kCodeLoads = kCodeBytes / 1024 / kWaves, kScaleLoads = kRows * 2 / 64 / kWaves;
     static_assert(kXLoads * 8 * kWaves == kTokens && kCodeLoads * 1024 * kWaves == kCodeBytes && kScaleLoads * 32 * kWaves == kRows, "whole loads of 1 KiB");
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     if (!grid.tile(blockIdx.x, &n_tile, &p_tile) || !find_tile(a, p_tile, kTokensLog2, &at)) return;
     const uint32_t lane = threadIdx.x & 63u, any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wave = any_wave % kWaves, wave_k = any_wave / kWaves;
-    const uint32_t wave_n = wave % kWN, wave_t = wave / kWN, i = lane & 31u, h = lane >> 5;
+    const uint32_t i = lane & 31u, h = lane >> 5;
     const uint32_t positions = at.last - at.first;
     const uint32_t out0 = n_tile * (a.gated ? kRows / 2 : kRows);  // the workgroup's first column of y
     const uint32_t last_unit = a.cols / (128u / kBits) - 1u;
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
 #pragma unroll
     for (uint32_t q = 0; q < kScaleLoads; q++) scale_from[q] = scale_row((q * kWaves + wave) * 32u + lane / 2u);
 #pragma unroll
-    for (uint32_t n = 0; n < kNT; n++) scale_own[n] = scale_row((wave_n * kNT + n) * 32u + i);
+    for (uint32_t n = 0; n < kNT; n++) scale_own[n] = scale_row((wave * kNT + n) * 32u + i);
     const auto scale_block = [&](uint32_t step, uint32_t half) { return grid.block_of(min(step * 2u + half, a.cols / 32u - 1u)) * grid.scale_col_bytes; };
 
     const auto load_x = [&](uint32_t step, uint32_t into) {
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     };
     // `in`: a step of the wave's run, from 0 on
     const auto read_codes = [&](uint32_t in, uint32_t n) {
-        const uint32_t r = (wave_n * kNT + n) * 32u + i, s = in % kSteps;
+        const uint32_t r = (wave * kNT + n) * 32u + i, s = in % kSteps;
         const char* const line = code_img + in / kSteps % kCodeRing * kCodeBytes + r * kLine;
         const uint32_t turn = r / kTurn % kUnits;
         Codes<kCode> c;
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
 #pragma unroll
         for (uint32_t n = 0; n < kNT; n++) {
             codes[n] = read_codes(in, n);
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(scale_img + in % Traits::kScaleRing * Traits::kScaleBytes + ((wave_n * kNT + n) * 32u + i) * 8u + h * 4u);
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(scale_img + in % Traits::kScaleRing * Traits::kScaleBytes + ((wave * kNT + n) * 32u + i) * 8u + h * 4u);
             rounded_scale[n] = dev::round_to<kF>(scale_of(masks, word, scale_own[n] + block));
             mine = mine && takes_short<kF, kCode>(rounded_scale[n]);
         }
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     const auto read_x = [&](auto tiles, uint32_t from, uint32_t m, u32x4* xv) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t t = 0; t < decltype(tiles)::value; t++) {
-            const uint32_t row = (wave_t * kTT + t) * 32u + i;
+            const uint32_t row = t * 32u + i;
             xv[t] = *reinterpret_cast<const u32x4*>(x_img + from * kXBytes + row * 128u + ((h * 4u + m) ^ ((row >> 1) & 7u)) * 16u);
         }
     };
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     float* const parts_of = reinterpret_cast<float*>(lds) + wave * kPart;  // those of the other waves along the columns behind it
     const bool pairs = a.gated && grid.splits == 1;                        // (with shared columns the rows are stored as they are)
     const uint32_t columns = pairs ? 16u * kNT : 32u * kNT, lanes = columns / 8u;
-    const uint32_t in = lane % lanes * 8u, own_col = out0 + wave_n * columns + in;
+    const uint32_t in = lane % lanes * 8u, own_col = out0 + wave * columns + in;
     f32x8 bias = {}, bias_up = {};
     if (grid.splits == 1 && own_col < a.out_cols) {
         bias = load_bias8(a, at.expert, own_col);
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
             __syncthreads();
         else
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const uint32_t p0 = at.first + (wave_t * kTT + t) * 32u;
+        const uint32_t p0 = at.first + t * 32u;
 #pragma unroll 1
         for (uint32_t r = (wave_k * 64u + lane) / lanes; r < 32; r += 64u * kWK / lanes) {
             const uint32_t p = p0 + r;
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
             };
             if (grid.splits > 1) {
                 // [part][position][row of W]: gated, 16 columns and then their 16 gated ones
-                const uint32_t row = wave_n * 32u * kNT + in, col = a.gated ? out0 + row / 32u * 16u + row % 16u : out0 + row;
+                const uint32_t row = wave * 32u * kNT + in, col = a.gated ? out0 + row / 32u * 16u + row % 16u : out0 + row;
                 if (col >= a.out_cols) continue;
                 const f32x8 v = sum_at(from);
                 float* const to = static_cast<float*>(a.workspace) +
@@ -348,22 +349,22 @@ __global__ __launch_bounds__(64 * kWN * kWT * kWK, (TilesTraits<kNT, kTT, kWN, k
     }
 }
 
-template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWT, int kWK, int kLine, int kXRing, int kCodeRing>
+template <dev::Float kF, int kCode, int kNT, int kTT, int kWN, int kWK, int kLine>
 hipError_t launch_tile(hipStream_t s, const MatmulArgs& a, uint32_t splits) {
-    using Traits = TilesTraits<kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>;
+    using Traits = TilesTraits<kNT, kTT, kWN, kWK, kLine>;
     const TilesGrid grid(a, Traits::kRows, Traits::kTokens, splits);
-    hipLaunchKernelGGL((matmul_tiles_kernel<kF, kCode, kNT, kTT, kWN, kWT, kWK, kLine, kXRing, kCodeRing>), dim3(grid.workgroups(), splits), dim3(64 * kWN * kWT * kWK), Traits::kLds, s, a, grid);
+    hipLaunchKernelGGL((matmul_tiles_kernel<kF, kCode, kNT, kTT, kWN, kWK, kLine>), dim3(grid.workgroups(), splits), dim3(64 * kWN * kWK), Traits::kLds, s, a, grid);
     return hipGetLastError();
 }
 
 template <dev::Float kF, int kCode>
 hipError_t launch_shape(hipStream_t s, const MatmulArgs& a, const TilesChoice& c) {
     switch (c.shape) {
-        case TilesShape::k256x128: return launch_tile<kF, kCode, 2, 4, 4, 1, 1, 64, 2, 2>(s, a, c.splits);
-        case TilesShape::k256x128x2: return launch_tile<kF, kCode, 2, 4, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
-        case TilesShape::k128x64: return launch_tile<kF, kCode, 1, 2, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
-        case TilesShape::k128x32: return launch_tile<kF, kCode, 1, 1, 4, 1, 2, 64, 2, 2>(s, a, c.splits);
-        case TilesShape::k32x32: return launch_tile<kF, kCode, 1, 1, 1, 1, 8, 128, 2, 2>(s, a, c.splits);
+        case TilesShape::k256x128: return launch_tile<kF, kCode, 2, 4, 4, 1, 64>(s, a, c.splits);
+        case TilesShape::k256x128x2: return launch_tile<kF, kCode, 2, 4, 4, 2, 64>(s, a, c.splits);
+        case TilesShape::k128x64: return launch_tile<kF, kCode, 1, 2, 4, 2, 64>(s, a, c.splits);
+        case TilesShape::k128x32: return launch_tile<kF, kCode, 1, 1, 4, 2, 64>(s, a, c.splits);
+        case TilesShape::k32x32: return launch_tile<kF, kCode, 1, 1, 1, 8, 128>(s, a, c.splits);
     }
     return hipErrorInvalidValue;
 }

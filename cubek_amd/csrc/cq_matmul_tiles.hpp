@@ -12,19 +12,18 @@ struct TilesChoice {
     uint32_t splits;  // workgroups that share the columns of a tile
 };
 
-// kNT, kTT: tiles of 32 rows and of 32 positions of a wave; kWN, kWT, kWK: waves along rows, positions and columns; kLine: bytes of a row in a
-// chunk of codes.
-// kXRing, kCodeRing: images of x (a step) and of codes (a chunk).
-template <int kNT, int kTT, int kWN, int kWT, int kWK, int kLine, int kXRing, int kCodeRing>
+// kNT, kTT: tiles of 32 rows and of 32 positions of a wave; kWN, kWK: waves along rows and along columns; kLine: bytes of a row in a chunk of
+// codes.
+template <int kNT, int kTT, int kWN, int kWK, int kLine>
 struct TilesTraits {
-    static constexpr uint32_t kRows = 32 * kNT * kWN, kTokens = 32 * kTT * kWT;
+    static constexpr uint32_t kRows = 32 * kNT * kWN, kTokens = 32 * kTT;
     static constexpr uint32_t kXBytes = kTokens * 128, kCodeBytes = kRows * kLine, kScaleBytes = kRows * 8;  // a step of x; a chunk of codes; a step's scales
-    static constexpr uint32_t kScaleRing = 4;
+    static constexpr uint32_t kXRing = 2, kCodeRing = 2, kScaleRing = 4;          // images of a step's x, a chunk's codes and a step's scales
     static constexpr uint32_t kPitch = 32 * kNT + 4;                              // of the sums on their way to y
-    static constexpr uint32_t kImage = kXRing * kXBytes + kCodeRing * kCodeBytes + kScaleRing * kScaleBytes, kImages = kWK * kImage, kParts = kWN * kWT * kWK * 32 * kPitch * 4;
+    static constexpr uint32_t kImage = kXRing * kXBytes + kCodeRing * kCodeBytes + kScaleRing * kScaleBytes, kImages = kWK * kImage, kParts = kWN * kWK * 32 * kPitch * 4;
     static constexpr uint32_t kLds = kImages > kParts ? kImages : kParts;
     static_assert(kLds <= 160 * 1024, "a compute unit's LDS");
-    static constexpr uint32_t kWaves = kWN * kWT * kWK, kFit = 160 * 1024 / kLds;
+    static constexpr uint32_t kWaves = kWN * kWK, kFit = 160 * 1024 / kLds;
     static constexpr uint32_t kMost = kNT * kTT >= 8 ? 2 : 4;  // waves of a SIMD that the registers of the sums leave room for
     static constexpr uint32_t kWavesPerSimd = kWaves / 4 * kFit < kMost ? kWaves / 4 * kFit : kMost;
 };

@@ -10,10 +10,8 @@ namespace {
 
 constexpr int bits_of(int code) { return code <= 8 ? code : (code == kCodeE2M1x2 ? 4 : 8); }
 
-// A stored scale of type `dtype` (uniform over the launch) at an address, as the word around it and as a number: apart, so that a load is
-// not waited for where it is issued, and without branches, which would cut a step's instructions into pieces.
-__device__ __forceinline__ uint32_t scale_word(const char* base, uint32_t offset) { return *reinterpret_cast<const uint32_t*>(base + (offset & ~3u)); }
-// All bits or none of a word, by the type of the scales: uniform over the launch.
+// A stored scale is loaded as the word around it and made a number later: a load is not waited for where it is issued.  By masks instead of
+// branches, which would cut a step's instructions into pieces: all bits or none of a word, by the type of the scales (uniform over the launch).
 struct ScaleMasks {
     uint32_t f32, bf16, f16;
     __device__ explicit ScaleMasks(int dtype) : f32(dtype == CQ_F32 ? ~0u : 0u), bf16(dtype == CQ_BF16 ? ~0u : 0u), f16(dtype == CQ_F16 ? ~0u : 0u) {}
