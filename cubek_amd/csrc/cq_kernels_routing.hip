@@ -125,12 +125,15 @@ __device__ __forceinline__ void choose(const RouteArgs& a, uint32_t token, uint3
             chosen(lane * kR + at);
         }
     }
-    // A sigmoid by exponentials of numbers up to 0, which do not overflow; where a token's are divided by their sum, all of them times exp(-largest) if
-    // that is below 0, so that small ones keep their quotients.  exp(-l) of -709.7827 and below leaves the range of 64 bits: masks of a type's lowest
-    // value weigh nothing, as those of -infinity do.
-    const float shift = a.normalize && largest < 0.0f ? largest : 0.0f;
+    // Sigmoids of a token that are all below 1/2 are divided by their sum as multiples of exp(largest), so that small ones keep their quotients where
+    // exp(-l) leaves the range of f32.  From -709.7827 down it leaves that of 64 bits: masks of a type's lowest value weigh nothing, as those of -infinity do.
+    const bool small = a.sigmoid && a.normalize && largest < 0.0f;
     const auto score = [&](float l) {
-        if (a.sigmoid) return l <= -709.7827f ? 0.0f : (l < 0.0f ? expf(l - shift) : 1.0f) / (1.0f + expf(-__builtin_fabsf(l)));
+        if (a.sigmoid) {
+            float s = 1.0f / (1.0f + expf(-l));
+            if (small) s = l <= -709.7827f ? 0.0f : expf(l - largest) / (1.0f + expf(l));
+            return s;
+        }
         // the largest itself scores 1 also where it is infinite; a token without any finite logit scores nothing
         return l == -__builtin_inff() ? 0.0f : (l == largest ? 1.0f : expf(l - largest));
     };

@@ -77,7 +77,7 @@ size_t cq_experts_workspace_bytes(const cq_tensor* values, const cq_scheme* sche
 
 typedef enum cq_score {
     CQ_SCORE_SOFTMAX = 0, /* over all experts of the token */
-    CQ_SCORE_SIGMOID = 1  /* 0 for logits of -709.7827 and below, such as masks of a type's lowest value: 1 / s passes the range of 64 bits */
+    CQ_SCORE_SIGMOID = 1
 } cq_score;
 
 #define CQ_MAX_EXPERTS 1024
@@ -90,7 +90,8 @@ typedef enum cq_score {
  *             expert.  NaN counts as -infinity.  1 <= chosen <= min(experts, CQ_MAX_CHOSEN).
  *   offsets : i32 [experts + 1]; rows : i32 [tokens * chosen], the token of each position; slots : i32 [tokens, chosen], the position of
  *             each pair.  All outputs contiguous.
- *   normalize : a token's weights are divided by their sum (0 stays 0).  A token whose logits are all -infinity gets weights of 0.
+ *   normalize : a token's weights are divided by their sum (0 stays 0), also where sigmoids are too small for f32 themselves: down to logits of
+ *             -709.78, past which, as masks of a type's lowest value are, they count 0.  A token whose logits are all -infinity gets weights of 0.
  *   workspace : cq_route_workspace_bytes() bytes of device memory, 16-byte aligned (0 for few tokens)
  * tokens <= 2^28 - 64 and tokens * chosen < 2^31.  No tokens: the offsets are set to 0. */
 cq_status cq_route(cq_stream_t stream, const cq_tensor* logits, const cq_tensor* weights, const cq_tensor* experts,
