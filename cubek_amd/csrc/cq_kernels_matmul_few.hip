@@ -8,7 +8,8 @@
 // time from a workgroup's start to its first stage and from its last one to its sums.
 //
 // bf16, 4 bits: one token on [4096, 4096] 5.6 us (a launch 3.5), on [28672, 8192] 35, 16 tokens 37; 32 positions of eight experts [28672, 4096]
-// gated 127 us, 4.6 TB/s, with 2.4 vector instructions per weight; 24 tokens on [28672, 4096] f16 gated 25 us.
+// gated 127 us, 4.6 TB/s, with 2.4 vector instructions per weight; 24 tokens on [28672, 4096] f16 gated 25 us, twice its read: 224 workgroups, each
+// with one stage of 20 KiB of codes and scales on its way, wait for memory.
 #include <hip/hip_runtime.h>
 
 #include "cq_gemv_operand.hpp"

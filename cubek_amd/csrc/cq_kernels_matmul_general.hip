@@ -3,7 +3,7 @@
 //
 // Every weight is decoded and rounded once per workgroup, F(F(scale) * F(code)), into LDS as f32, where a thread takes its numbers of x and of W
 // with one access each for its FMAs; the next step's words are on their way meanwhile.  Bound by the decoding value by value and by the
-// FMAs: 14 TFLOP/s of the vector units' 157 (f32 x, [4096, 4096] 4 bits, 4096 positions 9.8 ms, 512 1.27 ms, 64 0.63 ms, 1 to 16 0.10 ms; with loads
+// FMAs: 14 TFLOP/s of the vector units' 157, without the matrix instructions that there are for f32 (f32 x, [4096, 4096] 4 bits, 4096 positions 9.8 ms, 512 1.27 ms, 64 0.63 ms, 1 to 16 0.10 ms; with loads
 // that waited for one another behind branches on the types 25.8, 3.2, 1.49 and 1.45 ms).
 #include "../../include/cubek_quant_device.hpp"
 #include "cq_matmul_epilogue.hpp"

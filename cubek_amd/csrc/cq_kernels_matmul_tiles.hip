@@ -12,8 +12,9 @@
 // so that the sixteen lanes of a read fall on different banks.
 //
 // Bound by power on large products (bf16 e2m1 [28672, 8192], 4096 tokens 1.83 ms, 1.05 PFLOP/s at 1.6 GHz; 1.73 without the dequantization, 1.86 without
-// the reads of x) and else by what a workgroup takes before its first products and after its last ones: 64 experts [2816, 2048] f16 8 bits gated, 6126
-// positions 173 us, a fifth of it.  256 x 128 rather than 256 x 256 or 512 x 128: two workgroups on a compute unit, no slower; rather than
+// the reads of x).  Smaller ones by their steps' loads, dequantization and barriers side by side, which half the positions hardly shorten, and by what a
+// workgroup takes before its first products and after its last ones: 64 experts [2816, 2048] f16 8 bits gated, 6126 positions 173 us, a fifth of it in
+// front and behind, the matrix units busy for a quarter.  Codes of 8 bits are waited for in every step, as a line of 64 bytes holds one.  256 x 128 rather than 256 x 256 or 512 x 128: two workgroups on a compute unit, no slower; rather than
 // one wave of 64 x 256 per SIMD: 2.09 ms.
 #include <hip/hip_runtime.h>
 

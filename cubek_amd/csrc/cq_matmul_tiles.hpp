@@ -28,7 +28,8 @@ struct TilesTraits {
     static constexpr uint32_t kWavesPerSimd = kWaves / 4 * kFit < kMost ? kWaves / 4 * kFit : kMost;
 };
 
-// n / each as 2 n ceil(2^31 / each) / 2^32, for n < 2^27 and each < 32; 0 for each = 0, one scale for everything
+// n / each as 2 n ceil(2^31 / each) / 2^32, for n < 2^27 and each <= 15: a scheme's blocks have at most 255 columns, 15 units of 16 bytes of 8-bit codes.
+// 0 for each = 0, one scale for everything.
 inline uint32_t magic_of(uint32_t each) { return each ? (0x80000000u + each - 1u) / each : 0u; }
 
 // Tiles of `size` positions that a launch may be taken to have: the experts' sizes lie in device memory, and as many end in half a tile as in a whole one.
@@ -137,7 +138,7 @@ struct FewGrid {
 };
 
 // Whether the kernels on the matrix cores take a product: 16-bit x, rows of whole 16-byte pieces on boundaries of 16 bytes, scales that serve
-// 32 columns at least, and distances within a tile that fit 32 bits.
+// 32 columns at least, and distances within a tile that fit 32 bits: half of a gated weight, and x where rows of it are picked, below 3.75 GiB.
 inline bool tiles_take(const MatmulArgs& a) {
     const auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
     const uint64_t scale_size = a.param_dtype == CQ_F32 ? 4 : 2, rows = 256 + (a.gated ? a.out_cols : 0);
