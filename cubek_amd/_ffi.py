@@ -15,6 +15,7 @@ from .scheme import _CScheme
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libcubek_quant_hip.so")
 MATMUL_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libcubek_matmul_hip.so")
+ATTENTION_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libcubek_attention_hip.so")
 
 #: every symbol include/cubek_quant.h declares
 EXPORTED_SYMBOLS = (
@@ -28,6 +29,9 @@ EXPORTED_SYMBOLS = (
 #: every symbol include/cubek_matmul.h declares
 MATMUL_SYMBOLS = ("cq_matmul_quantized", "cq_matmul_workspace_bytes", "cq_experts_quantized", "cq_experts_workspace_bytes", "cq_route",
                   "cq_route_workspace_bytes", "cq_combine", "cq_matmul_last_hip_error")
+
+#: every symbol include/cubek_attention.h declares
+ATTENTION_SYMBOLS = ("cq_cache_append", "cq_cache_copy", "cq_attention", "cq_attention_workspace_bytes", "cq_attention_last_hip_error")
 
 
 class CTensor(ctypes.Structure):
@@ -53,6 +57,25 @@ class CEpilogue(ctypes.Structure):
     ]
 
 
+class CCache(ctypes.Structure):
+    """Binary layout of ``cq_cache`` (include/cubek_attention.h)."""
+
+    _fields_ = [(name, ctypes.POINTER(CTensor)) for name in ("keys", "key_scales", "values", "value_scales")] + [("scheme", ctypes.POINTER(_CScheme))]
+
+
+class CRotary(ctypes.Structure):
+    """Binary layout of ``cq_rotary``."""
+
+    _fields_ = [("frequencies", ctypes.POINTER(CTensor)), ("magnitude", ctypes.c_float), ("interleaved", ctypes.c_uint32)]
+
+
+class CScores(ctypes.Structure):
+    """Binary layout of ``cq_scores``."""
+
+    _fields_ = [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("window", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+                ("slopes", ctypes.POINTER(CTensor)), ("prefix", ctypes.POINTER(CTensor))]
+
+
 class QuantError(RuntimeError):
     """A non-zero cq_status.  ``status`` holds the code (include/cubek_quant.h)."""
 
@@ -68,6 +91,7 @@ OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED_SCHEME, ERR_BLOCK_NOT_DIVISIBLE, ERR_S
 
 _lib = None
 _matmul_lib = None
+_attention_lib = None
 _calls = None
 
 
@@ -154,6 +178,43 @@ def matmul_lib() -> ctypes.CDLL:
     return L
 
 
+def attention_lib() -> ctypes.CDLL:
+    """The library of include/cubek_attention.h: a cache of keys and values in pages, attention over it."""
+    global _attention_lib
+    if _attention_lib is not None:
+        return _attention_lib
+    if not os.path.exists(ATTENTION_LIB_PATH):
+        raise RuntimeError(f"native library not built: {ATTENTION_LIB_PATH} is missing; there is no fallback path. "
+                           "Build it with `make -C cubek_amd/csrc` (needs hipcc).")
+    lib()
+    L = ctypes.CDLL(ATTENTION_LIB_PATH)
+    tp, cp, rp, op = (ctypes.POINTER(c) for c in (CTensor, CCache, CRotary, CScores))
+    L.cq_cache_append.restype = ctypes.c_int
+    L.cq_cache_append.argtypes = [ctypes.c_void_p, cp] + [tp] * 6 + [rp, ctypes.c_int]
+    L.cq_attention.restype = ctypes.c_int
+    L.cq_attention.argtypes = [ctypes.c_void_p, cp] + [tp] * 5 + [op, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]
+    L.cq_attention_workspace_bytes.restype = ctypes.c_size_t
+    L.cq_attention_workspace_bytes.argtypes = [cp, tp, tp, ctypes.c_int]
+    L.cq_cache_copy.restype = ctypes.c_int
+    L.cq_cache_copy.argtypes = [ctypes.c_void_p, tp, ctypes.c_uint32, tp]
+    L.cq_attention_last_hip_error.restype = ctypes.c_int
+    L.cq_attention_last_hip_error.argtypes = []
+    _attention_lib = L
+    return L
+
+
+def cache_to_c(cache) -> CCache:
+    """The ``cq_cache`` of a ``Cache``; its tensors live as long as their handles."""
+    c = CCache()
+    for name in ("keys", "key_scales", "values", "value_scales"):
+        t = getattr(cache, name)
+        if t is not None:
+            setattr(c, name, ctypes.pointer(t.as_c()))
+    if cache.scheme is not None:
+        c.scheme = ctypes.pointer(cache.scheme.to_c())
+    return c
+
+
 def epilogue_to_c(epilogue) -> CEpilogue:
     """The ``cq_epilogue`` of an ``Epilogue``; its tensors live as long as their handles."""
     c = CEpilogue(int(epilogue.activation), int(epilogue.gated))
@@ -194,6 +255,13 @@ def check_matmul(status: int) -> None:
     """check() for the calls of include/cubek_matmul.h, whose library keeps its own last HIP error."""
     if status == ERR_HIP:
         raise QuantError(status, f"{lib().cq_strerror(status).decode()} (hipError_t {matmul_lib().cq_matmul_last_hip_error()})")
+    check(status)
+
+
+def check_attention(status: int) -> None:
+    """check() for the calls of include/cubek_attention.h, whose library keeps its own last HIP error."""
+    if status == ERR_HIP:
+        raise QuantError(status, f"{lib().cq_strerror(status).decode()} (hipError_t {attention_lib().cq_attention_last_hip_error()})")
     check(status)
 
 

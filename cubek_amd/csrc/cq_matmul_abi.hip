@@ -1,4 +1,5 @@
 // C ABI of libcubek_matmul_hip.so (include/cubek_matmul.h): argument checks, the choice of a kernel, launches.
+#include "cq_abi_checks.hpp"
 #include "cq_matmul_tiles.hpp"
 
 namespace {
@@ -14,51 +15,7 @@ cq_status hip_status(hipError_t e) {
 // The launchers read hipGetLastError() after each launch: an error that earlier HIP calls of the caller left would be taken for theirs.
 void drop_stale_hip_error() { (void)hipGetLastError(); }
 
-constexpr uint64_t kMostExtent = 0x7fffffffull;  // rows, columns, positions and tokens are 32-bit numbers in the kernels
 constexpr uint64_t kMostRouted = (cq::kLaunchThreads / 1024 - 1) * 64;  // tokens of a routing: 64 of them are a workgroup of 1024 threads
-
-uint32_t dtype_size(int dtype) { return dtype == CQ_F32 ? 4u : 2u; }
-bool valid_dtype(int dtype) { return dtype == CQ_F32 || dtype == CQ_F16 || dtype == CQ_BF16; }
-bool has_elements(const cq_tensor* t) {
-    for (uint32_t d = 0; d < t->rank; d++)
-        if (t->shape[d] == 0) return false;
-    return true;
-}
-
-// A tensor without elements may come without an address.
-bool tensor_ok(const cq_tensor* t) {
-    return t && t->shape && t->strides && t->rank >= 1 && t->rank <= CQ_MAX_RANK && (t->ptr || !has_elements(t));
-}
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
-bool is_contiguous(const cq_tensor* t) {
-    if (!has_elements(t)) return true;
-    uint64_t expect = 1;
-    for (int d = static_cast<int>(t->rank) - 1; d >= 0; d--) {
-        if (t->shape[d] != 1 && t->strides[d] != expect) return false;
-        expect *= t->shape[d];
-    }
-    return true;
-}
-
-// The stride of dimension d; one entry counts as 0, whatever the tensor says, and keeps no product from a kernel by its alignment.
-uint64_t stride_of(const cq_tensor* t, uint32_t d) { return t->shape[d] > 1 ? t->strides[d] : 0; }
-
-cq_status check_scheme(const cq_scheme* s) {
-    if (!s) return CQ_ERR_INVALID_ARGUMENT;
-    if (cq_value_size_bits(s->value) == 0 || s->param > CQ_PARAM_BF16 || s->store > CQ_STORE_NATIVE || s->level > CQ_LEVEL_BLOCK || s->reserved != 0)
-        return CQ_ERR_INVALID_ARGUMENT;
-    if (s->mode != CQ_MODE_SYMMETRIC) return CQ_ERR_UNSUPPORTED_SCHEME;
-    if (s->level == CQ_LEVEL_BLOCK) {
-        if (s->block_rank < 1 || s->block_rank > CQ_MAX_BLOCK_DIMS) return CQ_ERR_INVALID_ARGUMENT;
-        for (uint32_t i = 0; i < s->block_rank; i++)
-            if (s->block[i] == 0) return CQ_ERR_INVALID_ARGUMENT;
-    }
-    // the native store holds i8, e4m3, e5m2 bytes or e2m1 pairs (crates/cubek-quant/src/quantize.rs:196-219)
-    if (s->store == CQ_STORE_NATIVE && (s->value == CQ_VALUE_Q4F || s->value == CQ_VALUE_Q4S || s->value == CQ_VALUE_Q2F || s->value == CQ_VALUE_Q2S))
-        return CQ_ERR_UNSUPPORTED_SCHEME;
-    return CQ_OK;
-}
 
 // The weights of a product: [rows, stored columns], or [experts, rows, stored columns].
 cq_status read_weights(const cq_tensor* values, const cq_tensor* params, const cq_scheme* scheme, bool experts, cq::MatmulArgs* a) {
@@ -158,15 +115,6 @@ cq_status read_activations(const cq_tensor* x, const cq_tensor* y, cq_dtype dtyp
     a->positions = static_cast<uint32_t>(positions);
     a->x_stride = last ? stride_of(x, 0) : 0;
     a->y_stride = last ? y->strides[0] : 0;
-    return CQ_OK;
-}
-
-// An i32 tensor [n], contiguous.
-cq_status read_indexes(const cq_tensor* t, uint64_t n, const int32_t** out) {
-    if (!tensor_ok(t) || !aligned(t->ptr, 4)) return CQ_ERR_INVALID_ARGUMENT;
-    if (t->rank != 1 || t->elem_size != 4 || t->shape[0] != n) return CQ_ERR_SHAPE_MISMATCH;
-    if (!is_contiguous(t)) return CQ_ERR_NON_CONTIGUOUS;
-    *out = static_cast<const int32_t*>(t->ptr);
     return CQ_OK;
 }
 

@@ -1,5 +1,5 @@
 // The package's calls without ctypes: a CPython module that reads the handles, the scheme and the numbers of a call from the
-// Python objects and calls the C ABI (include/cubek_quant.h, include/cubek_matmul.h).
+// Python objects and calls the C ABI (include/cubek_quant.h, include/cubek_matmul.h, include/cubek_attention.h).
 //
 // A call that launches one kernel takes the HIP runtime 3.2 us of the host.  Through ctypes (a lookup of the scheme's
 // struct by its hash, a cached struct per handle, a conversion per argument) the package added 1.2 us to that: quantize
@@ -10,8 +10,11 @@
 
 #include <cstring>
 #include <initializer_list>
+#include <new>
 #include <utility>
+#include <vector>
 
+#include "../../include/cubek_attention.h"
 #include "../../include/cubek_matmul.h"
 #include "../../include/cubek_quant.h"
 
@@ -371,6 +374,95 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return status_of([&] { return cq_combine(static_cast<cq_stream_t>(stream), &h.t, &slots.t, &weights.t, residual.t, &y.t, h_elem, y_elem); });
 }
 
+// keys, key scales, values, value scales, scheme (None: floats)
+struct CacheArg {
+    Tensor keys, values;
+    OptionalTensor key_scales, value_scales;
+    cq_scheme scheme;
+    cq_cache c{};
+    static constexpr Py_ssize_t kArgs = 5;
+
+    bool read(PyObject* const* a) {
+        if (!keys.read(a[0]) || !key_scales.read(a[1]) || !values.read(a[2]) || !value_scales.read(a[3])) return false;
+        c.keys = &keys.t, c.key_scales = key_scales.t, c.values = &values.t, c.value_scales = value_scales.t;
+        if (a[4] == Py_None) return true;
+        c.scheme = &scheme;
+        return read_scheme(a[4], &scheme);
+    }
+};
+
+bool real(PyObject* o, float* out) {
+    const double v = PyFloat_AsDouble(o);
+    *out = static_cast<float>(v);
+    return !(v == -1.0 && PyErr_Occurred());
+}
+
+// stream, cache, k, v, slots, q, q_out, positions, frequencies, magnitude, interleaved, elem
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* stream;
+    CacheArg cache;
+    Tensor k, v, slots;
+    OptionalTensor q, q_out, positions, frequencies;
+    cq_rotary rotary{};
+    uint64_t interleaved;
+    cq_dtype elem;
+    if (!count(n, 11 + cache.kArgs) || !pointer(a[0], &stream) || !cache.read(a + 1) || !k.read(a[6]) || !v.read(a[7]) || !slots.read(a[8]) || !q.read(a[9]) ||
+        !q_out.read(a[10]) || !positions.read(a[11]) || !frequencies.read(a[12]) || !real(a[13], &rotary.magnitude) || !number(a[14], &interleaved) ||
+        !Common<1>::read_elem(a[15], &elem))
+        return nullptr;
+    rotary.frequencies = frequencies.t;
+    rotary.interleaved = static_cast<uint32_t>(interleaved);
+    return status_of([&] {
+        return cq_cache_append(static_cast<cq_stream_t>(stream), &cache.c, &k.t, &v.t, &slots.t, q.t, q_out.t, positions.t, frequencies.t ? &rotary : nullptr, elem);
+    });
+}
+
+// stream, cache, q, y, table, offsets, lengths, scale, cap, window, slopes, prefix, elem, workspace, bytes
+PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void *stream, *workspace;
+    CacheArg cache;
+    Tensor q, y, table, offsets, lengths;
+    OptionalTensor slopes, prefix;
+    cq_scores scores{};
+    uint64_t window, bytes;
+    cq_dtype elem;
+    if (!count(n, 14 + cache.kArgs) || !pointer(a[0], &stream) || !cache.read(a + 1) || !q.read(a[6]) || !y.read(a[7]) || !table.read(a[8]) ||
+        !offsets.read(a[9]) || !lengths.read(a[10]) || !real(a[11], &scores.scale) || !real(a[12], &scores.cap) || !number(a[13], &window) ||
+        !slopes.read(a[14]) || !prefix.read(a[15]) || !Common<1>::read_elem(a[16], &elem) || !pointer(a[17], &workspace) || !integer(a[18], &bytes))
+        return nullptr;
+    if (window > 0xffffffffull) {
+        PyErr_SetString(PyExc_OverflowError, "a window is a number of 32 bits");
+        return nullptr;
+    }
+    scores.window = static_cast<uint32_t>(window);
+    scores.slopes = slopes.t;
+    scores.prefix = prefix.t;
+    return status_of([&] {
+        return cq_attention(static_cast<cq_stream_t>(stream), &cache.c, &q.t, &y.t, &table.t, &offsets.t, &lengths.t, &scores, elem, workspace, bytes);
+    });
+}
+
+// stream, tensors, pairs
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* stream;
+    Tensor pairs;
+    if (!count(n, 3) || !pointer(a[0], &stream) || !pairs.read(a[2])) return nullptr;
+    const Ref fast(PySequence_Fast(a[1], "tensors are a sequence"));
+    if (!fast) return nullptr;
+    const Py_ssize_t of = PySequence_Fast_GET_SIZE(fast.p);
+    try {
+        std::vector<Tensor> held(static_cast<size_t>(of));
+        std::vector<cq_tensor> tensors(static_cast<size_t>(of));
+        for (Py_ssize_t i = 0; i < of; i++) {
+            if (!held[static_cast<size_t>(i)].read(PySequence_Fast_GET_ITEM(fast.p, i))) return nullptr;
+            tensors[static_cast<size_t>(i)] = held[static_cast<size_t>(i)].t;
+        }
+        return status_of([&] { return cq_cache_copy(static_cast<cq_stream_t>(stream), tensors.data(), static_cast<uint32_t>(of), &pairs.t); });
+    } catch (const std::bad_alloc&) {
+        return PyErr_NoMemory();
+    }
+}
+
 template <class F>
 constexpr PyMethodDef method(const char* name, F f) {
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr};
@@ -391,6 +483,7 @@ PyMethodDef methods[] = {
     method("quantize_dynamic", quantize_dynamic), method("quantize_dynamic_static", quantize_dynamic_static),
     method("gemv", gemv), method("max_abs", max_abs), method("repack", repack),
     method("matmul", matmul), method("experts", experts), method("route", route), method("combine", combine),
+    method("append", append), method("attention", attention), method("copy_pages", copy_pages),
     {"bind", bind, METH_VARARGS, "bind(TensorHandleRef, QuantScheme)"}, {nullptr, nullptr, 0, nullptr},
 };
 
