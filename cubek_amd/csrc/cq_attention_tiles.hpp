@@ -1,0 +1,138 @@
+// What the attention kernels on the matrix cores share: codes to operands, tiles of rows, the partial results of a split.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "cq_attention_internal.hpp"
+#include "cq_device.hpp"
+
+namespace cq {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2E = 1.44269504088896340736f;
+
+template <int kCode>
+constexpr uint32_t kCodeBits = kCode == kCacheFloat ? 16u : (kCode == kCacheInt4 || kCode == kCacheE2M1 ? 4u : 8u);
+
+// What may be infinite or not a number in a code; else only its scale can.
+template <int kCode>
+constexpr bool kCodeHasNaN = kCode == kCacheFloat || kCode == kCacheE4M3 || kCode == kCacheE5M2;
+
+// The entry that stands at place i of eight decoded ones: 4-bit integers come in pairs (k, k + 4).
+template <int kCode>
+__device__ __forceinline__ constexpr uint32_t place_of(uint32_t i) {
+    return kCode == kCacheInt4 ? i / 2u + i % 2u * 4u : i;
+}
+
+// Eight codes (8 bits: `low` then `high`; 4 bits: `low`) as numbers of f16, exactly.
+//   i8 : the byte, its sign bit turned, under the exponent of 1024, less 1024 + 128
+//   4-bit integers : nibbles 0 and 4 under the exponent of 1024, less 1024 + 8; nibbles 1 and 5 as 16 times themselves there, times 1/16, less 64 + 8
+//   fp8, fp4 : one conversion for two
+template <int kCode>
+__device__ __forceinline__ u32x4 numbers(uint32_t low, uint32_t high) {
+    const auto bits = [](f16x2 v) { return __builtin_bit_cast(uint32_t, v); };
+    const auto half2 = [](uint32_t v) { return __builtin_bit_cast(f16x2, v); };
+    if constexpr (kCode == kCacheInt8) {
+        const f16x2 less = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+        low ^= 0x80808080u, high ^= 0x80808080u;
+        return u32x4{bits(half2(__builtin_amdgcn_perm(0x64646464u, low, 0x04010400u)) + less), bits(half2(__builtin_amdgcn_perm(0x64646464u, low, 0x04030402u)) + less),
+                     bits(half2(__builtin_amdgcn_perm(0x64646464u, high, 0x04010400u)) + less), bits(half2(__builtin_amdgcn_perm(0x64646464u, high, 0x04030402u)) + less)};
+    } else if constexpr (kCode == kCacheInt4) {
+        const f16x2 less = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)}, less16 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)},
+                    by = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+        low ^= 0x88888888u;
+        const uint32_t next = low >> 8;
+        return u32x4{bits(half2((low & 0x000f000fu) | 0x64006400u) + less), bits(__builtin_elementwise_fma(half2((low & 0x00f000f0u) | 0x64006400u), by, less16)),
+                     bits(half2((next & 0x000f000fu) | 0x64006400u) + less), bits(__builtin_elementwise_fma(half2((next & 0x00f000f0u) | 0x64006400u), by, less16))};
+    } else if constexpr (kCode == kCacheE2M1) {
+        return u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(low, 1.0f, 0)), bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(low, 1.0f, 1)),
+                     bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(low, 1.0f, 2)), bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(low, 1.0f, 3))};
+    } else if constexpr (kCode == kCacheE4M3) {
+        return u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, 1.0f, false)), bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, 1.0f, true)),
+                     bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(high, 1.0f, false)), bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(high, 1.0f, true))};
+    } else {
+        return u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8(low, 1.0f, false)), bits(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8(low, 1.0f, true)),
+                     bits(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8(high, 1.0f, false)), bits(__builtin_amdgcn_cvt_scalef32_pk_f16_bf8(high, 1.0f, true))};
+    }
+}
+
+// Two f32 to a pair of 16 bits, each to the nearest.
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+    if constexpr (kBF16) return BF16::pack2(a, b);
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
+template <bool kBF16>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (kBF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// The larger of a value's copies in the four groups of 16 lanes.
+__device__ __forceinline__ float max_of_groups(float v) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+    v = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
+    const auto quarters = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+    return fmaxf(bits_f32(quarters[0]), bits_f32(quarters[1]));
+}
+__device__ __forceinline__ float sum_of_groups(float v) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+    v = bits_f32(halves[0]) + bits_f32(halves[1]);
+    const auto quarters = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+    return bits_f32(quarters[0]) + bits_f32(quarters[1]);
+}
+
+// A stored scale is loaded as the word around it and made a number later, by masks instead of branches: a load is not waited for where it is
+// issued.  All bits or none of a word, by the type of the scales (uniform over the launch).
+struct ScaleWords {
+    uint32_t f32, bf16, f16, log2;
+    __device__ explicit ScaleWords(uint32_t dtype)
+        : f32(dtype == CQ_F32 ? ~0u : 0u), bf16(dtype == CQ_BF16 ? ~0u : 0u), f16(dtype == CQ_F16 ? ~0u : 0u), log2(dtype == CQ_F32 ? 2u : 1u) {}
+    __device__ __forceinline__ uint32_t load(const char* scales, uint64_t i) const {
+        return *reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(scales + (i << log2)) & ~static_cast<uintptr_t>(3));
+    }
+    // which half of its word a scale of 16 bits is
+    __device__ __forceinline__ uint32_t half(const char* scales, uint64_t i) const {
+        return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(scales + (i << log2)) >> 1) & 1u;
+    }
+    __device__ __forceinline__ float number(uint32_t word, uint32_t half) const {
+        const uint32_t bits = word >> (half * 16u);
+        const uint32_t from_f16 = f32_bits(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits))));
+        return bits_f32((word & f32) | (bits << 16 & bf16) | (from_f16 & f16));
+    }
+};
+
+// The tile of rows (token, head of a group) that a workgroup has: tile t of a sequence's own begins at its row t * rows.  Sequence s owns the tiles from
+// offsets[s] * group / rows + s on, which is room enough: floor(a + b) - floor(a) + 1 >= ceil(b).
+struct RowTile {
+    Sequence s;
+    uint32_t row0, rows;  // first row within the sequence and how many there are
+};
+__device__ __forceinline__ bool find_rows(const AttentionArgs& a, uint32_t tile, uint32_t rows_log2, RowTile* out) {
+    const auto begin = [&](uint32_t i) {
+        const int32_t o = a.offsets[i];
+        return (static_cast<uint64_t>(min(static_cast<uint32_t>(max(o, 0)), a.tokens)) * a.group >> rows_log2) + i;
+    };
+    const uint32_t s = __builtin_amdgcn_readfirstlane(last_at_or_below(a.seqs, tile, begin));
+    const Sequence q = sequence_of(a, s);
+    const uint64_t first = begin(s), rows = static_cast<uint64_t>(q.last - q.first) * a.group;
+    if (tile < first) return false;
+    const uint64_t row0 = (tile - first) << rows_log2;
+    if (row0 >= rows) return false;
+    out->s = q;
+    out->row0 = static_cast<uint32_t>(row0);
+    out->rows = static_cast<uint32_t>(min(rows - row0, static_cast<uint64_t>(1u << rows_log2)));
+    return true;
+}
+
+}  // namespace
+}  // namespace cq

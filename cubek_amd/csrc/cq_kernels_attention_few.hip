@@ -1,0 +1,570 @@
+// Attention of few rows (token, head of a group) over long caches: decode steps, drafts of some tokens.  An object per kind of code (CQ_TU_CODE).
+//
+// A workgroup takes a tile of 16 or 32 rows that share a head of the cache, and a split of the keys they see; its four waves take steps
+// of 32 keys (64 of 4 bits) in turn, each with a running maximum, sum and result of its own, which meet in LDS at the end; the results of several
+// splits meet in attention_join_kernel.  Everything else stays in registers:
+//   S^T = K Q^T by 16 x 16 x 32 matrix instructions: lane (i, g) has 16 bytes of key i, and gets the scores of row i with the keys 4 g ... 4 g + 3 of a
+//   tile of 16, which are the operand that the second product takes: O^T = V^T P^T with the keys in that order.
+//   V goes through LDS, each wave's own part (no barrier), and comes back by transposing reads, a lane eight keys of one entry.
+// Codes enter as themselves, exact in f16, keys' scales in f32 behind the first product, values' scales in front of the second, on the weights: no
+// entry is rounded, and a value of the cache costs 1.25 vector instructions at 8 bits (0.5 of fp8) instead of the 2.5 to 4 of its dequantization.
+// Where a scale covers 32 entries of a longer head, lanes swap parts so that one instruction has one block (`kPer` > 1).
+// Queries are scaled by a power of two per row, weights by one per step, so that f16 holds them whatever the range of bf16.
+#include <hip/hip_runtime.h>
+
+#include "cq_attention_tiles.hpp"
+#include "cq_magic_div.hpp"
+
+namespace cq {
+namespace {
+
+#define CQ_LDS_AT(T, p) ((__attribute__((address_space(3))) T*)(p))
+typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+
+// Between a wave's writes to its part of LDS and its reads from it: LDS serves a wave in order, so only the compiler has to keep it.
+__device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+    v = max(v, dpp<kDppXor1>(v));
+    v = max(v, dpp<kDppXor2>(v));
+    v = max(v, dpp<kDppHalfMirror>(v));
+    v = max(v, dpp<kDppMirror>(v));
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(halves[0], halves[1]);
+    const auto quarters = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(quarters[0], quarters[1]);
+}
+
+template <int kCode, int kDim, int kPer>
+struct Shape {
+    static constexpr uint32_t kBits = kCodeBits<kCode>;
+    static constexpr uint32_t kKeyTiles = kBits == 4 ? 4 : 2, kKeys = 16 * kKeyTiles;  // of a step
+    static constexpr uint32_t kRow = kDim * kBits / 8;                                 // bytes of a key
+    static constexpr uint32_t kUnits = kRow >= 64 ? kRow / 64 : 1, kWords = kRow >= 64 ? 4 : 2;  // loads of a lane for a key; words of one
+    static constexpr uint32_t kSlices = kDim / 32;                                     // matrix instructions of a tile of keys
+    static constexpr uint32_t kLane = 16, kLanes = kRow / kLane, kLoads = kKeys * kRow / 1024;  // of values: bytes of a lane, lanes of a row, loads of a step
+    static constexpr uint32_t kPitch = kRow + 16;                                      // bytes of a row in LDS: 16 keys' reads fall on different banks
+    static constexpr uint32_t kScaleLoads = kCode == kCacheFloat ? 0 : kPer * kKeyTiles / 2;
+    static constexpr uint32_t kValueBytes = kKeys * kPitch, kScaleBytes = kCode == kCacheFloat ? 0 : 2 * kPer * kKeys * 4, kWaveBytes = kValueBytes + kScaleBytes;
+};
+
+// Where a lane's eight entries of slice t begin within a row, as the first product takes them.
+template <int kCode, int kDim, int kPer>
+__device__ __forceinline__ uint32_t slice_entry(uint32_t t, uint32_t g) {
+    using S = Shape<kCode, kDim, kPer>;
+    if constexpr (S::kBits == 16) {
+        return 32u * t + 8u * g;
+    } else if constexpr (kPer == 1) {
+        constexpr uint32_t kEntries = S::kWords * 32 / S::kBits, kOf = kEntries / 8;  // a lane's entries of a unit; slices of a unit
+        return t / kOf * (4u * kEntries) + g * kEntries + t % kOf * 8u;
+    } else {
+        return 32u * t + 8u * g;  // placed by swaps, see below; the order within 32 is slice_order()
+    }
+}
+
+// With blocks of 32 entries a unit's words are exchanged between the groups of lanes.  16 entries a lane (8 bits; 4 bits of 64 entries): words of
+// eight entries w0, w1; after the swap of halves group g has, in slice 0, entries 0 - 7, 16 - 23, 8 - 15, 24 - 31 for g = 0 ... 3, in slice 1 the same
+// of the next block.  32 entries a lane (4 bits): a transposition of four words between four groups, after which group g has word g's place.
+template <int kCode, int kDim>
+__device__ __forceinline__ uint32_t slice_order(uint32_t g) {
+    using S = Shape<kCode, kDim, 2>;
+    constexpr uint32_t kEntries = S::kWords * 32 / S::kBits;
+    if constexpr (kEntries == 16) return (g & 1u) * 16u + (g >> 1) * 8u;
+    return 8u * g;
+}
+
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+__device__ __forceinline__ void swap_quarters(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+
+template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
+__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, FewSplit split) {
+    using S = Shape<kCode, kDim, kPer>;
+    constexpr bool kFloat = kCode == kCacheFloat;
+    constexpr uint32_t kRowsLog2 = kTiles == 1 ? 4 : 5, kRows = 16 * kTiles;
+    constexpr uint32_t kOut = kDim / 16;  // tiles of 16 entries of the result
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15u, g = lane >> 4;
+    const uint32_t part = blockIdx.x % split.splits, tile = blockIdx.x / split.splits, kv_head = blockIdx.y, dim = a.cache.dim;
+    char* const mine = lds + wave * S::kWaveBytes;
+    float* const scales_at = reinterpret_cast<float*>(mine + S::kValueBytes);
+
+    RowTile at;
+    if (!find_rows(a, tile, kRowsLog2, &at)) return;
+    // the keys that some row of the tile sees, and those that all of them do
+    const int32_t first_position = at.s.position + static_cast<int32_t>(at.row0 / a.group), last_position = at.s.position + static_cast<int32_t>((at.row0 + at.rows - 1u) / a.group);
+    const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, last_position);
+    const int32_t low = first.low, high = last.high, all_low = last.low, all_high = first.high;
+    const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
+    const uint32_t each = (steps_all + split.splits - 1u) / split.splits;
+    const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
+    const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
+
+    // queries: row i of each tile of 16
+    u32x4 q[kTiles][S::kSlices];
+    float times[kTiles], slope[kTiles];
+    int32_t position[kTiles], row_low[kTiles], row_high[kTiles];
+#pragma unroll
+    for (uint32_t r = 0; r < kTiles; r++) {
+        const uint32_t row = min(r * 16u + i, at.rows - 1u) + at.row0, token = at.s.first + row / a.group, head = kv_head * a.group + row % a.group;
+        position[r] = at.s.position + static_cast<int32_t>(row / a.group);
+        const Seen seen = seen_from(a, at.s, position[r]);
+        row_low[r] = seen.low, row_high[r] = r * 16u + i < at.rows ? seen.high : -1;
+        slope[r] = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
+        const char* const from_q = a.q + (token * a.q_token + head * a.q_head) * 2u;
+        float most = 0.0f;
+#pragma unroll
+        for (uint32_t t = 0; t < S::kSlices; t++) {
+            const uint32_t d = kPer == 1 || kFloat ? slice_entry<kCode, kDim, kPer>(t, g) : 32u * t + slice_order<kCode, kDim>(g);
+            q[r][t] = d < dim ? *reinterpret_cast<const u32x4*>(from_q + d * 2u) : u32x4{0, 0, 0, 0};
+        }
+        if constexpr (!kFloat) {
+            float v[8];
+            const bool bf16 = a.dtype == CQ_BF16;
+#pragma unroll
+            for (uint32_t t = 0; t < S::kSlices; t++) {
+                if (bf16)
+                    BF16::unpack(q[r][t], v);
+                else
+                    F16::unpack(q[r][t], v);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) most = fmaxf(most, fabsf(v[e]));
+            }
+            most = max_of_groups(most);
+            // 2^-p with 2^p <= most < 2^(p + 1): the largest entry between 1 and 2 (none, infinite: as it is)
+            const uint32_t field = f32_bits(most) >> 23;
+            const uint32_t power = bf16 && field > 0u && field < 255u ? min(max(field, 1u), 253u) : 127u;
+            const float down = bits_f32((254u - power) << 23);
+#pragma unroll
+            for (uint32_t t = 0; t < S::kSlices; t++) {
+                if (bf16)
+                    BF16::unpack(q[r][t], v);
+                else
+                    F16::unpack(q[r][t], v);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) q[r][t][e] = pair_of<false>(v[place_of<kCode>(2 * e)] * down, v[place_of<kCode>(2 * e + 1)] * down);
+            }
+            times[r] = a.scale * bits_f32(power << 23);
+        } else {
+            times[r] = a.scale;
+        }
+        // with a cap: 2 log2(e) t / cap, the exponent of its tanh; else log2(e) t
+        times[r] *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
+    }
+    const float cap = a.cap * kLog2E;
+
+    // Pages of the wave's next 64 / kKeyTiles steps, a lane a tile of 16 keys.
+    const uint32_t tiles_of_page = a.cache.page_size / 16u;
+    const auto tile_of = [&](uint32_t step, uint32_t k) { return min((step0 + step) * S::kKeyTiles + k, last_tile); };
+    constexpr uint32_t kAhead = 64 / S::kKeyTiles;
+    uint32_t pages = 0;
+    const auto look_up = [&](uint32_t step) {
+        const uint32_t t = tile_of(step + lane / S::kKeyTiles * 4u, lane % S::kKeyTiles);
+        pages = page_of(a, at.s, magic_div(t, split.page_magic, split.page_shift));
+    };
+
+    // A step's loads.
+    struct Raw {
+        uint32_t k[S::kKeyTiles][S::kUnits][S::kWords];
+        u32x4 v[S::kLoads];
+        uint32_t scale[S::kScaleLoads ? S::kScaleLoads : 1], halves;
+    };
+    const ScaleWords words(a.cache.param_dtype);
+    const uint32_t row_bytes = dim * S::kBits / 8u;
+    const auto key_byte = [&](uint32_t u) { return u * 64u + g * (4u * S::kWords); };
+    uint32_t key_offset[S::kUnits], value_offset[S::kLoads];
+#pragma unroll
+    for (uint32_t u = 0; u < S::kUnits; u++) key_offset[u] = i * static_cast<uint32_t>(a.cache.keys.slot) + min(key_byte(u), row_bytes - 4u * S::kWords);
+#pragma unroll
+    for (uint32_t n = 0; n < S::kLoads; n++) {
+        const uint32_t key = (n * 64u + lane) / S::kLanes;
+        value_offset[n] = key % 16u * static_cast<uint32_t>(a.cache.values.slot) + min(lane % S::kLanes * S::kLane, row_bytes - S::kLane);
+    }
+    // The scales that a lane loads: of 32 keys those of the key (lanes 0 - 31) and of the value (32 - 63) at once, of 64 one after the other.
+    const uint32_t scale_key = lane % S::kKeys;
+    const auto of_values = [&](uint32_t n) { return S::kKeyTiles == 2 ? lane >= 32u : n >= kPer; };
+    const auto place_of_tile = [&](uint32_t t) { return (t - magic_div(t, split.page_magic, split.page_shift) * tiles_of_page) * 16u; };
+    const auto load = [&](uint32_t step, uint32_t nth, Raw& raw) {
+        uint32_t page[S::kKeyTiles], place[S::kKeyTiles];
+#pragma unroll
+        for (uint32_t k = 0; k < S::kKeyTiles; k++) {
+            page[k] = __builtin_amdgcn_readlane(pages, (nth % kAhead) * S::kKeyTiles + k);
+            place[k] = place_of_tile(tile_of(step, k));
+            const char* const key_rows = a.cache.keys.base + page[k] * a.cache.keys.page + kv_head * a.cache.keys.head + place[k] * a.cache.keys.slot;
+#pragma unroll
+            for (uint32_t u = 0; u < S::kUnits; u++) {
+                if constexpr (S::kWords == 4) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(key_rows + key_offset[u]);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) raw.k[k][u][e] = w[e];
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(key_rows + key_offset[u]);
+                    raw.k[k][u][0] = w[0], raw.k[k][u][1] = w[1];
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < S::kLoads; n++) {
+            constexpr uint32_t kKeysOfLoad = 64 / S::kLanes;  // 32 where rows are 32 bytes
+            const uint32_t k = n * kKeysOfLoad / 16u;
+            uint64_t rows = page[k] * a.cache.values.page + place[k] * a.cache.values.slot;
+            if constexpr (kKeysOfLoad > 16) {
+                const uint64_t second = page[k + 1] * a.cache.values.page + place[k + 1] * a.cache.values.slot;
+                rows = lane / S::kLanes >= 16u ? second : rows;
+            }
+            raw.v[n] = *reinterpret_cast<const u32x4*>(a.cache.values.base + rows + kv_head * a.cache.values.head + value_offset[n]);
+        }
+        if constexpr (!kFloat) {
+            uint32_t my_page = page[0], my_place = place[0];
+#pragma unroll
+            for (uint32_t k = 1; k < S::kKeyTiles; k++) {
+                my_page = scale_key / 16u == k ? page[k] : my_page;
+                my_place = scale_key / 16u == k ? place[k] : my_place;
+            }
+            raw.halves = 0;
+#pragma unroll
+            for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                const CacheSide& side = of_values(n) ? a.cache.values : a.cache.keys;
+                const uint64_t index = my_page * side.scale_page + kv_head * side.scale_head + (my_place + scale_key % 16u) * side.scale_slot +
+                                       (min(n % kPer * 32u, dim - 1u) >> split.block_log2) * side.scale_block;
+                raw.scale[n] = words.load(side.scales, index);
+                raw.halves |= words.half(side.scales, index) << n;
+            }
+        }
+    };
+
+    f32x4 out[kTiles][kOut] = {};
+    float top[kTiles], sum[kTiles];
+#pragma unroll
+    for (uint32_t r = 0; r < kTiles; r++) top[r] = -INFINITY, sum[r] = 0.0f;
+    int32_t power = -126;  // of the largest scale of the values so far: they are taken times 2^-power
+
+    Raw raw, next;
+    uint32_t nth = 0;
+    if (from + wave < to) {
+        look_up(from + wave);
+        load(from + wave, 0, raw);
+    }
+    for (uint32_t step = from + wave; step < to; step += 4, nth++) {
+        if ((nth + 1u) % kAhead == 0) look_up(step + 4u);
+        load(step + 4u, nth + 1u, next);
+        const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys);
+        const bool partial = key0 < all_low || key0 + static_cast<int32_t>(S::kKeys) - 1 > all_high;
+
+        // this step's values and scales into LDS
+#pragma unroll
+        for (uint32_t n = 0; n < S::kLoads; n++)
+            *reinterpret_cast<u32x4*>(mine + (n * 64u + lane) / S::kLanes * S::kPitch + lane % S::kLanes * S::kLane) = raw.v[n];
+        if constexpr (!kFloat) {
+            const int32_t key = key0 + static_cast<int32_t>(scale_key);
+            const bool any = key >= low && key <= high;  // what no row sees is not looked at
+            float scale[S::kScaleLoads];
+            uint32_t most = 0;
+#pragma unroll
+            for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                const float v = words.number(raw.scale[n], raw.halves >> n & 1u);
+                scale[n] = any ? v : 0.0f;
+                const uint32_t field = f32_bits(scale[n]) >> 23 & 255u;
+                if (of_values(n)) most = max(most, field == 255u ? 0u : field);
+            }
+            const int32_t now = static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave_max_bits(most))) - 127;
+            if (now > power) {
+                const float shrink = ldexpf(1.0f, power - min(now, 126));
+                power = min(now, 126);
+#pragma unroll
+                for (uint32_t r = 0; r < kTiles; r++)
+#pragma unroll
+                    for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
+            }
+            const float down = bits_f32(static_cast<uint32_t>(127 - power) << 23);
+#pragma unroll
+            for (uint32_t n = 0; n < S::kScaleLoads; n++) scales_at[((of_values(n) ? kPer : 0u) + n % kPer) * S::kKeys + scale_key] = of_values(n) ? scale[n] * down : scale[n];
+        }
+        fence();
+
+        // scores
+        f32x4 s[kTiles][S::kKeyTiles];
+#pragma unroll
+        for (uint32_t k = 0; k < S::kKeyTiles; k++) {
+            u32x4 operand[S::kSlices];
+#pragma unroll
+            for (uint32_t u = 0; u < S::kUnits; u++) {
+                uint32_t* const w = raw.k[k][u];
+                if (row_bytes < S::kRow) {  // a shorter head: what lies past its end
+#pragma unroll
+                    for (uint32_t e = 0; e < S::kWords; e++) w[e] = key_byte(u) < row_bytes ? w[e] : 0u;
+                }
+                if constexpr (kPer > 1 && S::kWords == 4) {
+                    swap_halves(w[0], w[2]), swap_halves(w[1], w[3]);
+                    if constexpr (S::kBits == 4) swap_quarters(w[0], w[1]), swap_quarters(w[2], w[3]);
+                } else if constexpr (kPer > 1) {
+                    swap_halves(w[0], w[1]);
+                }
+                if constexpr (kFloat) {
+                    operand[u] = u32x4{w[0], w[1], w[2], w[3]};
+                } else if constexpr (S::kBits == 8) {
+                    operand[2 * u] = numbers<kCode>(w[0], w[1]);
+                    operand[2 * u + 1] = numbers<kCode>(w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < S::kWords; e++) operand[u * S::kWords + e] = numbers<kCode>(w[e], 0);
+                }
+            }
+            if constexpr (kPer == 1) {
+                f32x4 by = {1.0f, 1.0f, 1.0f, 1.0f};
+                if constexpr (!kFloat) by = *reinterpret_cast<const f32x4*>(scales_at + k * 16u + 4u * g);
+#pragma unroll
+                for (uint32_t r = 0; r < kTiles; r++) {
+                    f32x4 v = {};
+#pragma unroll
+                    for (uint32_t t = 0; t < S::kSlices; t++) v = mfma16<kBF16>(operand[t], q[r][t], v);
+                    s[r][k] = kFloat ? v : v * by;
+                }
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < S::kSlices; t++) {
+                    const f32x4 by = *reinterpret_cast<const f32x4*>(scales_at + t * S::kKeys + k * 16u + 4u * g);
+#pragma unroll
+                    for (uint32_t r = 0; r < kTiles; r++) {
+                        const f32x4 v = mfma16<kBF16>(operand[t], q[r][t], f32x4{});
+                        s[r][k] = t == 0 ? v * by : __builtin_elementwise_fma(v, by, s[r][k]);
+                    }
+                }
+            }
+        }
+
+        // weights: exp2(t - top) * 2^13, which f16 holds down to 2^-37 of the largest
+        float p[kTiles][S::kKeyTiles * 4];
+#pragma unroll
+        for (uint32_t r = 0; r < kTiles; r++) {
+            float most = -INFINITY;
+#pragma unroll
+            for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    float t = s[r][k][e] * times[r];
+                    const int32_t key = key0 + static_cast<int32_t>(k * 16u + 4u * g + e);
+                    if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
+                    if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
+                    if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
+                    p[r][k * 4 + e] = t;
+                    most = fmaxf(most, t);
+                }
+            most = max_of_groups(most);
+            if (__builtin_amdgcn_ballot_w64(most > top[r])) {
+                const float before = top[r];
+                top[r] = fmaxf(top[r], most);
+                const float shrink = top[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - top[r]);
+                sum[r] *= shrink;
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
+            }
+            const float less = 13.0f - (top[r] == -INFINITY ? 0.0f : top[r]);
+#pragma unroll
+            for (uint32_t k = 0; k < S::kKeyTiles * 4; k++) {
+                p[r][k] = __builtin_amdgcn_exp2f(p[r][k] + less);
+                sum[r] += p[r][k];
+            }
+        }
+
+        // the second product; `hide`: entries that the row `only` of each tile does not see count as nothing, and only that row is computed
+        const auto weights_of = [&](uint32_t r, uint32_t block, uint32_t half, bool hide, bool mine_only) {
+            float w[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 2; k++) {
+                f32x4 by = {1.0f, 1.0f, 1.0f, 1.0f};
+                if constexpr (!kFloat) by = *reinterpret_cast<const f32x4*>(scales_at + (kPer + block) * S::kKeys + (half * 2u + k) * 16u + 4u * g);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    const float of = p[r][(half * 2u + k) * 4u + e];
+                    float v = kFloat ? of : of * by[e];
+                    if (partial) v = of == 0.0f ? 0.0f : v;  // a scale that is not a number, of an entry that is not seen
+                    w[k * 4 + e] = !hide || mine_only ? v : 0.0f;
+                }
+            }
+            u32x4 packed;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) packed[e] = pair_of<kBF16>(w[place_of<kCode>(2 * e)], w[place_of<kCode>(2 * e + 1)]);
+            return packed;
+        };
+        constexpr uint32_t kHalves = S::kKeyTiles / 2;  // matrix instructions of a step and a tile of entries
+        const auto values_of = [&](uint32_t e, u32x4* v) {
+            if constexpr (kFloat) {
+#pragma unroll
+                for (uint32_t k = 0; k < 2; k++) {
+                    const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(CQ_LDS_AT(i16x4, mine + (k * 16u + 4u * g + i / 4u) * S::kPitch + e * 32u + i % 4u * 8u));
+                    const u32x2 w = __builtin_bit_cast(u32x2, four);
+                    v[0][2 * k] = w[0], v[0][2 * k + 1] = w[1];
+                }
+            } else if constexpr (S::kBits == 8) {
+                const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(CQ_LDS_AT(i32x2, mine + (i / 8u * 16u + 4u * g + i / 2u % 4u) * S::kPitch + e * 16u + i % 2u * 8u));
+                v[0] = numbers<kCode>(w[0], w[1]);
+            } else {
+                const auto w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(CQ_LDS_AT(i32x2, mine + (i / 4u * 16u + 4u * g + i % 4u) * S::kPitch + e * 8u));
+                v[0] = numbers<kCode>(w[0], 0), v[1] = numbers<kCode>(w[1], 0);
+            }
+        };
+        const auto multiply = [&](bool hide, uint32_t only) {
+            u32x4 w[kTiles][kHalves];
+#pragma unroll
+            for (uint32_t e = 0; e < kOut; e++) {
+                if (e == 0 || (kPer > 1 && e % 2 == 0))
+#pragma unroll
+                    for (uint32_t r = 0; r < kTiles; r++)
+#pragma unroll
+                        for (uint32_t half = 0; half < kHalves; half++) w[r][half] = weights_of(r, kPer > 1 ? e / 2u : 0u, half, hide, i == only);
+                u32x4 entries[kHalves];
+                values_of(e, entries);
+#pragma unroll
+                for (uint32_t r = 0; r < kTiles; r++)
+#pragma unroll
+                    for (uint32_t half = 0; half < kHalves; half++) {
+                        u32x4 seen = entries[half];
+                        if (hide) {
+                            const int32_t of_low = __builtin_amdgcn_readlane(row_low[r], only), of_high = __builtin_amdgcn_readlane(row_high[r], only);
+#pragma unroll
+                            for (uint32_t pair = 0; pair < 4; pair++)
+#pragma unroll
+                                for (uint32_t k = 0; k < 2; k++) {
+                                    const uint32_t nth_key = place_of<kCode>(2 * pair + k);
+                                    const int32_t key = key0 + static_cast<int32_t>((half * 2u + nth_key / 4u) * 16u + 4u * g + nth_key % 4u);
+                                    if (key < of_low || key > of_high) seen[pair] &= k ? 0x0000ffffu : 0xffff0000u;
+                                }
+                        }
+                        const f32x4 v = mfma16<kBF16>(seen, w[r][half], out[r][e]);
+                        out[r][e] = !hide || i == only ? v : out[r][e];  // for other rows than `only` a weight of zero may have met an infinity
+                    }
+            }
+        };
+        bool odd = false;
+        if constexpr (kCodeHasNaN<kCode>) {
+            // Entries that are infinite or not a number, among keys that not every row sees: weights of zero do not keep them out of a sum.
+            if (partial) {
+                constexpr uint32_t kExponent = kBF16 ? 0x7f80u : 0x7c00u;
+                bool found = false;
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++) {
+                    u32x4 v[kHalves];
+                    values_of(e, v);
+#pragma unroll
+                    for (uint32_t half = 0; half < kHalves; half++)
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; k++)
+                            found = found || (v[half][k] & kExponent) == kExponent || (v[half][k] >> 16 & kExponent) == kExponent;
+                }
+                odd = __builtin_amdgcn_ballot_w64(found) != 0;
+            }
+        }
+        if (!odd)
+            multiply(false, 0);
+        else
+            for (uint32_t only = 0; only < 16; only++) multiply(true, only);
+        fence();
+        raw = next;
+    }
+
+    // The four waves' results, each over its own sum, by their shares of the whole.
+    __syncthreads();
+    constexpr uint32_t kOutPitch = kDim + 4;
+    float* const result = reinterpret_cast<float*>(lds);
+    float* const tops = result + kRows * kOutPitch;  // [wave][row]
+    float* const sums = tops + 4 * kRows;
+    const float up = ldexpf(1.0f, power);
+#pragma unroll
+    for (uint32_t r = 0; r < kTiles; r++) {
+        sum[r] = sum_of_groups(sum[r]);
+        if (g == 0) tops[wave * kRows + r * 16u + i] = top[r], sums[wave * kRows + r * 16u + i] = sum[r];
+    }
+    __syncthreads();
+    const auto share_of = [&](uint32_t row, uint32_t of, float* most_out, float* all_out) {
+        float most = -INFINITY, all = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < 4; w++) most = fmaxf(most, tops[w * kRows + row]);
+        const float zero = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+        for (uint32_t w = 0; w < 4; w++) all += sums[w * kRows + row] * __builtin_amdgcn_exp2f(tops[w * kRows + row] - zero);
+        *most_out = most, *all_out = all;
+        return __builtin_amdgcn_exp2f(tops[of * kRows + row] - zero);
+    };
+    for (uint32_t w = 0; w < 4; w++) {
+        if (wave == w)
+#pragma unroll
+            for (uint32_t r = 0; r < kTiles; r++) {
+                float most, all;
+                const float share = share_of(r * 16u + i, w, &most, &all);
+                const float by = sum[r] == 0.0f ? 0.0f : share / all;
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++) {
+                    f32x4* const to_row = reinterpret_cast<f32x4*>(result + (r * 16u + i) * kOutPitch + e * 16u + 4u * g);
+                    f32x4 v = {};
+                    if (by != 0.0f || sum[r] != 0.0f) v = out[r][e] * by * (kFloat ? 1.0f : up);
+                    *to_row = w == 0 ? v : *to_row + v;
+                }
+            }
+        __syncthreads();
+    }
+    const uint32_t fours = dim / 4u;
+    for (uint32_t n = threadIdx.x; n < at.rows * fours; n += 256) {
+        const uint32_t row = n / fours, d = n % fours * 4u, in_sequence = at.row0 + row;
+        const uint32_t token = at.s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(result + row * kOutPitch + d);
+        if (split.splits == 1) {
+            const bool bf16 = a.dtype == CQ_BF16;
+            const u32x2 w = bf16 ? u32x2{pair_of<true>(v[0], v[1]), pair_of<true>(v[2], v[3])} : u32x2{pair_of<false>(v[0], v[1]), pair_of<false>(v[2], v[3])};
+            *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) = w;
+        } else {
+            const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
+            *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = v;
+            if (d == 0) {
+                float most, all;
+                (void)share_of(row, 0, &most, &all);
+                split.stats[2 * of] = most, split.stats[2 * of + 1] = all;
+            }
+        }
+    }
+}
+
+template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
+hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+    using S = Shape<kCode, kDim, kPer>;
+    const uint32_t waves = 4 * S::kWaveBytes, join = 16 * kTiles * (kDim + 4 + 8) * 4;
+    hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(split.tiles * split.splits, a.cache.kv_heads), dim3(256),
+                       waves > join ? waves : join, s, a, split);
+    return hipGetLastError();
+}
+
+template <int kCode, int kDim, int kPer>
+hipError_t launch_tiles(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+    const auto by_type = [&](auto tiles) {
+        if constexpr (kCode == kCacheFloat)
+            if (a.dtype == CQ_BF16) return launch_few<kCode, kDim, kPer, tiles.value, true>(s, a, split);
+        return launch_few<kCode, kDim, kPer, tiles.value, false>(s, a, split);
+    };
+    if (split.row_tiles == 1) return by_type(std::integral_constant<int, 1>{});
+    return by_type(std::integral_constant<int, 2>{});
+}
+
+template <int kCode, int kDim>
+hipError_t launch_blocks(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+    if constexpr (kCode != kCacheFloat)
+        if (a.cache.block < a.cache.dim) return launch_tiles<kCode, kDim, kDim / 32>(s, a, split);
+    return launch_tiles<kCode, kDim, 1>(s, a, split);
+}
+
+}  // namespace
+
+#define CQ_FEW_NAME2(c) launch_attention_few_##c
+#define CQ_FEW_NAME(c) CQ_FEW_NAME2(c)
+hipError_t CQ_FEW_NAME(CQ_TU_CODE)(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+    if (a.cache.dim <= 64) return launch_blocks<CQ_TU_CODE, 64>(s, a, split);
+    if (a.cache.dim <= 128) return launch_blocks<CQ_TU_CODE, 128>(s, a, split);
+    return launch_blocks<CQ_TU_CODE, 256>(s, a, split);
+}
+
+}  // namespace cq
