@@ -31,54 +31,57 @@ bool tiles_take(const AttentionArgs& a) {
     return rows(c.keys) && rows(c.values) && on(a.q, 16) && a.q_token % 8 == 0 && a.q_head % 8 == 0 && on(a.y, 8) && a.y_token % 4 == 0 && a.y_head % 4 == 0;
 }
 
-// Sequences of up to 32 rows on the mean go by tiles of 16 or 32.
-bool few_rows(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.group <= 64ull * a.seqs; }
-
 constexpr uint32_t kMostSplits = 64;  // a lane each in attention_join_kernel
 
-// Enough splits that about four workgroups come to a compute unit, none of less than 512 keys.
-FewSplit few_split(const AttentionArgs& a, uint64_t room) {
-    FewSplit f{};
+uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4; }
+
+// Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (128 of longer
+// heads) by attention_many_kernel.  The keys are split so that `wanted` workgroups come to the GPU, none with less than `fewest` keys.
+Split split_of(const AttentionArgs& a, uint64_t room) {
+    Split f{};
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, mean = (rows + a.seqs - 1) / a.seqs;
-    f.row_tiles = mean <= 16 ? 1 : 2;
-    f.tiles = static_cast<uint32_t>(rows / (16 * f.row_tiles) + a.seqs);
-    const uint64_t busy = a.seqs * ((mean + 16 * f.row_tiles - 1) / (16 * f.row_tiles)) * a.cache.kv_heads;
-    const uint64_t keys = static_cast<uint64_t>(a.width) * a.cache.page_size;
-    uint64_t splits = (1024 + busy - 1) / busy, most = keys / 512;
+    f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? 2 : 0;
+    const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : 256;
+    const uint64_t wanted = f.row_tiles ? 1024 : 256, fewest = f.row_tiles ? 512 : 1024;
+    f.tiles = static_cast<uint32_t>(rows / of_tile + a.seqs);
+    const uint64_t busy = a.seqs * ((mean + of_tile - 1) / of_tile) * a.cache.kv_heads;
+    const uint64_t most = static_cast<uint64_t>(a.width) * a.cache.page_size / fewest;
+    uint64_t splits = (wanted + busy - 1) / busy;
     splits = splits < most ? splits : most;
     splits = splits < kMostSplits ? splits : kMostSplits;
-    const uint64_t each = static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4;
-    if (splits > 1 && each * splits > room) splits = room / each;
+    if (splits > 1 && part_bytes(a) * splits > room) splits = room / part_bytes(a);
     f.splits = splits > 1 ? static_cast<uint32_t>(splits) : 1;
     f.parts = static_cast<float*>(a.workspace);
     f.stats = f.parts + static_cast<uint64_t>(a.tokens) * a.heads * f.splits * a.cache.dim;
     magic_of(a.cache.page_size / 16, &f.page_magic, &f.page_shift);
-    f.block_log2 = log2_below(a.cache.block);
+    f.block_log2 = a.cache.block == a.cache.dim ? 31 : log2_below(a.cache.block);
     return f;
 }
 
-bool fits_a_launch(const FewSplit& f) { return static_cast<uint64_t>(f.tiles) * f.splits * 256 < kLaunchThreads; }
+bool fits_a_launch(const AttentionArgs& a, const Split& f) {
+    return static_cast<uint64_t>(f.tiles) * f.splits * (f.row_tiles ? 1 : a.cache.kv_heads) * 256 < kLaunchThreads;
+}
 
 }  // namespace
 
 uint64_t attention_workspace_bytes(const AttentionArgs& a) {
-    if (a.tokens == 0 || a.heads == 0 || a.seqs == 0 || !tiles_take(a) || !few_rows(a)) return 0;
-    const FewSplit f = few_split(a, ~0ull);
-    return f.splits == 1 ? 0 : static_cast<uint64_t>(a.tokens) * a.heads * f.splits * (a.cache.dim + 2) * 4;
+    if (a.tokens == 0 || a.heads == 0 || a.seqs == 0 || !tiles_take(a)) return 0;
+    const Split f = split_of(a, ~0ull);
+    return f.splits == 1 ? 0 : part_bytes(a) * f.splits;
 }
 
 hipError_t launch_attention(hipStream_t s, const AttentionArgs& a) {
-    if (!tiles_take(a) || !few_rows(a)) return launch_attention_general(s, a);
-    const FewSplit f = few_split(a, a.workspace_bytes);
-    if (!fits_a_launch(f)) return launch_attention_general(s, a);
-    const auto few = [&]() -> hipError_t {
+    if (!tiles_take(a)) return launch_attention_general(s, a);
+    const Split f = split_of(a, a.workspace_bytes);
+    if (!fits_a_launch(a, f)) return launch_attention_general(s, a);
+    const auto tiles = [&]() -> hipError_t {
         switch (a.cache.code) {
-#define CQ_CASE_FEW(c) case c: return launch_attention_few_##c(s, a, f);
-            CQ_FOR_CODES(CQ_CASE_FEW)
+#define CQ_CASE_TILES(c) case c: return f.row_tiles ? launch_attention_few_##c(s, a, f) : launch_attention_many_##c(s, a, f);
+            CQ_FOR_CODES(CQ_CASE_TILES)
             default: return hipErrorInvalidValue;
         }
     };
-    const hipError_t e = few();
+    const hipError_t e = tiles();
     return e != hipSuccess || f.splits == 1 ? e : launch_attention_join(s, a, f);
 }
 

@@ -65,17 +65,19 @@ uint64_t attention_workspace_bytes(const AttentionArgs& a);
 hipError_t launch_attention(hipStream_t s, const AttentionArgs& a);
 hipError_t launch_attention_general(hipStream_t s, const AttentionArgs& a);
 
-// How the few rows of attention_few_kernel and the keys they see are shared out.
-struct FewSplit {
-    uint32_t tiles, row_tiles;  // workgroups for rows; tiles of 16 rows of one
+// How rows and the keys they see are shared out between workgroups.
+struct Split {
+    uint32_t tiles, row_tiles;  // workgroups for rows; tiles of 16 rows of one (attention_few_kernel)
     uint32_t splits;            // of the keys
     uint32_t page_magic, page_shift, block_log2;  // division by the tiles of 16 keys of a page; log2 of a scale's entries
     float *parts, *stats;  // splits > 1: [token][head][split][dim], each over its own sum; [token][head][split]{largest score, sum}
 };
 #define CQ_FOR_CODES(x) x(0) x(1) x(2) x(3) x(4) x(5)
-#define CQ_DECLARE_FEW(c) hipError_t launch_attention_few_##c(hipStream_t s, const AttentionArgs& a, const FewSplit& split);
-CQ_FOR_CODES(CQ_DECLARE_FEW)
-hipError_t launch_attention_join(hipStream_t s, const AttentionArgs& a, const FewSplit& split);
+#define CQ_DECLARE_TILES(c)                                                                            \
+    hipError_t launch_attention_few_##c(hipStream_t s, const AttentionArgs& a, const Split& split); \
+    hipError_t launch_attention_many_##c(hipStream_t s, const AttentionArgs& a, const Split& split);
+CQ_FOR_CODES(CQ_DECLARE_TILES)
+hipError_t launch_attention_join(hipStream_t s, const AttentionArgs& a, const Split& split);
 
 constexpr uint32_t kCopyTensors = 32;
 struct CopyArgs {

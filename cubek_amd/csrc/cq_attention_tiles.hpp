@@ -77,6 +77,36 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+template <bool kBF16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (kBF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+#define CQ_LDS_AT(T, p) ((__attribute__((address_space(3))) T*)(p))
+typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+
+// The exponent field of the power of two that a row of queries is divided by, so that its largest entry lies between 1 and 2; f16 stays as it is, and
+// so does a row of zeros or with an infinity.
+__device__ __forceinline__ uint32_t power_of_row(float most, bool bf16) {
+    const uint32_t field = f32_bits(most) >> 23;
+    return bf16 && field > 0u && field < 255u ? min(field, 253u) : 127u;
+}
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+    v = max(v, dpp<kDppXor1>(v));
+    v = max(v, dpp<kDppXor2>(v));
+    v = max(v, dpp<kDppHalfMirror>(v));
+    v = max(v, dpp<kDppMirror>(v));
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(halves[0], halves[1]);
+    const auto quarters = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(quarters[0], quarters[1]);
+}
+
 // The larger of a value's copies in the four groups of 16 lanes.
 __device__ __forceinline__ float max_of_groups(float v) {
     const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);

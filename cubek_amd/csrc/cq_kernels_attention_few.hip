@@ -18,23 +18,8 @@
 namespace cq {
 namespace {
 
-#define CQ_LDS_AT(T, p) ((__attribute__((address_space(3))) T*)(p))
-typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
-typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
-
 // Between a wave's writes to its part of LDS and its reads from it: LDS serves a wave in order, so only the compiler has to keep it.
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
-
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
-    v = max(v, dpp<kDppXor1>(v));
-    v = max(v, dpp<kDppXor2>(v));
-    v = max(v, dpp<kDppHalfMirror>(v));
-    v = max(v, dpp<kDppMirror>(v));
-    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = max(halves[0], halves[1]);
-    const auto quarters = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return max(quarters[0], quarters[1]);
-}
 
 template <int kCode, int kDim, int kPer>
 struct Shape {
@@ -84,7 +69,7 @@ __device__ __forceinline__ void swap_quarters(uint32_t& a, uint32_t& b) {
 }
 
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
-__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, FewSplit split) {
+__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Split split) {
     using S = Shape<kCode, kDim, kPer>;
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kRowsLog2 = kTiles == 1 ? 4 : 5, kRows = 16 * kTiles;
@@ -137,9 +122,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Few
                 for (uint32_t e = 0; e < 8; e++) most = fmaxf(most, fabsf(v[e]));
             }
             most = max_of_groups(most);
-            // 2^-p with 2^p <= most < 2^(p + 1): the largest entry between 1 and 2 (none, infinite: as it is)
-            const uint32_t field = f32_bits(most) >> 23;
-            const uint32_t power = bf16 && field > 0u && field < 255u ? min(max(field, 1u), 253u) : 127u;
+            const uint32_t power = power_of_row(most, bf16);
             const float down = bits_f32((254u - power) << 23);
 #pragma unroll
             for (uint32_t t = 0; t < S::kSlices; t++) {
@@ -531,7 +514,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Few
 }
 
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
-hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const Split& split) {
     using S = Shape<kCode, kDim, kPer>;
     const uint32_t waves = 4 * S::kWaveBytes, join = 16 * kTiles * (kDim + 4 + 8) * 4;
     hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(split.tiles * split.splits, a.cache.kv_heads), dim3(256),
@@ -540,7 +523,7 @@ hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const FewSplit& spl
 }
 
 template <int kCode, int kDim, int kPer>
-hipError_t launch_tiles(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+hipError_t launch_tiles(hipStream_t s, const AttentionArgs& a, const Split& split) {
     const auto by_type = [&](auto tiles) {
         if constexpr (kCode == kCacheFloat)
             if (a.dtype == CQ_BF16) return launch_few<kCode, kDim, kPer, tiles.value, true>(s, a, split);
@@ -551,7 +534,7 @@ hipError_t launch_tiles(hipStream_t s, const AttentionArgs& a, const FewSplit& s
 }
 
 template <int kCode, int kDim>
-hipError_t launch_blocks(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+hipError_t launch_blocks(hipStream_t s, const AttentionArgs& a, const Split& split) {
     if constexpr (kCode != kCacheFloat)
         if (a.cache.block < a.cache.dim) return launch_tiles<kCode, kDim, kDim / 32>(s, a, split);
     return launch_tiles<kCode, kDim, 1>(s, a, split);
@@ -561,7 +544,7 @@ hipError_t launch_blocks(hipStream_t s, const AttentionArgs& a, const FewSplit& 
 
 #define CQ_FEW_NAME2(c) launch_attention_few_##c
 #define CQ_FEW_NAME(c) CQ_FEW_NAME2(c)
-hipError_t CQ_FEW_NAME(CQ_TU_CODE)(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+hipError_t CQ_FEW_NAME(CQ_TU_CODE)(hipStream_t s, const AttentionArgs& a, const Split& split) {
     if (a.cache.dim <= 64) return launch_blocks<CQ_TU_CODE, 64>(s, a, split);
     if (a.cache.dim <= 128) return launch_blocks<CQ_TU_CODE, 128>(s, a, split);
     return launch_blocks<CQ_TU_CODE, 256>(s, a, split);

@@ -9,7 +9,7 @@
 namespace cq {
 namespace {
 
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, FewSplit split, uint32_t row0) {
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Split split, uint32_t row0) {
     const uint32_t lane = threadIdx.x & 63u, row = row0 + blockIdx.x * 4u + (threadIdx.x >> 6);
     if (row >= a.tokens * a.heads) return;
     const uint32_t token = row / a.heads, head = row % a.heads;
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Fe
 
 }  // namespace
 
-hipError_t launch_attention_join(hipStream_t s, const AttentionArgs& a, const FewSplit& split) {
+hipError_t launch_attention_join(hipStream_t s, const AttentionArgs& a, const Split& split) {
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
     constexpr uint64_t kPiece = (kLaunchThreads / 256 - 1) * 4;
     for (uint64_t row = 0; row < rows; row += kPiece) {

@@ -1,0 +1,442 @@
+// Attention of many rows (token, head of a group): prompts and their chunks.  An object per kind of code (CQ_TU_CODE).
+//
+// A workgroup takes 256 rows (128 of heads longer than 128) that share a head of the cache, a wave 64 of them.  Keys come 64 at a time: the
+// workgroup loads their codes one step ahead, makes numbers of f16 of them (a cache of floats: as they are) and lays keys and values into LDS, two
+// steps in turn, one barrier a step.  Each wave then computes S^T = K Q^T and O^T = V^T P^T by 32 x 32 x 16 matrix instructions with queries,
+// weights and results in registers: the scores that lane (n, h) gets are those of row n, and stand in the order of keys in which the second product takes
+// its weights; values are read transposed.
+// 64 rows a wave, so that LDS is read at half of what it can give; a step is 2048 cycles of matrix instructions beside about as many of the
+// softmax's vector instructions.
+// Entries are scaled by powers of two (of the largest scale so far, one for keys, one for values; queries by one per row), so that f16 holds them whatever
+// the range of bf16; each is rounded once to 11 bits, where dequantize for bf16 would round to 8.
+#include <hip/hip_runtime.h>
+
+#include "cq_attention_tiles.hpp"
+#include "cq_magic_div.hpp"
+
+namespace cq {
+namespace {
+
+template <int kCode, int kDim>
+struct Many {
+    static constexpr uint32_t kBits = kCodeBits<kCode>, kKeys = 64, kRowTiles = kDim > 128 ? 1 : 2, kRowsLog2 = kRowTiles == 1 ? 7 : 8;
+    static constexpr uint32_t kRow = kDim * kBits / 8;                                                  // bytes of a key as it is stored
+    static constexpr uint32_t kChunk = kRow == 32 ? 8 : 16, kLanes = kRow / kChunk;                      // of a thread; threads of a row
+    static constexpr uint32_t kEntries = kChunk * 8 / kBits, kChunks = kKeys * kLanes / 256;             // entries of a chunk; chunks of a thread
+    static constexpr uint32_t kPitch = kDim * 2 + 16, kSide = kKeys * kPitch, kBuffer = 2 * kSide;       // bytes in LDS: of a row, of keys or values, of both
+};
+
+// Eight numbers in the order of their entries.
+template <int kCode>
+__device__ __forceinline__ u32x4 in_order(u32x4 v) {
+    if constexpr (kCode != kCacheInt4) return v;
+    return u32x4{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x05040100u), __builtin_amdgcn_perm(v[1], v[0], 0x07060302u),
+                 __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
+}
+
+template <int kCode, int kDim, bool kBF16>
+__global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel(AttentionArgs a, Split split) {
+    using S = Many<kCode, kDim>;
+    constexpr bool kFloat = kCode == kCacheFloat;
+    constexpr uint32_t kR = S::kRowTiles, kSlices = kDim / 16, kOut = kDim / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][wave][keys, values]
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31u, h = lane >> 5;
+    // neighbours in the grid are heads of the cache: with eight of them each die keeps one in its L2.  The tiles with most keys come first.
+    const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads, part = rest % split.splits;
+    const uint32_t tile = split.tiles - 1u - rest / split.splits, dim = a.cache.dim;
+
+    RowTile at;
+    if (!find_rows(a, tile, S::kRowsLog2, &at)) return;
+    const auto position_of = [&](uint32_t row) { return at.s.position + static_cast<int32_t>((at.row0 + row) / a.group); };
+    const int32_t low = seen_from(a, at.s, position_of(0)).low, high = seen_from(a, at.s, position_of(at.rows - 1u)).high;
+    const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
+    const uint32_t each = (steps_all + split.splits - 1u) / split.splits;
+    const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
+    const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
+
+    // the wave's rows, and the keys that some of them see and that all of them do
+    const uint32_t wave_row = wave * (32u * kR), wave_last = min(wave_row + 32u * kR, at.rows) - 1u;
+    const bool rows_here = wave_row < at.rows;
+    const Seen first = seen_from(a, at.s, position_of(min(wave_row, at.rows - 1u))), last = seen_from(a, at.s, position_of(rows_here ? wave_last : at.rows - 1u));
+    const int32_t wave_low = first.low, wave_high = rows_here ? last.high : -1, all_low = last.low, all_high = first.high;
+
+    u32x4 q[kR][kSlices];
+    float times[kR], slope[kR];
+    int32_t position[kR], row_low[kR], row_high[kR];
+#pragma unroll
+    for (uint32_t r = 0; r < kR; r++) {
+        const uint32_t own = wave_row + r * 32u + n, row = min(own, at.rows - 1u) + at.row0, token = at.s.first + row / a.group, head = kv_head * a.group + row % a.group;
+        position[r] = at.s.position + static_cast<int32_t>(row / a.group);
+        const Seen seen = seen_from(a, at.s, position[r]);
+        row_low[r] = seen.low, row_high[r] = own < at.rows ? seen.high : -1;
+        slope[r] = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
+        const char* const from_q = a.q + (token * a.q_token + head * a.q_head) * 2u;
+#pragma unroll
+        for (uint32_t t = 0; t < kSlices; t++) {
+            const uint32_t d = 16u * t + 8u * h;
+            q[r][t] = d < dim ? *reinterpret_cast<const u32x4*>(from_q + d * 2u) : u32x4{0, 0, 0, 0};
+        }
+        times[r] = a.scale;
+        if constexpr (!kFloat) {
+            float most = 0.0f, v[8];
+            const bool bf16 = a.dtype == CQ_BF16;
+            const auto unpack = [&](u32x4 w) { bf16 ? BF16::unpack(w, v) : F16::unpack(w, v); };
+#pragma unroll
+            for (uint32_t t = 0; t < kSlices; t++) {
+                unpack(q[r][t]);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) most = fmaxf(most, fabsf(v[e]));
+            }
+            const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
+            most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
+            const uint32_t down = power_of_row(most, bf16);
+#pragma unroll
+            for (uint32_t t = 0; t < kSlices; t++) {
+                unpack(q[r][t]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) q[r][t][e] = pair_of<false>(v[2 * e] * bits_f32((254u - down) << 23), v[2 * e + 1] * bits_f32((254u - down) << 23));
+            }
+            times[r] *= bits_f32(down << 23);
+        }
+        times[r] *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
+    }
+    const float cap = a.cap * kLog2E;
+
+    // Pages of the next 16 steps, a lane a tile of 16 keys.
+    const uint32_t tiles_of_page = a.cache.page_size / 16u;
+    const auto tile_of = [&](uint32_t step, uint32_t k) { return min((step0 + step) * 4u + k, last_tile); };
+    uint32_t pages = 0;
+    const auto look_up = [&](uint32_t step) { pages = page_of(a, at.s, magic_div(tile_of(step + lane / 4u, lane % 4u), split.page_magic, split.page_shift)); };
+    const auto place_of_tile = [&](uint32_t t) { return (t - magic_div(t, split.page_magic, split.page_shift) * tiles_of_page) * 16u; };
+
+    // What a thread brings of a step: chunks of keys and of values, and their scales.
+    struct Raw {
+        uint32_t k[S::kChunks][S::kChunk / 4], v[S::kChunks][S::kChunk / 4];
+    };
+    struct Scales {
+        uint32_t k[S::kChunks], v[S::kChunks], halves;
+    };
+    const ScaleWords words(a.cache.param_dtype);
+    const uint32_t row_bytes = dim * S::kBits / 8u, byte = threadIdx.x % S::kLanes * S::kChunk, entry = byte * 8u / S::kBits;
+    const uint32_t block = min(entry, dim - 1u) >> split.block_log2;
+    const auto key_of = [&](uint32_t c) { return (c * 256u + threadIdx.x) / S::kLanes; };
+    // the page of a chunk's tile of 16 keys (the same for the wave) and the row in it
+    const auto place = [&](uint32_t step, uint32_t c, uint32_t* page, uint32_t* slot) {
+        const uint32_t k = __builtin_amdgcn_readfirstlane(key_of(c) / 16u);
+        *page = __builtin_amdgcn_readlane(pages, (step - from) % 16u * 4u + k);
+        *slot = place_of_tile(tile_of(step, k)) + key_of(c) % 16u;
+    };
+    const auto load = [&](uint32_t step, Raw& raw) {
+#pragma unroll
+        for (uint32_t c = 0; c < S::kChunks; c++) {
+            uint32_t page, slot;
+            place(step, c, &page, &slot);
+            const uint64_t at_byte = min(byte, row_bytes - S::kChunk);
+            const char* const k = a.cache.keys.base + page * a.cache.keys.page + kv_head * a.cache.keys.head + slot * a.cache.keys.slot + at_byte;
+            const char* const v = a.cache.values.base + page * a.cache.values.page + kv_head * a.cache.values.head + slot * a.cache.values.slot + at_byte;
+            if constexpr (S::kChunk == 16) {
+                const u32x4 kw = *reinterpret_cast<const u32x4*>(k), vw = *reinterpret_cast<const u32x4*>(v);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) raw.k[c][e] = kw[e], raw.v[c][e] = vw[e];
+            } else {
+                const u32x2 kw = *reinterpret_cast<const u32x2*>(k), vw = *reinterpret_cast<const u32x2*>(v);
+                raw.k[c][0] = kw[0], raw.k[c][1] = kw[1], raw.v[c][0] = vw[0], raw.v[c][1] = vw[1];
+            }
+        }
+    };
+    const auto load_scales = [&](uint32_t step, Scales& s) {
+        s.halves = 0;
+#pragma unroll
+        for (uint32_t c = 0; c < S::kChunks; c++) {
+            uint32_t page, slot;
+            place(step, c, &page, &slot);
+            const auto index = [&](const CacheSide& side) { return page * side.scale_page + kv_head * side.scale_head + slot * side.scale_slot + block * side.scale_block; };
+            const uint64_t k = index(a.cache.keys), v = index(a.cache.values);
+            s.k[c] = words.load(a.cache.keys.scales, k);
+            s.v[c] = words.load(a.cache.values.scales, v);
+            s.halves |= words.half(a.cache.keys.scales, k) << (2 * c) | words.half(a.cache.values.scales, v) << (2 * c + 1);
+        }
+    };
+    // The exponents of the largest scales of a step that any row sees, for the workgroup.
+    const auto publish = [&](uint32_t step, const Scales& s) {
+        uint32_t of_keys = 0, of_values = 0;
+#pragma unroll
+        for (uint32_t c = 0; c < S::kChunks; c++) {
+            const int32_t key = static_cast<int32_t>((step0 + step) * S::kKeys + key_of(c));
+            const auto field = [&](float v) {
+                const uint32_t f = f32_bits(v) >> 23 & 255u;
+                return key < low || key > high || f == 255u ? 0u : f;
+            };
+            of_keys = max(of_keys, field(words.number(s.k[c], s.halves >> (2 * c) & 1u)));
+            of_values = max(of_values, field(words.number(s.v[c], s.halves >> (2 * c + 1) & 1u)));
+        }
+        of_keys = wave_max_bits(of_keys), of_values = wave_max_bits(of_values);
+        if (lane == 0) powers[(step & 1u) * 8u + wave * 2u] = of_keys, powers[(step & 1u) * 8u + wave * 2u + 1u] = of_values;
+    };
+
+    f32x16 out[kR][kOut] = {};
+    float top[kR], sum[kR];
+#pragma unroll
+    for (uint32_t r = 0; r < kR; r++) top[r] = -INFINITY, sum[r] = 0.0f;
+    int32_t key_power = -126, value_power = -126;  // of the largest scales so far: entries are taken times 2^-power / 2
+
+    // A step's codes as numbers into LDS.
+    const auto lay = [&](uint32_t step, Raw& raw, const Scales& s) {
+        char* const to_keys = lds + (step & 1u) * S::kBuffer;
+        float down_keys = 0.0f, down_values = 0.0f;
+        if constexpr (!kFloat) {
+            uint32_t of_keys = 0, of_values = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < 4; w++) of_keys = max(of_keys, powers[(step & 1u) * 8u + w * 2u]), of_values = max(of_values, powers[(step & 1u) * 8u + w * 2u + 1u]);
+            const int32_t now_keys = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of_keys)) - 127, 126);
+            const int32_t now_values = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of_values)) - 127, 126);
+            key_power = max(key_power, now_keys);
+            if (now_values > value_power) {
+                const float shrink = ldexpf(1.0f, value_power - now_values);
+                value_power = now_values;
+#pragma unroll
+                for (uint32_t r = 0; r < kR; r++)
+#pragma unroll
+                    for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
+            }
+            down_keys = 0.5f * bits_f32(static_cast<uint32_t>(127 - key_power) << 23), down_values = 0.5f * bits_f32(static_cast<uint32_t>(127 - value_power) << 23);
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < S::kChunks; c++) {
+            char* const row = to_keys + key_of(c) * S::kPitch + entry * 2u;
+            if (byte >= row_bytes) {  // a shorter head: nothing past its end
+#pragma unroll
+                for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.k[c][e] = 0, raw.v[c][e] = 0;
+            }
+            if constexpr (kFloat) {
+                *reinterpret_cast<u32x4*>(row) = u32x4{raw.k[c][0], raw.k[c][1], raw.k[c][2], raw.k[c][3]};
+                *reinterpret_cast<u32x4*>(row + S::kSide) = u32x4{raw.v[c][0], raw.v[c][1], raw.v[c][2], raw.v[c][3]};
+            } else {
+                constexpr uint32_t kEach = S::kBits == 8 ? 2 : 1;  // words of eight entries
+                const auto put = [&](char* to, const uint32_t* w, float scale) {
+                    const uint32_t both = pair_of<false>(scale, scale);
+                    const f16x2 by = __builtin_bit_cast(f16x2, both);
+#pragma unroll
+                    for (uint32_t e = 0; e < S::kChunk / 4; e += kEach) {
+                        u32x4 v = in_order<kCode>(numbers<kCode>(w[e], kEach == 2 ? w[e + kEach - 1] : 0u));
+#pragma unroll
+                        for (uint32_t p = 0; p < 4; p++) {
+                            const uint32_t word = v[p];
+                            v[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, word) * by);
+                        }
+                        *reinterpret_cast<u32x4*>(to + e / kEach * 16u) = v;
+                    }
+                };
+                put(row, raw.k[c], words.number(s.k[c], s.halves >> (2 * c) & 1u) * down_keys);
+                put(row + S::kSide, raw.v[c], words.number(s.v[c], s.halves >> (2 * c + 1) & 1u) * down_values);
+            }
+        }
+    };
+
+    // Scores, weights and results of 32 keys.
+    const auto compute = [&](uint32_t step, uint32_t k) {
+        const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys + 32u * k);
+        if (key0 > wave_high || key0 + 31 < wave_low) return;
+        const bool partial = key0 < all_low || key0 + 31 > all_high;
+        const char* const keys = lds + (step & 1u) * S::kBuffer + 32u * k * S::kPitch;
+        const char* const values = keys + S::kSide;
+        f32x16 s[kR] = {};
+#pragma unroll
+        for (uint32_t t = 0; t < kSlices; t++) {
+            const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + n * S::kPitch + t * 32u + h * 16u);
+#pragma unroll
+            for (uint32_t r = 0; r < kR; r++) s[r] = mfma32<kBF16>(operand, q[r][t], s[r]);
+        }
+        u32x4 w[kR][2];
+#pragma unroll
+        for (uint32_t r = 0; r < kR; r++) {
+            float p[16], most = -INFINITY;
+            const float by = kFloat ? times[r] : times[r] * 2.0f * bits_f32(static_cast<uint32_t>(127 + key_power) << 23);
+            if (partial || a.cap > 0.0f || a.slopes) {
+#pragma unroll
+                for (uint32_t v = 0; v < 16; v++) {
+                    float t = s[r][v] * by;
+                    const int32_t key = key0 + static_cast<int32_t>(v / 4u * 8u + 4u * h + v % 4u);
+                    if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
+                    if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
+                    if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
+                    p[v] = t;
+                    most = fmaxf(most, t);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t v = 0; v < 16; v++) p[v] = s[r][v] * by, most = fmaxf(most, p[v]);
+            }
+            const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
+            most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
+            if (__builtin_amdgcn_ballot_w64(most > top[r])) {
+                const float before = top[r];
+                top[r] = fmaxf(top[r], most);
+                const float shrink = top[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - top[r]);
+                sum[r] *= shrink;
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
+            }
+            const float less = 13.0f - (top[r] == -INFINITY ? 0.0f : top[r]);
+#pragma unroll
+            for (uint32_t v = 0; v < 16; v++) {
+                p[v] = __builtin_amdgcn_exp2f(p[v] + less);
+                sum[r] += p[v];
+            }
+#pragma unroll
+            for (uint32_t v = 0; v < 16; v += 2) w[r][v / 8][v % 8 / 2] = pair_of<kBF16>(p[v], p[v + 1]);
+        }
+        // lane (n, h): entry n of 32, keys 4 h ... 4 h + 3 and 8 more
+        const auto values_of = [&](uint32_t e, uint32_t half) {
+            u32x4 v;
+#pragma unroll
+            for (uint32_t eight = 0; eight < 2; eight++) {
+                const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    CQ_LDS_AT(i16x4, values + (half * 16u + eight * 8u + 4u * h + lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + lane % 4u * 8u));
+                const u32x2 two = __builtin_bit_cast(u32x2, four);
+                v[2 * eight] = two[0], v[2 * eight + 1] = two[1];
+            }
+            return v;
+        };
+        bool odd = false;
+        if (partial) {
+            // Entries that are infinite or not a number, among keys that not every row sees: weights of zero do not keep them out of a sum.
+            constexpr uint32_t kExponent = kBF16 ? 0x7f80u : 0x7c00u;
+            bool found = false;
+#pragma unroll
+            for (uint32_t e = 0; e < kOut; e++)
+#pragma unroll
+                for (uint32_t half = 0; half < 2; half++) {
+                    const u32x4 v = values_of(e, half);
+#pragma unroll
+                    for (uint32_t p = 0; p < 4; p++) found = found || (v[p] & kExponent) == kExponent || (v[p] >> 16 & kExponent) == kExponent;
+                }
+            odd = __builtin_amdgcn_ballot_w64(found) != 0;
+        }
+        if (!odd) {
+#pragma unroll
+            for (uint32_t e = 0; e < kOut; e++)
+#pragma unroll
+                for (uint32_t half = 0; half < 2; half++) {
+                    const u32x4 v = values_of(e, half);
+#pragma unroll
+                    for (uint32_t r = 0; r < kR; r++) out[r][e] = mfma32<kBF16>(v, w[r][half], out[r][e]);
+                }
+            return;
+        }
+        for (uint32_t only = 0; only < 32; only++)  // a row of each tile by itself, with the entries that it sees
+#pragma unroll
+            for (uint32_t r = 0; r < kR; r++) {
+                const int32_t of_low = __builtin_amdgcn_readlane(row_low[r], only), of_high = __builtin_amdgcn_readlane(row_high[r], only);
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++)
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; half++) {
+                        u32x4 v = values_of(e, half);
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; i++) {
+                            const int32_t key = key0 + static_cast<int32_t>(half * 16u + i / 4u * 8u + 4u * h + i % 4u);
+                            if (key < of_low || key > of_high) v[i / 2] &= i % 2 ? 0x0000ffffu : 0xffff0000u;
+                        }
+                        const f32x16 with = mfma32<kBF16>(v, w[r][half], out[r][e]);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i++) out[r][e][i] = n == only ? with[i] : out[r][e][i];
+                    }
+            }
+    };
+
+    if (from < to) {
+        Raw raw;
+        Scales scales{}, scales_next{};
+        look_up(from);
+        load(from, raw);
+        if constexpr (!kFloat) {
+            load_scales(from, scales);
+            load_scales(from + 1u, scales_next);
+            publish(from, scales);
+            __syncthreads();
+        }
+        lay(from, raw, scales);
+        if constexpr (!kFloat) {
+            scales = scales_next;
+            publish(from + 1u, scales);
+        }
+        for (uint32_t step = from; step < to; step++) {
+            __syncthreads();
+            // pages are looked up for sixteen steps from `from` on; scales are asked for two steps ahead
+            const uint32_t done = step - from;
+            if (step + 1u < to) {
+                if ((done + 1u) % 16u == 0 && kFloat) look_up(step + 1u);
+                load(step + 1u, raw);
+            }
+            if constexpr (!kFloat) {
+                if ((done + 2u) % 16u == 0) look_up(step + 2u);
+                load_scales(step + 2u, scales_next);
+            }
+            compute(step, 0);
+            compute(step, 1);
+            if (step + 1u < to) {
+                lay(step + 1u, raw, scales);
+                if constexpr (!kFloat) {
+                    scales = scales_next;
+                    publish(step + 2u, scales);
+                }
+            }
+        }
+    }
+
+    const float up = kFloat ? 1.0f : 2.0f * ldexpf(1.0f, value_power);
+#pragma unroll
+    for (uint32_t r = 0; r < kR; r++) {
+        const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum[r]), f32_bits(sum[r]), false, false);
+        const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
+        const float by = all == 0.0f ? 0.0f : 1.0f / all;
+        const uint32_t own = wave_row + r * 32u + n;
+        if (own >= at.rows) continue;
+        const uint32_t row = own + at.row0, token = at.s.first + row / a.group, head = kv_head * a.group + row % a.group;
+        const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
+        if (split.splits > 1 && h == 0) split.stats[2 * of] = top[r], split.stats[2 * of + 1] = all;
+#pragma unroll
+        for (uint32_t e = 0; e < kOut; e++)
+#pragma unroll
+            for (uint32_t v = 0; v < 16; v += 4) {
+                const uint32_t d = e * 32u + v * 2u + 4u * h;
+                if (d >= dim) continue;
+                f32x4 four;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) four[i] = all == 0.0f ? 0.0f : out[r][e][v + i] * by * up;
+                if (split.splits > 1)
+                    *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = four;
+                else
+                    *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) =
+                        a.dtype == CQ_BF16 ? u32x2{pair_of<true>(four[0], four[1]), pair_of<true>(four[2], four[3])} : u32x2{pair_of<false>(four[0], four[1]), pair_of<false>(four[2], four[3])};
+            }
+    }
+}
+
+template <int kCode, int kDim, bool kBF16>
+hipError_t launch_many(hipStream_t s, const AttentionArgs& a, const Split& split) {
+    constexpr uint32_t kLds = 2 * Many<kCode, kDim>::kBuffer + 64;
+    hipLaunchKernelGGL((attention_many_kernel<kCode, kDim, kBF16>), dim3(split.tiles * split.splits * a.cache.kv_heads), dim3(256), kLds, s, a, split);
+    return hipGetLastError();
+}
+
+template <int kCode, int kDim>
+hipError_t launch_type(hipStream_t s, const AttentionArgs& a, const Split& split) {
+    if constexpr (kCode == kCacheFloat)
+        if (a.dtype == CQ_BF16) return launch_many<kCode, kDim, true>(s, a, split);
+    return launch_many<kCode, kDim, false>(s, a, split);
+}
+
+}  // namespace
+
+#define CQ_MANY_NAME2(c) launch_attention_many_##c
+#define CQ_MANY_NAME(c) CQ_MANY_NAME2(c)
+hipError_t CQ_MANY_NAME(CQ_TU_CODE)(hipStream_t s, const AttentionArgs& a, const Split& split) {
+    if (a.cache.dim <= 64) return launch_type<CQ_TU_CODE, 64>(s, a, split);
+    if (a.cache.dim <= 128) return launch_type<CQ_TU_CODE, 128>(s, a, split);
+    return launch_type<CQ_TU_CODE, 256>(s, a, split);
+}
+
+}  // namespace cq
