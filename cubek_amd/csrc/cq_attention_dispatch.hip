@@ -35,13 +35,13 @@ constexpr uint32_t kMostSplits = 64;  // a lane each in attention_join_kernel
 
 uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4; }
 
-// Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (128 of longer
-// heads) by attention_many_kernel.  The keys are split so that `wanted` workgroups come to the GPU, none with less than `fewest` keys.
+// Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (512, 128 of heads up
+// to 64, past 128) by attention_many_kernel.  The keys are split so that `wanted` workgroups come to the GPU, none with less than `fewest` keys.
 Split split_of(const AttentionArgs& a, uint64_t room) {
     Split f{};
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, mean = (rows + a.seqs - 1) / a.seqs;
     f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? 2 : 0;
-    const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : 256;
+    const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : a.cache.dim > 64 ? 256 : 512;
     const uint64_t wanted = f.row_tiles ? 1024 : 256, fewest = f.row_tiles ? 512 : 1024;
     f.tiles = static_cast<uint32_t>(rows / of_tile + a.seqs);
     const uint64_t busy = a.seqs * ((mean + of_tile - 1) / of_tile) * a.cache.kv_heads;

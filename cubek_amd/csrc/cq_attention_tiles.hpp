@@ -3,8 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
-#include "cq_attention_internal.hpp"
-#include "cq_device.hpp"
+#include "cq_attention_rows.hpp"
 
 namespace cq {
 namespace {
@@ -15,6 +14,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2E = 1.44269504088896340736f;
+// Weights are exp2(t - largest t) * 2^13, which f16 holds down to 2^-37 of the largest.
+constexpr float kWeightLog2 = 13.0f, kWeightOne = 8192.0f;
 
 template <int kCode>
 constexpr uint32_t kCodeBits = kCode == kCacheFloat ? 16u : (kCode == kCacheInt4 || kCode == kCacheE2M1 ? 4u : 8u);
@@ -121,6 +122,19 @@ __device__ __forceinline__ float sum_of_groups(float v) {
     return bits_f32(quarters[0]) + bits_f32(quarters[1]);
 }
 
+// Whether eight entries of 16 bits have one that is infinite or not a number.
+template <bool kBF16>
+__device__ __forceinline__ bool has_odd(u32x4 v) {
+    constexpr uint32_t kExponent = kBF16 ? 0x7f80u : 0x7c00u;
+    bool found = false;
+#pragma unroll
+    for (uint32_t p = 0; p < 4; p++) {
+        const uint32_t w = v[p];
+        found = found || (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+    }
+    return found;
+}
+
 // A stored scale is loaded as the word around it and made a number later, by masks instead of branches: a load is not waited for where it is
 // issued.  All bits or none of a word, by the type of the scales (uniform over the launch).
 struct ScaleWords {
@@ -162,6 +176,46 @@ __device__ __forceinline__ bool find_rows(const AttentionArgs& a, uint32_t tile,
     out->row0 = static_cast<uint32_t>(row0);
     out->rows = static_cast<uint32_t>(min(rows - row0, static_cast<uint64_t>(1u << rows_log2)));
     return true;
+}
+
+// The rows of a tile once more, one by one, over the keys from first to last: taken where an entry of a value that is infinite or not a number lies among
+// keys that not every row of the tile sees.  A weight of zero does not keep such an entry out of a product of tiles.  All threads of the workgroup
+// come here, with its LDS free for (kDim + 64) floats a wave.
+template <uint32_t kDim, class Put>
+__device__ __forceinline__ void rows_one_by_one(const AttentionArgs& a, const RowTile& at, uint32_t kv_head, int64_t first, int64_t last, float* lds, Put put) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    float* const query = lds + wave * (kDim + 64u);
+    for (uint32_t row = wave; row < at.rows; row += blockDim.x / 64u) {
+        const uint32_t in_sequence = at.row0 + row, token = at.s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
+        const int32_t position = at.s.position + static_cast<int32_t>(in_sequence / a.group);
+        const Seen seen = seen_from(a, at.s, position);
+        for (uint32_t d = lane; d < a.cache.dim; d += 64) query[d] = load_dtype(a.dtype, a.q, token * a.q_token + head * a.q_head + d);
+        __builtin_amdgcn_wave_barrier();
+        float top, sum, acc[kDim / 64];
+        attend_row<kDim / 64>(a, at.s, kv_head, position, a.slopes ? a.slopes[head] : 0.0f, query, query + kDim, max(first, static_cast<int64_t>(seen.low)), 64,
+                              min(last, static_cast<int64_t>(seen.high)), &top, &sum, acc);
+#pragma unroll
+        for (uint32_t i = 0; i < kDim / 64; i++) acc[i] = sum != 0.0f ? acc[i] / sum : 0.0f;
+        put(token, head, top * kLog2E, sum, acc);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// A row's result, lane l with its entries l, l + 64 ..., to y or as a part.
+template <uint32_t kDim>
+__device__ __forceinline__ void put_row(const AttentionArgs& a, const Split& split, uint32_t part, uint32_t token, uint32_t head, float top, float sum, const float* v) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
+#pragma unroll
+    for (uint32_t i = 0; i < kDim / 64; i++) {
+        const uint32_t d = i * 64u + lane;
+        if (d >= a.cache.dim) continue;
+        if (split.splits > 1)
+            split.parts[of * a.cache.dim + d] = v[i];
+        else
+            store_dtype(a.dtype, a.y, token * a.y_token + head * a.y_head + d, v[i]);
+    }
+    if (split.splits > 1 && lane == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = sum * kWeightOne;
 }
 
 }  // namespace

@@ -68,6 +68,21 @@ __device__ __forceinline__ void swap_quarters(uint32_t& a, uint32_t& b) {
     a = r[0], b = r[1];
 }
 
+// Whether 16 bytes of codes have one that is infinite or not a number.
+template <int kCode, bool kBF16>
+__device__ __forceinline__ bool code_is_odd(u32x4 v) {
+    if constexpr (kCode == kCacheFloat) return has_odd<kBF16>(v);
+    constexpr uint32_t kMask = kCode == kCacheE4M3 ? 0x7fu : 0x7cu;  // e4m3 has one NaN; e5m2's largest exponent is infinity and NaN
+    bool found = false;
+#pragma unroll
+    for (uint32_t p = 0; p < 4; p++) {
+        const uint32_t w = v[p];
+#pragma unroll
+        for (uint32_t b = 0; b < 32; b += 8) found = found || (w >> b & kMask) == kMask;
+    }
+    return found;
+}
+
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
 __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Split split) {
     using S = Shape<kCode, kDim, kPer>;
@@ -226,6 +241,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
     float top[kTiles], sum[kTiles];
 #pragma unroll
     for (uint32_t r = 0; r < kTiles; r++) top[r] = -INFINITY, sum[r] = 0.0f;
+    bool found = false;    // values that are no numbers, among keys that not every row sees
     int32_t power = -126;  // of the largest scale of the values so far: they are taken times 2^-power
 
     Raw raw, next;
@@ -240,7 +256,19 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
         const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys);
         const bool partial = key0 < all_low || key0 + static_cast<int32_t>(S::kKeys) - 1 > all_high;
 
-        // this step's values and scales into LDS
+        // this step's values and scales into LDS; of values that can be no numbers those that no row sees become zeros, and others are reported
+        if constexpr (kCodeHasNaN<kCode>) {
+            if (partial) {
+                bool odd = false;
+#pragma unroll
+                for (uint32_t n = 0; n < S::kLoads; n++) {
+                    const int32_t key = key0 + static_cast<int32_t>((n * 64u + lane) / S::kLanes);
+                    if (key < low || key > high) raw.v[n] = u32x4{0, 0, 0, 0};
+                    odd = odd || code_is_odd<kCode, kBF16>(raw.v[n]);
+                }
+                found = found || __builtin_amdgcn_ballot_w64(odd) != 0;
+            }
+        }
 #pragma unroll
         for (uint32_t n = 0; n < S::kLoads; n++)
             *reinterpret_cast<u32x4*>(mine + (n * 64u + lane) / S::kLanes * S::kPitch + lane % S::kLanes * S::kLane) = raw.v[n];
@@ -322,7 +350,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
             }
         }
 
-        // weights: exp2(t - top) * 2^13, which f16 holds down to 2^-37 of the largest
+        // weights
         float p[kTiles][S::kKeyTiles * 4];
 #pragma unroll
         for (uint32_t r = 0; r < kTiles; r++) {
@@ -348,7 +376,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
 #pragma unroll
                 for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
             }
-            const float less = 13.0f - (top[r] == -INFINITY ? 0.0f : top[r]);
+            const float less = kWeightLog2 - (top[r] == -INFINITY ? 0.0f : top[r]);
 #pragma unroll
             for (uint32_t k = 0; k < S::kKeyTiles * 4; k++) {
                 p[r][k] = __builtin_amdgcn_exp2f(p[r][k] + less);
@@ -356,8 +384,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
             }
         }
 
-        // the second product; `hide`: entries that the row `only` of each tile does not see count as nothing, and only that row is computed
-        const auto weights_of = [&](uint32_t r, uint32_t block, uint32_t half, bool hide, bool mine_only) {
+        const auto weights_of = [&](uint32_t r, uint32_t block, uint32_t half) {
             float w[8];
 #pragma unroll
             for (uint32_t k = 0; k < 2; k++) {
@@ -368,7 +395,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
                     const float of = p[r][(half * 2u + k) * 4u + e];
                     float v = kFloat ? of : of * by[e];
                     if (partial) v = of == 0.0f ? 0.0f : v;  // a scale that is not a number, of an entry that is not seen
-                    w[k * 4 + e] = !hide || mine_only ? v : 0.0f;
+                    w[k * 4 + e] = v;
                 }
             }
             u32x4 packed;
@@ -393,65 +420,33 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
                 v[0] = numbers<kCode>(w[0], 0), v[1] = numbers<kCode>(w[1], 0);
             }
         };
-        const auto multiply = [&](bool hide, uint32_t only) {
-            u32x4 w[kTiles][kHalves];
+        u32x4 w[kTiles][kHalves];
 #pragma unroll
-            for (uint32_t e = 0; e < kOut; e++) {
-                if (e == 0 || (kPer > 1 && e % 2 == 0))
-#pragma unroll
-                    for (uint32_t r = 0; r < kTiles; r++)
-#pragma unroll
-                        for (uint32_t half = 0; half < kHalves; half++) w[r][half] = weights_of(r, kPer > 1 ? e / 2u : 0u, half, hide, i == only);
-                u32x4 entries[kHalves];
-                values_of(e, entries);
+        for (uint32_t e = 0; e < kOut; e++) {
+            if (e == 0 || (kPer > 1 && e % 2 == 0))
 #pragma unroll
                 for (uint32_t r = 0; r < kTiles; r++)
 #pragma unroll
-                    for (uint32_t half = 0; half < kHalves; half++) {
-                        u32x4 seen = entries[half];
-                        if (hide) {
-                            const int32_t of_low = __builtin_amdgcn_readlane(row_low[r], only), of_high = __builtin_amdgcn_readlane(row_high[r], only);
+                    for (uint32_t half = 0; half < kHalves; half++) w[r][half] = weights_of(r, kPer > 1 ? e / 2u : 0u, half);
+            u32x4 v[kHalves];
+            values_of(e, v);
 #pragma unroll
-                            for (uint32_t pair = 0; pair < 4; pair++)
+            for (uint32_t half = 0; half < kHalves; half++)
 #pragma unroll
-                                for (uint32_t k = 0; k < 2; k++) {
-                                    const uint32_t nth_key = place_of<kCode>(2 * pair + k);
-                                    const int32_t key = key0 + static_cast<int32_t>((half * 2u + nth_key / 4u) * 16u + 4u * g + nth_key % 4u);
-                                    if (key < of_low || key > of_high) seen[pair] &= k ? 0x0000ffffu : 0xffff0000u;
-                                }
-                        }
-                        const f32x4 v = mfma16<kBF16>(seen, w[r][half], out[r][e]);
-                        out[r][e] = !hide || i == only ? v : out[r][e];  // for other rows than `only` a weight of zero may have met an infinity
-                    }
-            }
-        };
-        bool odd = false;
-        if constexpr (kCodeHasNaN<kCode>) {
-            // Entries that are infinite or not a number, among keys that not every row sees: weights of zero do not keep them out of a sum.
-            if (partial) {
-                constexpr uint32_t kExponent = kBF16 ? 0x7f80u : 0x7c00u;
-                bool found = false;
-#pragma unroll
-                for (uint32_t e = 0; e < kOut; e++) {
-                    u32x4 v[kHalves];
-                    values_of(e, v);
-#pragma unroll
-                    for (uint32_t half = 0; half < kHalves; half++)
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; k++)
-                            found = found || (v[half][k] & kExponent) == kExponent || (v[half][k] >> 16 & kExponent) == kExponent;
-                }
-                odd = __builtin_amdgcn_ballot_w64(found) != 0;
-            }
+                for (uint32_t r = 0; r < kTiles; r++) out[r][e] = mfma16<kBF16>(v[half], w[r][half], out[r][e]);
         }
-        if (!odd)
-            multiply(false, 0);
-        else
-            for (uint32_t only = 0; only < 16; only++) multiply(true, only);
         fence();
         raw = next;
     }
 
+    if constexpr (kCodeHasNaN<kCode>) {
+        if (__syncthreads_or(found)) {
+            const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
+            rows_one_by_one<kDim>(a, at, kv_head, first_key, last_key, reinterpret_cast<float*>(lds),
+                                  [&](uint32_t token, uint32_t head, float most, float all, const float* v) { put_row<kDim>(a, split, part, token, head, most, all, v); });
+            return;
+        }
+    }
     // The four waves' results, each over its own sum, by their shares of the whole.
     __syncthreads();
     constexpr uint32_t kOutPitch = kDim + 4;

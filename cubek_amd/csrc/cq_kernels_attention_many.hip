@@ -19,10 +19,12 @@ namespace {
 
 template <int kCode, int kDim>
 struct Many {
-    static constexpr uint32_t kBits = kCodeBits<kCode>, kKeys = 64, kRowTiles = kDim > 128 ? 1 : 2, kRowsLog2 = kRowTiles == 1 ? 7 : 8;
+    static constexpr uint32_t kBits = kCodeBits<kCode>, kKeys = 64;
+    static constexpr uint32_t kWaves = kDim > 128 ? 4 : 8, kThreads = 64 * kWaves, kRowTiles = kDim > 64 ? 1 : 2;       // tiles of 32 rows of a wave
+    static constexpr uint32_t kRows = kWaves * 32 * kRowTiles, kRowsLog2 = kRows == 512 ? 9 : kRows == 256 ? 8 : 7;
     static constexpr uint32_t kRow = kDim * kBits / 8;                                                  // bytes of a key as it is stored
-    static constexpr uint32_t kChunk = kRow == 32 ? 8 : 16, kLanes = kRow / kChunk;                      // of a thread; threads of a row
-    static constexpr uint32_t kEntries = kChunk * 8 / kBits, kChunks = kKeys * kLanes / 256;             // entries of a chunk; chunks of a thread
+    static constexpr uint32_t kChunk = kRow * kKeys / kThreads < 16 ? kRow * kKeys / kThreads : 16, kLanes = kRow / kChunk;  // of a thread; threads of a row
+    static constexpr uint32_t kEntries = kChunk * 8 / kBits, kChunks = kKeys * kLanes / kThreads;             // entries of a chunk; chunks of a thread
     static constexpr uint32_t kPitch = kDim * 2 + 16, kSide = kKeys * kPitch, kBuffer = 2 * kSide;       // bytes in LDS: of a row, of keys or values, of both
 };
 
@@ -35,12 +37,13 @@ __device__ __forceinline__ u32x4 in_order(u32x4 v) {
 }
 
 template <int kCode, int kDim, bool kBF16>
-__global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel(AttentionArgs a, Split split) {
+__global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_kernel(AttentionArgs a, Split split) {
     using S = Many<kCode, kDim>;
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kR = S::kRowTiles, kSlices = kDim / 16, kOut = kDim / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][wave][keys, values]
+    uint32_t* const found = powers + 4 * S::kWaves;                              // whether values that are no numbers need rows one by one
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31u, h = lane >> 5;
     // neighbours in the grid are heads of the cache: with eight of them each die keeps one in its L2.  The tiles with most keys come first.
     const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads, part = rest % split.splits;
@@ -49,7 +52,8 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
     RowTile at;
     if (!find_rows(a, tile, S::kRowsLog2, &at)) return;
     const auto position_of = [&](uint32_t row) { return at.s.position + static_cast<int32_t>((at.row0 + row) / a.group); };
-    const int32_t low = seen_from(a, at.s, position_of(0)).low, high = seen_from(a, at.s, position_of(at.rows - 1u)).high;
+    const Seen top_row = seen_from(a, at.s, position_of(0)), bottom_row = seen_from(a, at.s, position_of(at.rows - 1u));
+    const int32_t low = top_row.low, high = bottom_row.high, tile_low = bottom_row.low, tile_high = top_row.high;  // seen by some, and by all
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
     const uint32_t each = (steps_all + split.splits - 1u) / split.splits;
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u, byte = threadIdx.x % S::kLanes * S::kChunk, entry = byte * 8u / S::kBits;
     const uint32_t block = min(entry, dim - 1u) >> split.block_log2;
-    const auto key_of = [&](uint32_t c) { return (c * 256u + threadIdx.x) / S::kLanes; };
+    const auto key_of = [&](uint32_t c) { return (c * S::kThreads + threadIdx.x) / S::kLanes; };
     // the page of a chunk's tile of 16 keys (the same for the wave) and the row in it
     const auto place = [&](uint32_t step, uint32_t c, uint32_t* page, uint32_t* slot) {
         const uint32_t k = __builtin_amdgcn_readfirstlane(key_of(c) / 16u);
@@ -135,7 +139,9 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
             const uint64_t at_byte = min(byte, row_bytes - S::kChunk);
             const char* const k = a.cache.keys.base + page * a.cache.keys.page + kv_head * a.cache.keys.head + slot * a.cache.keys.slot + at_byte;
             const char* const v = a.cache.values.base + page * a.cache.values.page + kv_head * a.cache.values.head + slot * a.cache.values.slot + at_byte;
-            if constexpr (S::kChunk == 16) {
+            if constexpr (S::kChunk == 4) {
+                raw.k[c][0] = *reinterpret_cast<const uint32_t*>(k), raw.v[c][0] = *reinterpret_cast<const uint32_t*>(v);
+            } else if constexpr (S::kChunk == 16) {
                 const u32x4 kw = *reinterpret_cast<const u32x4*>(k), vw = *reinterpret_cast<const u32x4*>(v);
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) raw.k[c][e] = kw[e], raw.v[c][e] = vw[e];
@@ -172,7 +178,7 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
             of_values = max(of_values, field(words.number(s.v[c], s.halves >> (2 * c + 1) & 1u)));
         }
         of_keys = wave_max_bits(of_keys), of_values = wave_max_bits(of_values);
-        if (lane == 0) powers[(step & 1u) * 8u + wave * 2u] = of_keys, powers[(step & 1u) * 8u + wave * 2u + 1u] = of_values;
+        if (lane == 0) powers[((step & 1u) * S::kWaves + wave) * 2u] = of_keys, powers[((step & 1u) * S::kWaves + wave) * 2u + 1u] = of_values;
     };
 
     f32x16 out[kR][kOut] = {};
@@ -181,14 +187,20 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
     for (uint32_t r = 0; r < kR; r++) top[r] = -INFINITY, sum[r] = 0.0f;
     int32_t key_power = -126, value_power = -126;  // of the largest scales so far: entries are taken times 2^-power / 2
 
-    // A step's codes as numbers into LDS.
+    // A step's codes as numbers into LDS.  In a step that some row sees only a part of, values that no row sees become zeros, and others that are no
+    // numbers are reported.
     const auto lay = [&](uint32_t step, Raw& raw, const Scales& s) {
         char* const to_keys = lds + (step & 1u) * S::kBuffer;
+        const int32_t step_key = static_cast<int32_t>((step0 + step) * S::kKeys);
+        const bool partial = step_key < tile_low || step_key + static_cast<int32_t>(S::kKeys) - 1 > tile_high;
         float down_keys = 0.0f, down_values = 0.0f;
         if constexpr (!kFloat) {
             uint32_t of_keys = 0, of_values = 0;
 #pragma unroll
-            for (uint32_t w = 0; w < 4; w++) of_keys = max(of_keys, powers[(step & 1u) * 8u + w * 2u]), of_values = max(of_values, powers[(step & 1u) * 8u + w * 2u + 1u]);
+            for (uint32_t w = 0; w < S::kWaves; w++) {
+                const uint32_t* const of = powers + ((step & 1u) * S::kWaves + w) * 2u;
+                of_keys = max(of_keys, of[0]), of_values = max(of_values, of[1]);
+            }
             const int32_t now_keys = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of_keys)) - 127, 126);
             const int32_t now_values = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of_values)) - 127, 126);
             key_power = max(key_power, now_keys);
@@ -209,12 +221,27 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
 #pragma unroll
                 for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.k[c][e] = 0, raw.v[c][e] = 0;
             }
+            float value_scale = 1.0f;
+            if constexpr (!kFloat) value_scale = words.number(s.v[c], s.halves >> (2 * c + 1) & 1u) * down_values;
+            if (partial) {
+                const int32_t key = step_key + static_cast<int32_t>(key_of(c));
+                if (key < low || key > high) {
+#pragma unroll
+                    for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.v[c][e] = 0;
+                    value_scale = 0.0f;
+                }
+            }
+            const auto look = [&](u32x4 v) {
+                if (partial && has_odd<kBF16>(v)) *found = 1u;
+            };
             if constexpr (kFloat) {
+                const u32x4 v = {raw.v[c][0], raw.v[c][1], raw.v[c][2], raw.v[c][3]};
+                look(v);
                 *reinterpret_cast<u32x4*>(row) = u32x4{raw.k[c][0], raw.k[c][1], raw.k[c][2], raw.k[c][3]};
-                *reinterpret_cast<u32x4*>(row + S::kSide) = u32x4{raw.v[c][0], raw.v[c][1], raw.v[c][2], raw.v[c][3]};
+                *reinterpret_cast<u32x4*>(row + S::kSide) = v;
             } else {
                 constexpr uint32_t kEach = S::kBits == 8 ? 2 : 1;  // words of eight entries
-                const auto put = [&](char* to, const uint32_t* w, float scale) {
+                const auto put = [&](char* to, const uint32_t* w, float scale, bool of_values) {
                     const uint32_t both = pair_of<false>(scale, scale);
                     const f16x2 by = __builtin_bit_cast(f16x2, both);
 #pragma unroll
@@ -225,11 +252,12 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
                             const uint32_t word = v[p];
                             v[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, word) * by);
                         }
+                        if (of_values) look(v);
                         *reinterpret_cast<u32x4*>(to + e / kEach * 16u) = v;
                     }
                 };
-                put(row, raw.k[c], words.number(s.k[c], s.halves >> (2 * c) & 1u) * down_keys);
-                put(row + S::kSide, raw.v[c], words.number(s.v[c], s.halves >> (2 * c + 1) & 1u) * down_values);
+                put(row, raw.k[c], words.number(s.k[c], s.halves >> (2 * c) & 1u) * down_keys, false);
+                put(row + S::kSide, raw.v[c], value_scale, true);
             }
         }
     };
@@ -278,7 +306,7 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
 #pragma unroll
                 for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
             }
-            const float less = 13.0f - (top[r] == -INFINITY ? 0.0f : top[r]);
+            const float less = kWeightLog2 - (top[r] == -INFINITY ? 0.0f : top[r]);
 #pragma unroll
             for (uint32_t v = 0; v < 16; v++) {
                 p[v] = __builtin_amdgcn_exp2f(p[v] + less);
@@ -299,53 +327,18 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
             }
             return v;
         };
-        bool odd = false;
-        if (partial) {
-            // Entries that are infinite or not a number, among keys that not every row sees: weights of zero do not keep them out of a sum.
-            constexpr uint32_t kExponent = kBF16 ? 0x7f80u : 0x7c00u;
-            bool found = false;
 #pragma unroll
-            for (uint32_t e = 0; e < kOut; e++)
+        for (uint32_t e = 0; e < kOut; e++)
 #pragma unroll
-                for (uint32_t half = 0; half < 2; half++) {
-                    const u32x4 v = values_of(e, half);
+            for (uint32_t half = 0; half < 2; half++) {
+                const u32x4 v = values_of(e, half);
 #pragma unroll
-                    for (uint32_t p = 0; p < 4; p++) found = found || (v[p] & kExponent) == kExponent || (v[p] >> 16 & kExponent) == kExponent;
-                }
-            odd = __builtin_amdgcn_ballot_w64(found) != 0;
-        }
-        if (!odd) {
-#pragma unroll
-            for (uint32_t e = 0; e < kOut; e++)
-#pragma unroll
-                for (uint32_t half = 0; half < 2; half++) {
-                    const u32x4 v = values_of(e, half);
-#pragma unroll
-                    for (uint32_t r = 0; r < kR; r++) out[r][e] = mfma32<kBF16>(v, w[r][half], out[r][e]);
-                }
-            return;
-        }
-        for (uint32_t only = 0; only < 32; only++)  // a row of each tile by itself, with the entries that it sees
-#pragma unroll
-            for (uint32_t r = 0; r < kR; r++) {
-                const int32_t of_low = __builtin_amdgcn_readlane(row_low[r], only), of_high = __builtin_amdgcn_readlane(row_high[r], only);
-#pragma unroll
-                for (uint32_t e = 0; e < kOut; e++)
-#pragma unroll
-                    for (uint32_t half = 0; half < 2; half++) {
-                        u32x4 v = values_of(e, half);
-#pragma unroll
-                        for (uint32_t i = 0; i < 8; i++) {
-                            const int32_t key = key0 + static_cast<int32_t>(half * 16u + i / 4u * 8u + 4u * h + i % 4u);
-                            if (key < of_low || key > of_high) v[i / 2] &= i % 2 ? 0x0000ffffu : 0xffff0000u;
-                        }
-                        const f32x16 with = mfma32<kBF16>(v, w[r][half], out[r][e]);
-#pragma unroll
-                        for (uint32_t i = 0; i < 16; i++) out[r][e][i] = n == only ? with[i] : out[r][e][i];
-                    }
+                for (uint32_t r = 0; r < kR; r++) out[r][e] = mfma32<kBF16>(v, w[r][half], out[r][e]);
             }
     };
 
+    if (threadIdx.x == 0) *found = 0u;
+    __syncthreads();
     if (from < to) {
         Raw raw;
         Scales scales{}, scales_next{};
@@ -386,6 +379,15 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
         }
     }
 
+    __syncthreads();
+    if (*found) {
+        const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
+        __syncthreads();
+        rows_one_by_one<kDim>(a, at, kv_head, first_key, last_key, reinterpret_cast<float*>(lds),
+                              [&](uint32_t token, uint32_t head, float most, float all, const float* v) { put_row<kDim>(a, split, part, token, head, most, all, v); });
+        return;
+    }
+
     const float up = kFloat ? 1.0f : 2.0f * ldexpf(1.0f, value_power);
 #pragma unroll
     for (uint32_t r = 0; r < kR; r++) {
@@ -417,8 +419,8 @@ __global__ __launch_bounds__(256, kDim <= 64 ? 2 : 1) void attention_many_kernel
 
 template <int kCode, int kDim, bool kBF16>
 hipError_t launch_many(hipStream_t s, const AttentionArgs& a, const Split& split) {
-    constexpr uint32_t kLds = 2 * Many<kCode, kDim>::kBuffer + 64;
-    hipLaunchKernelGGL((attention_many_kernel<kCode, kDim, kBF16>), dim3(split.tiles * split.splits * a.cache.kv_heads), dim3(256), kLds, s, a, split);
+    constexpr uint32_t kLds = 2 * Many<kCode, kDim>::kBuffer + Many<kCode, kDim>::kWaves * 16 + 16;
+    hipLaunchKernelGGL((attention_many_kernel<kCode, kDim, kBF16>), dim3(split.tiles * split.splits * a.cache.kv_heads), dim3(Many<kCode, kDim>::kThreads), kLds, s, a, split);
     return hipGetLastError();
 }
 
