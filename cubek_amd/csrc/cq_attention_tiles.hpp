@@ -14,8 +14,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2E = 1.44269504088896340736f;
-// Weights are exp2(t - largest t) * 2^13, which f16 holds down to 2^-37 of the largest.
-constexpr float kWeightLog2 = 13.0f, kWeightOne = 8192.0f;
+// Weights are exp2(t - top) * 2^5, with a `top` that the largest score so far exceeds by at most kLazy: f16 holds them up to 2^13 and down to 2^-29 of that of
+// `top`.  A new largest score costs all results a product, so most of them are let pass.
+constexpr float kLazy = 8.0f, kWeightLog2 = 5.0f, kWeightOne = 32.0f;
 
 template <int kCode>
 constexpr uint32_t kCodeBits = kCode == kCacheFloat ? 16u : (kCode == kCacheInt4 || kCode == kCacheE2M1 ? 4u : 8u);

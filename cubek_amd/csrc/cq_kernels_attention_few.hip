@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
                     most = fmaxf(most, t);
                 }
             most = max_of_groups(most);
-            if (__builtin_amdgcn_ballot_w64(most > top[r])) {
+            if (__builtin_amdgcn_ballot_w64(most > top[r] + kLazy)) {
                 const float before = top[r];
                 top[r] = fmaxf(top[r], most);
                 const float shrink = top[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - top[r]);

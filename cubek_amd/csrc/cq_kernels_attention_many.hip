@@ -25,7 +25,7 @@ struct Many {
     static constexpr uint32_t kRow = kDim * kBits / 8;                                                  // bytes of a key as it is stored
     static constexpr uint32_t kChunk = kRow * kKeys / kThreads < 16 ? kRow * kKeys / kThreads : 16, kLanes = kRow / kChunk;  // of a thread; threads of a row
     static constexpr uint32_t kEntries = kChunk * 8 / kBits, kChunks = kKeys * kLanes / kThreads;             // entries of a chunk; chunks of a thread
-    static constexpr uint32_t kPitch = kDim * 2 + 16, kSide = kKeys * kPitch, kBuffer = 2 * kSide;       // bytes in LDS: of a row, of keys or values, of both
+    static constexpr uint32_t kPitch = kDim * 2 + 32, kSide = kKeys * kPitch, kBuffer = 2 * kSide;       // bytes in LDS: of a row, of keys or values, of both
 };
 
 // Eight numbers in the order of their entries.
@@ -81,7 +81,11 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
             const uint32_t d = 16u * t + 8u * h;
             q[r][t] = d < dim ? *reinterpret_cast<const u32x4*>(from_q + d * 2u) : u32x4{0, 0, 0, 0};
         }
-        times[r] = a.scale;
+        if (a.scale < 0.0f) {  // into the queries: the largest score is that of the largest product
+#pragma unroll
+            for (uint32_t t = 0; t < kSlices; t++) q[r][t] ^= 0x80008000u;
+        }
+        times[r] = fabsf(a.scale);
         if constexpr (!kFloat) {
             float most = 0.0f, v[8];
             const bool bf16 = a.dtype == CQ_BF16;
@@ -279,9 +283,11 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
         u32x4 w[kR][2];
 #pragma unroll
         for (uint32_t r = 0; r < kR; r++) {
-            float p[16], most = -INFINITY;
+            // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
             const float by = kFloat ? times[r] : times[r] * 2.0f * bits_f32(static_cast<uint32_t>(127 + key_power) << 23);
-            if (partial || a.cap > 0.0f || a.slopes) {
+            const bool plain = !partial && a.cap == 0.0f && !a.slopes;
+            float most = -INFINITY;
+            if (!plain) {
 #pragma unroll
                 for (uint32_t v = 0; v < 16; v++) {
                     float t = s[r][v] * by;
@@ -289,16 +295,16 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
                     if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
                     if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
                     if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
-                    p[v] = t;
-                    most = fmaxf(most, t);
+                    s[r][v] = t;
                 }
-            } else {
-#pragma unroll
-                for (uint32_t v = 0; v < 16; v++) p[v] = s[r][v] * by, most = fmaxf(most, p[v]);
             }
+#pragma unroll
+            for (uint32_t v = 0; v < 16; v++) most = fmaxf(most, s[r][v]);
+            const float times_now = plain ? by : 1.0f;
+            most *= times_now;
             const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
             most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
-            if (__builtin_amdgcn_ballot_w64(most > top[r])) {
+            if (__builtin_amdgcn_ballot_w64(most > top[r] + kLazy)) {
                 const float before = top[r];
                 top[r] = fmaxf(top[r], most);
                 const float shrink = top[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - top[r]);
@@ -307,9 +313,10 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
                 for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
             }
             const float less = kWeightLog2 - (top[r] == -INFINITY ? 0.0f : top[r]);
+            float p[16];
 #pragma unroll
             for (uint32_t v = 0; v < 16; v++) {
-                p[v] = __builtin_amdgcn_exp2f(p[v] + less);
+                p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][v], times_now, less));
                 sum[r] += p[v];
             }
 #pragma unroll
