@@ -21,13 +21,16 @@ uint32_t log2_below(uint64_t v) {
 }
 
 // Whether the matrix cores take a call: 16-bit queries, heads of whole 32 entries up to 256, pages of whole 16 slots, a scale for 32, 64, 128 ...
-// entries or for a head, rows on 16-byte boundaries.
+// entries or for a head, rows on 16-byte boundaries, a page within 32 bits.
 bool tiles_take(const AttentionArgs& a) {
     const CacheArgs& c = a.cache;
     if (a.dtype == CQ_F32 || c.dim % 32 || c.dim > 256 || c.page_size % 16) return false;
     if (c.block != c.dim && (c.block < 32 || (c.block & (c.block - 1)))) return false;
     const auto on = [](const void* p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
-    const auto rows = [&](const CacheSide& s) { return on(s.base, 16) && s.page % 16 == 0 && s.head % 16 == 0 && s.slot % 16 == 0 && s.slot < (1u << 26); };
+    const auto rows = [&](const CacheSide& s) {
+        return on(s.base, 16) && s.page % 16 == 0 && s.head % 16 == 0 && s.slot % 16 == 0 && s.page < (1ull << 32) && s.slot < (1u << 26) &&
+               s.slot * c.page_size < (1ull << 32) && s.scale_page < (1ull << 32) && s.scale_slot < (1u << 24) && s.scale_slot * c.page_size < (1ull << 32) && s.scale_block < (1u << 24);
+    };
     return rows(c.keys) && rows(c.values) && on(a.q, 16) && a.q_token % 8 == 0 && a.q_head % 8 == 0 && on(a.y, 8) && a.y_token % 4 == 0 && a.y_head % 4 == 0;
 }
 

@@ -181,9 +181,21 @@ __device__ __forceinline__ bool find_rows(const AttentionArgs& a, uint32_t tile,
 
 // The rows of a tile once more, one by one, over the keys from first to last: taken where an entry of a value that is infinite or not a number lies among
 // keys that not every row of the tile sees.  A weight of zero does not keep such an entry out of a product of tiles.  All threads of the workgroup
-// come here, with its LDS free for (kDim + 64) floats a wave.
-template <uint32_t kDim, class Put>
-__device__ __forceinline__ void rows_one_by_one(const AttentionArgs& a, const RowTile& at, uint32_t kv_head, int64_t first, int64_t last, float* lds, Put put) {
+// come here, with its LDS free for (kDim + 64) floats a wave.  The arguments, the kernel's first two, are read again, so that what is needed here alone
+// takes no registers from what comes before.
+template <uint32_t kDim>
+__device__ __forceinline__ void rows_one_by_one(uint32_t rows_log2, uint32_t tile, uint32_t part, uint32_t kv_head, int64_t first, int64_t last, float* lds) {
+    struct Arguments {
+        AttentionArgs a;
+        Split split;
+    };
+    uint64_t again = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(again));
+    const Arguments& arguments = *reinterpret_cast<const Arguments*>(again);
+    const AttentionArgs& a = arguments.a;
+    const Split& split = arguments.split;
+    RowTile at;
+    if (!find_rows(a, tile, rows_log2, &at)) return;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     float* const query = lds + wave * (kDim + 64u);
     for (uint32_t row = wave; row < at.rows; row += blockDim.x / 64u) {
@@ -192,31 +204,23 @@ __device__ __forceinline__ void rows_one_by_one(const AttentionArgs& a, const Ro
         const Seen seen = seen_from(a, at.s, position);
         for (uint32_t d = lane; d < a.cache.dim; d += 64) query[d] = load_dtype(a.dtype, a.q, token * a.q_token + head * a.q_head + d);
         __builtin_amdgcn_wave_barrier();
-        float top, sum, acc[kDim / 64];
+        float top, sum, v[kDim / 64];
         attend_row<kDim / 64>(a, at.s, kv_head, position, a.slopes ? a.slopes[head] : 0.0f, query, query + kDim, max(first, static_cast<int64_t>(seen.low)), 64,
-                              min(last, static_cast<int64_t>(seen.high)), &top, &sum, acc);
+                              min(last, static_cast<int64_t>(seen.high)), &top, &sum, v);
+        const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
 #pragma unroll
-        for (uint32_t i = 0; i < kDim / 64; i++) acc[i] = sum != 0.0f ? acc[i] / sum : 0.0f;
-        put(token, head, top * kLog2E, sum, acc);
+        for (uint32_t i = 0; i < kDim / 64; i++) {
+            const uint32_t d = i * 64u + lane;
+            if (d >= a.cache.dim) continue;
+            const float y = sum != 0.0f ? v[i] / sum : 0.0f;
+            if (split.splits > 1)
+                split.parts[of * a.cache.dim + d] = y;
+            else
+                store_dtype(a.dtype, a.y, token * a.y_token + head * a.y_head + d, y);
+        }
+        if (split.splits > 1 && lane == 0) split.stats[2 * of] = top * kLog2E, split.stats[2 * of + 1] = sum * kWeightOne;
         __builtin_amdgcn_wave_barrier();
     }
-}
-
-// A row's result, lane l with its entries l, l + 64 ..., to y or as a part.
-template <uint32_t kDim>
-__device__ __forceinline__ void put_row(const AttentionArgs& a, const Split& split, uint32_t part, uint32_t token, uint32_t head, float top, float sum, const float* v) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
-#pragma unroll
-    for (uint32_t i = 0; i < kDim / 64; i++) {
-        const uint32_t d = i * 64u + lane;
-        if (d >= a.cache.dim) continue;
-        if (split.splits > 1)
-            split.parts[of * a.cache.dim + d] = v[i];
-        else
-            store_dtype(a.dtype, a.y, token * a.y_token + head * a.y_head + d, v[i]);
-    }
-    if (split.splits > 1 && lane == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = sum * kWeightOne;
 }
 
 }  // namespace

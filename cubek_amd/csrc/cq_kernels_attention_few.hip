@@ -27,36 +27,25 @@ struct Shape {
     static constexpr uint32_t kKeyTiles = kBits == 4 ? 4 : 2, kKeys = 16 * kKeyTiles;  // of a step
     static constexpr uint32_t kRow = kDim * kBits / 8;                                 // bytes of a key
     static constexpr uint32_t kUnits = kRow >= 64 ? kRow / 64 : 1, kWords = kRow >= 64 ? 4 : 2;  // loads of a lane for a key; words of one
+    static constexpr uint32_t kEntries = kWords * 32 / kBits, kCover = 4 * kEntries, kUnit = kDim / kPer;               // of a lane's load; of its four groups; of a scale
     static constexpr uint32_t kSlices = kDim / 32;                                     // matrix instructions of a tile of keys
     static constexpr uint32_t kLane = 16, kLanes = kRow / kLane, kLoads = kKeys * kRow / 1024;  // of values: bytes of a lane, lanes of a row, loads of a step
     static constexpr uint32_t kPitch = kRow + 16;                                      // bytes of a row in LDS: 16 keys' reads fall on different banks
-    static constexpr uint32_t kScaleLoads = kCode == kCacheFloat ? 0 : kPer * kKeyTiles / 2;
+    static constexpr uint32_t kScaleLoads = kCode == kCacheFloat ? 0 : (kPer * 16 + 63) / 64;           // of 16 keys' scales, of keys or of values
     static constexpr uint32_t kValueBytes = kKeys * kPitch, kScaleBytes = kCode == kCacheFloat ? 0 : 2 * kPer * kKeys * 4, kWaveBytes = kValueBytes + kScaleBytes;
 };
 
-// Where a lane's eight entries of slice t begin within a row, as the first product takes them.
+// The first product takes entries in slices of 32, eight of a lane.  A lane's load of a key has kEntries of them in a row, and the four groups of lanes have
+// kCover together.  Where a scale covers as many or more, a slice is what the lanes' words at one place are.  Where it covers half of them, lanes 0 - 31
+// and 32 - 63 exchange words (swap_halves), where a quarter also neighbouring groups (swap_quarters), so that every slice has one scale.
 template <int kCode, int kDim, int kPer>
 __device__ __forceinline__ uint32_t slice_entry(uint32_t t, uint32_t g) {
     using S = Shape<kCode, kDim, kPer>;
-    if constexpr (S::kBits == 16) {
-        return 32u * t + 8u * g;
-    } else if constexpr (kPer == 1) {
-        constexpr uint32_t kEntries = S::kWords * 32 / S::kBits, kOf = kEntries / 8;  // a lane's entries of a unit; slices of a unit
-        return t / kOf * (4u * kEntries) + g * kEntries + t % kOf * 8u;
-    } else {
-        return 32u * t + 8u * g;  // placed by swaps, see below; the order within 32 is slice_order()
-    }
-}
-
-// With blocks of 32 entries a unit's words are exchanged between the groups of lanes.  16 entries a lane (8 bits; 4 bits of 64 entries): words of
-// eight entries w0, w1; after the swap of halves group g has, in slice 0, entries 0 - 7, 16 - 23, 8 - 15, 24 - 31 for g = 0 ... 3, in slice 1 the same
-// of the next block.  32 entries a lane (4 bits): a transposition of four words between four groups, after which group g has word g's place.
-template <int kCode, int kDim>
-__device__ __forceinline__ uint32_t slice_order(uint32_t g) {
-    using S = Shape<kCode, kDim, 2>;
-    constexpr uint32_t kEntries = S::kWords * 32 / S::kBits;
-    if constexpr (kEntries == 16) return (g & 1u) * 16u + (g >> 1) * 8u;
-    return 8u * g;
+    if constexpr (S::kBits == 16 || S::kUnit * 4 == S::kCover) return 32u * t + 8u * g;
+    constexpr uint32_t kOf = S::kEntries / 8;  // slices of a load
+    const uint32_t from = t / kOf * S::kCover, in = t % kOf;
+    if constexpr (S::kUnit * 2 == S::kCover) return from + in / (kOf / 2) * (S::kCover / 2) + g % 2u * S::kEntries + g / 2u * (S::kEntries / 2) + in % (kOf / 2) * 8u;
+    return from + g * S::kEntries + in * 8u;
 }
 
 __device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
@@ -83,8 +72,16 @@ __device__ __forceinline__ bool code_is_odd(u32x4 v) {
     return found;
 }
 
+// Waves per SIMD that registers are kept for: results, queries, codes on their way, scores and weights, and what else there is.
+template <int kCode, int kDim, int kTiles>
+constexpr int waves_of() {
+    using S = Shape<kCode, kDim, 1>;
+    constexpr int kRegisters = kDim * kTiles * 3 / 8 + S::kKeys * S::kRow / 128 + kTiles * S::kKeyTiles * 8 + 60;
+    return kRegisters <= 128 ? 4 : kRegisters <= 168 ? 3 : kRegisters <= 256 ? 2 : 1;
+}
+
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
-__global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Split split) {
+__global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attention_few_kernel(AttentionArgs a, Split split) {
     using S = Shape<kCode, kDim, kPer>;
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kRowsLog2 = kTiles == 1 ? 4 : 5, kRows = 16 * kTiles;
@@ -121,8 +118,12 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
         float most = 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < S::kSlices; t++) {
-            const uint32_t d = kPer == 1 || kFloat ? slice_entry<kCode, kDim, kPer>(t, g) : 32u * t + slice_order<kCode, kDim>(g);
+            const uint32_t d = slice_entry<kCode, kDim, kPer>(t, g);
             q[r][t] = d < dim ? *reinterpret_cast<const u32x4*>(from_q + d * 2u) : u32x4{0, 0, 0, 0};
+        }
+        if (a.scale < 0.0f) {  // into the queries: the largest score is that of the largest product
+#pragma unroll
+            for (uint32_t t = 0; t < S::kSlices; t++) q[r][t] ^= 0x80008000u;
         }
         if constexpr (!kFloat) {
             float v[8];
@@ -148,9 +149,9 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) q[r][t][e] = pair_of<false>(v[place_of<kCode>(2 * e)] * down, v[place_of<kCode>(2 * e + 1)] * down);
             }
-            times[r] = a.scale * bits_f32(power << 23);
+            times[r] = fabsf(a.scale) * bits_f32(power << 23);
         } else {
-            times[r] = a.scale;
+            times[r] = fabsf(a.scale);
         }
         // with a cap: 2 log2(e) t / cap, the exponent of its tanh; else log2(e) t
         times[r] *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
     struct Raw {
         uint32_t k[S::kKeyTiles][S::kUnits][S::kWords];
         u32x4 v[S::kLoads];
-        uint32_t scale[S::kScaleLoads ? S::kScaleLoads : 1], halves;
+        uint32_t scale[2][S::kKeyTiles][S::kScaleLoads ? S::kScaleLoads : 1], halves;  // of keys, of values
     };
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u;
@@ -184,55 +185,80 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
         const uint32_t key = (n * 64u + lane) / S::kLanes;
         value_offset[n] = key % 16u * static_cast<uint32_t>(a.cache.values.slot) + min(lane % S::kLanes * S::kLane, row_bytes - S::kLane);
     }
-    // The scales that a lane loads: of 32 keys those of the key (lanes 0 - 31) and of the value (32 - 63) at once, of 64 one after the other.
-    const uint32_t scale_key = lane % S::kKeys;
-    const auto of_values = [&](uint32_t n) { return S::kKeyTiles == 2 ? lane >= 32u : n >= kPer; };
+    // The scales of a tile of 16 keys: lane l has unit l % kPer of key l / kPer (of 256 entries in two loads).
+    uint32_t scale_offset[2][S::kScaleLoads ? S::kScaleLoads : 1];
+    const auto scale_unit = [&](uint32_t n) { return (n * 64u + lane) % kPer; };
+    const auto scale_key = [&](uint32_t n) { return (n * 64u + lane) / kPer % 16u; };
+    if constexpr (!kFloat) {
+#pragma unroll
+        for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+            const uint32_t block = min(scale_unit(n) * S::kUnit, dim - 1u) >> split.block_log2;
+            scale_offset[0][n] = (scale_key(n) * static_cast<uint32_t>(a.cache.keys.scale_slot) + block * static_cast<uint32_t>(a.cache.keys.scale_block)) << words.log2;
+            scale_offset[1][n] = (scale_key(n) * static_cast<uint32_t>(a.cache.values.scale_slot) + block * static_cast<uint32_t>(a.cache.values.scale_block)) << words.log2;
+        }
+    }
+    const char* const keys_base = a.cache.keys.base + kv_head * a.cache.keys.head;
+    const char* const values_base = a.cache.values.base + kv_head * a.cache.values.head;
+    const char* const key_scales = a.cache.keys.scales + (kv_head * a.cache.keys.scale_head << words.log2);
+    const char* const value_scales = a.cache.values.scales + (kv_head * a.cache.values.scale_head << words.log2);
     const auto place_of_tile = [&](uint32_t t) { return (t - magic_div(t, split.page_magic, split.page_shift) * tiles_of_page) * 16u; };
-    const auto load = [&](uint32_t step, uint32_t nth, Raw& raw) {
-        uint32_t page[S::kKeyTiles], place[S::kKeyTiles];
+    // where a tile of 16 keys lies: its page (of the wave's next steps, by readlane) and its first slot there
+    const auto find_tile = [&](uint32_t step, uint32_t nth, uint32_t k, uint32_t* page, uint32_t* place) {
+        *page = __builtin_amdgcn_readlane(pages, (nth % kAhead) * S::kKeyTiles + k);
+        *place = place_of_tile(tile_of(step, k));
+    };
+    const auto offset_of = [](uint32_t page, uint64_t page_stride, uint32_t place, uint64_t slot_stride) {
+        return static_cast<uint64_t>(page) * static_cast<uint32_t>(page_stride) + place * static_cast<uint32_t>(slot_stride);
+    };
+    const auto load_keys = [&](uint32_t step, uint32_t nth, Raw& raw) {
 #pragma unroll
         for (uint32_t k = 0; k < S::kKeyTiles; k++) {
-            page[k] = __builtin_amdgcn_readlane(pages, (nth % kAhead) * S::kKeyTiles + k);
-            place[k] = place_of_tile(tile_of(step, k));
-            const char* const key_rows = a.cache.keys.base + page[k] * a.cache.keys.page + kv_head * a.cache.keys.head + place[k] * a.cache.keys.slot;
+            uint32_t page, place;
+            find_tile(step, nth, k, &page, &place);
+            const char* const rows = keys_base + offset_of(page, a.cache.keys.page, place, a.cache.keys.slot);
 #pragma unroll
             for (uint32_t u = 0; u < S::kUnits; u++) {
                 if constexpr (S::kWords == 4) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(key_rows + key_offset[u]);
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(rows + key_offset[u]);
 #pragma unroll
                     for (uint32_t e = 0; e < 4; e++) raw.k[k][u][e] = w[e];
                 } else {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(key_rows + key_offset[u]);
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(rows + key_offset[u]);
                     raw.k[k][u][0] = w[0], raw.k[k][u][1] = w[1];
                 }
             }
         }
+    };
+    const auto load_values = [&](uint32_t step, uint32_t nth, Raw& raw) {
+        uint32_t page[S::kKeyTiles], place[S::kKeyTiles];
+#pragma unroll
+        for (uint32_t k = 0; k < S::kKeyTiles; k++) find_tile(step, nth, k, &page[k], &place[k]);
 #pragma unroll
         for (uint32_t n = 0; n < S::kLoads; n++) {
             constexpr uint32_t kKeysOfLoad = 64 / S::kLanes;  // 32 where rows are 32 bytes
             const uint32_t k = n * kKeysOfLoad / 16u;
-            uint64_t rows = page[k] * a.cache.values.page + place[k] * a.cache.values.slot;
+            uint64_t rows = offset_of(page[k], a.cache.values.page, place[k], a.cache.values.slot);
             if constexpr (kKeysOfLoad > 16) {
-                const uint64_t second = page[k + 1] * a.cache.values.page + place[k + 1] * a.cache.values.slot;
+                const uint64_t second = offset_of(page[k + 1], a.cache.values.page, place[k + 1], a.cache.values.slot);
                 rows = lane / S::kLanes >= 16u ? second : rows;
             }
-            raw.v[n] = *reinterpret_cast<const u32x4*>(a.cache.values.base + rows + kv_head * a.cache.values.head + value_offset[n]);
+            raw.v[n] = *reinterpret_cast<const u32x4*>(values_base + rows + value_offset[n]);
         }
         if constexpr (!kFloat) {
-            uint32_t my_page = page[0], my_place = place[0];
-#pragma unroll
-            for (uint32_t k = 1; k < S::kKeyTiles; k++) {
-                my_page = scale_key / 16u == k ? page[k] : my_page;
-                my_place = scale_key / 16u == k ? place[k] : my_place;
-            }
             raw.halves = 0;
 #pragma unroll
-            for (uint32_t n = 0; n < S::kScaleLoads; n++) {
-                const CacheSide& side = of_values(n) ? a.cache.values : a.cache.keys;
-                const uint64_t index = my_page * side.scale_page + kv_head * side.scale_head + (my_place + scale_key % 16u) * side.scale_slot +
-                                       (min(n % kPer * 32u, dim - 1u) >> split.block_log2) * side.scale_block;
-                raw.scale[n] = words.load(side.scales, index);
-                raw.halves |= words.half(side.scales, index) << n;
+            for (uint32_t k = 0; k < S::kKeyTiles; k++) {
+                const char* const of[2] = {key_scales + (offset_of(page[k], a.cache.keys.scale_page, place[k], a.cache.keys.scale_slot) << words.log2),
+                                           value_scales + (offset_of(page[k], a.cache.values.scale_page, place[k], a.cache.values.scale_slot) << words.log2)};
+#pragma unroll
+                for (uint32_t side = 0; side < 2; side++)
+#pragma unroll
+                    for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                        // the word around it: from a word's start on, and half a word further where the tile's first scale is
+                        const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(of[side])) & 2u, offset = scale_offset[side][n] + odd;
+                        raw.scale[side][k][n] = *reinterpret_cast<const uint32_t*>(of[side] - odd + (offset & ~3u));
+                        raw.halves |= (offset >> 1 & 1u) << ((side * S::kKeyTiles + k) * S::kScaleLoads + n);
+                    }
             }
         }
     };
@@ -244,15 +270,15 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
     bool found = false;    // values that are no numbers, among keys that not every row sees
     int32_t power = -126;  // of the largest scale of the values so far: they are taken times 2^-power
 
-    Raw raw, next;
+    Raw raw;
     uint32_t nth = 0;
     if (from + wave < to) {
         look_up(from + wave);
-        load(from + wave, 0, raw);
+        load_values(from + wave, 0, raw);
+        load_keys(from + wave, 0, raw);
     }
     for (uint32_t step = from + wave; step < to; step += 4, nth++) {
         if ((nth + 1u) % kAhead == 0) look_up(step + 4u);
-        load(step + 4u, nth + 1u, next);
         const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys);
         const bool partial = key0 < all_low || key0 + static_cast<int32_t>(S::kKeys) - 1 > all_high;
 
@@ -273,31 +299,48 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
         for (uint32_t n = 0; n < S::kLoads; n++)
             *reinterpret_cast<u32x4*>(mine + (n * 64u + lane) / S::kLanes * S::kPitch + lane % S::kLanes * S::kLane) = raw.v[n];
         if constexpr (!kFloat) {
-            const int32_t key = key0 + static_cast<int32_t>(scale_key);
-            const bool any = key >= low && key <= high;  // what no row sees is not looked at
-            float scale[S::kScaleLoads];
+            bool odd_scale = false;
+            const auto number = [&](uint32_t side, uint32_t k, uint32_t n) {
+                const int32_t key = key0 + static_cast<int32_t>(k * 16u + scale_key(n));
+                const float v = words.number(raw.scale[side][k][n], raw.halves >> ((side * S::kKeyTiles + k) * S::kScaleLoads + n) & 1u);
+                if (!partial) return v;
+                if (key < low || key > high) return 0.0f;  // what no row sees is not looked at
+                if (side == 1 && !(fabsf(v) < INFINITY)) odd_scale = true;
+                return v;
+            };
+            float scale[S::kKeyTiles][S::kScaleLoads];
             uint32_t most = 0;
 #pragma unroll
-            for (uint32_t n = 0; n < S::kScaleLoads; n++) {
-                const float v = words.number(raw.scale[n], raw.halves >> n & 1u);
-                scale[n] = any ? v : 0.0f;
-                const uint32_t field = f32_bits(scale[n]) >> 23 & 255u;
-                if (of_values(n)) most = max(most, field == 255u ? 0u : field);
-            }
-            const int32_t now = static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave_max_bits(most))) - 127;
-            if (now > power) {
-                const float shrink = ldexpf(1.0f, power - min(now, 126));
-                power = min(now, 126);
+            for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                    scale[k][n] = number(1, k, n);
+                    const uint32_t field = f32_bits(scale[k][n]) >> 23 & 255u;
+                    most = max(most, field == 255u ? 0u : field);
+                }
+            if (__builtin_amdgcn_ballot_w64(static_cast<int32_t>(most) - 127 > power)) {
+                const int32_t now = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave_max_bits(most))) - 127, 126);
+                const float shrink = ldexpf(1.0f, power - now);
+                power = now;
 #pragma unroll
                 for (uint32_t r = 0; r < kTiles; r++)
 #pragma unroll
                     for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
             }
+            if (partial) found = found || __builtin_amdgcn_ballot_w64(odd_scale) != 0;
             const float down = bits_f32(static_cast<uint32_t>(127 - power) << 23);
 #pragma unroll
-            for (uint32_t n = 0; n < S::kScaleLoads; n++) scales_at[((of_values(n) ? kPer : 0u) + n % kPer) * S::kKeys + scale_key] = of_values(n) ? scale[n] * down : scale[n];
+            for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                    float* const to = scales_at + scale_unit(n) * S::kKeys + k * 16u + scale_key(n);  // (of 16 or 32 scales some lanes write the same)
+                    to[0] = number(0, k, n);
+                    to[kPer * S::kKeys] = scale[k][n] * down;
+                }
         }
         fence();
+        // the next step's, into the registers that have gone to LDS; its keys behind this step's scores
+        load_values(step + 4u, nth + 1u, raw);
 
         // scores
         f32x4 s[kTiles][S::kKeyTiles];
@@ -311,11 +354,12 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
 #pragma unroll
                     for (uint32_t e = 0; e < S::kWords; e++) w[e] = key_byte(u) < row_bytes ? w[e] : 0u;
                 }
-                if constexpr (kPer > 1 && S::kWords == 4) {
-                    swap_halves(w[0], w[2]), swap_halves(w[1], w[3]);
-                    if constexpr (S::kBits == 4) swap_quarters(w[0], w[1]), swap_quarters(w[2], w[3]);
-                } else if constexpr (kPer > 1) {
-                    swap_halves(w[0], w[1]);
+                if constexpr (!kFloat && S::kUnit < S::kCover) {
+                    if constexpr (S::kWords == 4)
+                        swap_halves(w[0], w[2]), swap_halves(w[1], w[3]);
+                    else
+                        swap_halves(w[0], w[1]);
+                    if constexpr (S::kUnit * 4 == S::kCover) swap_quarters(w[0], w[1]), swap_quarters(w[2], w[3]);
                 }
                 if constexpr (kFloat) {
                     operand[u] = u32x4{w[0], w[1], w[2], w[3]};
@@ -339,35 +383,46 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
                 }
             } else {
 #pragma unroll
-                for (uint32_t t = 0; t < S::kSlices; t++) {
-                    const f32x4 by = *reinterpret_cast<const f32x4*>(scales_at + t * S::kKeys + k * 16u + 4u * g);
+                for (uint32_t unit = 0; unit < kPer; unit++) {
+                    const f32x4 by = *reinterpret_cast<const f32x4*>(scales_at + unit * S::kKeys + k * 16u + 4u * g);
 #pragma unroll
                     for (uint32_t r = 0; r < kTiles; r++) {
-                        const f32x4 v = mfma16<kBF16>(operand[t], q[r][t], f32x4{});
-                        s[r][k] = t == 0 ? v * by : __builtin_elementwise_fma(v, by, s[r][k]);
+                        f32x4 v = {};
+#pragma unroll
+                        for (uint32_t t = unit * S::kUnit / 32; t < (unit + 1) * S::kUnit / 32; t++) v = mfma16<kBF16>(operand[t], q[r][t], v);
+                        s[r][k] = unit == 0 ? v * by : __builtin_elementwise_fma(v, by, s[r][k]);
                     }
                 }
             }
         }
+
+        load_keys(step + 4u, nth + 1u, raw);
 
         // weights
         float p[kTiles][S::kKeyTiles * 4];
 #pragma unroll
         for (uint32_t r = 0; r < kTiles; r++) {
             float most = -INFINITY;
+            const bool plain = !partial && a.cap == 0.0f && !a.slopes;
+            if (!plain) {
+#pragma unroll
+                for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) {
+                        float t = s[r][k][e] * times[r];
+                        const int32_t key = key0 + static_cast<int32_t>(k * 16u + 4u * g + e);
+                        if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
+                        if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
+                        if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
+                        s[r][k][e] = t;
+                    }
+            }
 #pragma unroll
             for (uint32_t k = 0; k < S::kKeyTiles; k++)
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) {
-                    float t = s[r][k][e] * times[r];
-                    const int32_t key = key0 + static_cast<int32_t>(k * 16u + 4u * g + e);
-                    if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
-                    if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
-                    if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
-                    p[r][k * 4 + e] = t;
-                    most = fmaxf(most, t);
-                }
-            most = max_of_groups(most);
+                for (uint32_t e = 0; e < 4; e++) most = fmaxf(most, s[r][k][e]);
+            const float times_now = plain ? times[r] : 1.0f;
+            most = max_of_groups(most * times_now);
             if (__builtin_amdgcn_ballot_w64(most > top[r] + kLazy)) {
                 const float before = top[r];
                 top[r] = fmaxf(top[r], most);
@@ -378,10 +433,12 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
             }
             const float less = kWeightLog2 - (top[r] == -INFINITY ? 0.0f : top[r]);
 #pragma unroll
-            for (uint32_t k = 0; k < S::kKeyTiles * 4; k++) {
-                p[r][k] = __builtin_amdgcn_exp2f(p[r][k] + less);
-                sum[r] += p[r][k];
-            }
+            for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    p[r][k * 4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][k][e], times_now, less));
+                    sum[r] += p[r][k * 4 + e];
+                }
         }
 
         const auto weights_of = [&](uint32_t r, uint32_t block, uint32_t half) {
@@ -393,9 +450,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) {
                     const float of = p[r][(half * 2u + k) * 4u + e];
-                    float v = kFloat ? of : of * by[e];
-                    if (partial) v = of == 0.0f ? 0.0f : v;  // a scale that is not a number, of an entry that is not seen
-                    w[k * 4 + e] = v;
+                    w[k * 4 + e] = kFloat ? of : of * by[e];
                 }
             }
             u32x4 packed;
@@ -423,11 +478,11 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
         u32x4 w[kTiles][kHalves];
 #pragma unroll
         for (uint32_t e = 0; e < kOut; e++) {
-            if (e == 0 || (kPer > 1 && e % 2 == 0))
+            if (e % (S::kUnit / 16) == 0)
 #pragma unroll
                 for (uint32_t r = 0; r < kTiles; r++)
 #pragma unroll
-                    for (uint32_t half = 0; half < kHalves; half++) w[r][half] = weights_of(r, kPer > 1 ? e / 2u : 0u, half);
+                    for (uint32_t half = 0; half < kHalves; half++) w[r][half] = weights_of(r, e / (S::kUnit / 16), half);
             u32x4 v[kHalves];
             values_of(e, v);
 #pragma unroll
@@ -436,16 +491,12 @@ __global__ __launch_bounds__(256) void attention_few_kernel(AttentionArgs a, Spl
                 for (uint32_t r = 0; r < kTiles; r++) out[r][e] = mfma16<kBF16>(v[half], w[r][half], out[r][e]);
         }
         fence();
-        raw = next;
     }
 
-    if constexpr (kCodeHasNaN<kCode>) {
-        if (__syncthreads_or(found)) {
-            const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
-            rows_one_by_one<kDim>(a, at, kv_head, first_key, last_key, reinterpret_cast<float*>(lds),
-                                  [&](uint32_t token, uint32_t head, float most, float all, const float* v) { put_row<kDim>(a, split, part, token, head, most, all, v); });
-            return;
-        }
+    if (__syncthreads_or(found)) {
+        const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
+        rows_one_by_one<kDim>(kRowsLog2, tile, part, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
+        return;
     }
     // The four waves' results, each over its own sum, by their shares of the whole.
     __syncthreads();
@@ -530,8 +581,18 @@ hipError_t launch_tiles(hipStream_t s, const AttentionArgs& a, const Split& spli
 
 template <int kCode, int kDim>
 hipError_t launch_blocks(hipStream_t s, const AttentionArgs& a, const Split& split) {
-    if constexpr (kCode != kCacheFloat)
-        if (a.cache.block < a.cache.dim) return launch_tiles<kCode, kDim, kDim / 32>(s, a, split);
+    if constexpr (kCode != kCacheFloat) {
+        const uint32_t block = a.cache.block;
+        if (block < a.cache.dim) {
+            if constexpr (kDim == 256) {
+                if (block == 32) return launch_tiles<kCode, kDim, 8>(s, a, split);
+                if (block == 64) return launch_tiles<kCode, kDim, 4>(s, a, split);
+            } else if constexpr (kDim == 128) {
+                if (block == 32) return launch_tiles<kCode, kDim, 4>(s, a, split);
+            }
+            return launch_tiles<kCode, kDim, 2>(s, a, split);
+        }
+    }
     return launch_tiles<kCode, kDim, 1>(s, a, split);
 }
 

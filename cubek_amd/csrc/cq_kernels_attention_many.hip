@@ -390,8 +390,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
     if (*found) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
         __syncthreads();
-        rows_one_by_one<kDim>(a, at, kv_head, first_key, last_key, reinterpret_cast<float*>(lds),
-                              [&](uint32_t token, uint32_t head, float most, float all, const float* v) { put_row<kDim>(a, split, part, token, head, most, all, v); });
+        rows_one_by_one<kDim>(S::kRowsLog2, tile, part, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
 
