@@ -39,17 +39,24 @@ constexpr uint32_t kMostSplits = 64;  // a lane each in attention_join_kernel
 uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4; }
 
 // Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (512, 128 of heads up
-// to 64, past 128) by attention_many_kernel.  The keys are split so that `wanted` workgroups come to the GPU, none with less than `fewest` keys.
+// to 64, past 128) by attention_many_kernel.  The keys are split so that `wanted` parts come to the GPU, none of fewer than `fewest` steps: how many of the
+// `splits` a sequence has goes by its length, which the device knows.
 Split split_of(const AttentionArgs& a, uint64_t room) {
     Split f{};
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, mean = (rows + a.seqs - 1) / a.seqs;
     f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? 2 : 0;
     const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : a.cache.dim > 64 ? 256 : 512;
-    const uint64_t wanted = f.row_tiles ? 1024 : 256, fewest = f.row_tiles ? 512 : 1024;
+    const uint64_t step = f.row_tiles && a.cache.code != kCacheInt4 && a.cache.code != kCacheE2M1 ? 32 : 64;
+    f.wanted = f.row_tiles ? 1536 : 256;
+    f.fewest = f.row_tiles ? 512 / step : 16;
     f.tiles = static_cast<uint32_t>(rows / of_tile + a.seqs);
     const uint64_t busy = a.seqs * ((mean + of_tile - 1) / of_tile) * a.cache.kv_heads;
-    const uint64_t most = static_cast<uint64_t>(a.width) * a.cache.page_size / fewest;
-    uint64_t splits = (wanted + busy - 1) / busy;
+    uint64_t keys = static_cast<uint64_t>(a.width) * a.cache.page_size;
+    const uint64_t behind = a.window + (static_cast<uint64_t>(a.tokens) + a.seqs - 1) / a.seqs;
+    if (a.window && behind < keys) keys = behind;
+    const uint64_t most = keys / (f.fewest * step);
+    uint64_t splits = (2ull * f.wanted + busy - 1) / busy;
+    if (a.seqs > 1024) splits = 1;  // their lengths are too many for every workgroup to look at
     splits = splits < most ? splits : most;
     splits = splits < kMostSplits ? splits : kMostSplits;
     if (splits > 1 && part_bytes(a) * splits > room) splits = room / part_bytes(a);
@@ -62,7 +69,7 @@ Split split_of(const AttentionArgs& a, uint64_t room) {
 }
 
 bool fits_a_launch(const AttentionArgs& a, const Split& f) {
-    return static_cast<uint64_t>(f.tiles) * f.splits * (f.row_tiles ? 1 : a.cache.kv_heads) * 256 < kLaunchThreads;
+    return static_cast<uint64_t>(f.tiles) * f.splits * a.cache.kv_heads * (f.row_tiles ? 256 : 512) < kLaunchThreads;
 }
 
 }  // namespace

@@ -162,21 +162,59 @@ struct RowTile {
     Sequence s;
     uint32_t row0, rows;  // first row within the sequence and how many there are
 };
-__device__ __forceinline__ bool find_rows(const AttentionArgs& a, uint32_t tile, uint32_t rows_log2, RowTile* out) {
-    const auto begin = [&](uint32_t i) {
-        const int32_t o = a.offsets[i];
-        return (static_cast<uint64_t>(min(static_cast<uint32_t>(max(o, 0)), a.tokens)) * a.group >> rows_log2) + i;
-    };
-    const uint32_t s = __builtin_amdgcn_readfirstlane(last_at_or_below(a.seqs, tile, begin));
-    const Sequence q = sequence_of(a, s);
-    const uint64_t first = begin(s), rows = static_cast<uint64_t>(q.last - q.first) * a.group;
+__device__ __forceinline__ uint64_t first_tile(const AttentionArgs& a, uint32_t seq, int32_t offset, uint32_t rows_log2) {
+    return (static_cast<uint64_t>(min(static_cast<uint32_t>(max(offset, 0)), a.tokens)) * a.group >> rows_log2) + seq;
+}
+__device__ __forceinline__ bool rows_of(const AttentionArgs& a, const Sequence& s, uint64_t first, uint32_t tile, uint32_t rows_log2, RowTile* out) {
+    const uint64_t rows = static_cast<uint64_t>(s.last - s.first) * a.group;
     if (tile < first) return false;
     const uint64_t row0 = (tile - first) << rows_log2;
     if (row0 >= rows) return false;
-    out->s = q;
+    out->s = s;
     out->row0 = static_cast<uint32_t>(row0);
     out->rows = static_cast<uint32_t>(min(rows - row0, static_cast<uint64_t>(1u << rows_log2)));
     return true;
+}
+__device__ __forceinline__ bool find_rows(const AttentionArgs& a, uint32_t tile, uint32_t rows_log2, RowTile* out) {
+    const uint32_t s = __builtin_amdgcn_readfirstlane(last_at_or_below(a.seqs, tile, [&](uint32_t i) { return first_tile(a, i, a.offsets[i], rows_log2); }));
+    return rows_of(a, sequence_of(a, s), first_tile(a, s, a.offsets[s], rows_log2), tile, rows_log2, out);
+}
+
+// The same, and the steps of `keys_log2` keys of a part, such that all tiles of all sequences come to about split.wanted parts, none of fewer than split.fewest
+// steps: every workgroup works it out from the lengths.  Up to 64 sequences take one round of loads.
+__device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, const Split& split, uint32_t tile, uint32_t rows_log2, uint32_t keys_log2, RowTile* out,
+                                                    uint32_t* steps) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const bool few = a.seqs <= 64;
+    Sequence s{};
+    int32_t offset = 0;
+    uint32_t total = 0;  // 2^31 keys at most of each sequence: 2^26 steps, of 64 sequences a lane each; saturates below
+    *steps = ~0u;
+    if (few || split.splits > 1) {
+        for (uint32_t i = lane; i < a.seqs; i += 64) {
+            s = sequence_of(a, i);
+            offset = a.offsets[i];
+            const uint32_t rows = (s.last - s.first) * a.group, tiles = (rows + (1u << rows_log2) - 1u) >> rows_log2;
+            const uint32_t seen = a.window ? min(static_cast<uint32_t>(s.length), max(a.window, 1u) + (s.last - s.first)) : static_cast<uint32_t>(s.length);
+            total = min(total + min(tiles * ((seen >> keys_log2) + 1u), 1u << 20), 1u << 20);
+        }
+        if (split.splits > 1) {
+            uint32_t all = total;
+#pragma unroll
+            for (int d = 32; d; d >>= 1) all += static_cast<uint32_t>(__shfl_xor(static_cast<int>(all), d, 64));
+            const uint64_t parts = static_cast<uint64_t>(all) * a.cache.kv_heads;
+            *steps = __builtin_amdgcn_readfirstlane(max(split.fewest, static_cast<uint32_t>((parts + split.wanted - 1u) / split.wanted)));
+        }
+    }
+    if (!few) return find_rows(a, tile, rows_log2, out);
+    const uint64_t first = first_tile(a, lane, offset, rows_log2);
+    const uint64_t below = __builtin_amdgcn_ballot_w64(lane < a.seqs && first <= tile);
+    const uint32_t at = below ? 63u - static_cast<uint32_t>(__builtin_clzll(below)) : 0u;
+    const auto from_lane = [&](auto v) { return static_cast<decltype(v)>(__builtin_amdgcn_readlane(static_cast<int>(v), at)); };
+    Sequence q;
+    q.index = at;
+    q.first = from_lane(s.first), q.last = from_lane(s.last), q.length = from_lane(s.length), q.position = from_lane(s.position), q.prefix = from_lane(s.prefix);
+    return rows_of(a, q, first_tile(a, at, from_lane(offset), rows_log2), tile, rows_log2, out);
 }
 
 // The rows of a tile once more, one by one, over the keys from first to last: taken where an entry of a value that is infinite or not a number lies among

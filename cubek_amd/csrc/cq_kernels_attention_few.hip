@@ -88,18 +88,20 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
     constexpr uint32_t kOut = kDim / 16;  // tiles of 16 entries of the result
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15u, g = lane >> 4;
-    const uint32_t part = blockIdx.x % split.splits, tile = blockIdx.x / split.splits, kv_head = blockIdx.y, dim = a.cache.dim;
+    // parts of a tile are far apart in the grid, so that those which have nothing come last
+    const uint32_t tile = blockIdx.x % split.tiles, rest = blockIdx.x / split.tiles, kv_head = rest % a.cache.kv_heads, part = rest / a.cache.kv_heads, dim = a.cache.dim;
     char* const mine = lds + wave * S::kWaveBytes;
     float* const scales_at = reinterpret_cast<float*>(mine + S::kValueBytes);
 
     RowTile at;
-    if (!find_rows(a, tile, kRowsLog2, &at)) return;
+    uint32_t steps_wanted;
+    if (!find_rows_and_steps(a, split, tile, kRowsLog2, S::kKeyTiles == 4 ? 6 : 5, &at, &steps_wanted)) return;
     // the keys that some row of the tile sees, and those that all of them do
     const int32_t first_position = at.s.position + static_cast<int32_t>(at.row0 / a.group), last_position = at.s.position + static_cast<int32_t>((at.row0 + at.rows - 1u) / a.group);
     const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, last_position);
     const int32_t low = first.low, high = last.high, all_low = last.low, all_high = first.high;
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
-    const uint32_t each = (steps_all + split.splits - 1u) / split.splits;
+    const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits), each = (steps_all + parts - 1u) / parts;
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
     const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
 
@@ -219,11 +221,11 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 #pragma unroll
             for (uint32_t u = 0; u < S::kUnits; u++) {
                 if constexpr (S::kWords == 4) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(rows + key_offset[u]);
+                    const u32x4 w = stream_load(reinterpret_cast<const u32x4*>(rows + key_offset[u]));
 #pragma unroll
                     for (uint32_t e = 0; e < 4; e++) raw.k[k][u][e] = w[e];
                 } else {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(rows + key_offset[u]);
+                    const u32x2 w = stream_load(reinterpret_cast<const u32x2*>(rows + key_offset[u]));
                     raw.k[k][u][0] = w[0], raw.k[k][u][1] = w[1];
                 }
             }
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
                 const uint64_t second = offset_of(page[k + 1], a.cache.values.page, place[k + 1], a.cache.values.slot);
                 rows = lane / S::kLanes >= 16u ? second : rows;
             }
-            raw.v[n] = *reinterpret_cast<const u32x4*>(values_base + rows + value_offset[n]);
+            raw.v[n] = stream_load(reinterpret_cast<const u32x4*>(values_base + rows + value_offset[n]));
         }
         if constexpr (!kFloat) {
             raw.halves = 0;
@@ -498,62 +500,54 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         rows_one_by_one<kDim>(kRowsLog2, tile, part, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
-    // The four waves' results, each over its own sum, by their shares of the whole.
-    __syncthreads();
-    constexpr uint32_t kOutPitch = kDim + 4;
-    float* const result = reinterpret_cast<float*>(lds);
-    float* const tops = result + kRows * kOutPitch;  // [wave][row]
+    // The four waves' results, each by its share of the whole over its sum.  A tile of 16 entries of the result is finished by the wave e % 4, which the others
+    // hand theirs.
+    float* const tops = reinterpret_cast<float*>(lds);  // [wave][row]
     float* const sums = tops + 4 * kRows;
-    const float up = ldexpf(1.0f, power);
+    f32x4* const handed = reinterpret_cast<f32x4*>(sums + 4 * kRows);  // [tile of rows][tile of entries][wave that hands][lane]
 #pragma unroll
     for (uint32_t r = 0; r < kTiles; r++) {
         sum[r] = sum_of_groups(sum[r]);
         if (g == 0) tops[wave * kRows + r * 16u + i] = top[r], sums[wave * kRows + r * 16u + i] = sum[r];
     }
     __syncthreads();
-    const auto share_of = [&](uint32_t row, uint32_t of, float* most_out, float* all_out) {
-        float most = -INFINITY, all = 0.0f;
+    const float up = kFloat ? 1.0f : ldexpf(1.0f, power);
+    float most[kTiles], all[kTiles];
 #pragma unroll
-        for (uint32_t w = 0; w < 4; w++) most = fmaxf(most, tops[w * kRows + row]);
-        const float zero = most == -INFINITY ? 0.0f : most;
+    for (uint32_t r = 0; r < kTiles; r++) {
+        most[r] = -INFINITY, all[r] = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < 4; w++) all += sums[w * kRows + row] * __builtin_amdgcn_exp2f(tops[w * kRows + row] - zero);
-        *most_out = most, *all_out = all;
-        return __builtin_amdgcn_exp2f(tops[of * kRows + row] - zero);
-    };
-    for (uint32_t w = 0; w < 4; w++) {
-        if (wave == w)
+        for (uint32_t w = 0; w < 4; w++) most[r] = fmaxf(most[r], tops[w * kRows + r * 16u + i]);
+        const float zero = most[r] == -INFINITY ? 0.0f : most[r];
 #pragma unroll
-            for (uint32_t r = 0; r < kTiles; r++) {
-                float most, all;
-                const float share = share_of(r * 16u + i, w, &most, &all);
-                const float by = sum[r] == 0.0f ? 0.0f : share / all;
+        for (uint32_t w = 0; w < 4; w++) all[r] += sums[w * kRows + r * 16u + i] * __builtin_amdgcn_exp2f(tops[w * kRows + r * 16u + i] - zero);
+        const float share = sum[r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top[r] - zero) / all[r];
 #pragma unroll
-                for (uint32_t e = 0; e < kOut; e++) {
-                    f32x4* const to_row = reinterpret_cast<f32x4*>(result + (r * 16u + i) * kOutPitch + e * 16u + 4u * g);
-                    f32x4 v = {};
-                    if (by != 0.0f || sum[r] != 0.0f) v = out[r][e] * by * (kFloat ? 1.0f : up);
-                    *to_row = w == 0 ? v : *to_row + v;
-                }
-            }
-        __syncthreads();
+        for (uint32_t e = 0; e < kOut; e++) {
+            out[r][e] = sum[r] == 0.0f ? f32x4{} : out[r][e] * share * up;
+            if (e % 4u != wave) handed[((r * kOut + e) * 3u + (wave - e % 4u - 1u) % 4u) * 64u + lane] = out[r][e];
+        }
     }
-    const uint32_t fours = dim / 4u;
-    for (uint32_t n = threadIdx.x; n < at.rows * fours; n += 256) {
-        const uint32_t row = n / fours, d = n % fours * 4u, in_sequence = at.row0 + row;
-        const uint32_t token = at.s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(result + row * kOutPitch + d);
-        if (split.splits == 1) {
-            const bool bf16 = a.dtype == CQ_BF16;
-            const u32x2 w = bf16 ? u32x2{pair_of<true>(v[0], v[1]), pair_of<true>(v[2], v[3])} : u32x2{pair_of<false>(v[0], v[1]), pair_of<false>(v[2], v[3])};
-            *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) = w;
-        } else {
-            const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
-            *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = v;
-            if (d == 0) {
-                float most, all;
-                (void)share_of(row, 0, &most, &all);
-                split.stats[2 * of] = most, split.stats[2 * of + 1] = all;
+    __syncthreads();
+    const bool bf16 = a.dtype == CQ_BF16;
+#pragma unroll
+    for (uint32_t r = 0; r < kTiles; r++) {
+        if (r * 16u + i >= at.rows) continue;
+        const uint32_t in_sequence = at.row0 + r * 16u + i, token = at.s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
+        const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
+        if (split.splits > 1 && wave == 0 && g == 0) split.stats[2 * of] = most[r], split.stats[2 * of + 1] = all[r];
+#pragma unroll
+        for (uint32_t e = 0; e < kOut; e++) {
+            const uint32_t d = e * 16u + 4u * g;
+            if (e % 4u != wave || d >= dim) continue;
+            f32x4 v = out[r][e];
+#pragma unroll
+            for (uint32_t w = 0; w < 3; w++) v += handed[((r * kOut + e) * 3u + w) * 64u + lane];
+            if (split.splits > 1) {
+                if (part < parts) *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = v;
+            } else {
+                const u32x2 w = bf16 ? u32x2{pair_of<true>(v[0], v[1]), pair_of<true>(v[2], v[3])} : u32x2{pair_of<false>(v[0], v[1]), pair_of<false>(v[2], v[3])};
+                *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) = w;
             }
         }
     }
@@ -562,9 +556,9 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
 hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const Split& split) {
     using S = Shape<kCode, kDim, kPer>;
-    const uint32_t waves = 4 * S::kWaveBytes, join = 16 * kTiles * (kDim + 4 + 8) * 4;
-    hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(split.tiles * split.splits, a.cache.kv_heads), dim3(256),
-                       waves > join ? waves : join, s, a, split);
+    const uint32_t waves = 4 * S::kWaveBytes, join = 8 * 16 * kTiles * 4 + kTiles * (kDim / 16) * 3 * 1024;
+    hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(split.tiles * a.cache.kv_heads * split.splits), dim3(256), waves > join ? waves : join,
+                       s, a, split);
     return hipGetLastError();
 }
 

@@ -9,15 +9,26 @@
 namespace cq {
 namespace {
 
+constexpr uint32_t kAtOnce = 8;  // parts on their way
+
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Split split, uint32_t row0) {
     const uint32_t lane = threadIdx.x & 63u, row = row0 + blockIdx.x * 4u + (threadIdx.x >> 6);
     if (row >= a.tokens * a.heads) return;
     const uint32_t token = row / a.heads, head = row % a.heads;
-    const Sequence s = sequence_of(a, last_at_or_below(a.seqs, token, [&](uint32_t i) { return static_cast<uint64_t>(max(a.offsets[i], 0)); }));
-    if (token < s.first || token >= s.last) return;
+    // every lane stays, as the others read its share
+    const uint32_t d = min(lane * 4u, a.cache.dim - 4u);
+    const float* const parts = split.parts + static_cast<uint64_t>(row) * split.splits * a.cache.dim + d;
+    f32x4 of[kAtOnce];
+    const auto load = [&](uint32_t p0) {
+#pragma unroll
+        for (uint32_t p = 0; p < kAtOnce; p++) of[p] = *reinterpret_cast<const f32x4*>(parts + static_cast<uint64_t>(min(p0 + p, split.splits - 1u)) * a.cache.dim);
+    };
+    load(0);
     const float* const stats = split.stats + 2ull * row * split.splits;
     const bool mine = lane < split.splits;
     const float top = mine ? stats[2 * lane] : -INFINITY, sum = mine ? stats[2 * lane + 1] : 0.0f;
+    // whether the token is anybody's, looked up while the parts are on their way: of one that is not, they are not numbers of ours
+    const Sequence s = sequence_of(a, last_at_or_below(a.seqs, token, [&](uint32_t i) { return static_cast<uint64_t>(max(a.offsets[i], 0)); }));
     float most = top;
 #pragma unroll
     for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
@@ -26,22 +37,18 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, Sp
 #pragma unroll
     for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d, 64);
     const float share = all == 0.0f ? 0.0f : weight / all;
-    const float* const parts = split.parts + static_cast<uint64_t>(row) * split.splits * a.cache.dim;
-    // every lane stays, as the others read its share
-    const uint32_t d = min(lane * 4u, a.cache.dim - 4u);
     f32x4 v = {};
-    for (uint32_t p0 = 0; p0 < split.splits; p0 += 8) {
-        f32x4 of[8];
+    for (uint32_t p0 = 0;;) {
 #pragma unroll
-        for (uint32_t p = 0; p < 8; p++) of[p] = *reinterpret_cast<const f32x4*>(parts + static_cast<uint64_t>(min(p0 + p, split.splits - 1u)) * a.cache.dim + d);
-#pragma unroll
-        for (uint32_t p = 0; p < 8; p++) {
+        for (uint32_t p = 0; p < kAtOnce; p++) {
             const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(f32_bits(share), min(p0 + p, 63u)));
-            // a part without keys may hold anything
-            if (p0 + p < split.splits && by != 0.0f) v = __builtin_elementwise_fma(of[p], f32x4{by, by, by, by}, v);
+            if (p0 + p < split.splits && by != 0.0f) v = __builtin_elementwise_fma(of[p], f32x4{by, by, by, by}, v);  // a part without keys may hold anything
         }
+        p0 += kAtOnce;
+        if (p0 >= split.splits) break;
+        load(p0);
     }
-    if (lane * 4u >= a.cache.dim) return;
+    if (token < s.first || token >= s.last || lane * 4u >= a.cache.dim) return;
     const uint64_t at = (token * a.y_token + head * a.y_head + d) * 2u;
     const u32x2 w = a.dtype == CQ_BF16 ? u32x2{pair_of<true>(v[0], v[1]), pair_of<true>(v[2], v[3])} : u32x2{pair_of<false>(v[0], v[1]), pair_of<false>(v[2], v[3])};
     *reinterpret_cast<u32x2*>(a.y + at) = w;

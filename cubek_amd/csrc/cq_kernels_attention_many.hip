@@ -50,12 +50,13 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
     const uint32_t tile = split.tiles - 1u - rest / split.splits, dim = a.cache.dim;
 
     RowTile at;
-    if (!find_rows(a, tile, S::kRowsLog2, &at)) return;
+    uint32_t steps_wanted;
+    if (!find_rows_and_steps(a, split, tile, S::kRowsLog2, 6, &at, &steps_wanted)) return;
     const auto position_of = [&](uint32_t row) { return at.s.position + static_cast<int32_t>((at.row0 + row) / a.group); };
     const Seen top_row = seen_from(a, at.s, position_of(0)), bottom_row = seen_from(a, at.s, position_of(at.rows - 1u));
     const int32_t low = top_row.low, high = bottom_row.high, tile_low = bottom_row.low, tile_high = top_row.high;  // seen by some, and by all
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
-    const uint32_t each = (steps_all + split.splits - 1u) / split.splits;
+    const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits), each = (steps_all + parts - 1u) / parts;
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
     const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
 
