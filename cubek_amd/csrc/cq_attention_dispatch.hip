@@ -38,14 +38,15 @@ constexpr uint32_t kMostSplits = 64;  // a lane each in attention_join_kernel
 
 uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4; }
 
-// Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (512, 128 of heads up
-// to 64, past 128) by attention_many_kernel.  The keys are split so that `wanted` parts come to the GPU, none of fewer than `fewest` steps: how many of the
-// `splits` a sequence has goes by its length, which the device knows.
+// Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (128 of heads past
+// 128) by attention_many_kernel.  The keys are split so that `wanted` parts come to the GPU, none of fewer than `fewest` steps: how many of the `splits` a
+// sequence has goes by its length, which the device knows.  Tiles of many rows that fill the GPU by themselves are not split (496 tiles: 80 us, and 129 with
+// up to two parts of each and their join).
 Split split_of(const AttentionArgs& a, uint64_t room) {
     Split f{};
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, mean = (rows + a.seqs - 1) / a.seqs;
     f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? 2 : 0;
-    const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : a.cache.dim > 64 ? 256 : 512;
+    const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : 256;
     const uint64_t step = f.row_tiles && a.cache.code != kCacheInt4 && a.cache.code != kCacheE2M1 ? 32 : 64;
     f.wanted = f.row_tiles ? 1536 : 256;
     f.fewest = f.row_tiles ? 512 / step : 16;
@@ -55,7 +56,7 @@ Split split_of(const AttentionArgs& a, uint64_t room) {
     const uint64_t behind = a.window + (static_cast<uint64_t>(a.tokens) + a.seqs - 1) / a.seqs;
     if (a.window && behind < keys) keys = behind;
     const uint64_t most = keys / (f.fewest * step);
-    uint64_t splits = (2ull * f.wanted + busy - 1) / busy;
+    uint64_t splits = !f.row_tiles && busy >= f.wanted ? 1 : (2ull * f.wanted + busy - 1) / busy;
     if (a.seqs > 1024) splits = 1;  // their lengths are too many for every workgroup to look at
     splits = splits < most ? splits : most;
     splits = splits < kMostSplits ? splits : kMostSplits;

@@ -156,6 +156,40 @@ struct ScaleWords {
     }
 };
 
+// What a row's products become before their weights: capped, with the bias of their distance, keys that the row does not see at -infinity.  `of` are a lane's
+// products with the keys key0 + place(i); what is returned is left to be multiplied by, `times` where nothing of this is wanted.  `behind`: no key is past
+// the position, so that the distance is linear and costs two instructions a score instead of five.  The conditions are uniform over the wave and each has a loop
+// of its own: as choices within one loop they are all computed for all scores (509 tokens with a bias behind 7681 keys: 214 us instead of 154).
+template <uint32_t kCount, class Place>
+__device__ __forceinline__ float shape_scores(float (&of)[kCount], float times, float cap, bool biased, float slope, int32_t position, int32_t key0, Place place, bool behind,
+                                              bool partial, int32_t row_low, int32_t row_high) {
+    if (cap > 0.0f) {  // cap tanh(t / cap) = cap - 2 cap / (1 + exp(2 t / cap)); `times` holds the 2 / cap
+#pragma unroll
+        for (uint32_t i = 0; i < kCount; i++) of[i] = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(of[i] * times)), cap);
+        times = 1.0f;
+    }
+    if (biased) {
+        if (behind) {
+            const float first = slope * static_cast<float>(key0 - position);
+#pragma unroll
+            for (uint32_t i = 0; i < kCount; i++) of[i] = __builtin_fmaf(of[i], times, __builtin_fmaf(slope, static_cast<float>(place(i)), first));
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kCount; i++) of[i] = __builtin_fmaf(of[i], times, -slope * static_cast<float>(abs(position - key0 - static_cast<int32_t>(place(i)))));
+        }
+        times = 1.0f;
+    }
+    if (partial) {
+#pragma unroll
+        for (uint32_t i = 0; i < kCount; i++) {
+            const int32_t key = key0 + static_cast<int32_t>(place(i));
+            of[i] = key >= row_low && key <= row_high ? of[i] * times : -INFINITY;
+        }
+        times = 1.0f;
+    }
+    return times;
+}
+
 // The tile of rows (token, head of a group) that a workgroup has: tile t of a sequence's own begins at its row t * rows.  Sequence s owns the tiles from
 // offsets[s] * group / rows + s on, which is room enough: floor(a + b) - floor(a) + 1 >= ceil(b).
 struct RowTile {
@@ -217,12 +251,24 @@ __device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, cons
     return rows_of(a, q, first_tile(a, at, from_lane(offset), rows_log2), tile, rows_log2, out);
 }
 
+// Parts of a tile's keys: [token][head][split] results over their own sums and {largest score, sum} (split.parts, split.stats).  A tile with one part writes y.
+// What the parts it does not have would have left is written by its first part: sums of zero, or kWhole where there is nothing to join.
+constexpr float kWhole = -1.0f;
+__device__ __forceinline__ void note_parts(const AttentionArgs& a, const Split& split, const RowTile& at, uint32_t kv_head, uint32_t parts) {
+    for (uint32_t r = threadIdx.x; r < at.rows; r += blockDim.x) {
+        const uint32_t row = at.row0 + r, token = at.s.first + row / a.group, head = kv_head * a.group + row % a.group;
+        float* const of = split.stats + 2ull * (static_cast<uint64_t>(token) * a.heads + head) * split.splits;
+        if (parts == 1) of[0] = -INFINITY, of[1] = kWhole;
+        for (uint32_t p = max(parts, 1u); p < split.splits; p++) of[2 * p] = -INFINITY, of[2 * p + 1] = 0.0f;
+    }
+}
+
 // The rows of a tile once more, one by one, over the keys from first to last: taken where an entry of a value that is infinite or not a number lies among
 // keys that not every row of the tile sees.  A weight of zero does not keep such an entry out of a product of tiles.  All threads of the workgroup
 // come here, with its LDS free for (kDim + 64) floats a wave.  The arguments, the kernel's first two, are read again, so that what is needed here alone
 // takes no registers from what comes before.
 template <uint32_t kDim>
-__device__ __forceinline__ void rows_one_by_one(uint32_t rows_log2, uint32_t tile, uint32_t part, uint32_t kv_head, int64_t first, int64_t last, float* lds) {
+__device__ __forceinline__ void rows_one_by_one(uint32_t rows_log2, uint32_t tile, uint32_t part, uint32_t parts, uint32_t kv_head, int64_t first, int64_t last, float* lds) {
     struct Arguments {
         AttentionArgs a;
         Split split;
@@ -251,12 +297,12 @@ __device__ __forceinline__ void rows_one_by_one(uint32_t rows_log2, uint32_t til
             const uint32_t d = i * 64u + lane;
             if (d >= a.cache.dim) continue;
             const float y = sum != 0.0f ? v[i] / sum : 0.0f;
-            if (split.splits > 1)
+            if (parts > 1)
                 split.parts[of * a.cache.dim + d] = y;
             else
                 store_dtype(a.dtype, a.y, token * a.y_token + head * a.y_head + d, y);
         }
-        if (split.splits > 1 && lane == 0) split.stats[2 * of] = top * kLog2E, split.stats[2 * of + 1] = sum * kWeightOne;
+        if (parts > 1 && lane == 0) split.stats[2 * of] = top * kLog2E, split.stats[2 * of + 1] = sum * kWeightOne;
         __builtin_amdgcn_wave_barrier();
     }
 }

@@ -102,6 +102,8 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
     const int32_t low = first.low, high = last.high, all_low = last.low, all_high = first.high;
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
     const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits), each = (steps_all + parts - 1u) / parts;
+    if (part >= parts) return;
+    if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
     const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
 
@@ -404,26 +406,14 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         float p[kTiles][S::kKeyTiles * 4];
 #pragma unroll
         for (uint32_t r = 0; r < kTiles; r++) {
+            float t[S::kKeyTiles * 4];
+#pragma unroll
+            for (uint32_t i = 0; i < S::kKeyTiles * 4; i++) t[i] = s[r][i / 4u][i % 4u];
+            const float times_now = shape_scores(t, times[r], cap, a.slopes, slope[r], position[r], key0 + static_cast<int32_t>(4u * g), [](uint32_t i) { return i / 4u * 16u + i % 4u; },
+                                                 key0 + static_cast<int32_t>(S::kKeys) - 1 <= first_position, partial, row_low[r], row_high[r]);
             float most = -INFINITY;
-            const bool plain = !partial && a.cap == 0.0f && !a.slopes;
-            if (!plain) {
 #pragma unroll
-                for (uint32_t k = 0; k < S::kKeyTiles; k++)
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; e++) {
-                        float t = s[r][k][e] * times[r];
-                        const int32_t key = key0 + static_cast<int32_t>(k * 16u + 4u * g + e);
-                        if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
-                        if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
-                        if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
-                        s[r][k][e] = t;
-                    }
-            }
-#pragma unroll
-            for (uint32_t k = 0; k < S::kKeyTiles; k++)
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++) most = fmaxf(most, s[r][k][e]);
-            const float times_now = plain ? times[r] : 1.0f;
+            for (uint32_t i = 0; i < S::kKeyTiles * 4; i++) most = fmaxf(most, t[i]);
             most = max_of_groups(most * times_now);
             if (__builtin_amdgcn_ballot_w64(most > top[r] + kLazy)) {
                 const float before = top[r];
@@ -435,12 +425,10 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
             }
             const float less = kWeightLog2 - (top[r] == -INFINITY ? 0.0f : top[r]);
 #pragma unroll
-            for (uint32_t k = 0; k < S::kKeyTiles; k++)
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++) {
-                    p[r][k * 4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][k][e], times_now, less));
-                    sum[r] += p[r][k * 4 + e];
-                }
+            for (uint32_t i = 0; i < S::kKeyTiles * 4; i++) {
+                p[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i], times_now, less));
+                sum[r] += p[r][i];
+            }
         }
 
         const auto weights_of = [&](uint32_t r, uint32_t block, uint32_t half) {
@@ -497,7 +485,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 
     if (__syncthreads_or(found)) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
-        rows_one_by_one<kDim>(kRowsLog2, tile, part, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
+        rows_one_by_one<kDim>(kRowsLog2, tile, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
     // The four waves' results, each by its share of the whole over its sum.  A tile of 16 entries of the result is finished by the wave e % 4, which the others
@@ -535,7 +523,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         if (r * 16u + i >= at.rows) continue;
         const uint32_t in_sequence = at.row0 + r * 16u + i, token = at.s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
         const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
-        if (split.splits > 1 && wave == 0 && g == 0) split.stats[2 * of] = most[r], split.stats[2 * of + 1] = all[r];
+        if (parts > 1 && wave == 0 && g == 0) split.stats[2 * of] = most[r], split.stats[2 * of + 1] = all[r];
 #pragma unroll
         for (uint32_t e = 0; e < kOut; e++) {
             const uint32_t d = e * 16u + 4u * g;
@@ -543,8 +531,8 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
             f32x4 v = out[r][e];
 #pragma unroll
             for (uint32_t w = 0; w < 3; w++) v += handed[((r * kOut + e) * 3u + w) * 64u + lane];
-            if (split.splits > 1) {
-                if (part < parts) *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = v;
+            if (parts > 1) {
+                *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = v;
             } else {
                 const u32x2 w = bf16 ? u32x2{pair_of<true>(v[0], v[1]), pair_of<true>(v[2], v[3])} : u32x2{pair_of<false>(v[0], v[1]), pair_of<false>(v[2], v[3])};
                 *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) = w;

@@ -1,6 +1,6 @@
 // Attention of many rows (token, head of a group): prompts and their chunks.  An object per kind of code (CQ_TU_CODE).
 //
-// A workgroup takes 256 rows (128 of heads longer than 128) that share a head of the cache, a wave 64 of them.  Keys come 64 at a time: the
+// A workgroup takes 256 rows (128 of heads longer than 128) that share a head of the cache, a wave 32 of them.  Keys come 64 at a time: the
 // workgroup loads their codes one step ahead, makes numbers of f16 of them (a cache of floats: as they are) and lays keys and values into LDS, two
 // steps in turn, one barrier a step.  Each wave then computes S^T = K Q^T and O^T = V^T P^T by 32 x 32 x 16 matrix instructions with queries,
 // weights and results in registers: the scores that lane (n, h) gets are those of row n, and stand in the order of keys in which the second product takes
@@ -20,8 +20,8 @@ namespace {
 template <int kCode, int kDim>
 struct Many {
     static constexpr uint32_t kBits = kCodeBits<kCode>, kKeys = 64;
-    static constexpr uint32_t kWaves = kDim > 128 ? 4 : 8, kThreads = 64 * kWaves, kRowTiles = kDim > 64 ? 1 : 2;       // tiles of 32 rows of a wave
-    static constexpr uint32_t kRows = kWaves * 32 * kRowTiles, kRowsLog2 = kRows == 512 ? 9 : kRows == 256 ? 8 : 7;
+    static constexpr uint32_t kWaves = kDim > 128 ? 4 : 8, kThreads = 64 * kWaves;
+    static constexpr uint32_t kRows = kWaves * 32, kRowsLog2 = kRows == 256 ? 8 : 7;
     static constexpr uint32_t kRow = kDim * kBits / 8;                                                  // bytes of a key as it is stored
     static constexpr uint32_t kChunk = kRow * kKeys / kThreads < 16 ? kRow * kKeys / kThreads : 16, kLanes = kRow / kChunk;  // of a thread; threads of a row
     static constexpr uint32_t kEntries = kChunk * 8 / kBits, kChunks = kKeys * kLanes / kThreads;             // entries of a chunk; chunks of a thread
@@ -37,10 +37,10 @@ __device__ __forceinline__ u32x4 in_order(u32x4 v) {
 }
 
 template <int kCode, int kDim, bool kBF16>
-__global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_kernel(AttentionArgs a, Split split) {
+__global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)) void attention_many_kernel(AttentionArgs a, Split split) {
     using S = Many<kCode, kDim>;
     constexpr bool kFloat = kCode == kCacheFloat;
-    constexpr uint32_t kR = S::kRowTiles, kSlices = kDim / 16, kOut = kDim / 32;
+    constexpr uint32_t kSlices = kDim / 16, kOut = kDim / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][wave][keys, values]
     uint32_t* const found = powers + 4 * S::kWaves;                              // whether values that are no numbers need rows one by one
@@ -57,59 +57,61 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
     const int32_t low = top_row.low, high = bottom_row.high, tile_low = bottom_row.low, tile_high = top_row.high;  // seen by some, and by all
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
     const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits), each = (steps_all + parts - 1u) / parts;
+    if (part >= parts) return;
+    if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
     const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
 
     // the wave's rows, and the keys that some of them see and that all of them do
-    const uint32_t wave_row = wave * (32u * kR), wave_last = min(wave_row + 32u * kR, at.rows) - 1u;
+    const uint32_t wave_row = wave * 32u, wave_last = min(wave_row + 32u, at.rows) - 1u;
     const bool rows_here = wave_row < at.rows;
-    const Seen first = seen_from(a, at.s, position_of(min(wave_row, at.rows - 1u))), last = seen_from(a, at.s, position_of(rows_here ? wave_last : at.rows - 1u));
+    const int32_t first_position = position_of(min(wave_row, at.rows - 1u));
+    const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, position_of(rows_here ? wave_last : at.rows - 1u));
     const int32_t wave_low = first.low, wave_high = rows_here ? last.high : -1, all_low = last.low, all_high = first.high;
 
-    u32x4 q[kR][kSlices];
-    float times[kR], slope[kR];
-    int32_t position[kR], row_low[kR], row_high[kR];
+    // the lane's row (past the tile's last one: that one, but nothing seen)
+    const uint32_t own = wave_row + n;
+    const auto row_of = [&] { return min(own, at.rows - 1u) + at.row0; };
+    const auto token_of = [&] { return static_cast<uint64_t>(at.s.first + row_of() / a.group); };
+    const auto head_of = [&] { return kv_head * a.group + row_of() % a.group; };
+    const int32_t position = position_of(min(own, at.rows - 1u));
+    const Seen seen = seen_from(a, at.s, position);
+    const int32_t row_low = seen.low, row_high = own < at.rows ? seen.high : -1;
+    const float slope = a.slopes ? a.slopes[head_of()] * kLog2E : 0.0f;
+    u32x4 q[kSlices];
+    const char* const from_q = a.q + (token_of() * a.q_token + head_of() * a.q_head) * 2u;
 #pragma unroll
-    for (uint32_t r = 0; r < kR; r++) {
-        const uint32_t own = wave_row + r * 32u + n, row = min(own, at.rows - 1u) + at.row0, token = at.s.first + row / a.group, head = kv_head * a.group + row % a.group;
-        position[r] = at.s.position + static_cast<int32_t>(row / a.group);
-        const Seen seen = seen_from(a, at.s, position[r]);
-        row_low[r] = seen.low, row_high[r] = own < at.rows ? seen.high : -1;
-        slope[r] = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
-        const char* const from_q = a.q + (token * a.q_token + head * a.q_head) * 2u;
+    for (uint32_t t = 0; t < kSlices; t++) {
+        const uint32_t d = 16u * t + 8u * h;
+        q[t] = d < dim ? *reinterpret_cast<const u32x4*>(from_q + d * 2u) : u32x4{0, 0, 0, 0};
+    }
+    if (a.scale < 0.0f) {  // into the queries: the largest score is that of the largest product
+#pragma unroll
+        for (uint32_t t = 0; t < kSlices; t++) q[t] ^= 0x80008000u;
+    }
+    float times = fabsf(a.scale);
+    if constexpr (!kFloat) {
+        float most = 0.0f, v[8];
+        const bool bf16 = a.dtype == CQ_BF16;
+        const auto unpack = [&](u32x4 w) { bf16 ? BF16::unpack(w, v) : F16::unpack(w, v); };
 #pragma unroll
         for (uint32_t t = 0; t < kSlices; t++) {
-            const uint32_t d = 16u * t + 8u * h;
-            q[r][t] = d < dim ? *reinterpret_cast<const u32x4*>(from_q + d * 2u) : u32x4{0, 0, 0, 0};
+            unpack(q[t]);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) most = fmaxf(most, fabsf(v[e]));
         }
-        if (a.scale < 0.0f) {  // into the queries: the largest score is that of the largest product
+        const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
+        most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
+        const uint32_t down = power_of_row(most, bf16);
 #pragma unroll
-            for (uint32_t t = 0; t < kSlices; t++) q[r][t] ^= 0x80008000u;
+        for (uint32_t t = 0; t < kSlices; t++) {
+            unpack(q[t]);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) q[t][e] = pair_of<false>(v[2 * e] * bits_f32((254u - down) << 23), v[2 * e + 1] * bits_f32((254u - down) << 23));
         }
-        times[r] = fabsf(a.scale);
-        if constexpr (!kFloat) {
-            float most = 0.0f, v[8];
-            const bool bf16 = a.dtype == CQ_BF16;
-            const auto unpack = [&](u32x4 w) { bf16 ? BF16::unpack(w, v) : F16::unpack(w, v); };
-#pragma unroll
-            for (uint32_t t = 0; t < kSlices; t++) {
-                unpack(q[r][t]);
-#pragma unroll
-                for (uint32_t e = 0; e < 8; e++) most = fmaxf(most, fabsf(v[e]));
-            }
-            const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
-            most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
-            const uint32_t down = power_of_row(most, bf16);
-#pragma unroll
-            for (uint32_t t = 0; t < kSlices; t++) {
-                unpack(q[r][t]);
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++) q[r][t][e] = pair_of<false>(v[2 * e] * bits_f32((254u - down) << 23), v[2 * e + 1] * bits_f32((254u - down) << 23));
-            }
-            times[r] *= bits_f32(down << 23);
-        }
-        times[r] *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
+        times *= bits_f32(down << 23);
     }
+    times *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
     const float cap = a.cap * kLog2E;
 
     // Pages of the next 16 steps, a lane a tile of 16 keys.
@@ -186,10 +188,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
         if (lane == 0) powers[((step & 1u) * S::kWaves + wave) * 2u] = of_keys, powers[((step & 1u) * S::kWaves + wave) * 2u + 1u] = of_values;
     };
 
-    f32x16 out[kR][kOut] = {};
-    float top[kR], sum[kR];
-#pragma unroll
-    for (uint32_t r = 0; r < kR; r++) top[r] = -INFINITY, sum[r] = 0.0f;
+    f32x16 out[kOut] = {};
+    float top = -INFINITY, sum = 0.0f;
     int32_t key_power = -126, value_power = -126;  // of the largest scales so far: entries are taken times 2^-power / 2
 
     // A step's codes as numbers into LDS.  In a step that some row sees only a part of, values that no row sees become zeros, and others that are no
@@ -213,9 +213,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
                 const float shrink = ldexpf(1.0f, value_power - now_values);
                 value_power = now_values;
 #pragma unroll
-                for (uint32_t r = 0; r < kR; r++)
-#pragma unroll
-                    for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
+                for (uint32_t e = 0; e < kOut; e++) out[e] *= shrink;
             }
             down_keys = 0.5f * bits_f32(static_cast<uint32_t>(127 - key_power) << 23), down_values = 0.5f * bits_f32(static_cast<uint32_t>(127 - value_power) << 23);
         }
@@ -274,55 +272,43 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
         const bool partial = key0 < all_low || key0 + 31 > all_high;
         const char* const keys = lds + (step & 1u) * S::kBuffer + 32u * k * S::kPitch;
         const char* const values = keys + S::kSide;
-        f32x16 s[kR] = {};
+        f32x16 s = {};
 #pragma unroll
         for (uint32_t t = 0; t < kSlices; t++) {
             const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + n * S::kPitch + t * 32u + h * 16u);
-#pragma unroll
-            for (uint32_t r = 0; r < kR; r++) s[r] = mfma32<kBF16>(operand, q[r][t], s[r]);
+            s = mfma32<kBF16>(operand, q[t], s);
         }
-        u32x4 w[kR][2];
+        u32x4 w[2];
+        // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
+        const float by = kFloat ? times : times * 2.0f * bits_f32(static_cast<uint32_t>(127 + key_power) << 23);
+        float t[16];
 #pragma unroll
-        for (uint32_t r = 0; r < kR; r++) {
-            // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
-            const float by = kFloat ? times[r] : times[r] * 2.0f * bits_f32(static_cast<uint32_t>(127 + key_power) << 23);
-            const bool plain = !partial && a.cap == 0.0f && !a.slopes;
-            float most = -INFINITY;
-            if (!plain) {
+        for (uint32_t v = 0; v < 16; v++) t[v] = s[v];
+        const float times_now = shape_scores(t, by, cap, a.slopes, slope, position, key0 + static_cast<int32_t>(4u * h), [](uint32_t v) { return v / 4u * 8u + v % 4u; },
+                                             key0 + 31 <= first_position, partial, row_low, row_high);
+        float most = -INFINITY;
 #pragma unroll
-                for (uint32_t v = 0; v < 16; v++) {
-                    float t = s[r][v] * by;
-                    const int32_t key = key0 + static_cast<int32_t>(v / 4u * 8u + 4u * h + v % 4u);
-                    if (a.cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)));
-                    if (a.slopes) t -= slope[r] * static_cast<float>(abs(position[r] - key));
-                    if (partial) t = key >= row_low[r] && key <= row_high[r] ? t : -INFINITY;
-                    s[r][v] = t;
-                }
-            }
+        for (uint32_t v = 0; v < 16; v++) most = fmaxf(most, t[v]);
+        most *= times_now;
+        const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
+        most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
+        if (__builtin_amdgcn_ballot_w64(most > top + kLazy)) {
+            const float before = top;
+            top = fmaxf(top, most);
+            const float shrink = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - top);
+            sum *= shrink;
 #pragma unroll
-            for (uint32_t v = 0; v < 16; v++) most = fmaxf(most, s[r][v]);
-            const float times_now = plain ? by : 1.0f;
-            most *= times_now;
-            const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
-            most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
-            if (__builtin_amdgcn_ballot_w64(most > top[r] + kLazy)) {
-                const float before = top[r];
-                top[r] = fmaxf(top[r], most);
-                const float shrink = top[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - top[r]);
-                sum[r] *= shrink;
-#pragma unroll
-                for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
-            }
-            const float less = kWeightLog2 - (top[r] == -INFINITY ? 0.0f : top[r]);
-            float p[16];
-#pragma unroll
-            for (uint32_t v = 0; v < 16; v++) {
-                p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][v], times_now, less));
-                sum[r] += p[v];
-            }
-#pragma unroll
-            for (uint32_t v = 0; v < 16; v += 2) w[r][v / 8][v % 8 / 2] = pair_of<kBF16>(p[v], p[v + 1]);
+            for (uint32_t e = 0; e < kOut; e++) out[e] *= shrink;
         }
+        const float less = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
+        float p[16];
+#pragma unroll
+        for (uint32_t v = 0; v < 16; v++) {
+            p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less));
+            sum += p[v];
+        }
+#pragma unroll
+        for (uint32_t v = 0; v < 16; v += 2) w[v / 8][v % 8 / 2] = pair_of<kBF16>(p[v], p[v + 1]);
         // lane (n, h): entry n of 32, keys 4 h ... 4 h + 3 and 8 more
         const auto values_of = [&](uint32_t e, uint32_t half) {
             u32x4 v;
@@ -340,8 +326,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
 #pragma unroll
             for (uint32_t half = 0; half < 2; half++) {
                 const u32x4 v = values_of(e, half);
-#pragma unroll
-                for (uint32_t r = 0; r < kR; r++) out[r][e] = mfma32<kBF16>(v, w[r][half], out[r][e]);
+                out[e] = mfma32<kBF16>(v, w[half], out[e]);
             }
     };
 
@@ -391,37 +376,32 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads)) void attention_many_
     if (*found) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
         __syncthreads();
-        rows_one_by_one<kDim>(S::kRowsLog2, tile, part, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
+        rows_one_by_one<kDim>(S::kRowsLog2, tile, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
 
     const float up = kFloat ? 1.0f : 2.0f * ldexpf(1.0f, value_power);
+    const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum), f32_bits(sum), false, false);
+    const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
+    const float by = all == 0.0f ? 0.0f : 1.0f / all;
+    if (own >= at.rows) return;
+    const uint64_t token = token_of(), of = (token * a.heads + head_of()) * split.splits + part;
+    if (parts > 1 && h == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = all;
 #pragma unroll
-    for (uint32_t r = 0; r < kR; r++) {
-        const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum[r]), f32_bits(sum[r]), false, false);
-        const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
-        const float by = all == 0.0f ? 0.0f : 1.0f / all;
-        const uint32_t own = wave_row + r * 32u + n;
-        if (own >= at.rows) continue;
-        const uint32_t row = own + at.row0, token = at.s.first + row / a.group, head = kv_head * a.group + row % a.group;
-        const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
-        if (split.splits > 1 && h == 0) split.stats[2 * of] = top[r], split.stats[2 * of + 1] = all;
+    for (uint32_t e = 0; e < kOut; e++)
 #pragma unroll
-        for (uint32_t e = 0; e < kOut; e++)
+        for (uint32_t v = 0; v < 16; v += 4) {
+            const uint32_t d = e * 32u + v * 2u + 4u * h;
+            if (d >= dim) continue;
+            f32x4 four;
 #pragma unroll
-            for (uint32_t v = 0; v < 16; v += 4) {
-                const uint32_t d = e * 32u + v * 2u + 4u * h;
-                if (d >= dim) continue;
-                f32x4 four;
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) four[i] = all == 0.0f ? 0.0f : out[r][e][v + i] * by * up;
-                if (split.splits > 1)
-                    *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = four;
-                else
-                    *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) =
-                        a.dtype == CQ_BF16 ? u32x2{pair_of<true>(four[0], four[1]), pair_of<true>(four[2], four[3])} : u32x2{pair_of<false>(four[0], four[1]), pair_of<false>(four[2], four[3])};
-            }
-    }
+            for (uint32_t i = 0; i < 4; i++) four[i] = all == 0.0f ? 0.0f : out[e][v + i] * by * up;
+            if (parts > 1)
+                *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = four;
+            else
+                *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head_of() * a.y_head + d) * 2u) =
+                    a.dtype == CQ_BF16 ? u32x2{pair_of<true>(four[0], four[1]), pair_of<true>(four[2], four[3])} : u32x2{pair_of<false>(four[0], four[1]), pair_of<false>(four[2], four[3])};
+        }
 }
 
 template <int kCode, int kDim, bool kBF16>
