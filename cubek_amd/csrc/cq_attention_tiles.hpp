@@ -136,25 +136,21 @@ __device__ __forceinline__ bool has_odd(u32x4 v) {
     return found;
 }
 
-// A stored scale is loaded as the word around it and made a number later, by masks instead of branches: a load is not waited for where it is
-// issued.  All bits or none of a word, by the type of the scales (uniform over the launch).
+// A stored scale is loaded as the word around it, from `offset & ~3` on, and made a number later: a load is not waited for where it is issued.
 struct ScaleWords {
-    uint32_t f32, bf16, f16, log2;
-    __device__ explicit ScaleWords(uint32_t dtype)
-        : f32(dtype == CQ_F32 ? ~0u : 0u), bf16(dtype == CQ_BF16 ? ~0u : 0u), f16(dtype == CQ_F16 ? ~0u : 0u), log2(dtype == CQ_F32 ? 2u : 1u) {}
-    __device__ __forceinline__ uint32_t load(const char* scales, uint64_t i) const {
-        return *reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(scales + (i << log2)) & ~static_cast<uintptr_t>(3));
-    }
-    // which half of its word a scale of 16 bits is
-    __device__ __forceinline__ uint32_t half(const char* scales, uint64_t i) const {
-        return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(scales + (i << log2)) >> 1) & 1u;
-    }
-    __device__ __forceinline__ float number(uint32_t word, uint32_t half) const {
-        const uint32_t bits = word >> (half * 16u);
-        const uint32_t from_f16 = f32_bits(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits))));
-        return bits_f32((word & f32) | (bits << 16 & bf16) | (from_f16 & f16));
+    uint32_t log2, up;
+    bool f16;
+    __device__ explicit ScaleWords(uint32_t dtype) : log2(dtype == CQ_F32 ? 2u : 1u), up(dtype == CQ_BF16 ? 16u : 0u), f16(dtype == CQ_F16) {}
+    __device__ __forceinline__ float number(uint32_t word, uint32_t offset) const {
+        const uint32_t bits = __builtin_amdgcn_alignbyte(0u, word, offset & 3u) << up;
+        return f16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits))) : bits_f32(bits);
     }
 };
+// The exponent field of a scale, zero of one that is no number.
+__device__ __forceinline__ uint32_t exponent_of(float v) {
+    const uint32_t field = f32_bits(v) >> 23 & 255u;
+    return field == 255u ? 0u : field;
+}
 
 // What a row's products become before their weights: capped, with the bias of their distance, keys that the row does not see at -infinity.  `of` are a lane's
 // products with the keys key0 + place(i); what is returned is left to be multiplied by, `times` where nothing of this is wanted.  `behind`: no key is past

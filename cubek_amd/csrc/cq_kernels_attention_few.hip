@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
     struct Raw {
         uint32_t k[S::kKeyTiles][S::kUnits][S::kWords];
         u32x4 v[S::kLoads];
-        uint32_t scale[2][S::kKeyTiles][S::kScaleLoads ? S::kScaleLoads : 1], halves;  // of keys, of values
+        uint32_t scale[2][S::kKeyTiles][S::kScaleLoads ? S::kScaleLoads : 1], odd;  // of keys, of values; bits 2 (side * kKeyTiles + tile) ...: half a word that a tile's begin with
     };
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u;
@@ -249,20 +249,19 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
             raw.v[n] = stream_load(reinterpret_cast<const u32x4*>(values_base + rows + value_offset[n]));
         }
         if constexpr (!kFloat) {
-            raw.halves = 0;
+            raw.odd = 0;
 #pragma unroll
             for (uint32_t k = 0; k < S::kKeyTiles; k++) {
                 const char* const of[2] = {key_scales + (offset_of(page[k], a.cache.keys.scale_page, place[k], a.cache.keys.scale_slot) << words.log2),
                                            value_scales + (offset_of(page[k], a.cache.values.scale_page, place[k], a.cache.values.scale_slot) << words.log2)};
 #pragma unroll
-                for (uint32_t side = 0; side < 2; side++)
+                for (uint32_t side = 0; side < 2; side++) {
+                    // words: from a word's start on, and half a word further where the tile's first scale is
+                    const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(of[side])) & 2u;
+                    raw.odd |= odd << (2 * (side * S::kKeyTiles + k));
 #pragma unroll
-                    for (uint32_t n = 0; n < S::kScaleLoads; n++) {
-                        // the word around it: from a word's start on, and half a word further where the tile's first scale is
-                        const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(of[side])) & 2u, offset = scale_offset[side][n] + odd;
-                        raw.scale[side][k][n] = *reinterpret_cast<const uint32_t*>(of[side] - odd + (offset & ~3u));
-                        raw.halves |= (offset >> 1 & 1u) << ((side * S::kKeyTiles + k) * S::kScaleLoads + n);
-                    }
+                    for (uint32_t n = 0; n < S::kScaleLoads; n++) raw.scale[side][k][n] = *reinterpret_cast<const uint32_t*>(of[side] - odd + ((scale_offset[side][n] + odd) & ~3u));
+                }
             }
         }
     };
@@ -303,27 +302,37 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         for (uint32_t n = 0; n < S::kLoads; n++)
             *reinterpret_cast<u32x4*>(mine + (n * 64u + lane) / S::kLanes * S::kPitch + lane % S::kLanes * S::kLane) = raw.v[n];
         if constexpr (!kFloat) {
-            bool odd_scale = false;
-            const auto number = [&](uint32_t side, uint32_t k, uint32_t n) {
-                const int32_t key = key0 + static_cast<int32_t>(k * 16u + scale_key(n));
-                const float v = words.number(raw.scale[side][k][n], raw.halves >> ((side * S::kKeyTiles + k) * S::kScaleLoads + n) & 1u);
-                if (!partial) return v;
-                if (key < low || key > high) return 0.0f;  // what no row sees is not looked at
-                if (side == 1 && !(fabsf(v) < INFINITY)) odd_scale = true;
-                return v;
-            };
-            float scale[S::kKeyTiles][S::kScaleLoads];
-            uint32_t most = 0;
+            float scale[2][S::kKeyTiles][S::kScaleLoads], most = 0.0f;
+#pragma unroll
+            for (uint32_t side = 0; side < 2; side++)
+#pragma unroll
+                for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                    for (uint32_t n = 0; n < S::kScaleLoads; n++)
+                        scale[side][k][n] = words.number(raw.scale[side][k][n], scale_offset[side][n] + (raw.odd >> (2 * (side * S::kKeyTiles + k)) & 2u));
+            if (partial) {
+                bool odd = false;
+#pragma unroll
+                for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                    for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                        const int32_t key = key0 + static_cast<int32_t>(k * 16u + scale_key(n));
+                        if (key < low || key > high) scale[0][k][n] = scale[1][k][n] = 0.0f;  // what no row sees is not looked at
+                        odd = odd || !(fabsf(scale[1][k][n]) < INFINITY);
+                    }
+                found = found || __builtin_amdgcn_ballot_w64(odd) != 0;
+            }
 #pragma unroll
             for (uint32_t k = 0; k < S::kKeyTiles; k++)
 #pragma unroll
-                for (uint32_t n = 0; n < S::kScaleLoads; n++) {
-                    scale[k][n] = number(1, k, n);
-                    const uint32_t field = f32_bits(scale[k][n]) >> 23 & 255u;
-                    most = max(most, field == 255u ? 0u : field);
-                }
-            if (__builtin_amdgcn_ballot_w64(static_cast<int32_t>(most) - 127 > power)) {
-                const int32_t now = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave_max_bits(most))) - 127, 126);
+                for (uint32_t n = 0; n < S::kScaleLoads; n++) most = fmaxf(most, fabsf(scale[1][k][n]));
+            if (__builtin_amdgcn_ballot_w64(!(most < bits_f32(static_cast<uint32_t>(128 + power) << 23)))) {  // 2^(power + 1)
+                uint32_t field = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < S::kKeyTiles; k++)
+#pragma unroll
+                    for (uint32_t n = 0; n < S::kScaleLoads; n++) field = max(field, exponent_of(scale[1][k][n]));
+                const int32_t now = max(power, min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave_max_bits(field))) - 127, 126));
                 const float shrink = ldexpf(1.0f, power - now);
                 power = now;
 #pragma unroll
@@ -331,15 +340,14 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 #pragma unroll
                     for (uint32_t e = 0; e < kOut; e++) out[r][e] *= shrink;
             }
-            if (partial) found = found || __builtin_amdgcn_ballot_w64(odd_scale) != 0;
             const float down = bits_f32(static_cast<uint32_t>(127 - power) << 23);
 #pragma unroll
             for (uint32_t k = 0; k < S::kKeyTiles; k++)
 #pragma unroll
                 for (uint32_t n = 0; n < S::kScaleLoads; n++) {
                     float* const to = scales_at + scale_unit(n) * S::kKeys + k * 16u + scale_key(n);  // (of 16 or 32 scales some lanes write the same)
-                    to[0] = number(0, k, n);
-                    to[kPer * S::kKeys] = scale[k][n] * down;
+                    to[0] = scale[0][k][n];
+                    to[kPer * S::kKeys] = scale[1][k][n] * down;
                 }
         }
         fence();

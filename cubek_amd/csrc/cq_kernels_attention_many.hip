@@ -42,8 +42,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kSlices = kDim / 16, kOut = kDim / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][wave][keys, values]
-    uint32_t* const found = powers + 4 * S::kWaves;                              // whether values that are no numbers need rows one by one
+    uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][keys, values]: exponents, the largest of every other step so far
+    uint32_t* const found = powers + 4;                                          // whether values that are no numbers need rows one by one
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31u, h = lane >> 5;
     // neighbours in the grid are heads of the cache: with eight of them each die keeps one in its L2.  The tiles with most keys come first.
     const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads, part = rest % split.splits;
@@ -126,26 +126,34 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         uint32_t k[S::kChunks][S::kChunk / 4], v[S::kChunks][S::kChunk / 4];
     };
     struct Scales {
-        uint32_t k[S::kChunks], v[S::kChunks], halves;
+        uint32_t k[S::kChunks], v[S::kChunks], odd;  // words; bits 2 c ... of keys and 16 + 2 c ... of values: half a word that their tile begins with
     };
+    constexpr uint32_t kPass = S::kThreads / S::kLanes;  // keys of the workgroup's chunks at once, 8 or a multiple of 16
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u, byte = threadIdx.x % S::kLanes * S::kChunk, entry = byte * 8u / S::kBits;
     const uint32_t block = min(entry, dim - 1u) >> split.block_log2;
-    const auto key_of = [&](uint32_t c) { return (c * S::kThreads + threadIdx.x) / S::kLanes; };
-    // the page of a chunk's tile of 16 keys (the same for the wave) and the row in it
+    const auto key_of = [&](uint32_t c) { return c * kPass + threadIdx.x / S::kLanes; };
+    // a thread's offsets from the tile of 16 keys that holds its key; what is left is the same for the wave
+    const uint32_t in_tile = threadIdx.x / S::kLanes % 16u, at_byte = min(byte, row_bytes - S::kChunk);
+    const uint32_t key_at = in_tile * static_cast<uint32_t>(a.cache.keys.slot) + at_byte, value_at = in_tile * static_cast<uint32_t>(a.cache.values.slot) + at_byte;
+    const auto scale_at = [&](const CacheSide& side) { return (in_tile * static_cast<uint32_t>(side.scale_slot) + block * static_cast<uint32_t>(side.scale_block)) << words.log2; };
+    const uint32_t key_scale_at = scale_at(a.cache.keys), value_scale_at = scale_at(a.cache.values);
+    // the page of a chunk's tile and the row in it
     const auto place = [&](uint32_t step, uint32_t c, uint32_t* page, uint32_t* slot) {
-        const uint32_t k = __builtin_amdgcn_readfirstlane(key_of(c) / 16u);
+        const uint32_t k = (c * kPass + wave * (64u / S::kLanes)) / 16u;
         *page = __builtin_amdgcn_readlane(pages, (step - from) % 16u * 4u + k);
-        *slot = place_of_tile(tile_of(step, k)) + key_of(c) % 16u;
+        *slot = place_of_tile(tile_of(step, k)) + c * kPass % 16u;
+    };
+    const auto rows_at = [&](const CacheSide& side, uint32_t page, uint32_t slot) {
+        return side.base + kv_head * side.head + static_cast<uint64_t>(page) * static_cast<uint32_t>(side.page) + slot * static_cast<uint32_t>(side.slot);
     };
     const auto load = [&](uint32_t step, Raw& raw) {
 #pragma unroll
         for (uint32_t c = 0; c < S::kChunks; c++) {
             uint32_t page, slot;
             place(step, c, &page, &slot);
-            const uint64_t at_byte = min(byte, row_bytes - S::kChunk);
-            const char* const k = a.cache.keys.base + page * a.cache.keys.page + kv_head * a.cache.keys.head + slot * a.cache.keys.slot + at_byte;
-            const char* const v = a.cache.values.base + page * a.cache.values.page + kv_head * a.cache.values.head + slot * a.cache.values.slot + at_byte;
+            const char* const k = rows_at(a.cache.keys, page, slot) + key_at;
+            const char* const v = rows_at(a.cache.values, page, slot) + value_at;
             if constexpr (S::kChunk == 4) {
                 raw.k[c][0] = *reinterpret_cast<const uint32_t*>(k), raw.v[c][0] = *reinterpret_cast<const uint32_t*>(v);
             } else if constexpr (S::kChunk == 16) {
@@ -159,55 +167,64 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         }
     };
     const auto load_scales = [&](uint32_t step, Scales& s) {
-        s.halves = 0;
+        s.odd = 0;
 #pragma unroll
         for (uint32_t c = 0; c < S::kChunks; c++) {
             uint32_t page, slot;
             place(step, c, &page, &slot);
-            const auto index = [&](const CacheSide& side) { return page * side.scale_page + kv_head * side.scale_head + slot * side.scale_slot + block * side.scale_block; };
-            const uint64_t k = index(a.cache.keys), v = index(a.cache.values);
-            s.k[c] = words.load(a.cache.keys.scales, k);
-            s.v[c] = words.load(a.cache.values.scales, v);
-            s.halves |= words.half(a.cache.keys.scales, k) << (2 * c) | words.half(a.cache.values.scales, v) << (2 * c + 1);
+            const auto from_word = [&](const CacheSide& side, uint32_t at, uint32_t shift) {
+                const char* const of = side.scales + ((kv_head * side.scale_head + static_cast<uint64_t>(page) * static_cast<uint32_t>(side.scale_page) + slot * static_cast<uint32_t>(side.scale_slot)) << words.log2);
+                const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(of)) & 2u;
+                s.odd |= odd << shift;
+                return *reinterpret_cast<const uint32_t*>(of - odd + ((at + odd) & ~3u));
+            };
+            s.k[c] = from_word(a.cache.keys, key_scale_at, 2 * c), s.v[c] = from_word(a.cache.values, value_scale_at, 16 + 2 * c);
         }
     };
-    // The exponents of the largest scales of a step that any row sees, for the workgroup.
+    int32_t key_power = -126, value_power = -126;  // of the largest scales so far: entries are taken times 2^-power / 2
+    // A step's scales as numbers, and for the workgroup the exponents of its largest ones that any row sees, where they pass what was there before.
+    float key_scale[S::kChunks], value_scale[S::kChunks];
     const auto publish = [&](uint32_t step, const Scales& s) {
-        uint32_t of_keys = 0, of_values = 0;
+        const int32_t step_key = static_cast<int32_t>((step0 + step) * S::kKeys);
+        float of_keys = 0.0f, of_values = 0.0f;
 #pragma unroll
         for (uint32_t c = 0; c < S::kChunks; c++) {
-            const int32_t key = static_cast<int32_t>((step0 + step) * S::kKeys + key_of(c));
-            const auto field = [&](float v) {
-                const uint32_t f = f32_bits(v) >> 23 & 255u;
-                return key < low || key > high || f == 255u ? 0u : f;
-            };
-            of_keys = max(of_keys, field(words.number(s.k[c], s.halves >> (2 * c) & 1u)));
-            of_values = max(of_values, field(words.number(s.v[c], s.halves >> (2 * c + 1) & 1u)));
+            key_scale[c] = words.number(s.k[c], key_scale_at + (s.odd >> (2 * c) & 2u));
+            value_scale[c] = words.number(s.v[c], value_scale_at + (s.odd >> (16 + 2 * c) & 2u));
         }
-        of_keys = wave_max_bits(of_keys), of_values = wave_max_bits(of_values);
-        if (lane == 0) powers[((step & 1u) * S::kWaves + wave) * 2u] = of_keys, powers[((step & 1u) * S::kWaves + wave) * 2u + 1u] = of_values;
+        if (step_key < low || step_key + static_cast<int32_t>(S::kKeys) - 1 > high) {
+#pragma unroll
+            for (uint32_t c = 0; c < S::kChunks; c++) {
+                const int32_t key = step_key + static_cast<int32_t>(key_of(c));
+                if (key < low || key > high) key_scale[c] = value_scale[c] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < S::kChunks; c++) of_keys = fmaxf(of_keys, fabsf(key_scale[c])), of_values = fmaxf(of_values, fabsf(value_scale[c]));
+        const auto limit = [](int32_t power) { return bits_f32(static_cast<uint32_t>(128 + power) << 23); };  // 2^(power + 1)
+        if (__builtin_amdgcn_ballot_w64(!(of_keys < limit(key_power)) || !(of_values < limit(value_power)))) {
+            uint32_t keys = 0, values = 0;
+#pragma unroll
+            for (uint32_t c = 0; c < S::kChunks; c++) keys = max(keys, exponent_of(key_scale[c])), values = max(values, exponent_of(value_scale[c]));
+            keys = wave_max_bits(keys), values = wave_max_bits(values);
+            if (lane == 0) atomicMax(powers + (step & 1u) * 2u, keys), atomicMax(powers + (step & 1u) * 2u + 1u, values);
+        }
     };
 
     f32x16 out[kOut] = {};
     float top = -INFINITY, sum = 0.0f;
-    int32_t key_power = -126, value_power = -126;  // of the largest scales so far: entries are taken times 2^-power / 2
 
     // A step's codes as numbers into LDS.  In a step that some row sees only a part of, values that no row sees become zeros, and others that are no
     // numbers are reported.
-    const auto lay = [&](uint32_t step, Raw& raw, const Scales& s) {
+    const auto lay = [&](uint32_t step, Raw& raw) {
         char* const to_keys = lds + (step & 1u) * S::kBuffer;
         const int32_t step_key = static_cast<int32_t>((step0 + step) * S::kKeys);
         const bool partial = step_key < tile_low || step_key + static_cast<int32_t>(S::kKeys) - 1 > tile_high;
         float down_keys = 0.0f, down_values = 0.0f;
         if constexpr (!kFloat) {
-            uint32_t of_keys = 0, of_values = 0;
-#pragma unroll
-            for (uint32_t w = 0; w < S::kWaves; w++) {
-                const uint32_t* const of = powers + ((step & 1u) * S::kWaves + w) * 2u;
-                of_keys = max(of_keys, of[0]), of_values = max(of_values, of[1]);
-            }
-            const int32_t now_keys = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of_keys)) - 127, 126);
-            const int32_t now_values = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of_values)) - 127, 126);
+            const uint32_t* const of = powers + (step & 1u) * 2u;
+            const int32_t now_keys = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of[0])) - 127, 126);
+            const int32_t now_values = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of[1])) - 127, 126);
             key_power = max(key_power, now_keys);
             if (now_values > value_power) {
                 const float shrink = ldexpf(1.0f, value_power - now_values);
@@ -220,18 +237,15 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
 #pragma unroll
         for (uint32_t c = 0; c < S::kChunks; c++) {
             char* const row = to_keys + key_of(c) * S::kPitch + entry * 2u;
-            if (byte >= row_bytes) {  // a shorter head: nothing past its end
+            if (row_bytes < S::kRow) {  // a shorter head: nothing past its end
 #pragma unroll
-                for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.k[c][e] = 0, raw.v[c][e] = 0;
+                for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.k[c][e] = byte < row_bytes ? raw.k[c][e] : 0u, raw.v[c][e] = byte < row_bytes ? raw.v[c][e] : 0u;
             }
-            float value_scale = 1.0f;
-            if constexpr (!kFloat) value_scale = words.number(s.v[c], s.halves >> (2 * c + 1) & 1u) * down_values;
             if (partial) {
                 const int32_t key = step_key + static_cast<int32_t>(key_of(c));
                 if (key < low || key > high) {
 #pragma unroll
                     for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.v[c][e] = 0;
-                    value_scale = 0.0f;
                 }
             }
             const auto look = [&](u32x4 v) {
@@ -259,8 +273,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
                         *reinterpret_cast<u32x4*>(to + e / kEach * 16u) = v;
                     }
                 };
-                put(row, raw.k[c], words.number(s.k[c], s.halves >> (2 * c) & 1u) * down_keys, false);
-                put(row + S::kSide, raw.v[c], value_scale, true);
+                put(row, raw.k[c], key_scale[c] * down_keys, false);
+                put(row + S::kSide, raw.v[c], value_scale[c] * down_values, true);
             }
         }
     };
@@ -330,24 +344,21 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
             }
     };
 
-    if (threadIdx.x == 0) *found = 0u;
+    if (threadIdx.x < 5) powers[threadIdx.x] = 0u;  // and *found
     __syncthreads();
     if (from < to) {
         Raw raw;
-        Scales scales{}, scales_next{};
+        Scales scales{};
         look_up(from);
         load(from, raw);
         if constexpr (!kFloat) {
             load_scales(from, scales);
-            load_scales(from + 1u, scales_next);
             publish(from, scales);
+            load_scales(from + 1u, scales);
             __syncthreads();
         }
-        lay(from, raw, scales);
-        if constexpr (!kFloat) {
-            scales = scales_next;
-            publish(from + 1u, scales);
-        }
+        lay(from, raw);
+        if constexpr (!kFloat) publish(from + 1u, scales);
         for (uint32_t step = from; step < to; step++) {
             __syncthreads();
             // pages are looked up for sixteen steps from `from` on; scales are asked for two steps ahead
@@ -358,16 +369,13 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
             }
             if constexpr (!kFloat) {
                 if ((done + 2u) % 16u == 0) look_up(step + 2u);
-                load_scales(step + 2u, scales_next);
+                load_scales(step + 2u, scales);
             }
             compute(step, 0);
             compute(step, 1);
             if (step + 1u < to) {
-                lay(step + 1u, raw, scales);
-                if constexpr (!kFloat) {
-                    scales = scales_next;
-                    publish(step + 2u, scales);
-                }
+                lay(step + 1u, raw);
+                if constexpr (!kFloat) publish(step + 2u, scales);
             }
         }
     }
@@ -406,7 +414,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
 
 template <int kCode, int kDim, bool kBF16>
 hipError_t launch_many(hipStream_t s, const AttentionArgs& a, const Split& split) {
-    constexpr uint32_t kLds = 2 * Many<kCode, kDim>::kBuffer + Many<kCode, kDim>::kWaves * 16 + 16;
+    constexpr uint32_t kLds = 2 * Many<kCode, kDim>::kBuffer + 32;
     hipLaunchKernelGGL((attention_many_kernel<kCode, kDim, kBF16>), dim3(split.tiles * split.splits * a.cache.kv_heads), dim3(Many<kCode, kDim>::kThreads), kLds, s, a, split);
     return hipGetLastError();
 }
