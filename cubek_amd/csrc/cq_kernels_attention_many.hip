@@ -181,7 +181,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
             s.k[c] = from_word(a.cache.keys, key_scale_at, 2 * c), s.v[c] = from_word(a.cache.values, value_scale_at, 16 + 2 * c);
         }
     };
-    int32_t key_power = -126, value_power = -126;  // of the largest scales so far: entries are taken times 2^-power / 2
+    int32_t key_power = -126, value_power = -126;  // of the largest scales of what was laid so far: entries are taken times 2^-power / 2
     // A step's scales as numbers, and for the workgroup the exponents of its largest ones that any row sees, where they pass what was there before.
     float key_scale[S::kChunks], value_scale[S::kChunks];
     const auto publish = [&](uint32_t step, const Scales& s) {
@@ -213,6 +213,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
 
     f32x16 out[kOut] = {};
     float top = -INFINITY, sum = 0.0f;
+    int32_t score_power = -126, out_power = -126;  // of the keys that scores are made of, and of the values in `out`
 
     // A step's codes as numbers into LDS.  In a step that some row sees only a part of, values that no row sees become zeros, and others that are no
     // numbers are reported.
@@ -226,12 +227,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
             const int32_t now_keys = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of[0])) - 127, 126);
             const int32_t now_values = min(static_cast<int32_t>(__builtin_amdgcn_readfirstlane(of[1])) - 127, 126);
             key_power = max(key_power, now_keys);
-            if (now_values > value_power) {
-                const float shrink = ldexpf(1.0f, value_power - now_values);
-                value_power = now_values;
-#pragma unroll
-                for (uint32_t e = 0; e < kOut; e++) out[e] *= shrink;
-            }
+            value_power = max(value_power, now_values);
             down_keys = 0.5f * bits_f32(static_cast<uint32_t>(127 - key_power) << 23), down_values = 0.5f * bits_f32(static_cast<uint32_t>(127 - value_power) << 23);
         }
 #pragma unroll
@@ -279,30 +275,33 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         }
     };
 
-    // Scores, weights and results of 32 keys.
-    const auto compute = [&](uint32_t step, uint32_t k) {
-        const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys + 32u * k);
-        if (key0 > wave_high || key0 + 31 < wave_low) return;
-        const bool partial = key0 < all_low || key0 + 31 > all_high;
-        const char* const keys = lds + (step & 1u) * S::kBuffer + 32u * k * S::kPitch;
+    // Scores, weights and results of kSpan keys: of all 64 of a step where registers allow it, which halves the waits for LDS and for the largest score
+    // (heads of 128: 633 us instead of 665 of a prompt of 8191 tokens); two waves of a head of 64 share a SIMD with two others, which hides them.
+    constexpr uint32_t kHalves = kDim == 128 ? 2 : 1, kSpan = 32 * kHalves;
+    const auto compute = [&](uint32_t step, uint32_t half) {
+        const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys + 32u * half);
+        if (key0 > wave_high || key0 + static_cast<int32_t>(kSpan) - 1 < wave_low) return;
+        const bool partial = key0 < all_low || key0 + static_cast<int32_t>(kSpan) - 1 > all_high;
+        const char* const keys = lds + (step & 1u) * S::kBuffer + 32u * half * S::kPitch;
         const char* const values = keys + S::kSide;
-        f32x16 s = {};
+        f32x16 s[kHalves] = {};
 #pragma unroll
-        for (uint32_t t = 0; t < kSlices; t++) {
-            const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + n * S::kPitch + t * 32u + h * 16u);
-            s = mfma32<kBF16>(operand, q[t], s);
-        }
-        u32x4 w[2];
-        // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
-        const float by = kFloat ? times : times * 2.0f * bits_f32(static_cast<uint32_t>(127 + key_power) << 23);
-        float t[16];
+        for (uint32_t t = 0; t < kSlices; t++)
 #pragma unroll
-        for (uint32_t v = 0; v < 16; v++) t[v] = s[v];
+            for (uint32_t k = 0; k < kHalves; k++) {
+                const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + (k * 32u + n) * S::kPitch + t * 32u + h * 16u);
+                s[k] = mfma32<kBF16>(operand, q[t], s[k]);
+            }
+        const float by = kFloat ? times : times * 2.0f * bits_f32(static_cast<uint32_t>(127 + score_power) << 23);
+        float t[kSpan / 2];
+#pragma unroll
+        for (uint32_t v = 0; v < kSpan / 2; v++) t[v] = s[v / 16u][v % 16u];
         const float times_now = shape_scores(t, by, cap, a.slopes, slope, position, key0 + static_cast<int32_t>(4u * h), [](uint32_t v) { return v / 4u * 8u + v % 4u; },
-                                             key0 + 31 <= first_position, partial, row_low, row_high);
+                                             key0 + static_cast<int32_t>(kSpan) - 1 <= first_position, partial, row_low, row_high);
+        // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
         float most = -INFINITY;
 #pragma unroll
-        for (uint32_t v = 0; v < 16; v++) most = fmaxf(most, t[v]);
+        for (uint32_t v = 0; v < kSpan / 2; v++) most = fmaxf(most, t[v]);
         most *= times_now;
         const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
         most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
@@ -315,33 +314,29 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
             for (uint32_t e = 0; e < kOut; e++) out[e] *= shrink;
         }
         const float less = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
-        float p[16];
+        u32x4 w[2 * kHalves];
 #pragma unroll
-        for (uint32_t v = 0; v < 16; v++) {
-            p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less));
-            sum += p[v];
+        for (uint32_t v = 0; v < kSpan / 2; v += 2) {
+            const float one = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less)), two = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v + 1], times_now, less));
+            sum += one, sum += two;
+            w[v / 8][v % 8 / 2] = pair_of<kBF16>(one, two);
         }
-#pragma unroll
-        for (uint32_t v = 0; v < 16; v += 2) w[v / 8][v % 8 / 2] = pair_of<kBF16>(p[v], p[v + 1]);
         // lane (n, h): entry n of 32, keys 4 h ... 4 h + 3 and 8 more
-        const auto values_of = [&](uint32_t e, uint32_t half) {
+        const auto values_of = [&](uint32_t e, uint32_t quarter) {
             u32x4 v;
 #pragma unroll
             for (uint32_t eight = 0; eight < 2; eight++) {
                 const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    CQ_LDS_AT(i16x4, values + (half * 16u + eight * 8u + 4u * h + lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + lane % 4u * 8u));
+                    CQ_LDS_AT(i16x4, values + (quarter * 16u + eight * 8u + 4u * h + lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + lane % 4u * 8u));
                 const u32x2 two = __builtin_bit_cast(u32x2, four);
                 v[2 * eight] = two[0], v[2 * eight + 1] = two[1];
             }
             return v;
         };
 #pragma unroll
-        for (uint32_t e = 0; e < kOut; e++)
+        for (uint32_t quarter = 0; quarter < 2 * kHalves; quarter++)
 #pragma unroll
-            for (uint32_t half = 0; half < 2; half++) {
-                const u32x4 v = values_of(e, half);
-                out[e] = mfma32<kBF16>(v, w[half], out[e]);
-            }
+            for (uint32_t e = 0; e < kOut; e++) out[e] = mfma32<kBF16>(values_of(e, quarter), w[quarter], out[e]);
     };
 
     if (threadIdx.x < 5) powers[threadIdx.x] = 0u;  // and *found
@@ -359,24 +354,40 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         }
         lay(from, raw);
         if constexpr (!kFloat) publish(from + 1u, scales);
+        if (from + 1u < to) load(from + 1u, raw);
+        if constexpr (!kFloat) load_scales(from + 2u, scales);
+        // The next step goes to LDS before this one is computed in one half of the waves and behind it in the other, so that the two waves of a SIMD do not
+        // want its matrix unit at the same time.
+        const bool early = S::kWaves == 8 && wave >= 4;
         for (uint32_t step = from; step < to; step++) {
             __syncthreads();
-            // pages are looked up for sixteen steps from `from` on; scales are asked for two steps ahead
-            const uint32_t done = step - from;
-            if (step + 1u < to) {
-                if ((done + 1u) % 16u == 0 && kFloat) look_up(step + 1u);
-                load(step + 1u, raw);
-            }
             if constexpr (!kFloat) {
-                if ((done + 2u) % 16u == 0) look_up(step + 2u);
-                load_scales(step + 2u, scales);
+                score_power = key_power;
+                if (value_power > out_power) {
+                    const float shrink = ldexpf(1.0f, out_power - value_power);
+                    out_power = value_power;
+#pragma unroll
+                    for (uint32_t e = 0; e < kOut; e++) out[e] *= shrink;
+                }
             }
-            compute(step, 0);
-            compute(step, 1);
-            if (step + 1u < to) {
-                lay(step + 1u, raw);
-                if constexpr (!kFloat) publish(step + 2u, scales);
-            }
+            // pages are looked up for sixteen steps from `from` on; codes are asked for a step before they are laid, scales two
+            const uint32_t done = step - from;
+            const auto next = [&]() __attribute__((always_inline)) {
+                if (step + 1u < to) {
+                    lay(step + 1u, raw);
+                    if constexpr (!kFloat) publish(step + 2u, scales);
+                }
+                if (kFloat && (done + 2u) % 16u == 0) look_up(step + 2u);
+                if (step + 2u < to) load(step + 2u, raw);
+                if constexpr (!kFloat) {
+                    if ((done + 3u) % 16u == 0) look_up(step + 3u);
+                    load_scales(step + 3u, scales);
+                }
+            };
+            if (early) next();
+#pragma unroll
+            for (uint32_t half = 0; half < 2; half += kHalves) compute(step, half);
+            if (!early) next();
         }
     }
 
@@ -388,7 +399,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         return;
     }
 
-    const float up = kFloat ? 1.0f : 2.0f * ldexpf(1.0f, value_power);
+    const float up = kFloat ? 1.0f : 2.0f * ldexpf(1.0f, out_power);
     const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum), f32_bits(sum), false, false);
     const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
     const float by = all == 0.0f ? 0.0f : 1.0f / all;
