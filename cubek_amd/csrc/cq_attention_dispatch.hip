@@ -48,7 +48,7 @@ Split split_of(const AttentionArgs& a, uint64_t room) {
     f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? 2 : 0;
     const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : 256;
     const uint64_t step = f.row_tiles && a.cache.code != kCacheInt4 && a.cache.code != kCacheE2M1 ? 32 : 64;
-    f.wanted = f.row_tiles ? 1536 : 256;
+    f.wanted = f.row_tiles ? 1024 : 256;
     f.fewest = f.row_tiles ? 512 / step : 16;
     f.tiles = static_cast<uint32_t>(rows / of_tile + a.seqs);
     const uint64_t busy = a.seqs * ((mean + of_tile - 1) / of_tile) * a.cache.kv_heads;

@@ -1,6 +1,6 @@
 // Attention of few rows (token, head of a group) over long caches: decode steps, drafts of some tokens.  An object per kind of code (CQ_TU_CODE).
 //
-// A workgroup takes a tile of 16 or 32 rows that share a head of the cache, and a split of the keys they see; its four waves take steps
+// A workgroup takes a tile of 16 or 32 rows that share a head of the cache, and a split of the keys they see; its four or eight waves take steps
 // of 32 keys (64 of 4 bits) in turn, each with a running maximum, sum and result of its own, which meet in LDS at the end; the results of several
 // splits meet in attention_join_kernel.  Everything else stays in registers:
 //   S^T = K Q^T by 16 x 16 x 32 matrix instructions: lane (i, g) has 16 bytes of key i, and gets the scores of row i with the keys 4 g ... 4 g + 3 of a
@@ -80,8 +80,12 @@ constexpr int waves_of() {
     return kRegisters <= 128 ? 4 : kRegisters <= 168 ? 3 : kRegisters <= 256 ? 2 : 1;
 }
 
+// of a workgroup, at most
+template <int kCode, int kDim, int kTiles>
+constexpr uint32_t kMostWaves = waves_of<kCode, kDim, kTiles>() == 1 ? 4 : 8;
+
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
-__global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attention_few_kernel(AttentionArgs a, Split split) {
+__global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<kCode, kDim, kTiles>())) void attention_few_kernel(AttentionArgs a, Split split) {
     using S = Shape<kCode, kDim, kPer>;
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kRowsLog2 = kTiles == 1 ? 4 : 5, kRows = 16 * kTiles;
@@ -90,6 +94,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15u, g = lane >> 4;
     // parts of a tile are far apart in the grid, so that those which have nothing come last
     const uint32_t tile = blockIdx.x % split.tiles, rest = blockIdx.x / split.tiles, kv_head = rest % a.cache.kv_heads, part = rest / a.cache.kv_heads, dim = a.cache.dim;
+    const uint32_t waves = split.waves;  // 4 or 8
     char* const mine = lds + wave * S::kWaveBytes;
     float* const scales_at = reinterpret_cast<float*>(mine + S::kValueBytes);
 
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
     constexpr uint32_t kAhead = 64 / S::kKeyTiles;
     uint32_t pages = 0;
     const auto look_up = [&](uint32_t step) {
-        const uint32_t t = tile_of(step + lane / S::kKeyTiles * 4u, lane % S::kKeyTiles);
+        const uint32_t t = tile_of(step + lane / S::kKeyTiles * waves, lane % S::kKeyTiles);
         pages = page_of(a, at.s, magic_div(t, split.page_magic, split.page_shift));
     };
 
@@ -280,8 +285,8 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         load_values(from + wave, 0, raw);
         load_keys(from + wave, 0, raw);
     }
-    for (uint32_t step = from + wave; step < to; step += 4, nth++) {
-        if ((nth + 1u) % kAhead == 0) look_up(step + 4u);
+    for (uint32_t step = from + wave; step < to; step += waves, nth++) {
+        if ((nth + 1u) % kAhead == 0) look_up(step + waves);
         const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys);
         const bool partial = key0 < all_low || key0 + static_cast<int32_t>(S::kKeys) - 1 > all_high;
 
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         }
         fence();
         // the next step's, into the registers that have gone to LDS; its keys behind this step's scores
-        load_values(step + 4u, nth + 1u, raw);
+        load_values(step + waves, nth + 1u, raw);
 
         // scores
         f32x4 s[kTiles][S::kKeyTiles];
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
             }
         }
 
-        load_keys(step + 4u, nth + 1u, raw);
+        load_keys(step + waves, nth + 1u, raw);
 
         // weights
         float p[kTiles][S::kKeyTiles * 4];
@@ -496,11 +501,11 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
         rows_one_by_one<kDim>(kRowsLog2, tile, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
-    // The four waves' results, each by its share of the whole over its sum.  A tile of 16 entries of the result is finished by the wave e % 4, which the others
+    // The waves' results, each by its share of the whole over its sum.  A tile of 16 entries of the result is finished by the wave e % waves, which the others
     // hand theirs.
     float* const tops = reinterpret_cast<float*>(lds);  // [wave][row]
-    float* const sums = tops + 4 * kRows;
-    f32x4* const handed = reinterpret_cast<f32x4*>(sums + 4 * kRows);  // [tile of rows][tile of entries][wave that hands][lane]
+    float* const sums = tops + waves * kRows;
+    f32x4* const handed = reinterpret_cast<f32x4*>(sums + waves * kRows);  // [tile of rows][tile of entries][wave that hands][lane]
 #pragma unroll
     for (uint32_t r = 0; r < kTiles; r++) {
         sum[r] = sum_of_groups(sum[r]);
@@ -512,16 +517,14 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 #pragma unroll
     for (uint32_t r = 0; r < kTiles; r++) {
         most[r] = -INFINITY, all[r] = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < 4; w++) most[r] = fmaxf(most[r], tops[w * kRows + r * 16u + i]);
+        for (uint32_t w = 0; w < waves; w++) most[r] = fmaxf(most[r], tops[w * kRows + r * 16u + i]);
         const float zero = most[r] == -INFINITY ? 0.0f : most[r];
-#pragma unroll
-        for (uint32_t w = 0; w < 4; w++) all[r] += sums[w * kRows + r * 16u + i] * __builtin_amdgcn_exp2f(tops[w * kRows + r * 16u + i] - zero);
+        for (uint32_t w = 0; w < waves; w++) all[r] += sums[w * kRows + r * 16u + i] * __builtin_amdgcn_exp2f(tops[w * kRows + r * 16u + i] - zero);
         const float share = sum[r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top[r] - zero) / all[r];
 #pragma unroll
         for (uint32_t e = 0; e < kOut; e++) {
             out[r][e] = sum[r] == 0.0f ? f32x4{} : out[r][e] * share * up;
-            if (e % 4u != wave) handed[((r * kOut + e) * 3u + (wave - e % 4u - 1u) % 4u) * 64u + lane] = out[r][e];
+            if ((e & (waves - 1u)) != wave) handed[((r * kOut + e) * (waves - 1u) + (wave - e - 1u & (waves - 1u))) * 64u + lane] = out[r][e];
         }
     }
     __syncthreads();
@@ -535,10 +538,9 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 #pragma unroll
         for (uint32_t e = 0; e < kOut; e++) {
             const uint32_t d = e * 16u + 4u * g;
-            if (e % 4u != wave || d >= dim) continue;
+            if ((e & (waves - 1u)) != wave || d >= dim) continue;
             f32x4 v = out[r][e];
-#pragma unroll
-            for (uint32_t w = 0; w < 3; w++) v += handed[((r * kOut + e) * 3u + w) * 64u + lane];
+            for (uint32_t w = 0; w < waves - 1u; w++) v += handed[((r * kOut + e) * (waves - 1u) + w) * 64u + lane];
             if (parts > 1) {
                 *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = v;
             } else {
@@ -552,9 +554,17 @@ __global__ __launch_bounds__(256, (waves_of<kCode, kDim, kTiles>())) void attent
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
 hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const Split& split) {
     using S = Shape<kCode, kDim, kPer>;
-    const uint32_t waves = 4 * S::kWaveBytes, join = 8 * 16 * kTiles * 4 + kTiles * (kDim / 16) * 3 * 1024;
-    hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(split.tiles * a.cache.kv_heads * split.splits), dim3(256), waves > join ? waves : join,
-                       s, a, split);
+    const auto lds_of = [](uint32_t waves) {
+        const uint32_t steps = waves * S::kWaveBytes, join = 2 * waves * 16 * kTiles * 4 + kTiles * (kDim / 16) * (waves - 1) * 1024;
+        return steps > join ? steps : join;
+    };
+    // Where there are not even as many workgroups as compute units, eight waves each, which ask for twice as much at a time (24 workgroups with up to
+    // 701 keys: 16.2 us of four waves, 14.2 of eight); their results have to fit in LDS.
+    Split by = split;
+    const uint32_t workgroups = split.tiles * a.cache.kv_heads * split.splits;
+    constexpr uint32_t kMost = kMostWaves<kCode, kDim, kTiles>;
+    by.waves = workgroups <= 256 && lds_of(kMost) <= 160 * 1024 - 512 ? kMost : 4;
+    hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(workgroups), dim3(64 * by.waves), lds_of(by.waves), s, a, by);
     return hipGetLastError();
 }
 
