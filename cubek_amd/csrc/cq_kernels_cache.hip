@@ -53,13 +53,14 @@ __device__ __forceinline__ float narrowed(double v) {
 }
 
 constexpr uint32_t kEach = 8;             // entries of a lane
-constexpr uint32_t kWorkEntries = 4096;   // of a workgroup
+constexpr uint32_t kTasks = 2;            // of a thread
+constexpr uint32_t kWorkEntries = 256 * kTasks * kEach;  // of a workgroup
 
-// Eight entries from a 16-byte boundary.
+// Eight entries, and eight to a 16-byte boundary.
 template <class F>
-__device__ __forceinline__ void load_each(const char* p, uint64_t i, float* v) {
+__device__ __forceinline__ void unpack_each(const u32x4* w, float* v) {
 #pragma unroll
-    for (uint32_t c = 0; c < kEach / F::kPerChunk; c++) F::unpack(reinterpret_cast<const u32x4*>(p + i * F::kBytes)[c], v + c * F::kPerChunk);
+    for (uint32_t c = 0; c < kEach / F::kPerChunk; c++) F::unpack(w[c], v + c * F::kPerChunk);
 }
 template <class F>
 __device__ __forceinline__ void store_each(char* p, uint64_t i, const float* v) {
@@ -73,7 +74,7 @@ template <class F, int kEnc, int kBits, bool kWide>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     extern __shared__ char lds[];
     double2* const turn = reinterpret_cast<double2*>(lds);
-    char* const rows = lds + a.pairs * sizeof(double2);
+    char* const rows = lds + a.pairs * sizeof(double2);  // not kWide
     const CacheArgs& c = a.cache;
     const uint32_t token = blockIdx.x, all = a.heads + 2u * c.kv_heads, row0 = blockIdx.y * a.rows, count = min(a.rows, all - row0), dim = c.dim;
     const int64_t slot = a.slots[token];
@@ -89,18 +90,28 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         *at = row < c.kv_heads ? token * a.k_token + row * a.k_head : token * a.v_token + (row - c.kv_heads) * a.v_head;
         return row < c.kv_heads ? a.k : a.v;
     };
-    constexpr uint32_t kStep = kWide ? kEach : 1u;
+    constexpr uint32_t kStep = kWide ? kEach : 1u, kChunks = kEach / F::kPerChunk;
     const uint32_t of_row = dim / kStep, tasks = count * of_row;
-    for (uint32_t t = threadIdx.x; t < tasks; t += 256) {
-        const uint32_t row = t / of_row, d = t % of_row * kStep;
-        uint64_t at;
-        const char* const from = source(row0 + row, &at);
-        if constexpr (kWide) {
+    // an entry's partner, and whether it turns at all
+    const auto partner_of = [&](uint32_t d) { return a.interleaved ? d ^ 1u : (d < a.pairs ? d + a.pairs : d - a.pairs); };
+    u32x4 own[kTasks][kChunks], partner[kTasks][kChunks];
+    if constexpr (kWide) {
 #pragma unroll
-            for (uint32_t i = 0; i < kEach / F::kPerChunk; i++)
-                reinterpret_cast<u32x4*>(rows + (row * dim + d) * F::kBytes)[i] = reinterpret_cast<const u32x4*>(from + (at + d) * F::kBytes)[i];
-        } else {
-            F::store(rows, row * dim + d, F::load(from, at + d));
+        for (uint32_t i = 0; i < kTasks; i++) {
+            const uint32_t t = min(threadIdx.x + 256u * i, tasks - 1u), row = t / of_row, d = t % of_row * kEach;
+            uint64_t at;
+            const char* const from = source(row0 + row, &at);
+#pragma unroll
+            for (uint32_t e = 0; e < kChunks; e++) {
+                own[i][e] = reinterpret_cast<const u32x4*>(from + (at + d) * F::kBytes)[e];
+                partner[i][e] = reinterpret_cast<const u32x4*>(from + (at + (a.interleaved || d >= 2u * a.pairs ? d : partner_of(d))) * F::kBytes)[e];
+            }
+        }
+    } else {
+        for (uint32_t t = threadIdx.x; t < tasks; t += 256) {
+            uint64_t at;
+            const char* const from = source(row0 + t / dim, &at);
+            F::store(rows, t, F::load(from, at + t % dim));
         }
     }
     if (row0 < a.heads + c.kv_heads)
@@ -109,6 +120,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
             cos_sin(static_cast<double>(a.positions[token]) * static_cast<double>(a.frequencies[p]), &cosine, &sine);
             turn[p] = double2{cosine * a.magnitude, sine * a.magnitude};
         }
+    // all of the rows are read before any of them is written: q_out may be q
+    if constexpr (kWide) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
 
     // entry d of a row, turned
@@ -120,9 +133,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const auto entry = [&](uint32_t row, uint32_t d, bool turns) {
         const float own = F::load(rows, row * dim + d);
         if (!turns || d >= 2u * a.pairs) return own;
-        const bool first = a.interleaved ? d % 2u == 0 : d < a.pairs;
-        const uint32_t other = a.interleaved ? d ^ 1u : (first ? d + a.pairs : d - a.pairs);
-        return turned(d, own, F::load(rows, row * dim + other), first);
+        return turned(d, own, F::load(rows, row * dim + partner_of(d)), a.interleaved ? d % 2u == 0 : d < a.pairs);
     };
 
     const uint32_t page = kept ? static_cast<uint32_t>(slot) / c.page_size : 0u, place = kept ? static_cast<uint32_t>(slot) % c.page_size : 0u;
@@ -131,7 +142,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const uint32_t group_log2 = kBits && kWide ? 31u - static_cast<uint32_t>(__builtin_clz(c.block / kEach)) : 0u;
     const uint32_t block = kBits && !kWide ? c.block : kStep, of_row2 = dim / block, tasks2 = count * of_row2;
     // whole waves, so that butterflies have all their lanes; past the last the last again
-    for (uint32_t t0 = threadIdx.x; t0 < (tasks2 + 63u) / 64u * 64u; t0 += 256) {
+    const auto task = [&](uint32_t t0, const u32x4* own, const u32x4* partner) {
         const uint32_t t = min(t0, tasks2 - 1u), row = t / of_row2, d0 = t % of_row2 * block, from = row0 + row;
         const bool is_query = from < a.heads, is_key = !is_query && from < a.heads + c.kv_heads;
         const uint32_t head = is_query ? from : (from - a.heads) % c.kv_heads;
@@ -140,7 +151,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         char* const to = side.base + page * side.page + head * side.head + place * side.slot;
         if constexpr (kWide) {
             float v[kEach];
-            load_each<F>(rows, row * dim + d0, v);
+            unpack_each<F>(own, v);
             if ((is_query || is_key) && d0 < 2u * a.pairs) {
                 if (a.interleaved) {
 #pragma unroll
@@ -152,13 +163,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
                 } else {
                     const bool first = d0 < a.pairs;
                     float p[kEach];
-                    load_each<F>(rows, row * dim + (first ? d0 + a.pairs : d0 - a.pairs), p);
+                    unpack_each<F>(partner, p);
 #pragma unroll
                     for (uint32_t e = 0; e < kEach; e++) v[e] = turned(d0 + e, v[e], p[e], first);
                 }
             }
             if constexpr (kBits == 0) {
-                if (t0 >= tasks2) continue;
+                if (t0 >= tasks2) return;
                 if (is_query)
                     store_each<F>(a.q_out, token * a.out_token + from * a.out_head + d0, v);
                 else if (kept)
@@ -168,7 +179,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 #pragma unroll
                 for (uint32_t e = 0; e < kEach; e++) most = fmaxf(most, fabsf(v[e]));
                 most = group_max_rt(most, group_log2);
-                if (t0 >= tasks2) continue;
+                if (t0 >= tasks2) return;
                 if (is_query) {
                     store_each<F>(a.q_out, token * a.out_token + from * a.out_head + d0, v);
                 } else if (kept) {
@@ -188,7 +199,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
                 }
             }
         } else {
-            if (t0 >= tasks2) continue;
+            if (t0 >= tasks2) return;
             if (is_query) {
                 for (uint32_t d = d0; d < d0 + block; d++) F::store(a.q_out, token * a.out_token + from * a.out_head + d, entry(row, d, true));
             } else if (kept) {
@@ -213,6 +224,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
                 }
             }
         }
+    };
+    if constexpr (kWide) {
+#pragma unroll
+        for (uint32_t i = 0; i < kTasks; i++)
+            if (threadIdx.x / 64u * 64u + 256u * i < tasks2) task(threadIdx.x + 256u * i, own[i], partner[i]);
+    } else {
+        for (uint32_t t = threadIdx.x; t < (tasks2 + 63u) / 64u * 64u; t += 256) task(t, nullptr, nullptr);
     }
 }
 
@@ -237,11 +255,11 @@ hipError_t launch_typed(hipStream_t s, AppendArgs a) {
     const uint32_t all = a.heads + 2u * a.cache.kv_heads;
     a.rows = kWorkEntries / a.cache.dim < all ? kWorkEntries / a.cache.dim : all;
     const dim3 grid(a.tokens, (all + a.rows - 1u) / a.rows);
-    const uint32_t lds = a.pairs * sizeof(double2) + a.rows * a.cache.dim * F::kBytes;
+    const uint32_t turns = a.pairs * sizeof(double2);
     if (takes_wide<F>(a, kBits))
-        hipLaunchKernelGGL((append_kernel<F, kEnc, kBits, true>), grid, dim3(256), lds, s, a);
+        hipLaunchKernelGGL((append_kernel<F, kEnc, kBits, true>), grid, dim3(256), turns, s, a);
     else
-        hipLaunchKernelGGL((append_kernel<F, kEnc, kBits, false>), grid, dim3(256), lds, s, a);
+        hipLaunchKernelGGL((append_kernel<F, kEnc, kBits, false>), grid, dim3(256), turns + a.rows * a.cache.dim * F::kBytes, s, a);
     return hipGetLastError();
 }
 
