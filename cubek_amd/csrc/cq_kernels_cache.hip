@@ -1,8 +1,9 @@
 // New tokens into a cache of pages.  An object per float type (CQ_TU_FLOAT).
 //
-// append_kernel: a workgroup takes some heads of one token, queries, keys and values alike.  Their rows come into LDS; meanwhile the first lanes
-// work out cosine and sine of the token's angles, each once for all heads; then a lane takes eight entries, turns them with their partners out of
-// LDS and stores them, or quantizes them as the flat quantize kernels do, the maximum of a block by a butterfly over the lanes that hold it.
+// append_kernel: a workgroup takes some heads of one token, queries, keys and values alike: a lane asks for eight entries and their partners; meanwhile
+// the first lanes work out cosine and sine of the token's angles, once for these heads; then each lane turns its entries and stores them, or quantizes them
+// as the flat quantize kernels do, the maximum of a block by a butterfly over the lanes that hold it.  (Rows whose strides do not allow that go through
+// LDS, an entry or a block a lane.)
 //
 // Angles and turning are in 64 bits: position * frequency is then exact to 2^-53 of itself (262144 positions: 2^-35), the turned entry is the
 // exact one but for the one rounding to F, and so codes do not depend on how cosines are computed.  It costs nothing that shows: 12 instructions of
@@ -53,8 +54,7 @@ __device__ __forceinline__ float narrowed(double v) {
 }
 
 constexpr uint32_t kEach = 8;             // entries of a lane
-constexpr uint32_t kTasks = 2;            // of a thread
-constexpr uint32_t kWorkEntries = 256 * kTasks * kEach;  // of a workgroup
+constexpr uint32_t kWorkEntries = 256 * kEach;  // of a workgroup: with two lots a thread, 33 us where it is 30
 
 // Eight entries, and eight to a 16-byte boundary.
 template <class F>
@@ -94,18 +94,15 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const uint32_t of_row = dim / kStep, tasks = count * of_row;
     // an entry's partner, and whether it turns at all
     const auto partner_of = [&](uint32_t d) { return a.interleaved ? d ^ 1u : (d < a.pairs ? d + a.pairs : d - a.pairs); };
-    u32x4 own[kTasks][kChunks], partner[kTasks][kChunks];
+    u32x4 own[kChunks], partner[kChunks];
     if constexpr (kWide) {
+        const uint32_t t = min(threadIdx.x, tasks - 1u), d = t % of_row * kEach;
+        uint64_t at;
+        const char* const from = source(row0 + t / of_row, &at);
 #pragma unroll
-        for (uint32_t i = 0; i < kTasks; i++) {
-            const uint32_t t = min(threadIdx.x + 256u * i, tasks - 1u), row = t / of_row, d = t % of_row * kEach;
-            uint64_t at;
-            const char* const from = source(row0 + row, &at);
-#pragma unroll
-            for (uint32_t e = 0; e < kChunks; e++) {
-                own[i][e] = reinterpret_cast<const u32x4*>(from + (at + d) * F::kBytes)[e];
-                partner[i][e] = reinterpret_cast<const u32x4*>(from + (at + (a.interleaved || d >= 2u * a.pairs ? d : partner_of(d))) * F::kBytes)[e];
-            }
+        for (uint32_t e = 0; e < kChunks; e++) {
+            own[e] = reinterpret_cast<const u32x4*>(from + (at + d) * F::kBytes)[e];
+            partner[e] = reinterpret_cast<const u32x4*>(from + (at + (a.interleaved || d >= 2u * a.pairs ? d : partner_of(d))) * F::kBytes)[e];
         }
     } else {
         for (uint32_t t = threadIdx.x; t < tasks; t += 256) {
@@ -114,26 +111,27 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
             F::store(rows, t, F::load(from, at + t % dim));
         }
     }
+    // A lane's eight entries begin with pair kPairs * n: pair k of them stands at n + k * stride, so that neighbouring lanes read neighbours.
+    const uint32_t pairs_log2 = kWide ? (a.interleaved ? 2u : 3u) : 0u, stride = a.pairs >> pairs_log2;
     if (row0 < a.heads + c.kv_heads)
         for (uint32_t p = threadIdx.x; p < a.pairs; p += 256) {
             double cosine, sine;
             cos_sin(static_cast<double>(a.positions[token]) * static_cast<double>(a.frequencies[p]), &cosine, &sine);
-            turn[p] = double2{cosine * a.magnitude, sine * a.magnitude};
+            turn[(p & ((1u << pairs_log2) - 1u)) * stride + (p >> pairs_log2)] = double2{cosine * a.magnitude, sine * a.magnitude};
         }
     // all of the rows are read before any of them is written: q_out may be q
     if constexpr (kWide) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
 
-    // entry d of a row, turned
-    const auto turned = [&](uint32_t d, float own, float partner, bool first) {
-        const double2 z = turn[a.interleaved ? d / 2u : (first ? d : d - a.pairs)];
+    const auto turned = [&](double2 z, float own, float partner, bool first) {
         const double x = own, p = partner;
         return narrowed<F>(__builtin_fma(first ? -p : p, z.y, x * z.x));
     };
     const auto entry = [&](uint32_t row, uint32_t d, bool turns) {
         const float own = F::load(rows, row * dim + d);
         if (!turns || d >= 2u * a.pairs) return own;
-        return turned(d, own, F::load(rows, row * dim + partner_of(d)), a.interleaved ? d % 2u == 0 : d < a.pairs);
+        const bool first = a.interleaved ? d % 2u == 0 : d < a.pairs;
+        return turned(turn[a.interleaved ? d / 2u : (first ? d : d - a.pairs)], own, F::load(rows, row * dim + partner_of(d)), first);
     };
 
     const uint32_t page = kept ? static_cast<uint32_t>(slot) / c.page_size : 0u, place = kept ? static_cast<uint32_t>(slot) % c.page_size : 0u;
@@ -142,7 +140,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const uint32_t group_log2 = kBits && kWide ? 31u - static_cast<uint32_t>(__builtin_clz(c.block / kEach)) : 0u;
     const uint32_t block = kBits && !kWide ? c.block : kStep, of_row2 = dim / block, tasks2 = count * of_row2;
     // whole waves, so that butterflies have all their lanes; past the last the last again
-    const auto task = [&](uint32_t t0, const u32x4* own, const u32x4* partner) {
+    const auto task = [&](uint32_t t0) {
         const uint32_t t = min(t0, tasks2 - 1u), row = t / of_row2, d0 = t % of_row2 * block, from = row0 + row;
         const bool is_query = from < a.heads, is_key = !is_query && from < a.heads + c.kv_heads;
         const uint32_t head = is_query ? from : (from - a.heads) % c.kv_heads;
@@ -157,15 +155,15 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 #pragma unroll
                     for (uint32_t e = 0; e < kEach; e += 2) {
                         const float x = v[e], y = v[e + 1];
-                        v[e] = turned(d0 + e, x, y, true);
-                        v[e + 1] = turned(d0 + e + 1, y, x, false);
+                        v[e] = turned(turn[d0 / kEach + e / 2u * stride], x, y, true);
+                        v[e + 1] = turned(turn[d0 / kEach + e / 2u * stride], y, x, false);
                     }
                 } else {
                     const bool first = d0 < a.pairs;
                     float p[kEach];
                     unpack_each<F>(partner, p);
 #pragma unroll
-                    for (uint32_t e = 0; e < kEach; e++) v[e] = turned(d0 + e, v[e], p[e], first);
+                    for (uint32_t e = 0; e < kEach; e++) v[e] = turned(turn[(first ? d0 : d0 - a.pairs) / kEach + e * stride], v[e], p[e], first);
                 }
             }
             if constexpr (kBits == 0) {
@@ -226,11 +224,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         }
     };
     if constexpr (kWide) {
-#pragma unroll
-        for (uint32_t i = 0; i < kTasks; i++)
-            if (threadIdx.x / 64u * 64u + 256u * i < tasks2) task(threadIdx.x + 256u * i, own[i], partner[i]);
+        if (threadIdx.x / 64u * 64u < tasks2) task(threadIdx.x);
     } else {
-        for (uint32_t t = threadIdx.x; t < (tasks2 + 63u) / 64u * 64u; t += 256) task(t, nullptr, nullptr);
+        for (uint32_t t = threadIdx.x; t < (tasks2 + 63u) / 64u * 64u; t += 256) task(t);
     }
 }
 
