@@ -36,14 +36,17 @@ __device__ __forceinline__ u32x4 in_order(u32x4 v) {
                  __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
 }
 
-template <int kCode, int kDim, bool kBF16>
-__global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)) void attention_many_kernel(AttentionArgs a, Split split) {
+// kExact: entries enter as their codes, scales in f32 behind the first product and on the weights; else as numbers of f16.
+template <int kCode, int kDim, bool kBF16, bool kExact>
+__global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExact ? 4 : 1)) void attention_many_kernel(AttentionArgs a, Split split) {
     using S = Many<kCode, kDim>;
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kSlices = kDim / 16, kOut = kDim / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][keys, values]: exponents, the largest of every other step so far
     uint32_t* const found = powers + 4;                                          // whether values that are no numbers need rows one by one
+    float* const scales_at = reinterpret_cast<float*>(powers + 8);               // kExact: [step % 2][keys, values][block][64]
+    constexpr uint32_t kScales = kDim / 32 * S::kKeys;                           // of a side of a step
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31u, h = lane >> 5;
     // neighbours in the grid are heads of the cache: with eight of them each die keeps one in its L2.  The tiles with most keys come first.
     const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads, part = rest % split.splits;
@@ -131,7 +134,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
     constexpr uint32_t kPass = S::kThreads / S::kLanes;  // keys of the workgroup's chunks at once, 8 or a multiple of 16
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u, byte = threadIdx.x % S::kLanes * S::kChunk, entry = byte * 8u / S::kBits;
-    const uint32_t block = min(entry, dim - 1u) >> split.block_log2;
+    const uint32_t block = min(entry, dim - 1u) >> split.block_log2, block_mask = (1u << split.block_log2) - 1u;
     const auto key_of = [&](uint32_t c) { return c * kPass + threadIdx.x / S::kLanes; };
     // a thread's offsets from the tile of 16 keys that holds its key; what is left is the same for the wave
     const uint32_t in_tile = threadIdx.x / S::kLanes % 16u, at_byte = min(byte, row_bytes - S::kChunk);
@@ -233,6 +236,13 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
 #pragma unroll
         for (uint32_t c = 0; c < S::kChunks; c++) {
             char* const row = to_keys + key_of(c) * S::kPitch + entry * 2u;
+            if constexpr (kExact) {
+                if ((entry & block_mask) == 0) {
+                    float* const to = scales_at + (step & 1u) * 2u * kScales + (entry >> split.block_log2) * S::kKeys + key_of(c);
+                    to[0] = key_scale[c], to[kScales] = value_scale[c] * 2.0f * down_values;
+                }
+                if (partial && !(fabsf(value_scale[c]) < INFINITY)) *found = 1u;
+            }
             if (row_bytes < S::kRow) {  // a shorter head: nothing past its end
 #pragma unroll
                 for (uint32_t e = 0; e < S::kChunk / 4; e++) raw.k[c][e] = byte < row_bytes ? raw.k[c][e] : 0u, raw.v[c][e] = byte < row_bytes ? raw.v[c][e] : 0u;
@@ -260,10 +270,12 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
 #pragma unroll
                     for (uint32_t e = 0; e < S::kChunk / 4; e += kEach) {
                         u32x4 v = in_order<kCode>(numbers<kCode>(w[e], kEach == 2 ? w[e + kEach - 1] : 0u));
+                        if constexpr (!kExact) {
 #pragma unroll
-                        for (uint32_t p = 0; p < 4; p++) {
-                            const uint32_t word = v[p];
-                            v[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, word) * by);
+                            for (uint32_t p = 0; p < 4; p++) {
+                                const uint32_t word = v[p];
+                                v[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, word) * by);
+                            }
                         }
                         if (of_values) look(v);
                         *reinterpret_cast<u32x4*>(to + e / kEach * 16u) = v;
@@ -277,25 +289,47 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
 
     // Scores, weights and results of kSpan keys: of all 64 of a step where registers allow it, which halves the waits for LDS and for the largest score
     // (heads of 128: 633 us instead of 665 of a prompt of 8191 tokens); two waves of a head of 64 share a SIMD with two others, which hides them.
-    constexpr uint32_t kHalves = kDim == 128 ? 2 : 1, kSpan = 32 * kHalves;
+    constexpr uint32_t kHalves = kDim == 128 && !kExact ? 2 : 1, kSpan = 32 * kHalves;
     const auto compute = [&](uint32_t step, uint32_t half) {
         const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys + 32u * half);
         if (key0 > wave_high || key0 + static_cast<int32_t>(kSpan) - 1 < wave_low) return;
         const bool partial = key0 < all_low || key0 + static_cast<int32_t>(kSpan) - 1 > all_high;
         const char* const keys = lds + (step & 1u) * S::kBuffer + 32u * half * S::kPitch;
         const char* const values = keys + S::kSide;
+        // the scales of lane (n, h)'s keys, of one block of entries: four behind one another of every eight
+        const auto scales_of = [&](uint32_t side, uint32_t block, uint32_t four) {
+            return *reinterpret_cast<const f32x4*>(scales_at + ((step & 1u) * 2u + side) * kScales + block * S::kKeys + 32u * half + four * 8u + 4u * h);
+        };
+        float t[kSpan / 2];
         f32x16 s[kHalves] = {};
+        if constexpr (kExact) {
 #pragma unroll
-        for (uint32_t t = 0; t < kSlices; t++)
+            for (uint32_t v = 0; v < 16; v++) t[v] = 0.0f;
+        }
+#pragma unroll
+        for (uint32_t slice = 0; slice < kSlices; slice++) {
 #pragma unroll
             for (uint32_t k = 0; k < kHalves; k++) {
-                const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + (k * 32u + n) * S::kPitch + t * 32u + h * 16u);
-                s[k] = mfma32<kBF16>(operand, q[t], s[k]);
+                const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + (k * 32u + n) * S::kPitch + slice * 32u + h * 16u);
+                s[k] = mfma32<kBF16>(operand, q[slice], s[k]);
             }
-        const float by = kFloat ? times : times * 2.0f * bits_f32(static_cast<uint32_t>(127 + score_power) << 23);
-        float t[kSpan / 2];
+            if constexpr (kExact) {
+                if (slice + 1 == kSlices || ((slice + 1) * 16u & block_mask) == 0) {  // the block's last
 #pragma unroll
-        for (uint32_t v = 0; v < kSpan / 2; v++) t[v] = s[v / 16u][v % 16u];
+                    for (uint32_t four = 0; four < 4; four++) {
+                        const f32x4 scale = scales_of(0, slice * 16u >> split.block_log2, four);
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; e++) t[four * 4 + e] = __builtin_fmaf(s[0][four * 4 + e], scale[e], t[four * 4 + e]);
+                    }
+                    s[0] = f32x16{};
+                }
+            }
+        }
+        const float by = kFloat || kExact ? times : times * 2.0f * bits_f32(static_cast<uint32_t>(127 + score_power) << 23);
+        if constexpr (!kExact) {
+#pragma unroll
+            for (uint32_t v = 0; v < kSpan / 2; v++) t[v] = s[v / 16u][v % 16u];
+        }
         const float times_now = shape_scores(t, by, cap, a.slopes, slope, position, key0 + static_cast<int32_t>(4u * h), [](uint32_t v) { return v / 4u * 8u + v % 4u; },
                                              key0 + static_cast<int32_t>(kSpan) - 1 <= first_position, partial, row_low, row_high);
         // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
@@ -317,9 +351,9 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         u32x4 w[2 * kHalves];
 #pragma unroll
         for (uint32_t v = 0; v < kSpan / 2; v += 2) {
-            const float one = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less)), two = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v + 1], times_now, less));
-            sum += one, sum += two;
-            w[v / 8][v % 8 / 2] = pair_of<kBF16>(one, two);
+            t[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less)), t[v + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v + 1], times_now, less));
+            sum += t[v], sum += t[v + 1];
+            if constexpr (!kExact) w[v / 8][v % 8 / 2] = pair_of<kBF16>(t[v], t[v + 1]);
         }
         // lane (n, h): entry n of 32, keys 4 h ... 4 h + 3 and 8 more
         const auto values_of = [&](uint32_t e, uint32_t quarter) {
@@ -333,10 +367,26 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
             }
             return v;
         };
+        if constexpr (kExact) {
 #pragma unroll
-        for (uint32_t quarter = 0; quarter < 2 * kHalves; quarter++)
+            for (uint32_t e = 0; e < kOut; e++) {
+                if ((e * 32u & block_mask) == 0) {  // a block's first: its weights
 #pragma unroll
-            for (uint32_t e = 0; e < kOut; e++) out[e] = mfma32<kBF16>(values_of(e, quarter), w[quarter], out[e]);
+                    for (uint32_t four = 0; four < 4; four++) {
+                        const f32x4 scale = scales_of(1, e * 32u >> split.block_log2, four);
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; i += 2) w[four / 2][four % 2 * 2 + i / 2] = pair_of<false>(t[four * 4 + i] * scale[i], t[four * 4 + i + 1] * scale[i + 1]);
+                    }
+                }
+#pragma unroll
+                for (uint32_t quarter = 0; quarter < 2; quarter++) out[e] = mfma32<kBF16>(values_of(e, quarter), w[quarter], out[e]);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t quarter = 0; quarter < 2 * kHalves; quarter++)
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++) out[e] = mfma32<kBF16>(values_of(e, quarter), w[quarter], out[e]);
+        }
     };
 
     if (threadIdx.x < 5) powers[threadIdx.x] = 0u;  // and *found
@@ -399,7 +449,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         return;
     }
 
-    const float up = kFloat ? 1.0f : 2.0f * ldexpf(1.0f, out_power);
+    const float up = kFloat ? 1.0f : (kExact ? 1.0f : 2.0f) * ldexpf(1.0f, out_power);
     const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum), f32_bits(sum), false, false);
     const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
     const float by = all == 0.0f ? 0.0f : 1.0f / all;
@@ -423,18 +473,25 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 ? 4 : 1)
         }
 }
 
-template <int kCode, int kDim, bool kBF16>
+template <int kCode, int kDim, bool kBF16, bool kExact>
 hipError_t launch_many(hipStream_t s, const AttentionArgs& a, const Split& split) {
-    constexpr uint32_t kLds = 2 * Many<kCode, kDim>::kBuffer + 32;
-    hipLaunchKernelGGL((attention_many_kernel<kCode, kDim, kBF16>), dim3(split.tiles * split.splits * a.cache.kv_heads), dim3(Many<kCode, kDim>::kThreads), kLds, s, a, split);
+    using S = Many<kCode, kDim>;
+    constexpr uint32_t kLds = 2 * S::kBuffer + 32 + (kExact ? 4 * (kDim / 32) * S::kKeys * 4 : 0);
+    hipLaunchKernelGGL((attention_many_kernel<kCode, kDim, kBF16, kExact>), dim3(split.tiles * split.splits * a.cache.kv_heads), dim3(S::kThreads), kLds, s, a, split);
     return hipGetLastError();
 }
 
+// A number of f16 is rounded to 11 bits: less than a result of bf16 shows (8191 tokens of fp8: off by 0.0021 of its norm, 0.0017 of it the result's own rounding),
+// more than one of f16 does (0.0012 and 0.0002), so those are made of the codes.
 template <int kCode, int kDim>
 hipError_t launch_type(hipStream_t s, const AttentionArgs& a, const Split& split) {
-    if constexpr (kCode == kCacheFloat)
-        if (a.dtype == CQ_BF16) return launch_many<kCode, kDim, true>(s, a, split);
-    return launch_many<kCode, kDim, false>(s, a, split);
+    if constexpr (kCode == kCacheFloat) {
+        if (a.dtype == CQ_BF16) return launch_many<kCode, kDim, true, false>(s, a, split);
+        return launch_many<kCode, kDim, false, false>(s, a, split);
+    } else {
+        if (a.dtype == CQ_BF16) return launch_many<kCode, kDim, false, false>(s, a, split);
+        return launch_many<kCode, kDim, false, true>(s, a, split);
+    }
 }
 
 }  // namespace
