@@ -34,8 +34,6 @@ bool tiles_take(const AttentionArgs& a) {
     return rows(c.keys) && rows(c.values) && on(a.q, 16) && a.q_token % 8 == 0 && a.q_head % 8 == 0 && on(a.y, 8) && a.y_token % 4 == 0 && a.y_head % 4 == 0;
 }
 
-constexpr uint32_t kMostSplits = 64;  // a lane each in attention_join_kernel
-
 uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4; }
 
 // Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (128 of heads past

@@ -65,6 +65,8 @@ uint64_t attention_workspace_bytes(const AttentionArgs& a);
 hipError_t launch_attention(hipStream_t s, const AttentionArgs& a);
 hipError_t launch_attention_general(hipStream_t s, const AttentionArgs& a);
 
+constexpr uint32_t kMostSplits = 64;  // a lane each in attention_join_kernel
+
 // How rows and the keys they see are shared out between workgroups.
 struct Split {
     uint32_t tiles, row_tiles;  // workgroups for rows, of one head and one split; tiles of 16 rows of one (attention_few_kernel)
