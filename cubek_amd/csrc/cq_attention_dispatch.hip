@@ -38,8 +38,12 @@ uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tok
 
 // Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (128 of heads past
 // 128) by attention_many_kernel.  The keys are split so that `wanted` parts come to the GPU, none of fewer than `fewest` steps: how many of the `splits` a
-// sequence has goes by its length, which the device knows.  Tiles of many rows that fill the GPU by themselves are not split (496 tiles: 80 us, and 129 with
-// up to two parts of each and their join).
+// sequence has goes by its length, which the device knows.  Measured, in us:
+//   16 sequences of 4000 to 8191 keys, 12 rows each: tiles of 16 rows 59, of 32 rows 70; 24 rows: of 16 rows 95, of 32 rows 75; 64 rows: of 32 rows 122, of 256 rows 167;
+//     128 rows: of 32 rows 201, of 256 rows 175
+//   parts wanted of few rows: 768, 1024, 1536, 2048: 64 sequences of 257 to 8191 keys 137, 138, 141, 145; of one length 115, 115, 113, 114
+//   of many rows: 128, 256, 512: 509 tokens behind 7681 keys 173, 112, 128; 1000 tokens behind 7190 307, 190, 202.  Tiles that fill the GPU by themselves are
+//     not split: 2040 tokens behind 6150 keys 332, and 343
 Split split_of(const AttentionArgs& a, uint64_t room) {
     Split f{};
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, mean = (rows + a.seqs - 1) / a.seqs;
