@@ -105,3 +105,24 @@ def test_slopes_on_either_side_of_the_position(oracle, length, tokens):
     case.check("prefix", slopes=slopes, prefix=[length, 5])
     case.check("causal", slopes=slopes)
     case.check("capped", slopes=slopes, prefix=[length, length], cap=4.0, window=25)
+
+
+@pytest.mark.parametrize("tokens", [2, 12, 200])
+@pytest.mark.parametrize("name", CODES)
+@pytest.mark.parametrize("elem", [BF16, F16], ids=lambda e: e.name)
+def test_a_last_key_that_is_not_a_number(oracle, tokens, name, elem):
+    """The last token sees it, the ones in front of it do not, in a sequence of several parts and in one of one."""
+    case = Attention(oracle, 6, [(tokens, 3000), (tokens, tokens + 40)], 4, 2, 128, 16, elem, scheme(name, 32))
+    want, bound = case.want()
+    for s, (_, length) in enumerate(case.sequences):
+        for pool in (case.k, case.v):
+            at = (int(case.table[s, (length - 1) // 16]), slice(None), (length - 1) % 16)
+            if pool.scales is None:
+                pool.stored[at] = float("nan")
+            else:
+                pool.scales[at] = float("nan")
+    got = case.call().double().cpu().numpy()
+    for s in range(2):
+        a, b = case.offsets[s], case.offsets[s + 1] - 1
+        check_rounded(got[a:b], want[a:b], bound[a:b], elem, s)
+        assert np.isnan(got[b]).all()
