@@ -210,41 +210,60 @@ __device__ __forceinline__ bool find_rows(const AttentionArgs& a, uint32_t tile,
     return rows_of(a, sequence_of(a, s), first_tile(a, s, a.offsets[s], rows_log2), tile, rows_log2, out);
 }
 
-// The same, and the steps of `keys_log2` keys of a part, such that all tiles of all sequences come to about split.wanted parts, none of fewer than split.fewest
-// steps: every workgroup works it out from the lengths.  Up to 64 sequences take one round of loads.
-__device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, const Split& split, uint32_t tile, uint32_t rows_log2, uint32_t keys_log2, RowTile* out,
-                                                    uint32_t* steps) {
+// Sums of the lanes up to each one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    const auto add = [&](uint32_t from) { v += from; };
+    add(__builtin_amdgcn_update_dpp(0u, v, 0x111, 0xf, 0xf, true));  // one to the right within rows of 16 lanes, two, four, eight
+    add(__builtin_amdgcn_update_dpp(0u, v, 0x112, 0xf, 0xf, true));
+    add(__builtin_amdgcn_update_dpp(0u, v, 0x114, 0xf, 0xf, true));
+    add(__builtin_amdgcn_update_dpp(0u, v, 0x118, 0xf, 0xf, true));
+    add(__builtin_amdgcn_update_dpp(0u, v, 0x142, 0xa, 0xf, false));  // the last of rows 0 and 2 to rows 1 and 3, that of row 1 to rows 2 and 3
+    add(__builtin_amdgcn_update_dpp(0u, v, 0x143, 0xc, 0xf, false));
+    return v;
+}
+
+// The rows and the part of the keys that workgroup `index` of a head has, and how many steps of 2^keys_log2 keys a part is to have, such that all tiles of
+// all sequences come to about split.wanted parts, none of fewer than split.fewest steps: every workgroup works it out from the offsets and lengths.  Parts lie far
+// apart in the grid, so that those which some tiles do not have come last.  Up to 64 sequences take one round of loads, and their tiles lie side by side.
+// More sequences' tiles have gaps between them (find_rows), which would leave every other die idle where a sequence has exactly a tile's rows (64 sequences of 16 rows:
+// 228 us with gaps, 127 without): every other one first, then the ones between.
+template <bool kReversed>
+__device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, const Split& split, uint32_t index, uint32_t rows_log2, uint32_t keys_log2, RowTile* out,
+                                                    uint32_t* steps, uint32_t* part) {
     const uint32_t lane = threadIdx.x & 63u;
     const bool few = a.seqs <= 64;
     Sequence s{};
-    int32_t offset = 0;
-    uint32_t total = 0;  // 2^31 keys at most of each sequence: 2^26 steps, of 64 sequences a lane each; saturates below
+    uint32_t total = 0, own = 0;  // steps of the lane's sequences, at most 2^20 of each and of all; tiles of its last one
     *steps = ~0u;
     if (few || split.splits > 1) {
         for (uint32_t i = lane; i < a.seqs; i += 64) {
             s = sequence_of(a, i);
-            offset = a.offsets[i];
-            const uint32_t rows = (s.last - s.first) * a.group, tiles = (rows + (1u << rows_log2) - 1u) >> rows_log2;
+            own = static_cast<uint32_t>((static_cast<uint64_t>(s.last - s.first) * a.group + ((1u << rows_log2) - 1u)) >> rows_log2);
             const uint32_t seen = a.window ? min(static_cast<uint32_t>(s.length), max(a.window, 1u) + (s.last - s.first)) : static_cast<uint32_t>(s.length);
-            total = min(total + min(tiles * ((seen >> keys_log2) + 1u), 1u << 20), 1u << 20);
+            total = static_cast<uint32_t>(min(total + static_cast<uint64_t>(own) * ((seen >> keys_log2) + 1u), static_cast<uint64_t>(1u << 20)));
         }
         if (split.splits > 1) {
-            uint32_t all = total;
-#pragma unroll
-            for (int d = 32; d; d >>= 1) all += static_cast<uint32_t>(__shfl_xor(static_cast<int>(all), d, 64));
-            const uint64_t parts = static_cast<uint64_t>(all) * a.cache.kv_heads;
-            *steps = __builtin_amdgcn_readfirstlane(max(split.fewest, static_cast<uint32_t>((parts + split.wanted - 1u) / split.wanted)));
+            const uint64_t parts = static_cast<uint64_t>(__builtin_amdgcn_readlane(wave_scan(total), 63)) * a.cache.kv_heads;
+            *steps = max(split.fewest, static_cast<uint32_t>((parts + split.wanted - 1u) / split.wanted));
         }
     }
-    if (!few) return find_rows(a, tile, rows_log2, out);
-    const uint64_t first = first_tile(a, lane, offset, rows_log2);
-    const uint64_t below = __builtin_amdgcn_ballot_w64(lane < a.seqs && first <= tile);
-    const uint32_t at = below ? 63u - static_cast<uint32_t>(__builtin_clzll(below)) : 0u;
+    const uint32_t upto = few ? wave_scan(own) : 0u, tiles = few ? static_cast<uint32_t>(__builtin_amdgcn_readlane(upto, 63)) : split.tiles;
+    if (tiles == 0) return false;
+    *part = index / tiles;
+    uint32_t tile = index % tiles;
+    if (*part >= split.splits) return false;
+    if (kReversed) tile = tiles - 1u - tile;
+    if (!few) {
+        const uint32_t half = (tiles + 1u) / 2u;
+        return find_rows(a, tile < half ? 2u * tile : 2u * (tile - half) + 1u, rows_log2, out);
+    }
+    const uint32_t at = static_cast<uint32_t>(__builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > tile)));
     const auto from_lane = [&](auto v) { return static_cast<decltype(v)>(__builtin_amdgcn_readlane(static_cast<int>(v), at)); };
-    Sequence q;
-    q.index = at;
-    q.first = from_lane(s.first), q.last = from_lane(s.last), q.length = from_lane(s.length), q.position = from_lane(s.position), q.prefix = from_lane(s.prefix);
-    return rows_of(a, q, first_tile(a, at, from_lane(offset), rows_log2), tile, rows_log2, out);
+    out->s.index = at;
+    out->s.first = from_lane(s.first), out->s.last = from_lane(s.last), out->s.length = from_lane(s.length), out->s.position = from_lane(s.position), out->s.prefix = from_lane(s.prefix);
+    out->row0 = (tile - (from_lane(upto) - from_lane(own))) << rows_log2;
+    out->rows = min((out->s.last - out->s.first) * a.group - out->row0, 1u << rows_log2);
+    return true;
 }
 
 // Parts of a tile's keys: [token][head][split] results over their own sums and {largest score, sum} (split.parts, split.stats).  A tile with one part writes y.
@@ -264,7 +283,7 @@ __device__ __forceinline__ void note_parts(const AttentionArgs& a, const Split& 
 // come here, with its LDS free for (kDim + 64) floats a wave.  The arguments, the kernel's first two, are read again, so that what is needed here alone
 // takes no registers from what comes before.
 template <uint32_t kDim>
-__device__ __forceinline__ void rows_one_by_one(uint32_t rows_log2, uint32_t tile, uint32_t part, uint32_t parts, uint32_t kv_head, int64_t first, int64_t last, float* lds) {
+__device__ __forceinline__ void rows_one_by_one(uint32_t seq, uint32_t row0, uint32_t rows, uint32_t part, uint32_t parts, uint32_t kv_head, int64_t first, int64_t last, float* lds) {
     struct Arguments {
         AttentionArgs a;
         Split split;
@@ -274,18 +293,17 @@ __device__ __forceinline__ void rows_one_by_one(uint32_t rows_log2, uint32_t til
     const Arguments& arguments = *reinterpret_cast<const Arguments*>(again);
     const AttentionArgs& a = arguments.a;
     const Split& split = arguments.split;
-    RowTile at;
-    if (!find_rows(a, tile, rows_log2, &at)) return;
+    const Sequence s = sequence_of(a, seq);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     float* const query = lds + wave * (kDim + 64u);
-    for (uint32_t row = wave; row < at.rows; row += blockDim.x / 64u) {
-        const uint32_t in_sequence = at.row0 + row, token = at.s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
-        const int32_t position = at.s.position + static_cast<int32_t>(in_sequence / a.group);
-        const Seen seen = seen_from(a, at.s, position);
+    for (uint32_t row = wave; row < rows; row += blockDim.x / 64u) {
+        const uint32_t in_sequence = row0 + row, token = s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
+        const int32_t position = s.position + static_cast<int32_t>(in_sequence / a.group);
+        const Seen seen = seen_from(a, s, position);
         for (uint32_t d = lane; d < a.cache.dim; d += 64) query[d] = load_dtype(a.dtype, a.q, token * a.q_token + head * a.q_head + d);
         __builtin_amdgcn_wave_barrier();
         float top, sum, v[kDim / 64];
-        attend_row<kDim / 64>(a, at.s, kv_head, position, a.slopes ? a.slopes[head] : 0.0f, query, query + kDim, max(first, static_cast<int64_t>(seen.low)), 64,
+        attend_row<kDim / 64>(a, s, kv_head, position, a.slopes ? a.slopes[head] : 0.0f, query, query + kDim, max(first, static_cast<int64_t>(seen.low)), 64,
                               min(last, static_cast<int64_t>(seen.high)), &top, &sum, v);
         const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
 #pragma unroll

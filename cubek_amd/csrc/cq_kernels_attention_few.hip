@@ -97,15 +97,15 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
     constexpr uint32_t kOut = kDim / 16;  // tiles of 16 entries of the result
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15u, g = lane >> 4;
-    // parts of a tile are far apart in the grid, so that those which have nothing come last
-    const uint32_t tile = blockIdx.x % split.tiles, rest = blockIdx.x / split.tiles, kv_head = rest % a.cache.kv_heads, part = rest / a.cache.kv_heads, dim = a.cache.dim;
+    // neighbours in the grid are heads of the cache, whose entries lie side by side
+    const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, dim = a.cache.dim;
     const uint32_t waves = split.waves;  // 4 or 8
     char* const mine = lds + wave * S::kWaveBytes;
     float* const scales_at = reinterpret_cast<float*>(mine + S::kValueBytes);
 
     RowTile at;
-    uint32_t steps_wanted;
-    if (!find_rows_and_steps(a, split, tile, kRowsLog2, S::kKeyTiles == 4 ? 6 : 5, &at, &steps_wanted)) return;
+    uint32_t steps_wanted, part;
+    if (!find_rows_and_steps<false>(a, split, blockIdx.x / a.cache.kv_heads, kRowsLog2, S::kKeyTiles == 4 ? 6 : 5, &at, &steps_wanted, &part)) return;
     // the keys that some row of the tile sees, and those that all of them do
     const int32_t first_position = at.s.position + static_cast<int32_t>(at.row0 / a.group), last_position = at.s.position + static_cast<int32_t>((at.row0 + at.rows - 1u) / a.group);
     const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, last_position);
@@ -513,7 +513,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
 
     if (__syncthreads_or(found)) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
-        rows_one_by_one<kDim>(kRowsLog2, tile, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
+        rows_one_by_one<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
     // The waves' results, each by its share of the whole over its sum.  A tile of 16 entries of the result is finished by the wave e % waves, which the others

@@ -54,12 +54,11 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     // Neighbours in the grid are heads of the cache: with eight of them each die keeps one in its L2.  The tiles with most keys come first, the parts that some
     // tiles do not have last (next to those that they have, they leave parts of the dies idle: 1000 tokens behind 7190 keys, whose
     // tiles have two of four parts, 190 us, and 322).
-    const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads, part = rest / split.tiles;
-    const uint32_t tile = split.tiles - 1u - rest % split.tiles, dim = a.cache.dim;
+    const uint32_t kv_head = blockIdx.x % a.cache.kv_heads, dim = a.cache.dim;
 
     RowTile at;
-    uint32_t steps_wanted;
-    if (!find_rows_and_steps(a, split, tile, S::kRowsLog2, 6, &at, &steps_wanted)) return;
+    uint32_t steps_wanted, part;
+    if (!find_rows_and_steps<true>(a, split, blockIdx.x / a.cache.kv_heads, S::kRowsLog2, 6, &at, &steps_wanted, &part)) return;
     const auto position_of = [&](uint32_t row) { return at.s.position + static_cast<int32_t>((at.row0 + row) / a.group); };
     const Seen top_row = seen_from(a, at.s, position_of(0)), bottom_row = seen_from(a, at.s, position_of(at.rows - 1u));
     const int32_t low = top_row.low, high = bottom_row.high, tile_low = bottom_row.low, tile_high = top_row.high;  // seen by some, and by all
@@ -450,7 +449,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     if (*found) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
         __syncthreads();
-        rows_one_by_one<kDim>(S::kRowsLog2, tile, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
+        rows_one_by_one<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;
     }
 
