@@ -37,12 +37,13 @@ bool tiles_take(const AttentionArgs& a) {
 uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tokens) * a.heads * (a.cache.dim + 2) * 4; }
 
 // Tiles of 16 or 32 rows (token, head of a group) by attention_few_kernel, whose sequences have up to 64 on the mean; else tiles of 256 (128 of heads past
-// 128) by attention_many_kernel.  The keys are split so that `wanted` parts come to the GPU, none of fewer than `fewest` steps: how many of the `splits` a
-// sequence has goes by its length, which the device knows.  Measured, in us:
+// 128) by attention_many_kernel.  The keys are split; how many of the `splits` a sequence has goes by its length, which the device knows.  Measured, in us:
 //   16 sequences of 4000 to 8191 keys, 12 rows each: tiles of 16 rows 59, of 32 rows 70; 24 rows: of 16 rows 95, of 32 rows 75; 64 rows: of 32 rows 122, of 256 rows 167;
 //     128 rows: of 32 rows 201, of 256 rows 175
-//   parts wanted of few rows: 768, 1024, 1536, 2048: 64 sequences of 257 to 8191 keys 137, 138, 141, 145; of one length 115, 115, 113, 114
-//   of many rows: 128, 256, 512: 509 tokens behind 7681 keys 173, 112, 128; 1000 tokens behind 7190 307, 190, 202.  Tiles that fill the GPU by themselves are
+//   parts of few rows, at most 768, 1024, 1536, 2048: 64 sequences of 257 to 8191 keys 120, 117, 119, 123; of 4096 keys 100, 100, 105, 110
+//     of 8, 16, 32 steps: one sequence of 3000 keys 14.7, 16.2, 22.5, of 8000 15.4, 16.7, 20.4, of 32000 23.2, 24.2, 23.0; eight of 8000 41, 39, 35;
+//     five tokens of eight within a window of 4096 52, 39, 36 (of four parts; 47 of five, which some compute units have two of)
+//   of many rows, 128, 256, 512: 509 tokens behind 7681 keys 173, 112, 128; 1000 tokens behind 7190 307, 190, 202.  Tiles that fill the GPU by themselves are
 //     not split: 2040 tokens behind 6150 keys 332, and 343
 Split split_of(const AttentionArgs& a, uint64_t room) {
     Split f{};
@@ -51,7 +52,8 @@ Split split_of(const AttentionArgs& a, uint64_t room) {
     const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : 256;
     const uint64_t step = f.row_tiles && a.cache.code != kCacheInt4 && a.cache.code != kCacheE2M1 ? 32 : 64;
     f.wanted = f.row_tiles ? 1024 : 256;
-    f.fewest = f.row_tiles ? 512 / step : 16;
+    f.fewest = f.row_tiles ? 8 : 16;
+    f.enough = f.row_tiles ? 32 : 16;
     f.tiles = static_cast<uint32_t>(rows / of_tile + a.seqs);
     const uint64_t busy = a.seqs * ((mean + of_tile - 1) / of_tile) * a.cache.kv_heads;
     uint64_t keys = static_cast<uint64_t>(a.width) * a.cache.page_size;

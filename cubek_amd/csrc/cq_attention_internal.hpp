@@ -72,7 +72,7 @@ struct Split {
     uint32_t tiles, row_tiles;  // workgroups for rows, of one head and one split; tiles of 16 rows of one (attention_few_kernel)
     uint32_t splits;            // of the keys, at most
     uint32_t waves;             // of a workgroup of attention_few_kernel
-    uint32_t wanted, fewest;    // parts of all tiles together that are aimed at; steps of the smallest part
+    uint32_t wanted, fewest, enough;  // parts of all tiles together, at most; steps of the smallest part, and of one that is as good as a larger one
     uint32_t page_magic, page_shift, block_log2;  // division by the tiles of 16 keys of a page; log2 of a scale's entries
     float *parts, *stats;  // splits > 1: [token][head][split][dim], each over its own sum; [token][head][split]{largest score, sum}
 };

@@ -222,8 +222,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
-// The rows and the part of the keys that workgroup `index` of a head has, and how many steps of 2^keys_log2 keys a part is to have, such that all tiles of
-// all sequences come to about split.wanted parts, none of fewer than split.fewest steps: every workgroup works it out from the offsets and lengths.  Parts lie far
+// The rows and the part of the keys that workgroup `index` of a head has, and how many steps of 2^keys_log2 keys a part is to have: as many as make a part for
+// most of 256 compute units, not below split.fewest; split.enough where that is fewer, for then some units would
+// have two parts and others one; more where all tiles of all sequences would come to more than about split.wanted parts.  Every workgroup works it out from the offsets and lengths.  Parts lie far
 // apart in the grid, so that those which some tiles do not have come last.  Up to 64 sequences take one round of loads, and their tiles lie side by side.
 // More sequences' tiles have gaps between them (find_rows), which would leave every other die idle where a sequence has exactly a tile's rows (64 sequences of 16 rows:
 // 228 us with gaps, 127 without): every other one first, then the ones between.
@@ -242,12 +243,15 @@ __device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, cons
             const uint32_t seen = a.window ? min(static_cast<uint32_t>(s.length), max(a.window, 1u) + (s.last - s.first)) : static_cast<uint32_t>(s.length);
             total = static_cast<uint32_t>(min(total + static_cast<uint64_t>(own) * ((seen >> keys_log2) + 1u), static_cast<uint64_t>(1u << 20)));
         }
-        if (split.splits > 1) {
-            const uint64_t parts = static_cast<uint64_t>(__builtin_amdgcn_readlane(wave_scan(total), 63)) * a.cache.kv_heads;
-            *steps = max(split.fewest, static_cast<uint32_t>((parts + split.wanted - 1u) / split.wanted));
-        }
     }
     const uint32_t upto = few ? wave_scan(own) : 0u, tiles = few ? static_cast<uint32_t>(__builtin_amdgcn_readlane(upto, 63)) : split.tiles;
+    if (split.splits > 1) {
+        const uint64_t all = static_cast<uint64_t>(__builtin_amdgcn_readlane(wave_scan(total), 63)) * a.cache.kv_heads;
+        const auto of = [&](uint32_t parts) { return static_cast<uint32_t>((all + parts - 1u) / parts); };
+        uint32_t each = of(250u);
+        if (each > split.enough + split.enough / 4u) each = split.enough;
+        *steps = max(max(each, split.fewest), of(split.wanted));
+    }
     if (tiles == 0) return false;
     *part = index / tiles;
     uint32_t tile = index % tiles;
@@ -265,6 +269,9 @@ __device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, cons
     out->rows = min((out->s.last - out->s.first) * a.group - out->row0, 1u << rows_log2);
     return true;
 }
+
+// Parts of `all` steps, of about `wanted` each: the nearest number, so that a few steps too many do not make another one.
+__device__ __forceinline__ uint32_t parts_of(uint32_t all, uint32_t wanted, uint32_t splits) { return min(max((all + wanted / 2u) / wanted, 1u), splits); }
 
 // Parts of a tile's keys: [token][head][split] results over their own sums and {largest score, sum} (split.parts, split.stats).  A tile with one part writes y.
 // What the parts it does not have would have left is written by its first part: sums of zero, or kWhole where there is nothing to join.

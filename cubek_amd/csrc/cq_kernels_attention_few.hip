@@ -111,13 +111,13 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
     const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, last_position);
     const int32_t low = first.low, high = last.high, all_low = last.low, all_high = first.high;
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
-    const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits);
+    const uint32_t parts = parts_of(steps_all, steps_wanted, split.splits);
     if (part >= parts) return;
     if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
     // Where there are more parts than the GPU holds at once, the later ones, which start last, are smaller, from 3/2 of the mean down to 1/2, so that all
-    // end together (64 sequences of 257 to 8191 keys: 139 us of equal parts, 135; 64 of 4096: 116 and 108); else all are equal (one of 131071: 46, and 52).
+    // end together (64 sequences of 257 to 8191 keys: 120 us of equal parts, 117; 200 of 257 to 4000: 187 and 181); else all are equal (one of 131071: 46, and 52).
     uint32_t from, to;
-    if (steps_wanted > split.fewest && split.splits < kMostSplits) {
+    if (steps_wanted > split.enough && split.splits < kMostSplits) {
         const float by = static_cast<float>(steps_all) / static_cast<float>(2u * parts * parts);
         const auto begin_of = [&](uint32_t p) { return static_cast<uint32_t>(by * static_cast<float>(p * (3u * parts - p))); };
         from = begin_of(part), to = part + 1u < parts ? begin_of(part + 1u) : steps_all;

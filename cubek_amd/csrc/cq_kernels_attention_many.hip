@@ -63,7 +63,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     const Seen top_row = seen_from(a, at.s, position_of(0)), bottom_row = seen_from(a, at.s, position_of(at.rows - 1u));
     const int32_t low = top_row.low, high = bottom_row.high, tile_low = bottom_row.low, tile_high = top_row.high;  // seen by some, and by all
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
-    const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits), each = (steps_all + parts - 1u) / parts;
+    const uint32_t parts = parts_of(steps_all, steps_wanted, split.splits), each = (steps_all + parts - 1u) / parts;
     if (part >= parts) return;
     if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
