@@ -270,9 +270,6 @@ __device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, cons
     return true;
 }
 
-// Parts of `all` steps, of about `wanted` each: the nearest number, so that a few steps too many do not make another one.
-__device__ __forceinline__ uint32_t parts_of(uint32_t all, uint32_t wanted, uint32_t splits) { return min(max((all + wanted / 2u) / wanted, 1u), splits); }
-
 // Parts of a tile's keys: [token][head][split] results over their own sums and {largest score, sum} (split.parts, split.stats).  A tile with one part writes y.
 // What the parts it does not have would have left is written by its first part: sums of zero, or kWhole where there is nothing to join.
 constexpr float kWhole = -1.0f;

@@ -111,7 +111,8 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
     const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, last_position);
     const int32_t low = first.low, high = last.high, all_low = last.low, all_high = first.high;
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
-    const uint32_t parts = parts_of(steps_all, steps_wanted, split.splits);
+    // the nearest number of parts, so that a few steps too many do not make another one (five tokens of eight sequences within a window of 4096: 36 us, and 46)
+    const uint32_t parts = min(max((steps_all + steps_wanted / 2u) / steps_wanted, 1u), split.splits);
     if (part >= parts) return;
     if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
     // Where there are more parts than the GPU holds at once, the later ones, which start last, are smaller, from 3/2 of the mean down to 1/2, so that all

@@ -23,8 +23,9 @@ namespace {
 template <int kCode, int kDim>
 struct Many {
     static constexpr uint32_t kBits = kCodeBits<kCode>, kKeys = 64;
-    static constexpr uint32_t kWaves = kDim > 128 ? 4 : 8, kThreads = 64 * kWaves;
-    static constexpr uint32_t kRows = kWaves * 32, kRowsLog2 = kRows == 256 ? 8 : 7;
+    // waves that share rows, each with a part of the result's entries: two have all the scores of 32 rows, and registers for half of 256 entries
+    static constexpr uint32_t kWaves = 8, kThreads = 64 * kWaves, kShare = kDim > 128 ? 2 : 1, kRowWaves = kWaves / kShare;
+    static constexpr uint32_t kRows = kRowWaves * 32, kRowsLog2 = kRows == 256 ? 8 : 7;
     static constexpr uint32_t kRow = kDim * kBits / 8;                                                  // bytes of a key as it is stored
     static constexpr uint32_t kChunk = kRow * kKeys / kThreads < 16 ? kRow * kKeys / kThreads : 16, kLanes = kRow / kChunk;  // of a thread; threads of a row
     static constexpr uint32_t kEntries = kChunk * 8 / kBits, kChunks = kKeys * kLanes / kThreads;             // entries of a chunk; chunks of a thread
@@ -44,7 +45,7 @@ template <int kCode, int kDim, bool kBF16, bool kExact>
 __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExact ? 4 : 1)) void attention_many_kernel(AttentionArgs a, Split split) {
     using S = Many<kCode, kDim>;
     constexpr bool kFloat = kCode == kCacheFloat;
-    constexpr uint32_t kSlices = kDim / 16, kOut = kDim / 32;
+    constexpr uint32_t kSlices = kDim / 16, kOut = kDim / 32 / S::kShare;  // tiles of 32 entries of the wave's part
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][keys, values]: exponents, the largest of every other step so far
     uint32_t* const found = powers + 4;                                          // whether values that are no numbers need rows one by one
@@ -63,14 +64,14 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     const Seen top_row = seen_from(a, at.s, position_of(0)), bottom_row = seen_from(a, at.s, position_of(at.rows - 1u));
     const int32_t low = top_row.low, high = bottom_row.high, tile_low = bottom_row.low, tile_high = top_row.high;  // seen by some, and by all
     const uint32_t step0 = static_cast<uint32_t>(low) / S::kKeys, steps_all = high < low ? 0u : static_cast<uint32_t>(high) / S::kKeys + 1u - step0;
-    const uint32_t parts = parts_of(steps_all, steps_wanted, split.splits), each = (steps_all + parts - 1u) / parts;
+    const uint32_t parts = min(max(steps_all / steps_wanted + (steps_all % steps_wanted != 0), 1u), split.splits), each = (steps_all + parts - 1u) / parts;
     if (part >= parts) return;
     if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
     const uint32_t from = min(part * each, steps_all), to = min(from + each, steps_all);
     const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
 
     // the wave's rows, and the keys that some of them see and that all of them do
-    const uint32_t wave_row = wave * 32u, wave_last = min(wave_row + 32u, at.rows) - 1u;
+    const uint32_t wave_row = wave % S::kRowWaves * 32u, first_out = wave / S::kRowWaves * kOut, wave_last = min(wave_row + 32u, at.rows) - 1u;
     const bool rows_here = wave_row < at.rows;
     const int32_t first_position = position_of(min(wave_row, at.rows - 1u));
     const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, position_of(rows_here ? wave_last : at.rows - 1u));
@@ -110,6 +111,9 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
         most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
         const uint32_t down = power_of_row(most, bf16);
+        // unpacked again, not kept: they would take twice the queries' registers
+#pragma unroll
+        for (uint32_t t = 0; t < kSlices; t++) asm volatile("" : "+v"(q[t]));
 #pragma unroll
         for (uint32_t t = 0; t < kSlices; t++) {
             unpack(q[t]);
@@ -317,6 +321,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
                 const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + (k * 32u + n) * S::kPitch + slice * 32u + h * 16u);
                 s[k] = mfma32<kBF16>(operand, q[slice], s[k]);
             }
+            if constexpr (kSlices > 8)
+                if (slice % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more operands at once than there are registers for
             if constexpr (kExact) {
                 if (slice + 1 == kSlices || ((slice + 1) * 16u & block_mask) == 0) {  // the block's last
 #pragma unroll
@@ -365,7 +371,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
 #pragma unroll
             for (uint32_t eight = 0; eight < 2; eight++) {
                 const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    CQ_LDS_AT(i16x4, values + (quarter * 16u + eight * 8u + 4u * h + lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + lane % 4u * 8u));
+                    CQ_LDS_AT(i16x4, values + first_out * 64u + (quarter * 16u + eight * 8u + 4u * h + lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + lane % 4u * 8u));
                 const u32x2 two = __builtin_bit_cast(u32x2, four);
                 v[2 * eight] = two[0], v[2 * eight + 1] = two[1];
             }
@@ -374,10 +380,10 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         if constexpr (kExact) {
 #pragma unroll
             for (uint32_t e = 0; e < kOut; e++) {
-                if ((e * 32u & block_mask) == 0) {  // a block's first: its weights
+                if (e == 0 || ((first_out + e) * 32u & block_mask) == 0) {  // a block's first, or the wave's: its weights
 #pragma unroll
                     for (uint32_t four = 0; four < 4; four++) {
-                        const f32x4 scale = scales_of(1, e * 32u >> split.block_log2, four);
+                        const f32x4 scale = scales_of(1, (first_out + e) * 32u >> split.block_log2, four);
 #pragma unroll
                         for (uint32_t i = 0; i < 4; i += 2) w[four / 2][four % 2 * 2 + i / 2] = pair_of<false>(t[four * 4 + i] * scale[i], t[four * 4 + i + 1] * scale[i + 1]);
                     }
@@ -412,7 +418,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         if constexpr (!kFloat) load_scales(from + 2u, scales);
         // The next step goes to LDS before this one is computed in one half of the waves and behind it in the other, so that the two waves of a SIMD do not
         // want its matrix unit at the same time.
-        const bool early = S::kWaves == 8 && wave >= 4;
+        const bool early = wave >= 4;
         for (uint32_t step = from; step < to; step++) {
             __syncthreads();
             if constexpr (!kFloat) {
@@ -459,12 +465,12 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     const float by = all == 0.0f ? 0.0f : 1.0f / all;
     if (own >= at.rows) return;
     const uint64_t token = token_of(), of = (token * a.heads + head_of()) * split.splits + part;
-    if (parts > 1 && h == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = all;
+    if (parts > 1 && h == 0 && first_out == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = all;
 #pragma unroll
     for (uint32_t e = 0; e < kOut; e++)
 #pragma unroll
         for (uint32_t v = 0; v < 16; v += 4) {
-            const uint32_t d = e * 32u + v * 2u + 4u * h;
+            const uint32_t d = (first_out + e) * 32u + v * 2u + 4u * h;
             if (d >= dim) continue;
             f32x4 four;
 #pragma unroll
