@@ -71,7 +71,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     const uint32_t last_tile = static_cast<uint32_t>(max(high, 0)) / 16u;
 
     // the wave's rows, and the keys that some of them see and that all of them do
-    const uint32_t wave_row = wave % S::kRowWaves * 32u, first_out = wave / S::kRowWaves * kOut, wave_last = min(wave_row + 32u, at.rows) - 1u;
+    const uint32_t wave_row = (S::kShare == 1 ? wave : wave % S::kRowWaves) * 32u, first_out = S::kShare == 1 ? 0u : wave / S::kRowWaves * kOut, wave_last = min(wave_row + 32u, at.rows) - 1u;
     const bool rows_here = wave_row < at.rows;
     const int32_t first_position = position_of(min(wave_row, at.rows - 1u));
     const Seen first = seen_from(a, at.s, first_position), last = seen_from(a, at.s, position_of(rows_here ? wave_last : at.rows - 1u));
@@ -111,9 +111,10 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(most), f32_bits(most), false, false);
         most = fmaxf(bits_f32(halves[0]), bits_f32(halves[1]));
         const uint32_t down = power_of_row(most, bf16);
-        // unpacked again, not kept: they would take twice the queries' registers
+        if constexpr (kSlices > 8) {  // unpacked again, not kept: they would take twice the queries' registers
 #pragma unroll
-        for (uint32_t t = 0; t < kSlices; t++) asm volatile("" : "+v"(q[t]));
+            for (uint32_t t = 0; t < kSlices; t++) asm volatile("" : "+v"(q[t]));
+        }
 #pragma unroll
         for (uint32_t t = 0; t < kSlices; t++) {
             unpack(q[t]);
