@@ -11,8 +11,8 @@
 // Where a scale covers 32 entries of a longer head, lanes swap parts so that one instruction has one block (`kPer` > 1).
 // Queries are scaled by a power of two per row, weights by one per step, so that f16 holds them whatever the range of bf16.
 //
-// Bound by the read of the cache where sequences are many and long (64 of 4096 keys, 8 heads of 128 of i8: 108 us, 5.1 TB/s; lengths from 257 to 8191: 131-139,
-// the last parts end apart); by vector instructions at 4 bits with a scale for 32 entries (one sequence of 131071 keys: 45 us of which 4.5 join 64 parts,
+// Bound by the read of the cache where sequences are many and long (64 of 4096 keys, 8 heads of 128 of i8: 100 us, 5.5 TB/s; lengths from 257 to 8191: 117,
+// 4.9 TB/s); by vector instructions at 4 bits with a scale for 32 entries (one sequence of 131071 keys: 45 us of which 4.5 join 64 parts,
 // 3.3 TB/s, vector units busy 54 %); where there is little to read, by a launch and four rounds of loads that need each other, lengths, pages, codes, and
 // then a wave's steps one after another (24 tiles of up to 701 keys: 14 us).
 #include <hip/hip_runtime.h>

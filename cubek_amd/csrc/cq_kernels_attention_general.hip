@@ -4,7 +4,7 @@
 // A workgroup takes one query.  Its four waves take 64 keys at a time in turn: a lane a key for the scores (its row against the query in LDS),
 // a lane eight entries of the result for the values; running maximum, sum and result are each wave's own and meet in LDS at the end.  Everything is
 // f32.  Bound by vector instructions, one value of the cache an element load, a conversion and an FMA: nothing is shared between queries (64 single tokens over
-// 257 to 8191 keys of 8 heads of i8, four queries a head: 10.4 ms, where the matrix cores take 0.14).
+// 257 to 8191 keys of 8 heads of i8, four queries a head: 10.4 ms, where the matrix cores take 0.12).
 #include <hip/hip_runtime.h>
 
 #include "cq_attention_rows.hpp"

@@ -23,7 +23,8 @@ namespace {
 template <int kCode, int kDim>
 struct Many {
     static constexpr uint32_t kBits = kCodeBits<kCode>, kKeys = 64;
-    // waves that share rows, each with a part of the result's entries: two have all the scores of 32 rows, and registers for half of 256 entries
+    // Waves that share rows: of heads past 128 two compute all scores of the same 32 rows and half of the result each, whose registers leave room for two waves a SIMD
+    // (4096 tokens of heads of 256: 513 us, and 616 with a wave's rows its own and one a SIMD).
     static constexpr uint32_t kWaves = 8, kThreads = 64 * kWaves, kShare = kDim > 128 ? 2 : 1, kRowWaves = kWaves / kShare;
     static constexpr uint32_t kRows = kRowWaves * 32, kRowsLog2 = kRows == 256 ? 8 : 7;
     static constexpr uint32_t kRow = kDim * kBits / 8;                                                  // bytes of a key as it is stored
@@ -140,7 +141,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     struct Scales {
         uint32_t k[S::kChunks], v[S::kChunks], odd;  // words; bits 2 c ... of keys and 16 + 2 c ... of values: half a word that their tile begins with
     };
-    constexpr uint32_t kPass = S::kThreads / S::kLanes;  // keys of the workgroup's chunks at once, 8 or a multiple of 16
+    constexpr uint32_t kPass = S::kThreads / S::kLanes;  // keys of the workgroup's chunks at once
+    static_assert(kPass % 16 == 0);
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u, byte = threadIdx.x % S::kLanes * S::kChunk, entry = byte * 8u / S::kBits;
     const uint32_t block = min(entry, dim - 1u) >> split.block_log2, block_mask = (1u << split.block_log2) - 1u;
@@ -154,7 +156,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     const auto place = [&](uint32_t step, uint32_t c, uint32_t* page, uint32_t* slot) {
         const uint32_t k = (c * kPass + wave * (64u / S::kLanes)) / 16u;
         *page = __builtin_amdgcn_readlane(pages, (step - from) % 16u * 4u + k);
-        *slot = place_of_tile(tile_of(step, k)) + c * kPass % 16u;
+        *slot = place_of_tile(tile_of(step, k));
     };
     const auto rows_at = [&](const CacheSide& side, uint32_t page, uint32_t slot) {
         return side.base + kv_head * side.head + static_cast<uint64_t>(page) * static_cast<uint32_t>(side.page) + slot * static_cast<uint32_t>(side.slot);
