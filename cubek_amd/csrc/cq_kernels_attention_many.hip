@@ -10,7 +10,7 @@
 // in f16, and puts their scales in f32 behind the first product and on the weights.
 //
 // A step of a head of 128 is 32 matrix instructions of a wave (1024 cycles) beside about 250 vector instructions, 150 of them the softmax's; with two waves on a
-// SIMD they overlap in part, and the card's power limits the rest: a prompt of 8191 tokens, 32 heads over 8 of fp8, 604-633 us, 870-910 TFLOP/s at 1.9 GHz,
+// SIMD they overlap in part, and the card's power limits the rest: a prompt of 8191 tokens, 32 heads over 8 of fp8, 604-640 us, 860-910 TFLOP/s at 1.9 GHz,
 // matrix units busy 39 %, vector units 47 %, LDS 49 %.
 #include <hip/hip_runtime.h>
 
