@@ -8,6 +8,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <dlfcn.h>
+
 #include <cstring>
 #include <initializer_list>
 #include <new>
@@ -397,6 +399,27 @@ bool real(PyObject* o, float* out) {
     return !(v == -1.0 && PyErr_Occurred());
 }
 
+// The calls of the third library, which is opened by the first one: linked, its code objects would cost the first launch of a process that only quantizes
+// 7 ms (32 instead of 25).  nullptr, with a Python error, where it is missing.
+struct AttentionCalls {
+    decltype(&cq_cache_append) append = nullptr;
+    decltype(&cq_attention) attention = nullptr;
+    decltype(&cq_cache_copy) copy = nullptr;
+    AttentionCalls() {
+        void* const library = dlopen("libcubek_attention_hip.so", RTLD_NOW | RTLD_LOCAL);  // beside this module, by its run path
+        if (!library) return;
+        append = reinterpret_cast<decltype(append)>(dlsym(library, "cq_cache_append"));
+        attention = reinterpret_cast<decltype(attention)>(dlsym(library, "cq_attention"));
+        copy = reinterpret_cast<decltype(copy)>(dlsym(library, "cq_cache_copy"));
+    }
+};
+const AttentionCalls* attention_calls() {
+    static const AttentionCalls calls;
+    if (calls.append && calls.attention && calls.copy) return &calls;
+    PyErr_SetString(PyExc_RuntimeError, "libcubek_attention_hip.so is missing or of another version; build it with `make -C cubek_amd/csrc` (needs hipcc)");
+    return nullptr;
+}
+
 // stream, cache, k, v, slots, q, q_out, positions, frequencies, magnitude, interleaved, elem
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream;
@@ -412,8 +435,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return nullptr;
     rotary.frequencies = frequencies.t;
     rotary.interleaved = static_cast<uint32_t>(interleaved);
+    const AttentionCalls* const calls = attention_calls();
+    if (!calls) return nullptr;
     return status_of([&] {
-        return cq_cache_append(static_cast<cq_stream_t>(stream), &cache.c, &k.t, &v.t, &slots.t, q.t, q_out.t, positions.t, frequencies.t ? &rotary : nullptr, elem);
+        return calls->append(static_cast<cq_stream_t>(stream), &cache.c, &k.t, &v.t, &slots.t, q.t, q_out.t, positions.t, frequencies.t ? &rotary : nullptr, elem);
     });
 }
 
@@ -437,8 +462,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     scores.window = static_cast<uint32_t>(window);
     scores.slopes = slopes.t;
     scores.prefix = prefix.t;
+    const AttentionCalls* const calls = attention_calls();
+    if (!calls) return nullptr;
     return status_of([&] {
-        return cq_attention(static_cast<cq_stream_t>(stream), &cache.c, &q.t, &y.t, &table.t, &offsets.t, &lengths.t, &scores, elem, workspace, bytes);
+        return calls->attention(static_cast<cq_stream_t>(stream), &cache.c, &q.t, &y.t, &table.t, &offsets.t, &lengths.t, &scores, elem, workspace, bytes);
     });
 }
 
@@ -457,7 +484,9 @@ PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (!held[static_cast<size_t>(i)].read(PySequence_Fast_GET_ITEM(fast.p, i))) return nullptr;
             tensors[static_cast<size_t>(i)] = held[static_cast<size_t>(i)].t;
         }
-        return status_of([&] { return cq_cache_copy(static_cast<cq_stream_t>(stream), tensors.data(), static_cast<uint32_t>(of), &pairs.t); });
+        const AttentionCalls* const calls = attention_calls();
+        if (!calls) return nullptr;
+        return status_of([&] { return calls->copy(static_cast<cq_stream_t>(stream), tensors.data(), static_cast<uint32_t>(of), &pairs.t); });
     } catch (const std::bad_alloc&) {
         return PyErr_NoMemory();
     }
