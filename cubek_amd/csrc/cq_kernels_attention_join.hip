@@ -26,7 +26,8 @@ struct Joined {
         float most = top;
 #pragma unroll
         for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
-        const float weight = top == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f(top - most);
+        // A part that has seen no key has a sum of zero; one whose scores are all not numbers has a sum that is none over a largest score of -infinity
+        const float weight = sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : top - most);
         float all = weight;
 #pragma unroll
         for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d, 64);
