@@ -152,6 +152,15 @@ __device__ __forceinline__ uint32_t exponent_of(float v) {
     return field == 255u ? 0u : field;
 }
 
+// Weights times the scales of values (few rows, and kExact of many), or entries (many rows), are held in f16 over the largest scale so far, 2^power.  Of scales
+// down to 2^-kSpread of it that leaves a weight 2^-16 of the largest one and an entry 2^-10 of its code's step.  A smaller one, unless it is zero, would lose
+// its bits to keys that a row may not even see: where there is one the tile's rows are taken one by one (rows_one_by_one).  A model's stay far within: from the
+// largest block of a cache to the smallest it is 2^10 or so.  A thread keeps the smallest of its scales, by twice their bits less one, so that zero is the
+// largest of all and its sign does not count: two instructions a scale, and one question at the end (asked in every step, prompt_longest took 650 us instead of 624).
+constexpr int32_t kSpread = 14;
+__device__ __forceinline__ uint32_t smaller_of(uint32_t least, float scale) { return min(least, 2u * f32_bits(scale) - 1u); }
+__device__ __forceinline__ bool lost_below(uint32_t least, int32_t power) { return least < max(static_cast<uint32_t>(max(127 + power - kSpread, 0)) << 24, 1u) - 1u; }
+
 // What a row's products become before their weights: capped, with the bias of their distance, keys that the row does not see at -infinity.  `of` are a lane's
 // products with the keys key0 + place(i); what is returned is left to be multiplied by, `times` where nothing of this is wanted.  `behind`: no key is past
 // the position, so that the distance is linear and costs two instructions a score instead of five.  The conditions are uniform over the wave and each has a loop
@@ -283,7 +292,8 @@ __device__ __forceinline__ void note_parts(const AttentionArgs& a, const Split& 
 }
 
 // The rows of a tile once more, one by one, over the keys from first to last: taken where an entry of a value that is infinite or not a number lies among
-// keys that not every row of the tile sees.  A weight of zero does not keep such an entry out of a product of tiles.  All threads of the workgroup
+// keys that not every row of the tile sees, for a weight of zero does not keep such an entry out of a product of tiles, and where scales are further apart than
+// f16 can hold (kSpread).  All threads of the workgroup
 // come here, with its LDS free for (kDim + 64) floats a wave.  The arguments, the kernel's first two, are read again, so that what is needed here alone
 // takes no registers from what comes before.
 template <uint32_t kDim>

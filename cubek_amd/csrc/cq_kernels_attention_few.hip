@@ -293,6 +293,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
     for (uint32_t r = 0; r < kTiles; r++) top[r] = -INFINITY, sum[r] = 0.0f;
     bool found = false;    // values that are no numbers, among keys that not every row sees
     int32_t power = -126;  // of the largest scale of the values so far: they are taken times 2^-power
+    uint32_t least = ~0u;  // of the smallest (smaller_of)
 
     Raw raw;
     uint32_t nth = 0;
@@ -346,7 +347,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
 #pragma unroll
             for (uint32_t k = 0; k < S::kKeyTiles; k++)
 #pragma unroll
-                for (uint32_t n = 0; n < S::kScaleLoads; n++) most = fmaxf(most, fabsf(scale[1][k][n]));
+                for (uint32_t n = 0; n < S::kScaleLoads; n++) most = fmaxf(most, fabsf(scale[1][k][n])), least = smaller_of(least, scale[1][k][n]);
             if (__builtin_amdgcn_ballot_w64(!(most < bits_f32(static_cast<uint32_t>(128 + power) << 23)))) {  // 2^(power + 1)
                 uint32_t field = 0;
 #pragma unroll
@@ -512,7 +513,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
         fence();
     }
 
-    if (__syncthreads_or(found)) {
+    if (__syncthreads_or(found || (!kFloat && lost_below(least, power)))) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
         rows_one_by_one<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
         return;

@@ -49,7 +49,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     constexpr uint32_t kSlices = kDim / 16, kOut = kDim / 32 / S::kShare;  // tiles of 32 entries of the wave's part
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][keys, values]: exponents, the largest of every other step so far
-    uint32_t* const found = powers + 4;                                          // whether values that are no numbers need rows one by one
+    uint32_t* const found = powers + 4;                                          // whether values that are no numbers, or scales far apart, need rows one by one
     float* const scales_at = reinterpret_cast<float*>(powers + 8);               // kExact: [step % 2][keys, values][block][64]
     constexpr uint32_t kScales = kDim / 32 * S::kKeys;                           // of a side of a step
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31u, h = lane >> 5;
@@ -196,6 +196,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         }
     };
     int32_t key_power = -126, value_power = -126;  // of the largest scales of what was laid so far: entries are taken times 2^-power / 2
+    uint32_t least_key = ~0u, least_value = ~0u;   // of the smallest (smaller_of)
     // A step's scales as numbers, and for the workgroup the exponents of its largest ones that any row sees, where they pass what was there before.
     float key_scale[S::kChunks], value_scale[S::kChunks];
     const auto publish = [&](uint32_t step, const Scales& s) {
@@ -247,6 +248,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
 #pragma unroll
         for (uint32_t c = 0; c < S::kChunks; c++) {
             char* const row = to_keys + key_of(c) * S::kPitch + entry * 2u;
+            if constexpr (!kFloat) least_value = smaller_of(least_value, value_scale[c]);
+            if constexpr (!kFloat && !kExact) least_key = smaller_of(least_key, key_scale[c]);
             if constexpr (kExact) {
                 if ((entry & block_mask) == 0) {
                     float* const to = scales_at + (step & 1u) * 2u * kScales + (entry >> split.block_log2) * S::kKeys + key_of(c);
@@ -454,6 +457,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         }
     }
 
+    if (!kFloat && (lost_below(least_value, value_power) || lost_below(least_key, key_power))) *found = 1u;
     __syncthreads();
     if (*found) {
         const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
