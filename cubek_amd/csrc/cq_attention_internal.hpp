@@ -129,7 +129,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, uint32_t
     const int64_t length = a.lengths[s];
     q.length = a.cache.pages ? static_cast<int32_t>(min(max(length, static_cast<int64_t>(0)), most)) : 0;
     q.position = q.length - static_cast<int32_t>(q.last - q.first);
-    q.prefix = a.prefix ? min(a.prefix[s], q.length) : 0;
+    q.prefix = a.prefix ? min(max(a.prefix[s], 0), q.length) : 0;  // (the lowest number less one would be the highest)
     return q;
 }
 

@@ -58,7 +58,8 @@ cq_status cq_cache_append(cq_stream_t stream, const cq_cache* cache, const cq_te
 /* What stands between queries and weights, in f32:
  *   t = scale * (q . k);  t = cap * tanh(t / cap) where cap > 0;  t -= slopes[head] * |position - key|
  * The query at position p sees the keys 0 <= j < length with j <= p or j < prefix, and, where window > 0, p - j < window.
- *   slopes : NULL or f32 [heads], contiguous;  prefix : NULL or i32 [sequences], contiguous
+ *   slopes : NULL or f32 [heads], contiguous
+ *   prefix : NULL or i32 [sequences], contiguous, each taken as the nearest number between 0 and the sequence's length
  * cap is 0 (none) or a positive number.  Every field not used is 0. */
 typedef struct cq_scores {
     float scale;
