@@ -179,9 +179,9 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
             times[r] = fabsf(a.scale);
         }
         // with a cap: 2 log2(e) t / cap, the exponent of its tanh; else log2(e) t
-        times[r] *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
+        times[r] = a.cap > 0.0f ? times_of_cap(times[r], a.cap) : times[r] * kLog2E;
     }
-    const float cap = a.cap * kLog2E;
+    const float cap = cap_log2(a.cap);
 
     // Pages of the wave's next 64 / kKeyTiles steps, a lane a tile of 16 keys.
     const uint32_t tiles_of_page = a.cache.page_size / 16u;

@@ -124,8 +124,8 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         }
         times *= bits_f32(down << 23);
     }
-    times *= a.cap > 0.0f ? 2.0f * kLog2E / a.cap : kLog2E;
-    const float cap = a.cap * kLog2E;
+    times = a.cap > 0.0f ? times_of_cap(times, a.cap) : times * kLog2E;
+    const float cap = cap_log2(a.cap);
 
     // Pages of the next 16 steps, a lane a tile of 16 keys.
     const uint32_t tiles_of_page = a.cache.page_size / 16u;
