@@ -40,6 +40,8 @@ uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tok
 // 128) by attention_many_kernel.  The keys are split; how many of the `splits` a sequence has goes by its length, which the device knows.  Measured, in us:
 //   16 sequences of 4000 to 8191 keys, 12 rows each: tiles of 16 rows 59, of 32 rows 70; 24 rows: of 16 rows 95, of 32 rows 75; 64 rows: of 32 rows 122, of 256 rows 167;
 //     128 rows: of 32 rows 201, of 256 rows 175
+//   heads past 128 of a quantized cache, whose tiles of 32 rows want more registers than there are: 8 sequences within a window of 4096 keys, i8 and 4 bits in blocks of 32, 20 rows
+//     each: of 16 rows 58 and 80, of 32 rows 112 and 151, of 128 rows 105 and 105; 28 rows twice over (56): of 16 rows 103 and 91, of 128 rows 110 and 108.  Of floats 20 rows: of 16 rows 89, of 32 rows 60
 //   parts of few rows, at most 768, 1024, 1536, 2048: 64 sequences of 257 to 8191 keys 120, 117, 119, 123; of 4096 keys 100, 100, 105, 110
 //     of 8, 16, 32 steps: one sequence of 3000 keys 14.7, 16.2, 22.5, of 8000 15.4, 16.7, 20.4, of 32000 23.2, 24.2, 23.0; eight of 8000 41, 39, 35;
 //     five tokens of eight within a window of 4096 52, 39, 36 (of four parts; 47 of five, which some compute units have two of)
@@ -48,7 +50,7 @@ uint64_t part_bytes(const AttentionArgs& a) { return static_cast<uint64_t>(a.tok
 Split split_of(const AttentionArgs& a, uint64_t room) {
     Split f{};
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.group, mean = (rows + a.seqs - 1) / a.seqs;
-    f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? 2 : 0;
+    f.row_tiles = mean <= 16 ? 1 : mean <= 64 ? (a.cache.dim > 128 && a.cache.code != kCacheFloat ? 1 : 2) : 0;
     const uint64_t of_tile = f.row_tiles ? 16 * f.row_tiles : a.cache.dim > 128 ? 128 : 256;
     const uint64_t step = f.row_tiles && a.cache.code != kCacheInt4 && a.cache.code != kCacheE2M1 ? 32 : 64;
     f.wanted = f.row_tiles ? 1024 : 256;

@@ -166,23 +166,30 @@ __device__ __forceinline__ bool lost_below(uint32_t least, int32_t power) { retu
 // the position, so that the distance is linear and costs two instructions a score instead of five.  The conditions are uniform over the wave and each has a loop
 // of its own: as choices within one loop they are all computed for all scores (509 tokens with a bias behind 7681 keys: 214 us instead of 154).
 // The exponential's difference is off by 2^-22 of the cap, whatever the score: up to a cap of 64 (times log2 e) that is 2^-16 of a score's unit, less than weights of 16 bits
-// show.  Of larger ones, |t / cap| < 1/4 takes tanh's series (what follows its last term is below 2^-21 of it); above, the difference is off by 2^-20 of itself.  A choice of each
-// score and not a loop of its own: that one moved what stands around it (prompt_longest, which has no cap, 650 us instead of 625).
+// show.  Of larger ones, |t / cap| < 1/4 takes tanh's series (what follows its last term is below 2^-21 of it); above, the difference is off by 2^-20 of itself.  kApart: small caps
+// in a loop of their own, which is faster (a draft of 20 rows 36.8 us instead of 40.3, prompt_longest in f16 885 instead of 920), but where it moves what stands around it: calls without any
+// cap took 650 us instead of 630 (prompt_longest), 121 instead of 116 (decode_batch).
 constexpr float kExponentialCap = 64.0f * kLog2E;
 // A cap as log2(e) times itself, and what `times` holds of it: no infinities of the highest and lowest numbers of f32 (a cap past 10^38 is 10^38).
 __device__ __forceinline__ float cap_log2(float cap) { return fminf(cap, 1e38f) * kLog2E; }
 __device__ __forceinline__ float times_of_cap(float times, float cap) { return fminf(times * fminf(2.0f * kLog2E / fminf(cap, 1e38f), 3e38f), 3e38f); }
-template <uint32_t kCount, class Place>
+template <bool kApart, uint32_t kCount, class Place>
 __device__ __forceinline__ float shape_scores(float (&of)[kCount], float times, float cap, bool biased, float slope, int32_t position, int32_t key0, Place place, bool behind,
                                               bool partial, int32_t row_low, int32_t row_high) {
     if (cap > 0.0f) {  // cap tanh(t / cap) = cap - 2 cap / (1 + exp(2 t / cap)); `times` holds the 2 / cap
         const auto of_exponential = [&](float v) { return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * times)), cap); };
-        const float edge = cap <= kExponentialCap ? 0.0f : 0.25f;
+        const bool small = cap <= kExponentialCap;
+        const float edge = small ? 0.0f : 0.25f;
+        if (kApart && small) {
 #pragma unroll
-        for (uint32_t i = 0; i < kCount; i++) {
-            const float x = of[i] * times * 0.34657359028f, x2 = x * x;  // t / cap: times ln(2) / 2
-            const float series = __builtin_fmaf(x2, __builtin_fmaf(x2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f);
-            of[i] = fabsf(x) < edge ? cap * __builtin_fmaf(x * x2, series, x) : of_exponential(of[i]);
+            for (uint32_t i = 0; i < kCount; i++) of[i] = of_exponential(of[i]);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kCount; i++) {
+                const float x = of[i] * times * 0.34657359028f, x2 = x * x;  // t / cap: times ln(2) / 2
+                const float series = __builtin_fmaf(x2, __builtin_fmaf(x2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f);
+                of[i] = fabsf(x) < edge ? cap * __builtin_fmaf(x * x2, series, x) : of_exponential(of[i]);
+            }
         }
         times = 1.0f;
     }

@@ -77,24 +77,31 @@ __device__ __forceinline__ bool code_is_odd(u32x4 v) {
     return found;
 }
 
-// Waves per SIMD that registers are kept for: results, queries, codes on their way, scores and weights, and what else there is.
-template <int kCode, int kDim, int kTiles>
+// Waves per SIMD that registers are kept for: the most that builds show to need no scratch memory.  (Compiled for one more, loads of spilled registers stood in the loop: 64 tokens
+// over 4 bits in blocks of 32, heads of 256, 604 us, 195 without them; five drafted tokens of 20 rows 178 and 80, over 8 bits 178 and 58.)
+template <int kCode, int kDim, int kPer, int kTiles>
 constexpr int waves_of() {
-    using S = Shape<kCode, kDim, 1>;
-    constexpr int kRegisters = kDim * kTiles * 3 / 8 + S::kKeys * S::kRow / 128 + kTiles * S::kKeyTiles * 8 + 60;
-    return kRegisters <= 128 ? 4 : kRegisters <= 168 ? 3 : kRegisters <= 256 ? 2 : 1;
+    constexpr bool kNibbles = kCodeBits<kCode> == 4;
+    if (kDim == 64) return kTiles == 1 ? 4 : kNibbles ? 2 : 3;
+    if (kDim == 128 && kTiles == 1) return kCode == kCacheFloat || (kNibbles && kPer > 1) ? 2 : 3;
+    if (kDim == 128) return kNibbles && kPer > 1 ? 1 : 2;
+    return kCode == kCacheFloat ? 1 : 2;
 }
+// Where that takes it, queries stay in LDS, the same for all waves, and the compiler may not move operands of one tile in front of another's.
+template <int kCode, int kDim, int kPer, int kTiles>
+constexpr bool kTight = kDim == 256 || kTiles == 2 || (kCodeBits<kCode> == 4 && kDim == 128 && kPer == 1);
 
 // of a workgroup, at most
-template <int kCode, int kDim, int kTiles>
-constexpr uint32_t kMostWaves = waves_of<kCode, kDim, kTiles>() == 1 ? 4 : 8;
+template <int kCode, int kDim, int kPer, int kTiles>
+constexpr uint32_t kMostWaves = waves_of<kCode, kDim, kPer, kTiles>() == 1 ? 4 : 8;
 
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
-__global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<kCode, kDim, kTiles>())) void attention_few_kernel(AttentionArgs a, Split split) {
+__global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kPer, kTiles>), (waves_of<kCode, kDim, kPer, kTiles>())) void attention_few_kernel(AttentionArgs a, Split split) {
     using S = Shape<kCode, kDim, kPer>;
     constexpr bool kFloat = kCode == kCacheFloat;
     constexpr uint32_t kRowsLog2 = kTiles == 1 ? 4 : 5, kRows = 16 * kTiles;
     constexpr uint32_t kOut = kDim / 16;  // tiles of 16 entries of the result
+    constexpr bool kShort = kTight<kCode, kDim, kPer, kTiles>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15u, g = lane >> 4;
     // neighbours in the grid are heads of the cache, whose entries lie side by side
@@ -182,6 +189,16 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
         times[r] = a.cap > 0.0f ? times_of_cap(times[r], a.cap) : times[r] * kLog2E;
     }
     const float cap = cap_log2(a.cap);
+    u32x4* const queries = reinterpret_cast<u32x4*>(lds + waves * S::kWaveBytes);  // [tile of rows][slice][lane], the same for all waves
+    if constexpr (kShort) {
+        if (wave == 0)
+#pragma unroll
+            for (uint32_t r = 0; r < kTiles; r++)
+#pragma unroll
+                for (uint32_t t = 0; t < S::kSlices; t++) queries[(r * S::kSlices + t) * 64u + lane] = q[r][t];
+        __syncthreads();
+    }
+    const auto query = [&](uint32_t r, uint32_t t) { return kShort ? queries[(r * S::kSlices + t) * 64u + lane] : q[r][t]; };
 
     // Pages of the wave's next 64 / kKeyTiles steps, a lane a tile of 16 keys.
     const uint32_t tiles_of_page = a.cache.page_size / 16u;
@@ -202,25 +219,30 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
     const ScaleWords words(a.cache.param_dtype);
     const uint32_t row_bytes = dim * S::kBits / 8u;
     const auto key_byte = [&](uint32_t u) { return u * 64u + g * (4u * S::kWords); };
-    uint32_t key_offset[S::kUnits], value_offset[S::kLoads];
+    constexpr uint32_t kKeysOfLoad = 64 / S::kLanes;  // 32 where rows are 32 bytes
+    constexpr bool kOwn = kDim < 256;                 // an offset for each load of values; else one, and what all lanes have in common beside it
+    const uint32_t key_row = i * static_cast<uint32_t>(a.cache.keys.slot);
+    uint32_t key_offset[S::kUnits];
 #pragma unroll
-    for (uint32_t u = 0; u < S::kUnits; u++) key_offset[u] = i * static_cast<uint32_t>(a.cache.keys.slot) + min(key_byte(u), row_bytes - 4u * S::kWords);
+    for (uint32_t u = 0; u < S::kUnits; u++) key_offset[u] = key_row + min(key_byte(u), row_bytes - 4u * S::kWords);
+    const auto key_at = [&](uint32_t u) {
+        if constexpr (!kFloat || kDim < 256) return key_offset[u];
+        uint32_t first = g * 16u;  // worked out at each load: eight of them take registers that there are not
+        asm volatile("" : "+v"(first));
+        return key_row + min(u * 64u + first, row_bytes - 16u);
+    };
+    uint32_t value_offset[kOwn ? S::kLoads : 1];
 #pragma unroll
-    for (uint32_t n = 0; n < S::kLoads; n++) {
-        const uint32_t key = (n * 64u + lane) / S::kLanes;
-        value_offset[n] = key % 16u * static_cast<uint32_t>(a.cache.values.slot) + min(lane % S::kLanes * S::kLane, row_bytes - S::kLane);
-    }
-    // The scales of a tile of 16 keys: lane l has unit l % kPer of key l / kPer (of 256 entries in two loads).
-    uint32_t scale_offset[2][S::kScaleLoads ? S::kScaleLoads : 1];
-    const auto scale_unit = [&](uint32_t n) { return (n * 64u + lane) % kPer; };
-    const auto scale_key = [&](uint32_t n) { return (n * 64u + lane) / kPer % 16u; };
+    for (uint32_t n = 0; n < (kOwn ? S::kLoads : 1); n++)
+        value_offset[n] = (n * 64u + lane) / S::kLanes % 16u * static_cast<uint32_t>(a.cache.values.slot) + min(lane % S::kLanes * S::kLane, row_bytes - S::kLane);
+    // The scales of a tile of 16 keys: lane l has unit l % kPer of key l / kPer (of 256 entries in two loads, whose keys are 64 / kPer apart: whole words).
+    const uint32_t scale_unit = lane % kPer, scale_lane_key = lane / kPer % 16u;
+    const auto scale_key = [&](uint32_t n) { return scale_lane_key + n * (64u / kPer); };
+    uint32_t scale_offset[2] = {};
     if constexpr (!kFloat) {
-#pragma unroll
-        for (uint32_t n = 0; n < S::kScaleLoads; n++) {
-            const uint32_t block = min(scale_unit(n) * S::kUnit, dim - 1u) >> split.block_log2;
-            scale_offset[0][n] = (scale_key(n) * static_cast<uint32_t>(a.cache.keys.scale_slot) + block * static_cast<uint32_t>(a.cache.keys.scale_block)) << words.log2;
-            scale_offset[1][n] = (scale_key(n) * static_cast<uint32_t>(a.cache.values.scale_slot) + block * static_cast<uint32_t>(a.cache.values.scale_block)) << words.log2;
-        }
+        const uint32_t block = min(scale_unit * S::kUnit, dim - 1u) >> split.block_log2;
+        scale_offset[0] = (scale_lane_key * static_cast<uint32_t>(a.cache.keys.scale_slot) + block * static_cast<uint32_t>(a.cache.keys.scale_block)) << words.log2;
+        scale_offset[1] = (scale_lane_key * static_cast<uint32_t>(a.cache.values.scale_slot) + block * static_cast<uint32_t>(a.cache.values.scale_block)) << words.log2;
     }
     const char* const keys_base = a.cache.keys.base + kv_head * a.cache.keys.head;
     const char* const values_base = a.cache.values.base + kv_head * a.cache.values.head;
@@ -244,11 +266,11 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
 #pragma unroll
             for (uint32_t u = 0; u < S::kUnits; u++) {
                 if constexpr (S::kWords == 4) {
-                    const u32x4 w = stream_load(reinterpret_cast<const u32x4*>(rows + key_offset[u]));
+                    const u32x4 w = stream_load(reinterpret_cast<const u32x4*>(rows + key_at(u)));
 #pragma unroll
                     for (uint32_t e = 0; e < 4; e++) raw.k[k][u][e] = w[e];
                 } else {
-                    const u32x2 w = stream_load(reinterpret_cast<const u32x2*>(rows + key_offset[u]));
+                    const u32x2 w = stream_load(reinterpret_cast<const u32x2*>(rows + key_at(u)));
                     raw.k[k][u][0] = w[0], raw.k[k][u][1] = w[1];
                 }
             }
@@ -260,14 +282,13 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
         for (uint32_t k = 0; k < S::kKeyTiles; k++) find_tile(step, nth, k, &page[k], &place[k]);
 #pragma unroll
         for (uint32_t n = 0; n < S::kLoads; n++) {
-            constexpr uint32_t kKeysOfLoad = 64 / S::kLanes;  // 32 where rows are 32 bytes
             const uint32_t k = n * kKeysOfLoad / 16u;
-            uint64_t rows = offset_of(page[k], a.cache.values.page, place[k], a.cache.values.slot);
+            uint64_t rows = offset_of(page[k], a.cache.values.page, place[k] + (kOwn ? 0u : n * kKeysOfLoad % 16u), a.cache.values.slot);
             if constexpr (kKeysOfLoad > 16) {
                 const uint64_t second = offset_of(page[k + 1], a.cache.values.page, place[k + 1], a.cache.values.slot);
                 rows = lane / S::kLanes >= 16u ? second : rows;
             }
-            raw.v[n] = stream_load(reinterpret_cast<const u32x4*>(values_base + rows + value_offset[n]));
+            raw.v[n] = stream_load(reinterpret_cast<const u32x4*>(values_base + rows + value_offset[kOwn ? n : 0]));
         }
         if constexpr (!kFloat) {
             raw.odd = 0;
@@ -281,7 +302,10 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
                     const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(of[side])) & 2u;
                     raw.odd |= odd << (2 * (side * S::kKeyTiles + k));
 #pragma unroll
-                    for (uint32_t n = 0; n < S::kScaleLoads; n++) raw.scale[side][k][n] = *reinterpret_cast<const uint32_t*>(of[side] - odd + ((scale_offset[side][n] + odd) & ~3u));
+                    for (uint32_t n = 0; n < S::kScaleLoads; n++) {
+                        const uint64_t further = n * (64u / kPer) * static_cast<uint64_t>(static_cast<uint32_t>((side == 0 ? a.cache.keys : a.cache.values).scale_slot)) << words.log2;
+                        raw.scale[side][k][n] = *reinterpret_cast<const uint32_t*>(of[side] + further - odd + ((scale_offset[side] + odd) & ~3u));
+                    }
                 }
             }
         }
@@ -331,7 +355,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
                 for (uint32_t k = 0; k < S::kKeyTiles; k++)
 #pragma unroll
                     for (uint32_t n = 0; n < S::kScaleLoads; n++)
-                        scale[side][k][n] = words.number(raw.scale[side][k][n], scale_offset[side][n] + (raw.odd >> (2 * (side * S::kKeyTiles + k)) & 2u));
+                        scale[side][k][n] = words.number(raw.scale[side][k][n], scale_offset[side] + (raw.odd >> (2 * (side * S::kKeyTiles + k)) & 2u));
             if (partial) {
                 bool odd = false;
 #pragma unroll
@@ -367,7 +391,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
             for (uint32_t k = 0; k < S::kKeyTiles; k++)
 #pragma unroll
                 for (uint32_t n = 0; n < S::kScaleLoads; n++) {
-                    float* const to = scales_at + scale_unit(n) * S::kKeys + k * 16u + scale_key(n);  // (of 16 or 32 scales some lanes write the same)
+                    float* const to = scales_at + scale_unit * S::kKeys + k * 16u + scale_key(n);  // (of 16 or 32 scales some lanes write the same)
                     to[0] = scale[0][k][n];
                     to[kPer * S::kKeys] = scale[1][k][n] * down;
                 }
@@ -380,11 +404,12 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
         f32x4 s[kTiles][S::kKeyTiles];
 #pragma unroll
         for (uint32_t k = 0; k < S::kKeyTiles; k++) {
+            if constexpr (kShort) __builtin_amdgcn_sched_barrier(0);
             u32x4 operand[S::kSlices];
 #pragma unroll
             for (uint32_t u = 0; u < S::kUnits; u++) {
                 uint32_t* const w = raw.k[k][u];
-                if (row_bytes < S::kRow) {  // a shorter head: what lies past its end
+                if constexpr (kCodeHasNaN<kCode>) {  // past a shorter head's end queries are zero, which these codes may not be multiplied by
 #pragma unroll
                     for (uint32_t e = 0; e < S::kWords; e++) w[e] = key_byte(u) < row_bytes ? w[e] : 0u;
                 }
@@ -412,7 +437,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
                 for (uint32_t r = 0; r < kTiles; r++) {
                     f32x4 v = {};
 #pragma unroll
-                    for (uint32_t t = 0; t < S::kSlices; t++) v = mfma16<kBF16>(operand[t], q[r][t], v);
+                    for (uint32_t t = 0; t < S::kSlices; t++) v = mfma16<kBF16>(operand[t], query(r, t), v);
                     s[r][k] = kFloat ? v : v * by;
                 }
             } else {
@@ -423,7 +448,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
                     for (uint32_t r = 0; r < kTiles; r++) {
                         f32x4 v = {};
 #pragma unroll
-                        for (uint32_t t = unit * S::kUnit / 32; t < (unit + 1) * S::kUnit / 32; t++) v = mfma16<kBF16>(operand[t], q[r][t], v);
+                        for (uint32_t t = unit * S::kUnit / 32; t < (unit + 1) * S::kUnit / 32; t++) v = mfma16<kBF16>(operand[t], query(r, t), v);
                         s[r][k] = unit == 0 ? v * by : __builtin_elementwise_fma(v, by, s[r][k]);
                     }
                 }
@@ -439,7 +464,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
             float t[S::kKeyTiles * 4];
 #pragma unroll
             for (uint32_t i = 0; i < S::kKeyTiles * 4; i++) t[i] = s[r][i / 4u][i % 4u];
-            const float times_now = shape_scores(t, times[r], cap, a.slopes, slope[r], position[r], key0 + static_cast<int32_t>(4u * g), [](uint32_t i) { return i / 4u * 16u + i % 4u; },
+            const float times_now = shape_scores<S::kBits == 8 && (kDim == 256 || kTiles == 2)>(t, times[r], cap, a.slopes, slope[r], position[r], key0 + static_cast<int32_t>(4u * g), [](uint32_t i) { return i / 4u * 16u + i % 4u; },
                                                  key0 + static_cast<int32_t>(S::kKeys) - 1 <= first_position, partial, row_low[r], row_high[r]);
             float most = -INFINITY;
 #pragma unroll
@@ -503,6 +528,8 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kTiles>), (waves_of<k
                 for (uint32_t r = 0; r < kTiles; r++)
 #pragma unroll
                     for (uint32_t half = 0; half < kHalves; half++) w[r][half] = weights_of(r, e / (S::kUnit / 16), half);
+            if constexpr (kShort)
+                if (e % 2 == 0) __builtin_amdgcn_sched_barrier(0);
             u32x4 v[kHalves];
             values_of(e, v);
 #pragma unroll
@@ -572,14 +599,14 @@ template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>
 hipError_t launch_few(hipStream_t s, const AttentionArgs& a, const Split& split) {
     using S = Shape<kCode, kDim, kPer>;
     const auto lds_of = [](uint32_t waves) {
-        const uint32_t steps = waves * S::kWaveBytes, join = 2 * waves * 16 * kTiles * 4 + kTiles * (kDim / 16) * (waves - 1) * 1024;
+        const uint32_t steps = waves * S::kWaveBytes + (kTight<kCode, kDim, kPer, kTiles> ? kTiles * S::kSlices * 1024 : 0), join = 2 * waves * 16 * kTiles * 4 + kTiles * (kDim / 16) * (waves - 1) * 1024;
         return steps > join ? steps : join;
     };
     // Where there are not even as many workgroups as compute units, eight waves each, which ask for twice as much at a time (24 workgroups with up to
     // 701 keys: 16.2 us of four waves, 14.2 of eight); their results have to fit in LDS.
     Split by = split;
     const uint32_t workgroups = split.tiles * a.cache.kv_heads * split.splits;
-    constexpr uint32_t kMost = kMostWaves<kCode, kDim, kTiles>;
+    constexpr uint32_t kMost = kMostWaves<kCode, kDim, kPer, kTiles>;
     by.waves = workgroups <= 256 && lds_of(kMost) <= 160 * 1024 - 512 ? kMost : 4;
     hipLaunchKernelGGL((attention_few_kernel<kCode, kDim, kPer, kTiles, kBF16>), dim3(workgroups), dim3(64 * by.waves), lds_of(by.waves), s, a, by);
     return hipGetLastError();
@@ -592,8 +619,9 @@ hipError_t launch_tiles(hipStream_t s, const AttentionArgs& a, const Split& spli
             if (a.dtype == CQ_BF16) return launch_few<kCode, kDim, kPer, tiles.value, true>(s, a, split);
         return launch_few<kCode, kDim, kPer, tiles.value, false>(s, a, split);
     };
-    if (split.row_tiles == 1) return by_type(std::integral_constant<int, 1>{});
-    return by_type(std::integral_constant<int, 2>{});
+    if constexpr (kDim < 256 || kCode == kCacheFloat)  // (split_of)
+        if (split.row_tiles == 2) return by_type(std::integral_constant<int, 2>{});
+    return by_type(std::integral_constant<int, 1>{});
 }
 
 template <int kCode, int kDim>

@@ -33,6 +33,11 @@ struct Many {
     static constexpr uint32_t kPitch = kDim * 2 + 32, kSide = kKeys * kPitch, kBuffer = 2 * kSide;       // bytes in LDS: of a row, of keys or values, of both
 };
 
+// Forms that would keep reading spilled registers from scratch memory work out their lanes' addresses in LDS again in every step (7 prompts of 33 to 2047 tokens over i8 of heads of
+// 256, f16: 735 us, and 769).  Heads of 64 put up to four registers away in front of their steps and take them back behind, which costs less than this would (99 us, and 102).
+template <int kDim, bool kExact>
+constexpr bool kAgain = kExact && kDim == 256;
+
 // Eight numbers in the order of their entries.
 template <int kCode>
 __device__ __forceinline__ u32x4 in_order(u32x4 v) {
@@ -308,6 +313,9 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         const int32_t key0 = static_cast<int32_t>((step0 + step) * S::kKeys + 32u * half);
         if (key0 > wave_high || key0 + static_cast<int32_t>(kSpan) - 1 < wave_low) return;
         const bool partial = key0 < all_low || key0 + static_cast<int32_t>(kSpan) - 1 > all_high;
+        uint32_t own_lane = lane;
+        if constexpr (kAgain<kDim, kExact>) asm volatile("" : "+v"(own_lane));
+        const uint32_t n = own_lane & 31u, h = own_lane >> 5;
         const char* const keys = lds + (step & 1u) * S::kBuffer + 32u * half * S::kPitch;
         const char* const values = keys + S::kSide;
         // the scales of lane (n, h)'s keys, of one block of entries: four behind one another of every eight
@@ -346,7 +354,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
 #pragma unroll
             for (uint32_t v = 0; v < kSpan / 2; v++) t[v] = s[v / 16u][v % 16u];
         }
-        const float times_now = shape_scores(t, by, cap, a.slopes, slope, position, key0 + static_cast<int32_t>(4u * h), [](uint32_t v) { return v / 4u * 8u + v % 4u; },
+        const float times_now = shape_scores<kExact>(t, by, cap, a.slopes, slope, position, key0 + static_cast<int32_t>(4u * h), [](uint32_t v) { return v / 4u * 8u + v % 4u; },
                                              key0 + static_cast<int32_t>(kSpan) - 1 <= first_position, partial, row_low, row_high);
         // largest scores are `top` + kLazy at most: results are taken down to a larger one only where it is needed
         float most = -INFINITY;
@@ -377,7 +385,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
 #pragma unroll
             for (uint32_t eight = 0; eight < 2; eight++) {
                 const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    CQ_LDS_AT(i16x4, values + first_out * 64u + (quarter * 16u + eight * 8u + 4u * h + lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + lane % 4u * 8u));
+                    CQ_LDS_AT(i16x4, values + first_out * 64u + (quarter * 16u + eight * 8u + 4u * h + own_lane % 16u / 4u) * S::kPitch + e * 64u + n / 16u * 32u + own_lane % 4u * 8u));
                 const u32x2 two = __builtin_bit_cast(u32x2, four);
                 v[2 * eight] = two[0], v[2 * eight + 1] = two[1];
             }
