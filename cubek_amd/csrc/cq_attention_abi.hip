@@ -123,6 +123,26 @@ cq_status read_floats(const cq_tensor* t, uint64_t n, const float** out) {
     return st;
 }
 
+// A tensor whose pages are copied.
+cq_status read_pool(const cq_tensor* t, cq::CopyArgs::Pool* p) {
+    if (!tensor_ok(t) || t->elem_size == 0) return CQ_ERR_INVALID_ARGUMENT;
+    uint64_t elements = 1;
+    for (uint32_t d = t->rank - 1; d > 0; d--) {
+        if (t->shape[d] > 1 && has_elements(t) && t->strides[d] != elements) return CQ_ERR_NON_CONTIGUOUS;
+        if (t->shape[d] > kMostExtent || elements > (1ull << 40) / (t->shape[d] ? t->shape[d] : 1)) return CQ_ERR_TOO_LARGE;
+        elements *= t->shape[d];
+    }
+    if (t->shape[0] > kMostExtent || elements * t->elem_size > (1ull << 36)) return CQ_ERR_TOO_LARGE;
+    p->base = static_cast<char*>(t->ptr);
+    p->stride = stride_of(t, 0) * t->elem_size;
+    p->bytes = elements * t->elem_size;
+    p->pages = static_cast<uint32_t>(t->shape[0]);
+    p->unit = 1;
+    for (uint32_t unit : {16u, 4u})
+        if (p->unit == 1 && aligned(p->base, unit) && p->stride % unit == 0 && p->bytes % unit == 0) p->unit = unit;
+    return cq::copy_groups(*p) > cq::kMostCopyGroups ? CQ_ERR_TOO_LARGE : CQ_OK;
+}
+
 // What a call's kernels are chosen by: cache, queries, table.
 cq_status read_shapes(const cq_cache* cache, const cq_tensor* q, const cq_tensor* table, cq_dtype dtype, cq::AttentionArgs* a) {
     if (!valid_dtype(dtype)) return CQ_ERR_INVALID_ARGUMENT;
@@ -223,34 +243,17 @@ cq_status cq_cache_copy(cq_stream_t stream, const cq_tensor* tensors, uint32_t c
     if (pairs->rank != 2 || pairs->elem_size != 4 || pairs->shape[1] != 2) return CQ_ERR_SHAPE_MISMATCH;
     if (!is_contiguous(pairs)) return CQ_ERR_NON_CONTIGUOUS;
     if (pairs->shape[0] > kMostTokens) return CQ_ERR_TOO_LARGE;
+    cq::CopyArgs::Pool pool;
     for (uint32_t i = 0; i < count; i++) {  // all of them before the first launch
-        const cq_tensor* const t = tensors + i;
-        if (!tensor_ok(t) || t->elem_size == 0) return CQ_ERR_INVALID_ARGUMENT;
-        uint64_t elements = 1;
-        for (uint32_t d = t->rank - 1; d > 0; d--) {
-            if (t->shape[d] > 1 && has_elements(t) && t->strides[d] != elements) return CQ_ERR_NON_CONTIGUOUS;
-            if (t->shape[d] > kMostExtent || elements > (1ull << 40) / (t->shape[d] ? t->shape[d] : 1)) return CQ_ERR_TOO_LARGE;
-            elements *= t->shape[d];
-        }
-        if (t->shape[0] > kMostExtent || elements * t->elem_size > (1ull << 36)) return CQ_ERR_TOO_LARGE;
+        const cq_status st = read_pool(tensors + i, &pool);
+        if (st != CQ_OK) return st;
     }
     if (pairs->shape[0] == 0 || count == 0) return CQ_OK;
     cq_status st = ready(stream);
     for (uint32_t first = 0; first < count && st == CQ_OK; first += cq::kCopyTensors) {
         cq::CopyArgs a{};
         const uint32_t n = count - first < cq::kCopyTensors ? count - first : cq::kCopyTensors;
-        for (uint32_t i = 0; i < n; i++) {
-            const cq_tensor* const t = tensors + first + i;
-            cq::CopyArgs::Pool& p = a.pools[i];
-            p.bytes = t->elem_size;
-            for (uint32_t d = 1; d < t->rank; d++) p.bytes *= t->shape[d];
-            p.base = static_cast<char*>(t->ptr);
-            p.stride = stride_of(t, 0) * t->elem_size;
-            p.pages = static_cast<uint32_t>(t->shape[0]);
-            p.unit = 1;
-            for (uint32_t unit : {16u, 4u})
-                if (p.unit == 1 && aligned(p.base, unit) && p.stride % unit == 0 && p.bytes % unit == 0) p.unit = unit;
-        }
+        for (uint32_t i = 0; i < n; i++) (void)read_pool(tensors + first + i, &a.pools[i]);
         a.pairs = static_cast<const int32_t*>(pairs->ptr);
         a.count = static_cast<uint32_t>(pairs->shape[0]);
         st = hip_status(cq::launch_copy(stream, a, n));

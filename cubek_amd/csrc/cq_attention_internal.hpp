@@ -84,6 +84,8 @@ CQ_FOR_CODES(CQ_DECLARE_TILES)
 hipError_t launch_attention_join(hipStream_t s, const AttentionArgs& a, const Split& split);
 
 constexpr uint32_t kCopyTensors = 32;
+constexpr uint64_t kCopyAccesses = 1024;                          // of a workgroup
+constexpr uint64_t kMostCopyGroups = kLaunchThreads / 256 - 1;  // workgroups of a page
 struct CopyArgs {
     struct Pool {
         char* base;
@@ -94,6 +96,7 @@ struct CopyArgs {
     uint32_t count;  // pairs
     uint32_t chunks;  // workgroups of a page
 };
+inline uint64_t copy_groups(const CopyArgs::Pool& p) { return (p.bytes + kCopyAccesses * p.unit - 1) / (kCopyAccesses * p.unit); }
 hipError_t launch_copy(hipStream_t s, const CopyArgs& a, uint32_t tensors);
 
 #if defined(__HIPCC__)

@@ -11,7 +11,8 @@
 namespace cq {
 namespace {
 
-constexpr uint32_t kPieces = 4, kChunk = 256 * kPieces;  // accesses of a lane and of a workgroup
+constexpr uint32_t kPieces = 4, kChunk = kCopyAccesses;  // accesses of a lane and of a workgroup
+static_assert(kChunk == 256 * kPieces);
 
 template <class T>
 __device__ __forceinline__ void copy_chunk(const char* from, char* to, uint64_t bytes, uint64_t chunk) {
@@ -48,13 +49,11 @@ hipError_t launch_copy(hipStream_t s, const CopyArgs& args, uint32_t tensors) {
     CopyArgs a = args;
     uint64_t chunks = 1;
     for (uint32_t t = 0; t < tensors; t++) {
-        const uint64_t n = (a.pools[t].bytes + static_cast<uint64_t>(kChunk) * a.pools[t].unit - 1) / (static_cast<uint64_t>(kChunk) * a.pools[t].unit);
+        const uint64_t n = copy_groups(a.pools[t]);  // kMostCopyGroups at most, as cq_cache_copy has seen to
         chunks = n > chunks ? n : chunks;
     }
-    constexpr uint64_t kMost = kLaunchThreads / 256 - 1;
-    if (chunks > kMost) return hipErrorInvalidValue;
     a.chunks = static_cast<uint32_t>(chunks);
-    const uint32_t piece = static_cast<uint32_t>(kMost / chunks);
+    const uint32_t piece = static_cast<uint32_t>(kMostCopyGroups / chunks);
     for (uint64_t pair = 0; pair < a.count; pair += piece) {
         const uint32_t n = a.count - pair < piece ? static_cast<uint32_t>(a.count - pair) : piece;
         hipLaunchKernelGGL(copy_pages_kernel, dim3(n * a.chunks, tensors), dim3(256), 0, s, a, static_cast<uint32_t>(pair));

@@ -92,7 +92,8 @@ size_t cq_attention_workspace_bytes(const cq_cache* cache, const cq_tensor* q, c
  * pairs[i, 0] to page pairs[i, 1], for a sequence that forks (a source as often as one likes) or a pool that is compacted.
  *   pairs : i32 [n, 2] in device memory, contiguous.  A pair with a page outside of a tensor copies nothing in it.  A page that is the destination of
  *           two pairs, or source of one and destination of another, may hold parts of both afterwards.
- * The tensors are handed over in launches of up to 32. */
+ * The tensors are handed over in launches of up to 32.  A page has 64 GiB at most, where its bytes, address or stride are no multiples of four less than 16 GiB (64 GiB less
+ * 4 KiB of fours). */
 cq_status cq_cache_copy(cq_stream_t stream, const cq_tensor* tensors, uint32_t count, const cq_tensor* pairs);
 
 /* hipError_t of the most recent failed HIP call of this library on the calling thread (0 if none). */

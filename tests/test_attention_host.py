@@ -20,3 +20,23 @@ def test_every_attention_object_is_built_without_packed_f32_and_contraction():
     assert len(lines) >= 18
     for line in lines:
         assert "-packed-fp32-ops" in line and "-ffp-contract=off" in line and "--offload-arch=gfx950" in line, line
+
+
+def test_pages_too_large_for_a_launch_are_refused_before_anything_is_copied():
+    """Bytes are copied one by one where a page allows nothing else, 1024 by a workgroup, of which a launch has fewer than 2^24; by fours and sixteens there is room for the largest pages."""
+    import pytest
+
+    from cubek_amd import ComputeClient, QuantError, TensorHandleRef, _ffi, cache
+
+    def pool(ptr, page, size=1):
+        return TensorHandleRef(ptr, (2, 1 << 10, page >> 10), (page, page >> 10, 1), size)
+
+    pairs = TensorHandleRef(1 << 20, (0, 2), (2, 1), 4)  # nothing to copy: what is taken returns without a GPU
+    small, large = pool(1 << 20, 1 << 20), 1 << 34
+    cache.copy_pages(ComputeClient(0), [small, pool(1 << 20, large)], pairs)
+    cache.copy_pages(ComputeClient(0), [small, pool((1 << 20) + 4, large)], pairs)
+    cache.copy_pages(ComputeClient(0), [small, pool((1 << 20) + 1, large - 1024)], pairs)
+    for tensors in ([pool((1 << 20) + 1, large)], [small] * 40 + [pool((1 << 20) + 2, large)]):
+        with pytest.raises(QuantError) as e:
+            cache.copy_pages(ComputeClient(0), tensors, pairs)
+        assert e.value.status == _ffi.ERR_TOO_LARGE
