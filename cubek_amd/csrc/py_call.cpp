@@ -474,14 +474,14 @@ PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream;
     Tensor pairs;
     if (!count(n, 3) || !pointer(a[0], &stream) || !pairs.read(a[2])) return nullptr;
-    const Ref fast(PySequence_Fast(a[1], "tensors are a sequence"));
+    const Ref fast(PySequence_Tuple(a[1]));  // what reading one of them runs may change a list
     if (!fast) return nullptr;
-    const Py_ssize_t of = PySequence_Fast_GET_SIZE(fast.p);
+    const Py_ssize_t of = PyTuple_GET_SIZE(fast.p);
     try {
         std::vector<Tensor> held(static_cast<size_t>(of));
         std::vector<cq_tensor> tensors(static_cast<size_t>(of));
         for (Py_ssize_t i = 0; i < of; i++) {
-            if (!held[static_cast<size_t>(i)].read(PySequence_Fast_GET_ITEM(fast.p, i))) return nullptr;
+            if (!held[static_cast<size_t>(i)].read(PyTuple_GET_ITEM(fast.p, i))) return nullptr;
             tensors[static_cast<size_t>(i)] = held[static_cast<size_t>(i)].t;
         }
         const AttentionCalls* const calls = attention_calls();
