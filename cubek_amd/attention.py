@@ -37,7 +37,9 @@ def launch_ref(client: ComputeClient, cache: Cache, q: TensorHandleRef, y: Tenso
     """``q``, ``y``: [tokens, heads, dim] of ``elem``; i32 on the device: ``table`` [sequences, pages] of each sequence, ``offsets``
     [sequences + 1] of its tokens, ``lengths`` [sequences] of its keys with the new ones, which are in the cache already.
     ``workspace``: device memory of ``workspace_bytes()``, optional."""
-    scale = scores.scale if scores.scale is not None else q.shape[-1] ** -0.5
+    scale = scores.scale
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.shape and q.shape[-1] else 1.0  # heads without entries are the library's to refuse
     rc = _ffi.calls().attention(client.stream, cache.keys, cache.key_scales, cache.values, cache.value_scales, cache.scheme, q, y, table, offsets, lengths,
                                 scale, scores.cap, scores.window, scores.slopes, scores.prefix, elem, workspace, workspace_size)
     if rc:

@@ -2,6 +2,10 @@
 import subprocess
 import sys
 
+import pytest
+
+from cubek_amd import Cache, ComputeClient, ElemType, QuantError, TensorHandleRef, _ffi, attention
+
 
 def test_a_list_of_tensors_that_changes_while_it_is_read():
     """What stands for a tensor may run code of its own (as_c), which empties the list it is read from: the call sees the tensors that it was given."""
@@ -19,3 +23,13 @@ print("read")
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert run.returncode == 0 and run.stdout.strip() == "read", run.stderr[-300:]
+
+
+@pytest.mark.parametrize("shape", [(), (5, 4, 0), (0,)])
+def test_queries_without_entries_are_refused_by_the_library(shape):
+    """The scale that stands for none given is worked out of the heads' size, where there is one."""
+    t = lambda s, size: TensorHandleRef(1 << 20, s, tuple(1 for _ in s), size)  # noqa: E731
+    held = Cache(TensorHandleRef(1 << 20, (9, 2, 16, 64), (2048, 1024, 64, 1), 2), TensorHandleRef(1 << 20, (9, 2, 16, 64), (2048, 1024, 64, 1), 2))
+    with pytest.raises(QuantError) as e:
+        attention.launch_ref(ComputeClient(0), held, t(shape, 2), t(shape, 2), t((3, 4), 4), t((4,), 4), t((3,), 4), ElemType.BF16)
+    assert e.value.status in (_ffi.ERR_SHAPE_MISMATCH, _ffi.ERR_INVALID_ARGUMENT)
