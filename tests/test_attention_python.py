@@ -4,7 +4,7 @@ import sys
 
 import pytest
 
-from cubek_amd import Cache, ComputeClient, ElemType, QuantError, TensorHandleRef, _ffi, attention
+from cubek_amd import Cache, ComputeClient, ElemType, QuantError, TensorHandleRef, _ffi, attention, rotary
 
 
 def test_a_list_of_tensors_that_changes_while_it_is_read():
@@ -33,3 +33,25 @@ def test_queries_without_entries_are_refused_by_the_library(shape):
     with pytest.raises(QuantError) as e:
         attention.launch_ref(ComputeClient(0), held, t(shape, 2), t(shape, 2), t((3, 4), 4), t((4,), 4), t((3,), 4), ElemType.BF16)
     assert e.value.status in (_ffi.ERR_SHAPE_MISMATCH, _ffi.ERR_INVALID_ARGUMENT)
+
+
+def test_a_ramp_of_frequencies_by_parts():
+    """Pairs by the number of times they turn within the trained length: with base e^4 and 16 entries, pair i turns trained / (2 pi) e^(-i / 2) times; more than 32 times: as it is; less than
+    once: slowed; between the indexes of both, rounded outwards, in a straight line."""
+    import math
+
+    base, trained, factor = math.exp(4.0), 600, 8.0
+    plain = rotary.frequencies(16, base)
+    turns = [trained * f / (2 * math.pi) for f in plain]
+    low = math.floor(2 * math.log(trained / (32 * 2 * math.pi)))  # 2
+    high = math.ceil(2 * math.log(trained / (2 * math.pi)))       # 10
+    got = rotary.frequencies_by_parts(16, factor, trained, base)
+    assert (low, high) == (2, 10)
+    for i, (f, n, g) in enumerate(zip(plain, turns, got)):
+        share = min(1.0, max(0.0, (i - low) / (high - low)))
+        assert abs(g - f * ((1.0 - share) + share / factor)) <= 1e-15 * f
+        if n > 32:
+            assert g == f
+    # within one length that turns every pair less than once all are slowed, and where all turn often none is
+    assert rotary.frequencies_by_parts(16, factor, 4, base) == [f / factor for f in plain]
+    assert rotary.frequencies_by_parts(16, factor, 10 ** 7, base) == plain
