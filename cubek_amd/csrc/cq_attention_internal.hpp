@@ -11,7 +11,7 @@ namespace cq {
 constexpr uint64_t kLaunchThreads = 1ull << 32;
 
 // How an entry of the cache is stored.
-enum CacheCode : uint32_t { kCacheInt8 = 0, kCacheInt4 = 1, kCacheE4M3 = 2, kCacheE5M2 = 3, kCacheE2M1 = 4, kCacheFloat = 5, kCacheCodes = 6 };
+enum CacheCode : uint32_t { kCacheInt8 = 0, kCacheInt4 = 1, kCacheE4M3 = 2, kCacheE5M2 = 3, kCacheE2M1 = 4, kCacheFloat = 5 };
 
 // Keys, or values: row `place` of head h of page p at base + p * page + h * head + place * slot, in bytes; its scales in elements.
 struct CacheSide {
@@ -150,12 +150,6 @@ __device__ __forceinline__ Seen seen_from(const AttentionArgs& a, const Sequence
 __device__ __forceinline__ uint32_t page_of(const AttentionArgs& a, const Sequence& s, uint32_t nth) {
     const int32_t page = a.table[s.index * a.table_row + nth];
     return min(static_cast<uint32_t>(max(page, 0)), a.cache.pages - 1u);
-}
-
-// A score in front of the softmax, t = scale * (q . k) given.
-__device__ __forceinline__ float capped(float cap, float t) {
-    // tanh u = 1 - 2 / (1 + exp 2u): off by a few 2^-24 of 1, of `cap` in the score
-    return cap * (1.0f - 2.0f / (1.0f + __expf(t * (2.0f / cap))));
 }
 
 #endif

@@ -269,7 +269,7 @@ __device__ __forceinline__ bool find_rows_and_steps(const AttentionArgs& a, cons
         for (uint32_t i = lane; i < a.seqs; i += 64) {
             s = sequence_of(a, i);
             own = static_cast<uint32_t>((static_cast<uint64_t>(s.last - s.first) * a.group + ((1u << rows_log2) - 1u)) >> rows_log2);
-            const uint32_t seen = a.window ? min(static_cast<uint32_t>(s.length), max(a.window, 1u) + (s.last - s.first)) : static_cast<uint32_t>(s.length);
+            const uint32_t length = static_cast<uint32_t>(s.length), seen = a.window && a.window < length ? min(length, a.window + (s.last - s.first)) : length;
             total = static_cast<uint32_t>(min(total + static_cast<uint64_t>(own) * ((seen >> keys_log2) + 1u), static_cast<uint64_t>(1u << 20)));
         }
     }

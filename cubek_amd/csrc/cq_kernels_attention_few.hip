@@ -122,8 +122,9 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kPer, kTiles>), (wave
     const uint32_t parts = min(max((steps_all + steps_wanted / 2u) / steps_wanted, 1u), split.splits);
     if (part >= parts) return;
     if (split.splits > 1 && part == 0) note_parts(a, split, at, kv_head, parts);
-    // Where there are more parts than the GPU holds at once, the later ones, which start last, are smaller, from 3/2 of the mean down to 1/2, so that all
-    // end together (64 sequences of 257 to 8191 keys: 120 us of equal parts, 117; 200 of 257 to 4000: 187 and 181); else all are equal (one of 131071: 46, and 52).
+    // Where all tiles together would have more parts than split.wanted, which is about as many as the GPU holds at once, the later ones, which start last, are smaller, from 3/2 of
+    // the mean down to 1/2, so that all end together (64 sequences of 257 to 8191 keys: 120 us of equal parts, 117; 200 of 257 to 4000: 187 and 181).  Else all are equal (one of
+    // 131071: 46, and 52), and so they are of few tiles (up to 32 with keys to split), whose kMostSplits parts each are no more than the GPU holds whatever their length.
     uint32_t from, to;
     if (steps_wanted > split.enough && split.splits < kMostSplits) {
         const float by = static_cast<float>(steps_all) / static_cast<float>(2u * parts * parts);
