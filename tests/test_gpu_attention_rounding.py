@@ -7,7 +7,7 @@ import pytest
 
 from attention_reference import Attention
 from cubek_amd import ElemType, QuantStore, QuantValue
-from matmul_reference import scheme_of
+from matmul_reference import check_rounded, scheme_of
 
 pytestmark = pytest.mark.gpu
 BF16 = ElemType.BF16
@@ -31,3 +31,16 @@ def test_a_keys_scale_is_not_rounded_by_itself(oracle, dim):
     want, _ = case.want()
     got = case.call().double().cpu().numpy()
     assert np.linalg.norm(got - want) <= 2.0 ** -9 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("tokens,length", [(1, 400), (1, 3000), (9, 700), (30, 500)])
+def test_weights_over_a_cache_of_bf16_have_16_bits(oracle, dim, tokens, length):
+    """Products of bf16 are exact in f32; a weight is two numbers of bf16, off by 2^-18 of it: what the second leaves of what the first leaves."""
+    case = Attention(oracle, 2, [(tokens, length), (tokens, tokens + 5)], 2, 1, dim, 16, BF16, None)
+    case.u = 0.0
+    want, bound = case.want()
+    held, case.v.entries = case.v.entries, np.abs(case.v.entries)
+    size, _ = case.want()
+    case.v.entries = held
+    check_rounded(case.call().double().cpu().numpy(), want, bound + size * 2.0 ** -17, BF16)
