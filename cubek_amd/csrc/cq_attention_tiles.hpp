@@ -152,14 +152,25 @@ __device__ __forceinline__ uint32_t exponent_of(float v) {
     return field == 255u ? 0u : field;
 }
 
-// Weights times the scales of values (few rows, and kExact of many), or entries (many rows), are held in f16 over the largest scale so far, 2^power.  Of scales
-// down to 2^-kSpread of it that leaves a weight 2^-16 of the largest one and an entry 2^-10 of its code's step.  A smaller one, unless it is zero, would lose
-// its bits to keys that a row may not even see: where there is one the tile's rows are taken one by one (rows_one_by_one).  A model's stay far within: from the
-// largest block of a cache to the smallest it is 2^10 or so.  A thread keeps the smallest of its scales, by twice their bits less one, so that zero is the
-// largest of all and its sign does not count: two instructions a scale, and one question at the end (asked in every step, prompt_longest took 650 us instead of 624).
-constexpr int32_t kSpread = 14;
+// Weights times the scales of values (few rows, and kExact of many), or entries (many rows), are held in f16 over the largest scale so far, 2^power, to half of its
+// smallest step, 2^-25.  Scales down to 2^-kSpread of the largest leave a weight 2^-18 of the largest one and an entry 2^-12 of its code's step.  A smaller one, unless it is zero,
+// loses bits to keys that a row may not even see, or give no weight; rows whose results are small enough to show that are taken once more (rows_again).  A model's scales lie within
+// 2^10 or so of one another.  A thread keeps the smallest of its scales, by twice their bits less one, so that zero is the largest of all and its sign does not count: two
+// instructions a scale, and one question at the end (asked in every step, prompt_longest took 650 us instead of 624).
+constexpr int32_t kSpread = 12;
 __device__ __forceinline__ uint32_t smaller_of(uint32_t least, float scale) { return min(least, 2u * f32_bits(scale) - 1u); }
 __device__ __forceinline__ bool lost_below(uint32_t least, int32_t power) { return least < max(static_cast<uint32_t>(max(127 + power - kSpread, 0)) << 24, 1u) - 1u; }
+// A row shows it if its scores may be off by more than kScoreOff, or if 32 neighbouring entries of its result are all below kShows times what they may be off by: else that is less
+// than 2^-11 of the largest of them, as it is of keys that have weight.
+constexpr float kScoreOff = 0x1p-12f, kShows = 0x1p11f;
+struct Losses {
+    float key, value;  // in a score (times log2 e) by the sum of |query|; in a result
+};
+template <int kCode>
+constexpr float kMostCode = kCode == kCacheInt8 ? 128.0f : kCode == kCacheInt4 ? 8.0f : kCode == kCacheE4M3 ? 448.0f : kCode == kCacheE5M2 ? 57344.0f : 6.0f;
+// Of `keys` weights each is off by 2^-25 times its code; their sum is 2^5 at least.
+template <int kCode>
+__device__ __forceinline__ float lost_by_weights(uint32_t keys, int32_t power) { return ldexpf(kMostCode<kCode> * static_cast<float>(keys), power - 30); }
 
 // What a row's products become before their weights: capped, with the bias of their distance, keys that the row does not see at -infinity.  `of` are a lane's
 // products with the keys key0 + place(i); what is returned is left to be multiplied by, `times` where nothing of this is wanted.  `behind`: no key is past
@@ -311,20 +322,25 @@ __device__ __forceinline__ void note_parts(const AttentionArgs& a, const Split& 
     }
 }
 
-// The rows of a tile once more, one by one, over the keys from first to last: taken where an entry of a value that is infinite or not a number lies among
-// keys that not every row of the tile sees, for a weight of zero does not keep such an entry out of a product of tiles, and where scales are further apart than
-// f16 can hold (kSpread).  All threads of the workgroup
-// come here, with its LDS free for (kDim + 64) floats a wave.  The arguments, the kernel's first two, are read again, so that what is needed here alone
-// takes no registers from what comes before.
-template <uint32_t kDim>
-__device__ __forceinline__ void rows_one_by_one(uint32_t seq, uint32_t row0, uint32_t rows, uint32_t part, uint32_t parts, uint32_t kv_head, int64_t first, int64_t last, float* lds) {
-    struct Arguments {
-        AttentionArgs a;
-        Split split;
-    };
+// A kernel's first two arguments, read again: what is only needed behind its steps takes no registers from them.
+struct Arguments {
+    AttentionArgs a;
+    Split split;
+};
+__device__ __forceinline__ const Arguments& arguments_again() {
     uint64_t again = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(again));
-    const Arguments& arguments = *reinterpret_cast<const Arguments*>(again);
+    return *reinterpret_cast<const Arguments*>(again);
+}
+
+// Rows of a tile once more, one by one, over the keys from first to last, in f32: all of them (`whole`) where an entry of a value that is infinite or not a number lies among
+// keys that not every row of the tile sees, for a weight of zero does not keep such an entry out of a product of tiles; else those that show that scales are far apart (kSpread),
+// whose results are written already.  All threads of the workgroup
+// come here, with its LDS free for (kDim + 64) floats a wave.
+template <uint32_t kDim>
+__device__ __forceinline__ void rows_again(uint32_t seq, uint32_t row0, uint32_t rows, uint32_t part, uint32_t parts, uint32_t kv_head, int64_t first, int64_t last, bool whole,
+                                           Losses losses, float* lds) {
+    const Arguments& arguments = arguments_again();
     const AttentionArgs& a = arguments.a;
     const Split& split = arguments.split;
     const Sequence s = sequence_of(a, seq);
@@ -332,14 +348,29 @@ __device__ __forceinline__ void rows_one_by_one(uint32_t seq, uint32_t row0, uin
     float* const query = lds + wave * (kDim + 64u);
     for (uint32_t row = wave; row < rows; row += blockDim.x / 64u) {
         const uint32_t in_sequence = row0 + row, token = s.first + in_sequence / a.group, head = kv_head * a.group + in_sequence % a.group;
+        const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
+        float of_query = 0.0f;
+        for (uint32_t d = lane; d < a.cache.dim; d += 64) {
+            const float q = load_dtype(a.dtype, a.q, token * a.q_token + head * a.q_head + d);
+            query[d] = q;
+            of_query += fabsf(q);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (!whole) {
+            bool shows = losses.key * wave_sum(of_query) > kScoreOff;
+            for (uint32_t d = lane; d < a.cache.dim; d += 64) {
+                float most = fabsf(parts > 1 ? split.parts[of * a.cache.dim + d] : load_dtype(a.dtype, a.y, token * a.y_token + head * a.y_head + d));
+#pragma unroll
+                for (int other = 16; other; other >>= 1) most = fmaxf(most, __shfl_xor(most, other, 64));  // of 32 entries, whose lanes are all here or none
+                shows |= most < kShows * losses.value;
+            }
+            if (__builtin_amdgcn_ballot_w64(shows) == 0) continue;
+        }
         const int32_t position = s.position + static_cast<int32_t>(in_sequence / a.group);
         const Seen seen = seen_from(a, s, position);
-        for (uint32_t d = lane; d < a.cache.dim; d += 64) query[d] = load_dtype(a.dtype, a.q, token * a.q_token + head * a.q_head + d);
-        __builtin_amdgcn_wave_barrier();
         float top, sum, v[kDim / 64];
         attend_row<kDim / 64>(a, s, kv_head, position, a.slopes ? a.slopes[head] : 0.0f, query, query + kDim, max(first, static_cast<int64_t>(seen.low)), 64,
                               min(last, static_cast<int64_t>(seen.high)), &top, &sum, v);
-        const uint64_t of = (static_cast<uint64_t>(token) * a.heads + head) * split.splits + part;
 #pragma unroll
         for (uint32_t i = 0; i < kDim / 64; i++) {
             const uint32_t d = i * 64u + lane;

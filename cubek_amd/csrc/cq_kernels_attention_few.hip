@@ -555,11 +555,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kPer, kTiles>), (wave
         fence();
     }
 
-    if (__syncthreads_or(found || (!kFloat && lost_below(least, power)))) {
-        const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
-        rows_one_by_one<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
-        return;
-    }
+    const bool whole = __syncthreads_or(found);
     // The waves' results, each by its share of the whole over its sum.  A tile of 16 entries of the result is finished by the wave e % waves, which the others
     // hand theirs.
     float* const tops = reinterpret_cast<float*>(lds);  // [wave][row]
@@ -570,7 +566,7 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kPer, kTiles>), (wave
         sum[r] = sum_of_groups(sum[r]);
         if (g == 0) tops[wave * kRows + r * 16u + i] = top[r], sums[wave * kRows + r * 16u + i] = sum[r];
     }
-    __syncthreads();
+    const bool far = __syncthreads_or(!kFloat && lost_below(least, power));
     const float up = kFloat ? 1.0f : ldexpf(1.0f, power);
     float most[kTiles], all[kTiles];
 #pragma unroll
@@ -608,6 +604,16 @@ __global__ __launch_bounds__((64 * kMostWaves<kCode, kDim, kPer, kTiles>), (wave
             }
         }
     }
+    if (!whole && !far) return;
+    float* const losses = reinterpret_cast<float*>(lds);  // [wave]
+    __syncthreads();
+    if (lane == 0) losses[wave] = kFloat ? 0.0f : lost_by_weights<kCode>((to - from) * S::kKeys, power);
+    __syncthreads();
+    float most_lost = 0.0f;
+    for (uint32_t w = 0; w < waves; w++) most_lost = fmaxf(most_lost, losses[w]);
+    __syncthreads();
+    rows_again<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, static_cast<int64_t>(step0 + from) * S::kKeys, static_cast<int64_t>(step0 + to) * S::kKeys - 1, whole,
+                     Losses{0.0f, most_lost}, reinterpret_cast<float*>(lds));
 }
 
 template <int kCode, int kDim, int kPer, int kTiles, bool kBF16>

@@ -10,7 +10,8 @@
 //   keys : scale * code in f32, once to the 11 bits of f16, where dequantize for bf16 would round to 8.  With its scale rounded to f16 first, as a value's is, all of a key's score is
 //     off by that: 8191 tokens of fp8 0.0021 of the result's norm instead of 0.0018 (0.0017 of it is the result's own rounding to bf16), for 2 % less time (641 us, and 653)
 //   values : the scale to 11 bits and the product to 11 bits, one instruction for two entries; once would take another 1.5 % and change 0.00175 to 0.00174
-//   weights : 11 bits, and over a bf16 cache of floats, which enters the matrix instructions as it is, the 8 of bf16: off by 0.0023 of the norm.  Their sum is of f32.
+//   weights : 11 bits, and over a bf16 cache of floats, which enters the matrix instructions as it is, the 8 of bf16: off by 0.0023 of the norm (7 prompts of 33 to 2047 tokens).  In two
+//     numbers of bf16, as attention_few_kernel has them, it is 0.0017, for half as many matrix instructions again: 562 us and 731 of 8191 tokens, 82 and 104 of these.  Their sum is f32.
 // For results of f16 rounded entries show (0.0012, where the result's own rounding is 0.0002): kExact keeps codes, exact in f16, and puts their scales in f32 behind the first product
 // and on the weights (0.0003).
 //
@@ -60,6 +61,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t* const powers = reinterpret_cast<uint32_t*>(lds + 2 * S::kBuffer);  // [step % 2][keys, values]: exponents, the largest of every other step so far
     uint32_t* const found = powers + 4;                                          // whether values that are no numbers, or scales far apart, need rows one by one
+    uint32_t* const lost = powers + 5;                                           // whether scales are far apart, of keys, of values
     float* const scales_at = reinterpret_cast<float*>(powers + 8);               // kExact: [step % 2][keys, values][block][64]
     constexpr uint32_t kScales = kDim / 32 * S::kKeys;                           // of a side of a step
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31u, h = lane >> 5;
@@ -340,13 +342,20 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
 #pragma unroll
             for (uint32_t v = 0; v < 16; v++) t[v] = 0.0f;
         }
+        const auto operand_of = [&](uint32_t slice, uint32_t k) { return *reinterpret_cast<const u32x4*>(keys + (k * 32u + n) * S::kPitch + slice * 32u + h * 16u); };
+        u32x4 ahead[kHalves];  // of the next slice, asked for in front of this one's products: so written, it stays so where registers are short
+#pragma unroll
+        for (uint32_t k = 0; k < kHalves; k++) ahead[k] = operand_of(0, k);
 #pragma unroll
         for (uint32_t slice = 0; slice < kSlices; slice++) {
+            u32x4 operand[kHalves];
 #pragma unroll
             for (uint32_t k = 0; k < kHalves; k++) {
-                const u32x4 operand = *reinterpret_cast<const u32x4*>(keys + (k * 32u + n) * S::kPitch + slice * 32u + h * 16u);
-                s[k] = mfma32<kBF16>(operand, q[slice], s[k]);
+                operand[k] = ahead[k];
+                if (slice + 1 < kSlices) ahead[k] = operand_of(slice + 1, k);
             }
+#pragma unroll
+            for (uint32_t k = 0; k < kHalves; k++) s[k] = mfma32<kBF16>(operand[k], q[slice], s[k]);
             if constexpr (kSlices > 8)
                 if (slice % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more operands at once than there are registers for
             if constexpr (kExact) {
@@ -384,13 +393,17 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
             for (uint32_t e = 0; e < kOut; e++) out[e] *= shrink;
         }
         const float less = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
-        u32x4 w[2 * kHalves];
+        // the weights of a quarter, sixteen keys
+        const auto weigh = [&](uint32_t quarter) {
+            u32x4 w = {};
 #pragma unroll
-        for (uint32_t v = 0; v < kSpan / 2; v += 2) {
-            t[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less)), t[v + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v + 1], times_now, less));
-            sum += t[v], sum += t[v + 1];
-            if constexpr (!kExact) w[v / 8][v % 8 / 2] = pair_of<kBF16>(t[v], t[v + 1]);
-        }
+            for (uint32_t v = quarter * 8u; v < quarter * 8u + 8u; v += 2) {
+                t[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v], times_now, less)), t[v + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[v + 1], times_now, less));
+                sum += t[v], sum += t[v + 1];
+                if constexpr (!kExact) w[v % 8 / 2] = pair_of<kBF16>(t[v], t[v + 1]);
+            }
+            return w;
+        };
         // lane (n, h): entry n of 32, keys 4 h ... 4 h + 3 and 8 more
         const auto values_of = [&](uint32_t e, uint32_t quarter) {
             u32x4 v;
@@ -404,6 +417,7 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
             return v;
         };
         if constexpr (kExact) {
+            u32x4 w[2] = {weigh(0), weigh(1)};
 #pragma unroll
             for (uint32_t e = 0; e < kOut; e++) {
                 if (e == 0 || ((first_out + e) * 32u & block_mask) == 0) {  // a block's first, or the wave's: its weights
@@ -419,13 +433,18 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
             }
         } else {
 #pragma unroll
-            for (uint32_t quarter = 0; quarter < 2 * kHalves; quarter++)
+            for (uint32_t quarter = 0; quarter < 2 * kHalves; quarter++) {
+                u32x4 v[kOut];  // asked for in front of the weights
 #pragma unroll
-                for (uint32_t e = 0; e < kOut; e++) out[e] = mfma32<kBF16>(values_of(e, quarter), w[quarter], out[e]);
+                for (uint32_t e = 0; e < kOut; e++) v[e] = values_of(e, quarter);
+                const u32x4 w = weigh(quarter);
+#pragma unroll
+                for (uint32_t e = 0; e < kOut; e++) out[e] = mfma32<kBF16>(v[e], w, out[e]);
+            }
         }
     };
 
-    if (threadIdx.x < 5) powers[threadIdx.x] = 0u;  // and *found
+    if (threadIdx.x < 7) powers[threadIdx.x] = 0u;  // and *found, lost
     __syncthreads();
     if (from < to) {
         Raw raw;
@@ -477,37 +496,59 @@ __global__ __launch_bounds__((Many<kCode, kDim>::kThreads), (kDim == 64 && !kExa
         }
     }
 
-    if (!kFloat && (lost_below(least_value, value_power) || lost_below(least_key, key_power))) *found = 1u;
+    const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum), f32_bits(sum), false, false);
+    const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
+    if constexpr (!kFloat) {
+        if (lost_below(least_key, key_power)) lost[0] = 1u;
+        if (lost_below(least_value, value_power)) lost[1] = 1u;
+    }
     __syncthreads();
-    if (*found) {
-        const int64_t first_key = static_cast<int64_t>(step0 + from) * S::kKeys, last_key = static_cast<int64_t>(step0 + to) * S::kKeys - 1;
+    const auto again = [&](bool whole, Losses losses) {
         __syncthreads();
-        rows_one_by_one<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, first_key, last_key, reinterpret_cast<float*>(lds));
+        rows_again<kDim>(at.s.index, at.row0, at.rows, part, parts, kv_head, static_cast<int64_t>(step0 + from) * S::kKeys, static_cast<int64_t>(step0 + to) * S::kKeys - 1, whole, losses,
+                         reinterpret_cast<float*>(lds));
+    };
+    if (*found) {
+        again(true, Losses{});
         return;
     }
 
-    const float up = kFloat ? 1.0f : (kExact ? 1.0f : 2.0f) * ldexpf(1.0f, out_power);
-    const auto halves = __builtin_amdgcn_permlane32_swap(f32_bits(sum), f32_bits(sum), false, false);
-    const float all = bits_f32(halves[0]) + bits_f32(halves[1]);
-    const float by = all == 0.0f ? 0.0f : 1.0f / all;
-    if (own >= at.rows) return;
-    const uint64_t token = token_of(), of = (token * a.heads + head_of()) * split.splits + part;
-    if (parts > 1 && h == 0 && first_out == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = all;
+    const auto store = [&](const AttentionArgs& a, const Split& split) {
+        if (own >= at.rows) return;
+        const float up = kFloat ? 1.0f : (kExact ? 1.0f : 2.0f) * ldexpf(1.0f, out_power), by = all == 0.0f ? 0.0f : 1.0f / all;
+        const uint32_t row = row_of(), head = kv_head * a.group + row % a.group;
+        const uint64_t token = at.s.first + row / a.group, of = (token * a.heads + head) * split.splits + part;
+        if (parts > 1 && h == 0 && first_out == 0) split.stats[2 * of] = top, split.stats[2 * of + 1] = all;
 #pragma unroll
-    for (uint32_t e = 0; e < kOut; e++)
+        for (uint32_t e = 0; e < kOut; e++)
 #pragma unroll
-        for (uint32_t v = 0; v < 16; v += 4) {
-            const uint32_t d = (first_out + e) * 32u + v * 2u + 4u * h;
-            if (d >= dim) continue;
-            f32x4 four;
+            for (uint32_t v = 0; v < 16; v += 4) {
+                const uint32_t d = (first_out + e) * 32u + v * 2u + 4u * h;
+                if (d >= dim) continue;
+                f32x4 four;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) four[i] = all == 0.0f ? 0.0f : out[e][v + i] * by * up;
-            if (parts > 1)
-                *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = four;
-            else
-                *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head_of() * a.y_head + d) * 2u) =
-                    a.dtype == CQ_BF16 ? u32x2{pair_of<true>(four[0], four[1]), pair_of<true>(four[2], four[3])} : u32x2{pair_of<false>(four[0], four[1]), pair_of<false>(four[2], four[3])};
-        }
+                for (uint32_t i = 0; i < 4; i++) four[i] = all == 0.0f ? 0.0f : out[e][v + i] * by * up;
+                if (parts > 1)
+                    *reinterpret_cast<f32x4*>(split.parts + of * dim + d) = four;
+                else
+                    *reinterpret_cast<u32x2*>(a.y + (token * a.y_token + head * a.y_head + d) * 2u) =
+                        a.dtype == CQ_BF16 ? u32x2{pair_of<true>(four[0], four[1]), pair_of<true>(four[2], four[3])} : u32x2{pair_of<false>(four[0], four[1]), pair_of<false>(four[2], four[3])};
+            }
+    };
+    if constexpr (kExact) {  // whose scalar registers are short (8191 tokens 912 us, and 926 with the arguments kept)
+        const Arguments& late = arguments_again();
+        store(late.a, late.split);
+    } else {
+        store(a, split);
+    }
+    if constexpr (!kFloat) {
+        if ((lost[0] | lost[1]) == 0u) return;
+        // a score is off by 2^-25 of numbers whose unit is 2^(key_power + 1), times the queries; a result by as much of values' scales, times a code, where those are numbers
+        Losses losses{};
+        if (lost[0]) losses.key = ldexpf(fabsf(a.scale) * kLog2E, key_power - 24);
+        if (lost[1]) losses.value = kExact ? lost_by_weights<kCode>((to - from) * S::kKeys, value_power) : ldexpf(kMostCode<kCode>, value_power - 24);
+        again(false, losses);
+    }
 }
 
 template <int kCode, int kDim, bool kBF16, bool kExact>

@@ -25,8 +25,9 @@ extern "C" {
  *   scheme : NULL for floats typed like the calls' dtype (no scales); else 8- or 4-bit values in blocks along the last dimension: i8, e4m3,
  *            e5m2 and e2m1 of the native store, the two's-complement fields of the U32 store of Q8*, Q4*, E2M1 and E2M1_OCP (codes and strides
  *            of the U32 store in words).  Else CQ_ERR_UNSUPPORTED_SCHEME.
- *   key_scales, value_scales : [pages, kv_heads, page_size, dim / block] typed scheme->param, any strides
- * The entries of a cache are scale * code, not rounded again. */
+ *   key_scales, value_scales : [pages, kv_heads, page_size, dim / block] typed scheme->param, any strides.  Scales of 16 bits are read as the aligned
+ *            four bytes around them: up to two bytes in front of such a tensor and behind it are read, and not used.
+ * The entries of a cache are scale * code; cq_attention says what becomes of them. */
 typedef struct cq_cache {
     const cq_tensor* keys;
     const cq_tensor* key_scales;
@@ -37,7 +38,7 @@ typedef struct cq_cache {
 
 /* Rotary positions: of each head the first 2 * (number of frequencies) entries are turned in pairs (a, b) by the angle position * frequency,
  *   a' = a c - b w, b' = b c + a w, with c = magnitude cos(angle) and w = magnitude sin(angle),
- * in 64 bits, rounded once; the other entries stay.  Longer contexts are a matter of the frequencies and of the magnitude.
+ * in 64 bits, rounded to f32 and from there to `dtype`; the other entries stay.  Longer contexts are a matter of the frequencies and of the magnitude.
  *   frequencies : f32 [n], contiguous, 2 n <= dim.  Angles of 2^31 and more have no meaning.
  *   interleaved : 0: entry i pairs with entry i + n; 1: entry 2 i with entry 2 i + 1 */
 typedef struct cq_rotary {
@@ -46,7 +47,7 @@ typedef struct cq_rotary {
     uint32_t interleaved;
 } cq_rotary;
 
-/* New tokens into their slots: keys turned by their positions, rounded to `dtype` and quantized, values quantized; queries turned.
+/* New tokens into their slots: keys turned by their positions (and so rounded to `dtype`) and quantized, values quantized; queries turned.
  *   k, v  : [tokens, kv_heads, dim] typed `dtype`, the last dimension contiguous (views of a common projection for one)
  *   slots : i32 [tokens], contiguous.  A token whose slot lies outside of the cache (-1 for one) is not stored.  Two tokens in one slot: what it
  *           holds afterwards may be parts of both.
@@ -60,7 +61,7 @@ cq_status cq_cache_append(cq_stream_t stream, const cq_cache* cache, const cq_te
  * The query at position p sees the keys 0 <= j < length with j <= p or j < prefix, and, where window > 0, p - j < window.
  *   slopes : NULL or f32 [heads], contiguous
  *   prefix : NULL or i32 [sequences], contiguous, each taken as the nearest number between 0 and the sequence's length
- * cap is 0 (none) or a positive number.  Every field not used is 0. */
+ * cap is 0 (none) or a positive number, of which those past 10^38 count as that.  Every field not used is 0. */
 typedef struct cq_scores {
     float scale;
     float cap;
@@ -79,7 +80,14 @@ typedef struct cq_scores {
  *             are taken as the nearest inside; tokens of no sequence are left unwritten.
  *   lengths : i32 [sequences], contiguous: keys of a sequence with its new ones: its last token is at position lengths[s] - 1.  Taken as the
  *             nearest number between 0 and what the table's row holds.
- * A token that sees no key gets zeros.  Entries of the cache that a token does not see do not enter its result, whatever they hold.
+ * A token that sees no key gets zeros.  Entries of the cache that a token does not see do not enter its result, whatever they hold; what it sees of infinities and NaN does, and
+ * so do those of its query.
+ * Scores, statistics and sums are f32, and for f32 queries so is everything else.  For 16-bit ones, on their way into matrix instructions, are rounded
+ *   weights, with a value's scale : to 11 bits (over a cache of bf16 floats to 16; to 8 for prompts)
+ *   queries of bf16 over a quantized cache : entries below 2^-14 of the largest of their head, to 2^-25 of it
+ *   entries of a quantized cache, for prompts of bf16 : keys to 11 bits, values twice, by their scale and by the product
+ * and what is 2^-18 of a token's largest weight, or 2^-12 of a step between two codes, is lost.  Where scales of a sequence lie further apart than 2^12 (zeros aside), tokens that
+ * would lose more to others' scales than 2^-11 of the largest of 32 neighbouring entries of their result are taken once more, one by one, in f32: many times slower.
  *   workspace : optional device scratch of cq_attention_workspace_bytes() bytes, 16-byte aligned; lets few tokens over long
  *             sequences spread over the GPU.  Without it they are right, and slower.  It holds nothing between calls: calls whose kernels
  *             do not run at the same time may share it. */

@@ -1,9 +1,10 @@
 """cq_attention where finite scales differ by many powers of two between keys: what a token does not see, or gives no weight, does not take bits from what it
 does see.
 
-Bounds are those of attention_reference.py for the entries that a token gives weight to.  Scales that differ by up to 2^14 stay on the matrix cores, where 16 bits below the
-largest scale hold: of a weight, half of f16's smallest step, 2^-25, of a largest weight of at least 2^5, times the ratio 2^14, so 2^-16 |v_j| of each key; of an entry
-that is made a number of f16, 2^-25 of numbers up to 2 (2^14 times its scale), so 2^-10 of its scale, of a key's entry times |q| in the score."""
+Bounds are those of attention_reference.py for the entries that a token gives weight to, and what 16 bits below the largest scale may lose on the matrix cores.
+Where scales differ by up to 2^12: of a weight, half of f16's smallest step, 2^-25, of a largest weight of at least 2^5, times 2^12, so 2^-18 |v_j| of each key; of an entry
+that is made a number of f16, 2^-25 of numbers up to 2 (2^12 times its scale), so 2^-12 of its scale, of a key's entry times |q| in the score.  Where they differ by more, tokens stay there
+whose results are 2^15 times what they may have lost, so 2^-15 of the largest of 16 or 32 neighbouring entries, and whose scores are off by 2^-12 (times ln 2) at most."""
 import numpy as np
 import pytest
 
@@ -23,17 +24,22 @@ def scheme(name, block, param=0):
     return scheme_of(CODES[name][0], [block], param, CODES[name][1])
 
 
+def far_bound(want, size):
+    """What is added to a bound for scales that differ by more than 2^12."""
+    tiles = np.abs(want).reshape(want.shape[:2] + (-1, 32)).max(-1).repeat(32, -1)
+    return 2.0 ** -15 * tiles + 2.0 * size * 2.0 ** -12 * np.log(2.0)
+
+
 def spread_bound(case, size, scale):
-    """What is added to a bound for scales that differ by up to 2^14: of weights and numbers of values, and of numbers of keys in the scores."""
+    """The same for those that differ by less."""
     of = [float(pool.scales.double().abs().max()) for pool in (case.k, case.v)]
     extra = np.zeros(case.q.shape)
     q = case.q.double().abs().sum(-1).numpy()[..., None]
     for s, (n, _) in enumerate(case.sequences):
         a = case.offsets[s]
         for head in range(case.q.shape[1]):
-            total = np.abs(case.of_sequence(case.v, s, head // case.group)).sum(0)
-            extra[a:a + n, head] = 2.0 ** -16 * total + 2.0 ** -10 * of[1]
-    return extra + 2.0 * size * scale * q * 2.0 ** -10 * of[0]
+            extra[a:a + n, head] = 2.0 ** -18 * np.abs(case.of_sequence(case.v, s, head // case.group)).sum(0)
+    return extra + 2.0 ** -12 * of[1] + 2.0 * size * scale * q * 2.0 ** -12 * of[0]
 
 
 def sizes(case, **scores):
@@ -74,7 +80,8 @@ def test_large_scales_of_a_last_token(oracle, name, tokens, elem):
         for seed, length in enumerate((tokens, 23 * 32 + tokens)):
             case = Attention(oracle, seed, [(tokens, length), (tokens, tokens + 3)], 4, 2, dim, 16, elem, scheme(name, block))
             want, bound = case.want()
-            bound = bound + spread_bound(case, sizes(case), dim ** -0.5)
+            size = sizes(case)
+            bound = bound + far_bound(want, size) + spread_bound(case, size, dim ** -0.5)
             rows = np.arange(case.tokens) != tokens - 1
             for of, factor in [("v", f) for f in FACTORS] + [("k", f) for f in FACTORS[1:]]:
                 with enlarged(case, of, 0, [length - 1], factor):
@@ -93,6 +100,7 @@ def test_large_scales_behind_a_window(oracle, name, tokens, elem):
     for dim, block in OF_CODE[name][:2]:
         case = Attention(oracle, 2, [(tokens, 700), (tokens, tokens + 3)], 4, 2, dim, 16, elem, scheme(name, block, 2))
         want, bound = case.want(window=100)
+        bound = bound + far_bound(want, sizes(case, window=100))
         for of in "vk":
             for factor in FACTORS[2:]:
                 with enlarged(case, of, 0, [700 - tokens - 99], factor):
@@ -111,6 +119,7 @@ def test_large_values_without_weight(oracle, name, tokens, elem):
         for back, slope in ((900, 0.5), (20, 16.0)):
             slopes = np.full(4, slope, np.float32)
             want, bound = case.want(slopes=slopes)
+            bound = bound + far_bound(want, sizes(case, slopes=slopes))
             for factor in FACTORS[2:]:
                 for workspace in (True, False):
                     with enlarged(case, "v", 0, [959 - back], factor):
