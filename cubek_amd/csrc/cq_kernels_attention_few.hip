@@ -9,11 +9,12 @@
 // Codes enter as themselves, exact in f16, keys' scales in f32 behind the first product, values' scales in front of the second, on the weights: no
 // entry is rounded, and a value of the cache costs 1.25 vector instructions at 8 bits (0.5 of fp8) instead of the 2.5 to 4 of its dequantization.
 // Where a scale covers 32 entries of a longer head, lanes swap parts so that one instruction has one block (`kPer` > 1).
-// Queries are scaled by a power of two per row, weights by one per step, so that f16 holds them whatever the range of bf16.
+// Queries are scaled by a power of two per row, weights by one of the largest scale so far, so that f16 holds them whatever the range of bf16 (kSpread says how far apart scales may
+// be).  Weights with their value's scale are rounded to the 11 bits of f16, and over bf16 floats to two numbers of bf16; of bf16 queries what is below 2^-14 of the largest loses bits.
 //
 // Bound by the read of the cache where sequences are many and long (64 of 4096 keys, 8 heads of 128 of i8: 100 us, 5.5 TB/s; lengths from 257 to 8191: 117,
-// 4.9 TB/s); by vector instructions at 4 bits with a scale for 32 entries (one sequence of 131071 keys: 45 us of which 4.5 join 64 parts,
-// 3.3 TB/s, vector units busy 54 %); where there is little to read, by a launch and four rounds of loads that need each other, lengths, pages, codes, and
+// 4.9 TB/s); by vector instructions at 4 bits with a scale for 32 entries (one sequence of 131071 keys: 46 us of which 5 join 64 parts,
+// 3.3 TB/s, vector units busy 53 %); where there is little to read, by a launch and four rounds of loads that need each other, lengths, pages, codes, and
 // then a wave's steps one after another (24 tiles of up to 701 keys: 14 us).
 #include <hip/hip_runtime.h>
 
@@ -78,7 +79,7 @@ __device__ __forceinline__ bool code_is_odd(u32x4 v) {
 }
 
 // Waves per SIMD that registers are kept for: the most that builds show to need no scratch memory.  (Compiled for one more, loads of spilled registers stood in the loop: 64 tokens
-// over 4 bits in blocks of 32, heads of 256, 604 us, 195 without them; five drafted tokens of 20 rows 178 and 80, over 8 bits 178 and 58.)
+// over 4 bits in blocks of 32, heads of 256, 604 us, 188 without them; five drafted tokens of 20 rows 178 and 76, over 8 bits 178 and 57.)
 template <int kCode, int kDim, int kPer, int kTiles>
 constexpr int waves_of() {
     constexpr bool kNibbles = kCodeBits<kCode> == 4;

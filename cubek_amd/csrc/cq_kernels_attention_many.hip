@@ -16,8 +16,8 @@
 // and on the weights (0.0003).
 //
 // A step of a head of 128 is 32 matrix instructions of a wave (1024 cycles) beside about 250 vector instructions, 150 of them the softmax's; with two waves on a
-// SIMD they overlap in part, and the card's power limits the rest: a prompt of 8191 tokens, 32 heads over 8 of fp8, 604-640 us, 860-910 TFLOP/s at 1.9 GHz,
-// matrix units busy 39 %, vector units 47 %, LDS 49 %.
+// SIMD they overlap in part, and no unit is full: a prompt of 8191 tokens, 32 heads over 8 of fp8, 630-645 us, 850-870 TFLOP/s at 1.8 GHz, vector units busy 47 %, matrix units
+// 36 %, LDS 46 %, waves waiting for a barrier or for LDS in 39 % of their cycles.
 #include <hip/hip_runtime.h>
 
 #include "cq_attention_tiles.hpp"
@@ -559,8 +559,8 @@ hipError_t launch_many(hipStream_t s, const AttentionArgs& a, const Split& split
     return hipGetLastError();
 }
 
-// A number of f16 is rounded to 11 bits: less than a result of bf16 shows (8191 tokens of fp8: off by 0.0021 of its norm, 0.0017 of it the result's own rounding),
-// more than one of f16 does (0.0012 and 0.0002), so those are made of the codes.
+// A number of f16 is rounded to 11 bits: hardly more than a result of bf16 shows (8191 tokens of fp8: off by 0.0018 of its norm, 0.0017 of it the result's own rounding; of codes 0.0017,
+// for 40 % more time), more than one of f16 does (0.0012 and 0.0002), so those are made of the codes.
 template <int kCode, int kDim>
 hipError_t launch_type(hipStream_t s, const AttentionArgs& a, const Split& split) {
     if constexpr (kCode == kCacheFloat) {

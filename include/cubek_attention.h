@@ -72,8 +72,8 @@ typedef struct cq_scores {
 } cq_scores;
 
 /* y = softmax(scores of q) V for the new tokens of all sequences, whose keys and values are in the cache already.
- *   q, y    : [tokens, heads, dim] typed `dtype`, last dimensions contiguous; heads is a multiple of kv_heads, and heads h * group ...
- *             h * group + group - 1 share head h of the cache
+ *   q, y    : [tokens, heads, dim] typed `dtype`, last dimensions contiguous, not in the same memory; heads is a multiple of kv_heads, and heads
+ *             h * group ... h * group + group - 1 share head h of the cache
  *   table   : i32 [sequences, most pages of one], rows contiguous: page j / page_size of a sequence holds its key j.  Entries behind a
  *             sequence's length are not read; one outside of the cache is taken as the nearest inside.
  *   offsets : i32 [sequences + 1], contiguous: tokens offsets[s] <= t < offsets[s + 1] are the newest of sequence s, in order.  Values outside
